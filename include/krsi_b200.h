@@ -186,6 +186,42 @@ int krsi_t5_bias_fwd(const void* table, float* pd, int64_t S, int64_t H, int num
 int krsi_t5_bias_bwd(const float* dpd, void* dtable, int64_t S, int64_t H, int num_buckets, int max_distance,
                      int bidirectional, int table_dtype, cudaStream_t stream);
 
+/* ---------------------------------------------------------------- embedding
+ * out[i] = scale * table[tokens[i]] and the table's gradient.  The reference has no embedding op (its
+ * models leave the lookup to torch).
+ * tokens: [n] of token_bits 32 or 64 (int32/int64); table, dtable: [V, d]; out, g: [n, d]; all but the
+ * tokens of `dtype`, contiguous.  A token outside [0, V) gives a row of NaN and no gradient. */
+int krsi_embedding_fwd(const void* tokens, int token_bits, const void* table, void* out, int64_t n,
+                       int64_t V, int64_t d, float scale, int dtype, cudaStream_t stream);
+
+/* Bytes of workspace krsi_embedding_bwd needs (the sorted positions and the partial rows of tokens
+ * that occur often). */
+int krsi_embedding_bwd_workspace_size(int64_t n, int64_t V, int64_t d, size_t* bytes);
+
+/* dtable[v] = scale * sum of g[i] over the i with tokens[i] = v, summed in fp32 in a fixed order over
+ * the sorted positions (deterministic, no atomics) and rounded once; every row of dtable is written.
+ * padding_idx: a token whose row gets no gradient, or -1.  workspace: 16-byte aligned. */
+int krsi_embedding_bwd(const void* tokens, int token_bits, const void* g, void* dtable, void* workspace,
+                       size_t workspace_bytes, int64_t n, int64_t V, int64_t d, float scale,
+                       int64_t padding_idx, int dtype, cudaStream_t stream);
+
+/* ---------------------------------------------------------------- GEGLU with an 8-bit checkpoint
+ * krsi_geglu_fwd/bwd with u kept for the backward in 8 bits.  No counterpart in the reference (its
+ * backward reads u in full, geglu.py:64-68).
+ * The checkpoint: q [rows, 2F] int8 and exponents [rows, ceil(F / 32), 2] uint8 (gate, value); in a
+ * group of 32 columns of a half-row u is kept as q * 2^(e - 127), with 2^(e - 127) = 2^-6 of the power
+ * of two at or below the group's largest magnitude (2^-126 at least) and q rounded to nearest even
+ * within [-127, 127].  e = 255 marks a group with a value that is not finite: it reads back as NaN.
+ * out = gelu_tanh(u[:, :F]) * u[:, F:] from u itself, in fp32, rounded once (krsi_geglu_fwd rounds
+ * gelu_tanh to dtype before the product).  q and exponents both null: no checkpoint, out alone. */
+int krsi_geglu_q8_fwd(const void* u, void* out, void* q, void* exponents, int64_t rows, int64_t F, int dtype,
+                      cudaStream_t stream);
+
+/* du = [d(gate) | d(value)] of GEGLU at the checkpoint's values, for g [rows, F]; and, where out is not
+ * null, out [rows, F] = GEGLU of those values (an operand of the down projection's weight gradient). */
+int krsi_geglu_q8_bwd(const void* g, const void* q, const void* exponents, void* du, void* out, int64_t rows,
+                      int64_t F, int dtype, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

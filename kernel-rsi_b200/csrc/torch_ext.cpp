@@ -275,6 +275,106 @@ at::Tensor t5_bias_bwd(const at::Tensor& dpd_in, const at::Tensor& table, int64_
   return dtable;
 }
 
+// ---------------------------------------------------------------- embedding
+int token_bits_of(const at::Tensor& t, const char* what) {
+  TORCH_CHECK(t.scalar_type() == at::kLong || t.scalar_type() == at::kInt, what, " must be int32 or int64, got ",
+              t.scalar_type());
+  return t.scalar_type() == at::kLong ? 64 : 32;
+}
+
+void check_same_device(const at::Tensor& a, const at::Tensor& b, const char* what) {
+  TORCH_CHECK(a.device() == b.device(), what, ": tensors on different devices (", a.device(), " and ", b.device(), ")");
+}
+
+// padding_idx is its registered gradient's: the lookup itself treats that token like any other.
+at::Tensor embedding_fwd(const at::Tensor& tokens_in, const at::Tensor& table_in, double scale, int64_t /*padding_idx*/) {
+  check_cuda(tokens_in, "tokens");
+  check_cuda(table_in, "table");
+  check_same_device(tokens_in, table_in, "embedding");
+  TORCH_CHECK(table_in.dim() == 2 && table_in.size(0) > 0 && table_in.size(1) > 0, "embedding: table must be [V, d]");
+  const int bits = token_bits_of(tokens_in, "embedding: tokens");
+  c10::cuda::CUDAGuard guard(table_in.device());
+  auto tokens = tokens_in.contiguous();
+  auto table = table_in.contiguous();
+  auto sizes = tokens.sizes().vec();
+  sizes.push_back(table.size(1));
+  auto out = at::empty(sizes, table.options());
+  check_rc(krsi_embedding_fwd(tokens.data_ptr(), bits, table.data_ptr(), out.data_ptr(), tokens.numel(), table.size(0),
+                              table.size(1), (float)scale, krsi_dtype_of(table), at::cuda::getCurrentCUDAStream()),
+           "krsi_embedding_fwd");
+  return out;
+}
+
+at::Tensor embedding_bwd(const at::Tensor& g_in, const at::Tensor& tokens_in, const at::Tensor& table, double scale,
+                         int64_t padding_idx) {
+  check_cuda(g_in, "g");
+  check_cuda(tokens_in, "tokens");
+  check_cuda(table, "table");
+  check_same_device(tokens_in, table, "embedding_bwd");
+  check_same_device(g_in, table, "embedding_bwd");
+  TORCH_CHECK(table.dim() == 2 && g_in.dim() > 0 && g_in.size(-1) == table.size(1) &&
+                  g_in.numel() == tokens_in.numel() * table.size(1),
+              "embedding_bwd: g must be [*tokens.shape, d]");
+  TORCH_CHECK(padding_idx >= -1 && padding_idx < table.size(0), "embedding_bwd: padding_idx out of range");
+  const int bits = token_bits_of(tokens_in, "embedding_bwd: tokens");
+  c10::cuda::CUDAGuard guard(table.device());
+  auto tokens = tokens_in.contiguous();
+  auto g = g_in.to(table.scalar_type()).contiguous();
+  auto dtable = at::empty(table.sizes(), table.options().memory_format(at::MemoryFormat::Contiguous));
+  const int64_t n = tokens.numel(), V = table.size(0), d = table.size(1);
+  size_t ws = 0;
+  check_rc(krsi_embedding_bwd_workspace_size(n, V, d, &ws), "krsi_embedding_bwd_workspace_size");
+  auto wsp = workspace(g, ws);
+  check_rc(krsi_embedding_bwd(tokens.data_ptr(), bits, g.data_ptr(), dtable.data_ptr(), wsp.data_ptr(),
+                              (size_t)wsp.numel(), n, V, d, (float)scale, padding_idx, krsi_dtype_of(table),
+                              at::cuda::getCurrentCUDAStream()),
+           "krsi_embedding_bwd");
+  return dtable;
+}
+
+// ---------------------------------------------------------------- GEGLU with an 8-bit checkpoint
+// (out, q, exponents): the checkpoint is empty unless it is to be kept.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> geglu_q8_fwd(const at::Tensor& u_in, bool keep) {
+  check_cuda(u_in, "u");
+  TORCH_CHECK(u_in.dim() == 2 && u_in.size(1) % 2 == 0, "geglu_q8: u must be [rows, 2F]");
+  c10::cuda::CUDAGuard guard(u_in.device());
+  auto u = u_in.contiguous();
+  const int64_t rows = u.size(0), F = u.size(1) / 2;
+  auto out = at::empty({rows, F}, u.options());
+  auto q = at::empty({keep ? rows : 0, 2 * F}, u.options().dtype(at::kChar));
+  auto ex = at::empty({keep ? rows : 0, (F + 31) / 32, 2}, u.options().dtype(at::kByte));
+  check_rc(krsi_geglu_q8_fwd(u.data_ptr(), out.data_ptr(), keep ? q.data_ptr() : nullptr,
+                             keep ? ex.data_ptr() : nullptr, rows, F, krsi_dtype_of(u),
+                             at::cuda::getCurrentCUDAStream()),
+           "krsi_geglu_q8_fwd");
+  return {out, q, ex};
+}
+
+// (du, out): out is GEGLU of the checkpoint's values, empty unless asked for.
+std::tuple<at::Tensor, at::Tensor> geglu_q8_bwd(const at::Tensor& g_in, const at::Tensor& q, const at::Tensor& ex,
+                                                bool want_out) {
+  check_cuda(g_in, "g");
+  check_cuda(q, "q");
+  check_cuda(ex, "exponents");
+  TORCH_CHECK(q.dim() == 2 && q.size(1) % 2 == 0 && q.scalar_type() == at::kChar && q.is_contiguous(),
+              "geglu_q8_bwd: q must be a contiguous int8 [rows, 2F]");
+  const int64_t rows = q.size(0), F = q.size(1) / 2;
+  TORCH_CHECK(g_in.dim() == 2 && g_in.size(0) == rows && g_in.size(1) == F, "geglu_q8_bwd: g must be [rows, F]");
+  TORCH_CHECK(ex.scalar_type() == at::kByte && ex.is_contiguous() && ex.numel() == rows * ((F + 31) / 32) * 2,
+              "geglu_q8_bwd: exponents must be a contiguous uint8 [rows, ceil(F / 32), 2]");
+  check_same_device(g_in, q, "geglu_q8_bwd");
+  check_same_device(ex, q, "geglu_q8_bwd");
+  c10::cuda::CUDAGuard guard(q.device());
+  auto g = g_in.contiguous();
+  auto du = at::empty({rows, 2 * F}, g.options());
+  auto out = at::empty({want_out ? rows : 0, F}, g.options());
+  check_rc(krsi_geglu_q8_bwd(g.data_ptr(), q.data_ptr(), ex.data_ptr(), du.data_ptr(),
+                             want_out ? out.data_ptr() : nullptr, rows, F, krsi_dtype_of(g),
+                             at::cuda::getCurrentCUDAStream()),
+           "krsi_geglu_q8_bwd");
+  return {du, out};
+}
+
 }  // namespace
 
 TORCH_LIBRARY(krsi, m) {
@@ -290,6 +390,10 @@ TORCH_LIBRARY(krsi, m) {
         "float scale) -> (Tensor, Tensor)");
   m.def("t5_bias_fwd(Tensor table, int S, int num_buckets, int max_distance, bool bidirectional) -> Tensor");
   m.def("t5_bias_bwd(Tensor dpd, Tensor table, int S, int num_buckets, int max_distance, bool bidirectional) -> Tensor");
+  m.def("embedding_fwd(Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
+  m.def("embedding_bwd(Tensor g, Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
+  m.def("geglu_q8_fwd(Tensor u, bool keep) -> (Tensor, Tensor, Tensor)");
+  m.def("geglu_q8_bwd(Tensor g, Tensor q, Tensor exponents, bool want_out) -> (Tensor, Tensor)");
 }
 
 TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
@@ -304,4 +408,8 @@ TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
   m.impl("relpos_attn_bwd", &relpos_attn_bwd);
   m.impl("t5_bias_fwd", &t5_bias_fwd);
   m.impl("t5_bias_bwd", &t5_bias_bwd);
+  m.impl("embedding_fwd", &embedding_fwd);
+  m.impl("embedding_bwd", &embedding_bwd);
+  m.impl("geglu_q8_fwd", &geglu_q8_fwd);
+  m.impl("geglu_q8_bwd", &geglu_q8_bwd);
 }

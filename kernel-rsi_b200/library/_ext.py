@@ -122,6 +122,26 @@ def _register_compile_support() -> None:
     def _(dpd, table, S, num_buckets, max_distance, bidirectional):
         return torch.empty_like(table)
 
+    @reg_fake("krsi::embedding_fwd")
+    def _(tokens, table, scale, padding_idx):
+        return table.new_empty((*tokens.shape, table.shape[1]))
+
+    @reg_fake("krsi::embedding_bwd")
+    def _(g, tokens, table, scale, padding_idx):
+        return table.new_empty(table.shape)
+
+    @reg_fake("krsi::geglu_q8_fwd")
+    def _(u, keep):
+        rows, F = u.shape[0], u.shape[1] // 2
+        kept = rows if keep else 0
+        return (u.new_empty((rows, F)), u.new_empty((kept, 2 * F), dtype=torch.int8),
+                u.new_empty((kept, (F + 31) // 32, 2), dtype=torch.uint8))
+
+    @reg_fake("krsi::geglu_q8_bwd")
+    def _(g, q, exponents, want_out):
+        rows, F = q.shape[0], q.shape[1] // 2
+        return g.new_empty((rows, 2 * F)), g.new_empty((rows if want_out else 0, F))
+
     # Autograd of the forward ops, used when a compiled graph contains them (the eager path
     # uses the autograd.Function classes of each module instead).
     def rms_setup(ctx, inputs, output):
@@ -176,6 +196,25 @@ def _register_compile_support() -> None:
         return ops.t5_bias_bwd(dpd.contiguous(), table, *ctx.args), None, None, None, None
 
     torch.library.register_autograd("krsi::t5_bias_fwd", t5_backward, setup_context=t5_setup)
+
+    def emb_setup(ctx, inputs, output):
+        tokens, table, scale, padding_idx = inputs
+        ctx.save_for_backward(tokens, table)
+        ctx.args = (scale, padding_idx)
+
+    def emb_backward(ctx, g):
+        tokens, table = ctx.saved_tensors
+        return None, ops.embedding_bwd(g, tokens, table, *ctx.args), None, None
+
+    torch.library.register_autograd("krsi::embedding_fwd", emb_backward, setup_context=emb_setup)
+
+    def q8_setup(ctx, inputs, output):
+        ctx.save_for_backward(output[1], output[2])
+
+    def q8_backward(ctx, g, _gq, _gex):
+        return ops.geglu_q8_bwd(g, *ctx.saved_tensors, False)[0], None
+
+    torch.library.register_autograd("krsi::geglu_q8_fwd", q8_backward, setup_context=q8_setup)
 
 
 _register_compile_support()
