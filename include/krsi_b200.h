@@ -222,6 +222,40 @@ int krsi_geglu_q8_fwd(const void* u, void* out, void* q, void* exponents, int64_
 int krsi_geglu_q8_bwd(const void* g, const void* q, const void* exponents, void* du, void* out, int64_t rows,
                       int64_t F, int dtype, cudaStream_t stream);
 
+/* ---------------------------------------------------------------- vocabulary cross entropy
+ * Softmax cross entropy of a projection onto the vocabulary, and both gradients, without the [N, V]
+ * logits in memory.  The reference has no loss op.
+ *   l = scale * x @ w^T, lse_i = log sum_v exp(l[i, v]),
+ *   loss_i = lse_i - l[i, t_i] + z_loss * lse_i^2, 0 for an ignored row.
+ * x, dx: [N, K]; w, dw: [V, K]; `dtype` BF16 or F16, contiguous, 16-byte aligned; K a multiple of 8.
+ * targets: [N] of target_bits 32 or 64; a row whose target is ignore_index has loss and gradients of
+ * zero, whatever its x holds; a target outside [0, V) that is not ignore_index makes the loss and the
+ * gradients NaN.  workspace: 256-byte aligned.  Needs clusters of two CTAs (KRSI_ERR_UNSUPPORTED where
+ * the device has none). */
+
+/* Bytes of workspace: mode 0 krsi_linear_ce_fwd without gradients, 1 with, 2 krsi_linear_ce_grad. */
+int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, int mode, size_t* bytes);
+
+/* loss: [N] fp32.  reduced: two floats or null: the sum of the losses (mean: divided by the number of
+ * rows that are not ignored, at least 1) and the weight of one row in it (1, or one over that number).
+ * dx, dw: null, or fp32 gradients of the sum of the losses without the factor `scale`, for
+ * krsi_linear_ce_finish: the logits are computed once for loss and gradients. */
+int krsi_linear_ce_fwd(const void* x, const void* w, const void* targets, int target_bits, float* loss,
+                       float* reduced, float* dx, float* dw, void* workspace, size_t workspace_bytes, int64_t N,
+                       int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss, int mean,
+                       int dtype, cudaStream_t stream);
+
+/* Gradients for the upstream gradient g of each row's loss (fp32, stride 1, or 0: one for all rows), times
+ * *weight where that is not null.  dx, dw: of `dtype`, one of them may be null. */
+int krsi_linear_ce_grad(const void* x, const void* w, const void* targets, int target_bits, const float* g,
+                        int64_t g_stride, const float* weight, void* dx, void* dw, void* workspace,
+                        size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index,
+                        float z_loss, int dtype, cudaStream_t stream);
+
+/* out = scale * *g * *weight * grad, rounded once (g, weight: device scalars or null); n a multiple of 8. */
+int krsi_linear_ce_finish(const float* grad, const float* g, const float* weight, void* out, int64_t n,
+                          float scale, int dtype, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

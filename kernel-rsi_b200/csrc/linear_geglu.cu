@@ -36,6 +36,7 @@
 #include "attn_common.cuh"
 #include "common.cuh"
 #include "gelu.cuh"
+#include "gemm_common.cuh"
 #include "watchdog.cuh"
 
 KRSI_DEFINE_WATCHDOG(gemm)
@@ -44,6 +45,9 @@ namespace krsi {
 namespace {
 
 using namespace sm100;
+using gemm::drain_loads;
+using gemm::kmajor_sw128;
+using gemm::make_map;
 
 constexpr int kBM = 128;                 // rows per tile (UMMA M)
 constexpr int kBF = 128;                 // F-columns per tile: UMMA N = 2 * kBF (gate | value)
@@ -80,20 +84,6 @@ struct GemmArgs {
 using gelu::Pair;
 using gelu::narrow;
 using gelu::widen;
-
-// After an abort: wait (bounded) until the last kStages K blocks the producer issued have landed, so
-// no TMA load is still writing this CTA's shared memory when it exits.
-template <int S>
-__device__ __forceinline__ void drain_loads(uint64_t* full, int issued, uint32_t limit) {
-  for (int j = issued > S ? issued - S : 0; j < issued; ++j) {
-    for (uint32_t n = 0; n < limit && !mbar_try_wait(&full[j % S], (j / S) & 1); ++n) {
-    }
-  }
-}
-
-// K-major operand in the 128-byte swizzle: 8-row groups of 8 x 128 B (SBO = 1024 B); the K step of
-// 16 elements inside the swizzle row advances the start address by 32 B.
-__device__ __forceinline__ uint64_t kmajor_sw128(uint32_t addr) { return smem_desc(addr, 16, 1024, kSw128); }
 
 // The forward epilogue of one warp (warps kEpiWarp0.. of a CTA): for each of the CTA's tiles, wait for
 // its accumulator, read it out 16 columns at a time, hand the accumulator back (`release`), and write u
@@ -929,23 +919,6 @@ linear_geglu_bwd_pair_kernel(const __grid_constant__ CUtensorMap dymap, const __
   if (warp == 1) tmem_dealloc_pair(tmem, kTmemCols);
 }
 
-// 2-D view (cols, rows) of a row-major 16-bit matrix with `pitch` elements between rows, copied in
-// boxes of box_cols x box_rows with the given swizzle.  Loads read elements past cols or rows as
-// zero; stores skip them.
-bool make_map(CUtensorMap* map, const void* base, int64_t rows, int64_t cols, int64_t pitch, bool f16,
-              uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
-  attn::EncodeTiledFn enc = attn::encode_fn();
-  if (!enc) return false;
-  memset(map, 0, sizeof(*map));
-  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
-  cuuint64_t strides[1] = {(cuuint64_t)pitch * 2};
-  cuuint32_t box[2] = {box_cols, box_rows};
-  cuuint32_t estr[2] = {1, 1};
-  CUresult r = enc(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2,
-                   const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-                   CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-  return r == CUDA_SUCCESS;
-}
 // The three box shapes: K-major operand tiles [128 rows x 64] (128-byte swizzle), MN-major weight tiles
 // [64 K-rows x 64 columns] (128-byte swizzle), and the epilogue's per-warp [32 rows x 16] boxes
 // (32-byte swizzle).

@@ -375,6 +375,104 @@ std::tuple<at::Tensor, at::Tensor> geglu_q8_bwd(const at::Tensor& g_in, const at
   return {du, out};
 }
 
+// ---------------------------------------------------------------- vocabulary cross entropy
+// The operands as the kernels take them, and a workspace of the mode's size.
+struct CeCall {
+  at::Tensor x, w, targets, ws;
+  int bits, dtype;
+  int64_t N, V, K;
+};
+CeCall ce_call(const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor& targets_in, int mode) {
+  check_cuda(x_in, "x2d");
+  check_cuda(w_in, "w");
+  check_cuda(targets_in, "targets");
+  check_same_device(x_in, w_in, "linear_cross_entropy");
+  check_same_device(x_in, targets_in, "linear_cross_entropy");
+  TORCH_CHECK(x_in.dim() == 2, "linear_cross_entropy: x2d must be 2-D, got ", x_in.dim(), "-D");
+  TORCH_CHECK(w_in.dim() == 2 && w_in.size(0) > 0 && w_in.size(1) == x_in.size(1),
+              "linear_cross_entropy: w must be [V, ", x_in.size(1), "]");
+  TORCH_CHECK(x_in.scalar_type() == w_in.scalar_type(), "linear_cross_entropy: x2d and w must have one dtype");
+  TORCH_CHECK(targets_in.dim() == 1 && targets_in.size(0) == x_in.size(0), "linear_cross_entropy: targets must be [",
+              x_in.size(0), "]");
+  const int bits = token_bits_of(targets_in, "linear_cross_entropy: targets");
+  // 16-byte aligned operands: a view that starts elsewhere is copied
+  auto aligned = [](const at::Tensor& t) {
+    auto c = t.contiguous();
+    return (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) == 0 ? c : c.clone();
+  };
+  CeCall c{aligned(x_in), aligned(w_in), targets_in.contiguous(), {}, bits, krsi_dtype_of(x_in),
+           x_in.size(0), w_in.size(0), x_in.size(1)};
+  size_t ws = 0;
+  check_rc(krsi_linear_ce_workspace_size(c.N, c.V, c.K, mode, &ws), "krsi_linear_ce_workspace_size");
+  c.ws = workspace(c.x, ws);
+  return c;
+}
+
+// (loss rows, [loss, row weight], dx, dw): the gradients are fp32, of the sum of the losses and without
+// `scale`, or empty.  reduction 0 none, 1 mean, 2 sum.
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(
+    const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor& targets_in, double scale, int64_t ignore_index,
+    double z_loss, int64_t reduction, bool want_dx, bool want_dw) {
+  TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const CeCall c = ce_call(x_in, w_in, targets_in, want_dx || want_dw ? 1 : 0);
+  auto f32 = c.x.options().dtype(at::kFloat);
+  auto loss = at::empty({c.N}, f32);
+  auto reduced = at::empty({reduction != 0 ? 2 : 0}, f32);
+  auto dx = at::empty({want_dx ? c.N : 0, c.K}, f32);
+  auto dw = at::empty({want_dw ? c.V : 0, c.K}, f32);
+  check_rc(krsi_linear_ce_fwd(c.x.data_ptr(), c.w.data_ptr(), c.targets.data_ptr(), c.bits, loss.data_ptr<float>(),
+                              reduction != 0 ? reduced.data_ptr<float>() : nullptr,
+                              want_dx ? dx.data_ptr<float>() : nullptr, want_dw ? dw.data_ptr<float>() : nullptr,
+                              c.ws.data_ptr(), (size_t)c.ws.numel(), c.N, c.V, c.K, (float)scale, ignore_index,
+                              (float)z_loss, reduction == 1, c.dtype, at::cuda::getCurrentCUDAStream()),
+           "krsi_linear_ce_fwd");
+  return {loss, reduced, dx, dw};
+}
+
+// Gradients in x2d's dtype for g, the upstream gradient of each row's loss ([N], or one for all), times
+// weight (one value, or empty).
+std::tuple<at::Tensor, at::Tensor> linear_ce_grad(const at::Tensor& g_in, const at::Tensor& weight_in,
+                                                  const at::Tensor& x_in, const at::Tensor& w_in,
+                                                  const at::Tensor& targets_in, double scale, int64_t ignore_index,
+                                                  double z_loss, bool want_dx, bool want_dw) {
+  TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const CeCall c = ce_call(x_in, w_in, targets_in, 2);
+  TORCH_CHECK(g_in.numel() == c.N || g_in.numel() == 1, "linear_ce_grad: g must have ", c.N, " values or one");
+  TORCH_CHECK(weight_in.numel() <= 1, "linear_ce_grad: weight must be one value or empty");
+  auto g = g_in.to(at::kFloat).contiguous();
+  auto weight = weight_in.to(at::kFloat).contiguous();
+  auto dx = at::empty({want_dx ? c.N : 0, c.K}, c.x.options());
+  auto dw = at::empty({want_dw ? c.V : 0, c.K}, c.x.options());
+  if (!want_dx && !want_dw) return {dx, dw};
+  check_rc(krsi_linear_ce_grad(c.x.data_ptr(), c.w.data_ptr(), c.targets.data_ptr(), c.bits, g.data_ptr<float>(),
+                               g.numel() == 1 ? 0 : 1, weight.numel() == 1 ? weight.data_ptr<float>() : nullptr,
+                               want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, c.ws.data_ptr(),
+                               (size_t)c.ws.numel(), c.N, c.V, c.K, (float)scale, ignore_index, (float)z_loss, c.dtype,
+                               at::cuda::getCurrentCUDAStream()),
+           "krsi_linear_ce_grad");
+  return {dx, dw};
+}
+
+// scale * g * weight * grad in `like`'s dtype (g, weight: one value each).
+at::Tensor linear_ce_finish(const at::Tensor& grad, const at::Tensor& g_in, const at::Tensor& weight, double scale,
+                            const at::Tensor& like) {
+  check_cuda(grad, "grad");
+  check_cuda(g_in, "g");
+  check_cuda(weight, "weight");
+  TORCH_CHECK(grad.scalar_type() == at::kFloat && grad.is_contiguous(), "linear_ce_finish: grad must be contiguous fp32");
+  TORCH_CHECK(g_in.numel() == 1 && weight.numel() == 1 && weight.scalar_type() == at::kFloat,
+              "linear_ce_finish: g and weight must be one value each");
+  c10::cuda::CUDAGuard guard(grad.device());
+  auto g = g_in.to(at::kFloat);
+  auto out = at::empty(grad.sizes(), grad.options().dtype(like.scalar_type()));
+  check_rc(krsi_linear_ce_finish(grad.data_ptr<float>(), g.data_ptr<float>(), weight.data_ptr<float>(), out.data_ptr(),
+                                 grad.numel(), (float)scale, krsi_dtype_of(like), at::cuda::getCurrentCUDAStream()),
+           "krsi_linear_ce_finish");
+  return out;
+}
+
 }  // namespace
 
 TORCH_LIBRARY(krsi, m) {
@@ -392,6 +490,11 @@ TORCH_LIBRARY(krsi, m) {
   m.def("t5_bias_bwd(Tensor dpd, Tensor table, int S, int num_buckets, int max_distance, bool bidirectional) -> Tensor");
   m.def("embedding_fwd(Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
   m.def("embedding_bwd(Tensor g, Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
+  m.def("linear_ce_fwd(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, "
+        "int reduction, bool want_dx, bool want_dw) -> (Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_ce_grad(Tensor g, Tensor weight, Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, "
+        "float z_loss, bool want_dx, bool want_dw) -> (Tensor, Tensor)");
+  m.def("linear_ce_finish(Tensor grad, Tensor g, Tensor weight, float scale, Tensor like) -> Tensor");
   m.def("geglu_q8_fwd(Tensor u, bool keep) -> (Tensor, Tensor, Tensor)");
   m.def("geglu_q8_bwd(Tensor g, Tensor q, Tensor exponents, bool want_out) -> (Tensor, Tensor)");
 }
@@ -410,6 +513,9 @@ TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
   m.impl("t5_bias_bwd", &t5_bias_bwd);
   m.impl("embedding_fwd", &embedding_fwd);
   m.impl("embedding_bwd", &embedding_bwd);
+  m.impl("linear_ce_fwd", &linear_ce_fwd);
+  m.impl("linear_ce_grad", &linear_ce_grad);
+  m.impl("linear_ce_finish", &linear_ce_finish);
   m.impl("geglu_q8_fwd", &geglu_q8_fwd);
   m.impl("geglu_q8_bwd", &geglu_q8_bwd);
 }

@@ -21,6 +21,9 @@ enum WatchdogRole : unsigned {
   kWdGemmLoad = 17,   // fused projection GEMM: TMA producer waiting for a free stage
   kWdGemmMma = 18,    // fused projection GEMM: MMA issuer waiting for data / a free accumulator
   kWdGemmEpilogue = 19,
+  kWdCeLoad = 25,     // vocabulary cross entropy GEMMs: the same three roles
+  kWdCeMma = 26,
+  kWdCeEpilogue = 27,
   kWdTest = 0x7f      // the self-test kernel's deliberately unsatisfied wait
 };
 
@@ -34,9 +37,10 @@ cudaError_t watchdog_read_attn_fwd(unsigned* word, bool clear);
 cudaError_t watchdog_read_attn_bwd(unsigned* word, bool clear);
 cudaError_t watchdog_read_diag(unsigned* word, bool clear);
 cudaError_t watchdog_read_gemm(unsigned* word, bool clear);
+cudaError_t watchdog_read_ce(unsigned* word, bool clear);
 
 inline cudaError_t watchdog_read(unsigned* word, bool clear) {
-  unsigned a = 0, b = 0, c = 0, d = 0;
+  unsigned a = 0, b = 0, c = 0, d = 0, f = 0;
   cudaError_t e = watchdog_read_attn_fwd(&a, clear);
   if (e != cudaSuccess) return e;
   e = watchdog_read_attn_bwd(&b, clear);
@@ -44,7 +48,9 @@ inline cudaError_t watchdog_read(unsigned* word, bool clear) {
   e = watchdog_read_diag(&c, clear);
   if (e != cudaSuccess) return e;
   e = watchdog_read_gemm(&d, clear);
-  *word = a | b | c | d;
+  if (e != cudaSuccess) return e;
+  e = watchdog_read_ce(&f, clear);
+  *word = a | b | c | d | f;
   return e;
 }
 

@@ -130,6 +130,22 @@ def _register_compile_support() -> None:
     def _(g, tokens, table, scale, padding_idx):
         return table.new_empty(table.shape)
 
+    @reg_fake("krsi::linear_ce_fwd")
+    def _(x2d, w, targets, scale, ignore_index, z_loss, reduction, want_dx, want_dw):
+        f32 = torch.float32
+        return (x2d.new_empty((x2d.shape[0],), dtype=f32), x2d.new_empty((2 if reduction else 0,), dtype=f32),
+                x2d.new_empty((x2d.shape[0] if want_dx else 0, x2d.shape[1]), dtype=f32),
+                x2d.new_empty((w.shape[0] if want_dw else 0, w.shape[1]), dtype=f32))
+
+    @reg_fake("krsi::linear_ce_grad")
+    def _(g, weight, x2d, w, targets, scale, ignore_index, z_loss, want_dx, want_dw):
+        return (x2d.new_empty((x2d.shape[0] if want_dx else 0, x2d.shape[1])),
+                x2d.new_empty((w.shape[0] if want_dw else 0, w.shape[1])))
+
+    @reg_fake("krsi::linear_ce_finish")
+    def _(grad, g, weight, scale, like):
+        return grad.new_empty(grad.shape, dtype=like.dtype)
+
     @reg_fake("krsi::geglu_q8_fwd")
     def _(u, keep):
         rows, F = u.shape[0], u.shape[1] // 2
@@ -207,6 +223,33 @@ def _register_compile_support() -> None:
         return None, ops.embedding_bwd(g, tokens, table, *ctx.args), None, None
 
     torch.library.register_autograd("krsi::embedding_fwd", emb_backward, setup_context=emb_setup)
+
+    def ce_setup(ctx, inputs, output):
+        x2d, w, targets, scale, ignore_index, z_loss, reduction, want_dx, want_dw = inputs
+        loss, reduced, dx, dw = output
+        ctx.args = (scale, ignore_index, z_loss)
+        ctx.reduction, ctx.kept, ctx.wanted = reduction, want_dx or want_dw, (want_dx, want_dw)
+        ctx.set_materialize_grads(False)
+        if ctx.kept:
+            ctx.save_for_backward(reduced, dx, dw, w)
+        else:
+            ctx.save_for_backward(reduced, x2d, w, targets)
+
+    def ce_backward(ctx, gloss, greduced, _gdx, _gdw):
+        g = gloss if ctx.reduction == 0 else greduced[0] if greduced is not None else None
+        none = (None,) * 7
+        if g is None:
+            return (None, None) + none
+        reduced, *saved = ctx.saved_tensors
+        if ctx.kept:
+            dx, dw, like = saved
+            return (ops.linear_ce_finish(dx, g, reduced[1:], ctx.args[0], like) if ctx.wanted[0] else None,
+                    ops.linear_ce_finish(dw, g, reduced[1:], ctx.args[0], like) if ctx.wanted[1] else None) + none
+        need = ctx.needs_input_grad[:2]
+        dx, dw = ops.linear_ce_grad(g, reduced[1:], *saved, *ctx.args, *need)
+        return (dx if need[0] else None, dw if need[1] else None) + none
+
+    torch.library.register_autograd("krsi::linear_ce_fwd", ce_backward, setup_context=ce_setup)
 
     def q8_setup(ctx, inputs, output):
         ctx.save_for_backward(output[1], output[2])
