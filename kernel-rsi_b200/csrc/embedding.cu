@@ -19,45 +19,44 @@ template <int DT>
 __device__ __forceinline__ typename Elem<DT>::T nan_of() { return Elem<DT>::store(__int_as_float(0x7fffffff)); }
 
 // ---------------------------------------------------------------- forward
-// One packet per work item, kFwdItems items per thread with their loads in flight together.
-constexpr int kFwdItems = 4;
+// A thread keeps one packet of columns and takes kFwdRows rows of a block's share, their loads in flight
+// together behind the loads of their tokens.
+constexpr int kFwdRows = 8;
 
 template <int DT, int VEC, typename I>
 __global__ void __launch_bounds__(256)
 embedding_fwd_kernel(const I* __restrict__ toks, const typename Elem<DT>::T* __restrict__ table,
-                     typename Elem<DT>::T* __restrict__ out, int64_t items, uint32_t packets, int64_t V, float scale) {
+                     typename Elem<DT>::T* __restrict__ out, int n, int rows, uint32_t packets, int64_t V, float scale) {
   pdl_enter();
   using E = Elem<DT>;
   using P = Pack<typename E::T, VEC>;
-  const P* tp = reinterpret_cast<const P*>(table);
-  P* op = reinterpret_cast<P*>(out);
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i0 < items; i0 += kFwdItems * stride) {
-    P r[kFwdItems];
+  const uint32_t c = blockIdx.y * blockDim.x + threadIdx.x;
+  const int row0 = (int)blockIdx.x * rows, m = min(rows, n - row0);
+  if (c >= packets) return;
+  const P* tp = reinterpret_cast<const P*>(table) + c;
+  P* op = reinterpret_cast<P*>(out) + (int64_t)row0 * packets + c;
+  I t[kFwdRows];
+  P r[kFwdRows];
 #pragma unroll
-    for (int k = 0; k < kFwdItems; ++k) {
-      const int64_t i = i0 + k * stride;
-      if (i >= items) break;
-      const int64_t row = i / packets;
-      const uint32_t c = (uint32_t)(i - row * packets);
-      const int64_t t = toks[row];
-      if (t >= 0 && t < V) {
-        r[k] = tp[t * packets + c];
-      } else {
+  for (int k = 0; k < kFwdRows; ++k) t[k] = k < m ? toks[row0 + k] : (I)0;
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) r[k].v[e] = nan_of<DT>();
-      }
+  for (int k = 0; k < kFwdRows; ++k) {
+    if (k >= m) break;
+    if (t[k] >= 0 && t[k] < (I)V) {
+      r[k] = tp[(int64_t)t[k] * packets];
+    } else {
+#pragma unroll
+      for (int e = 0; e < VEC; ++e) r[k].v[e] = nan_of<DT>();
     }
+  }
 #pragma unroll
-    for (int k = 0; k < kFwdItems; ++k) {
-      const int64_t i = i0 + k * stride;
-      if (i >= items) break;
-      if (scale != 1.0f) {   // else the row's own bits
+  for (int k = 0; k < kFwdRows; ++k) {
+    if (k >= m) break;
+    if (scale != 1.0f) {   // else the row's own bits
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) r[k].v[e] = E::store(scale * E::load(r[k].v[e]));
-      }
-      op[i] = r[k];
+      for (int e = 0; e < VEC; ++e) r[k].v[e] = E::store(scale * E::load(r[k].v[e]));
     }
+    op[(int64_t)k * packets] = r[k];
   }
 }
 
@@ -99,15 +98,17 @@ template <int DT, int VEC>
 int fwd(const void* toks, int token_bits, const void* table, void* out, int64_t n, int64_t V, int64_t d, float scale,
         cudaStream_t stream) {
   using T = typename Elem<DT>::T;
-  const int64_t items = n * (d / VEC);
-  const int64_t per_block = 256 * kFwdItems;
-  const dim3 grid((unsigned)std::min<int64_t>((items + per_block - 1) / per_block, 1 << 20));
+  const uint32_t packets = (uint32_t)(d / VEC);
+  const int threads = (int)std::min<uint32_t>(256, std::max<uint32_t>(32, (packets + 31) / 32 * 32));
+  // as many rows a block as still leave a block for every SM
+  const int rows = (int)std::max<int64_t>(1, std::min<int64_t>(kFwdRows, n / kNumSMsB200));
+  const dim3 grid((unsigned)((n + rows - 1) / rows), (packets + threads - 1) / threads);
   if (token_bits == 64)
-    KRSI_CUDA_TRY(launch_pdl(embedding_fwd_kernel<DT, VEC, long long>, grid, dim3(256), 0, stream,
-                             (const long long*)toks, (const T*)table, (T*)out, items, (uint32_t)(d / VEC), V, scale));
+    KRSI_CUDA_TRY(launch_pdl(embedding_fwd_kernel<DT, VEC, long long>, grid, dim3(threads), 0, stream,
+                             (const long long*)toks, (const T*)table, (T*)out, (int)n, rows, packets, V, scale));
   else
-    KRSI_CUDA_TRY(launch_pdl(embedding_fwd_kernel<DT, VEC, int>, grid, dim3(256), 0, stream, (const int*)toks,
-                             (const T*)table, (T*)out, items, (uint32_t)(d / VEC), V, scale));
+    KRSI_CUDA_TRY(launch_pdl(embedding_fwd_kernel<DT, VEC, int>, grid, dim3(threads), 0, stream, (const int*)toks,
+                             (const T*)table, (T*)out, (int)n, rows, packets, V, scale));
   return KRSI_OK;
 }
 

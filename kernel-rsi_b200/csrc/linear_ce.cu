@@ -51,7 +51,6 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMaxLift = 64.f;                    // log2: e <= 2^64 in bf16, sums far below fp32's range
 constexpr float kHalfScale = 1024.f;                // f16: e = 2^10 p
 constexpr int kIgnored = -2, kInvalid = -1;         // targets: ignored, outside [0, V)
-constexpr int64_t kDirectRows = 1024;               // rows up to which dw leaves the GEMM in 16 bits
 
 // ---------------------------------------------------------------- CTA-pair GEMM pipeline
 constexpr int kBM = 128;                            // rows of A per CTA (256 per pair)
@@ -63,13 +62,13 @@ constexpr int kEpiWarp0 = 4;
 constexpr int kEpiWarps = 8;
 constexpr uint32_t kATile = kBM * kBK * 2;          // 16 KB
 constexpr uint32_t kMnBox = 64 * kBK * 2;           // one [64 K-rows x 64 columns] MN-major box: 8 KB
-constexpr uint32_t kRingBytes = 6 * 32768;          // the operand ring: 192 KB, as many stages as fit
-constexpr uint32_t kBoxBytes = 4096;                // one epilogue warp's staged box
-constexpr uint32_t kBarOff = kRingBytes + kEpiWarps * kBoxBytes;
+// Shared memory: the epilogue warps' staged boxes, the barriers, then the operand ring.
+constexpr uint32_t kLogitsBox = 4096;               // [32 rows x 64 columns] of 16 bits
+constexpr uint32_t kGradsBox = 2048;                // [32 rows x 16 columns] of fp32
 constexpr int kNumBars = 2 * kMaxStages + 2 + 2 + 1;   // full, empty, acc_full, acc_empty, drain
-constexpr uint32_t kMiscOff = kBarOff + kNumBars * 8;
-constexpr uint32_t kSmem = kMiscOff + 16 + 1024;    // + slack for the 1024-byte alignment
-static_assert(kSmem <= 232448, "shared memory budget");
+constexpr uint32_t kSmem = 232448;
+constexpr uint32_t kUsable = kSmem - 1024 - 1024;   // less the 1024-byte alignment and the barriers' KB
+static_assert(kNumBars * 8 + 16 <= 1024, "barriers");
 constexpr uint32_t kTmemCols = 512;
 
 // MN-major operand in the 128-byte swizzle: 64-column atoms of 8 K-rows x 128 B (SBO = 1024 B), the next
@@ -82,8 +81,13 @@ __device__ __forceinline__ uint64_t mnmajor_sw128(uint32_t addr) { return smem_d
 // of B (8 KB per 64 columns), the second MMA's 16 KB after the first's.
 struct Pipe {
   int cols;
+  uint32_t box_bytes;   // one epilogue warp's staged box
+  __device__ __forceinline__ uint32_t bars_at() const { return kEpiWarps * box_bytes; }
+  __device__ __forceinline__ uint32_t ring_at() const { return bars_at() + 1024; }
   __device__ __forceinline__ uint32_t stage_bytes() const { return kATile + (cols / 128) * kMnBox; }
-  __device__ __forceinline__ int stages() const { return min((int)(kRingBytes / stage_bytes()), kMaxStages); }
+  __device__ __forceinline__ int stages() const {
+    return min((int)((kUsable - kEpiWarps * box_bytes) / stage_bytes()), kMaxStages);
+  }
   __device__ __forceinline__ int accs() const { return cols <= kBN ? 2 : 1; }
 };
 
@@ -106,13 +110,14 @@ struct MmaShape {
 template <typename ItemOf, typename Load, typename Shape, typename Prepare, typename Epilogue>
 __device__ __forceinline__ void pair_gemm(uint8_t* smem, const Pipe pipe, int n_items, uint32_t limit, ItemOf item_of,
                                           Load load, Shape shape, Prepare prepare, Epilogue epilogue) {
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kBarOff);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + pipe.bars_at());
   uint64_t* empty = full + kMaxStages;
   uint64_t* acc_full = empty + kMaxStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drain = acc_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kMiscOff);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kMiscOff + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint8_t* ring = smem + pipe.ring_at();
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const bool even = cluster_ctarank() == 0;
   const uint32_t stage_bytes = pipe.stage_bytes();
@@ -155,7 +160,7 @@ __device__ __forceinline__ void pair_gemm(uint8_t* smem, const Pipe pipe, int n_
         }
         if (lane == 0) {
           if (even) mbar_arrive_expect_tx(&full[s], 2 * stage_bytes);
-          load(item, kb, smem + s * stage_bytes, mapa_shared(&full[s], 0));
+          load(item, kb, ring + s * stage_bytes, mapa_shared(&full[s], 0));
         }
         __syncwarp();
         if (++s == stages) s = 0, ++round;
@@ -318,12 +323,14 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
     for (int r = 0; r < a.n_rt; ++r) n_rt += a.marked[r] != 0;
   }
   const int n_tiles = n_rt * a.n_vt;
+  if (n_tiles == 0) return;   // nothing is marked (the same for every CTA)
   struct Tile {
     int rt, vt, n_kb;
   };
 
+  const Pipe pipe{kBN, kLogitsBox};
   pair_gemm(
-      smem, Pipe{kBN}, pair < n_tiles ? (n_tiles - 1 - pair) / n_pairs + 1 : 0, a.limit,
+      smem, pipe, pair < n_tiles ? (n_tiles - 1 - pair) / n_pairs + 1 : 0, a.limit,
       [&](int i) {
         const int t = pair + i * n_pairs;
         int rt = t % n_rt;
@@ -340,7 +347,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
         tma_load_2d_pair(st + kATile, &wmap, bar, kb * kBK, m.vt * kBN + rank * kBM);
       },
       [&](const Tile&) {
-        const uint32_t s0 = smem_u32(smem);
+        const uint32_t s0 = smem_u32(smem + pipe.ring_at());
         return MmaShape{kmajor_sw128(s0), kmajor_sw128(s0 + kATile), 32 >> 4, 32 >> 4,
                         idesc_f16(2 * kBM, kBN, F16 ? 0u : 1u, false, false), 0u};
       },
@@ -355,7 +362,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
         float ref = in ? a.ref[row] : 0.f;
         const bool live = t != kIgnored;
         const uint32_t keep = live ? 0xffffffffu : 0u;   // an ignored row's e is 0 whatever its logits are
-        uint8_t* box = smem + kRingBytes + ew * kBoxBytes;
+        uint8_t* box = smem + ew * kLogitsBox;
         const uint32_t acc = taddr + half * 128;
         // One pass over the 128 columns, 32 at a time: y = l - ref in log2 units, -inf at the target and
         // past the vocabulary; sum += 2^y, top = max y, and (store) e in 16 bits through the staged box.
@@ -413,9 +420,9 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
               if ((j & 1) == 1) {
                 fence_async_shared();
                 __syncwarp();
-                const int bc = c0 - 32;
-                if (lane == 0 && bc < a.V && row0 < a.rows) {   // the map clips rows and columns
-                  tma_store_2d(&emap, box, bc, row0);
+                const int panel = (c0 - 32) / 64;   // stored whole: zeros past the vocabulary
+                if (lane == 0 && panel * 64 < a.V && row0 < a.rows) {   // the map clips rows
+                  tma_store_3d(&emap, box, 0, row0, panel);
                   bulk_commit_group();
                 }
               }
@@ -472,9 +479,17 @@ ce_join_kernel(const JoinArgs a) {
   const int t = a.tgt[row];
   const float l2t = a.l2t[row];
   const float2* pr = a.part + (int64_t)row * a.n_part;
+  const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.K;
+  constexpr int kAhead = 5;   // packets of the row on their way while the sums are added
+  Vec16<T> xv[kAhead];
+  if (a.coef != nullptr) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (lane * 8 + j * 256 < a.K) xv[j] = ldg16(xr + lane * 8 + j * 256);
+  }
   float s = 0.f, top = l2t;
   bool lifted = !(l2t == l2t);
-#pragma unroll 4
+#pragma unroll 8
   for (int k = lane; k < a.n_part; k += 32) {
     const float2 p = pr[k];
     lifted |= p.x != l2t;
@@ -520,15 +535,16 @@ ce_join_kernel(const JoinArgs a) {
     if (lifted && !dead) a.marked[row / (2 * kBM)] = 1;   // every writer writes the same
   }
   const float f = soft / unit;
-  const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.K;
   T* xo = reinterpret_cast<T*>(a.xs) + (int64_t)row * a.K;
-#pragma unroll 4
-  for (int k = lane * 8; k < a.K; k += 256) {
-    auto v = ldg16(xr + k);
+  auto put = [&](int k, Vec16<T> v) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v.v[e] = E::store(dead ? 0.f : f * E::load(v.v[e]));
     stg16(xo + k, v);
-  }
+  };
+#pragma unroll
+  for (int j = 0; j < kAhead; ++j)
+    if (lane * 8 + j * 256 < a.K) put(lane * 8 + j * 256, xv[j]);
+  for (int k = lane * 8 + kAhead * 256; k < a.K; k += 256) put(k, ldg16(xr + k));
 }
 
 // The reduced loss and the weight of each row in it, one block, in a fixed order.
@@ -539,6 +555,7 @@ ce_reduce_kernel(const float* __restrict__ loss, const int* __restrict__ tgt, fl
   __shared__ int counts[32];
   double s = 0.0;
   int c = 0;
+#pragma unroll 8
   for (int i = threadIdx.x; i < n; i += 1024) {
     s += (double)loss[i];
     c += tgt[i] != kIgnored;
@@ -573,6 +590,7 @@ ce_gtop_kernel(const float* __restrict__ g, int64_t g_stride, const float* __res
   pdl_enter();
   __shared__ float tops[32];
   float m = 0.f;
+#pragma unroll 8
   for (int i = threadIdx.x; i < n; i += 1024)
     if (tgt[i] != kIgnored) m = fmaxf(m, fabsf(g[i * g_stride]));
 #pragma unroll
@@ -602,10 +620,11 @@ struct GradArgs {
   const float* coef;
   const void* w;
   // dw: fp32 sums, stored or added; or, scaled and rounded, with the rows of `base` added for the tokens
-  // that occur (start[v] < start[v + 1])
+  // that occur (token_rows.cuh's start)
   int dw32, accumulate;
   const float* base;
   const int* start;
+  tokens::Order order;
   const float* g_top;
   float alpha;             // of the dw sums
   float scale;
@@ -617,11 +636,31 @@ struct GradArgs {
 struct GradItem {
   int is_dx, tile, ct, split, n_kb;
 };
-// One epilogue thread's row of an item: out = mul * sum + add, add from w_t or from base.
+// One epilogue thread's row of an item: out = mul * sum + add, add being coef * w_t (16 bits) or the row
+// of base (fp32); `add` holds the 16 columns that come next.
+template <typename T>
+union GradAdd {
+  Vec16<T> w[2];
+  Vec16<float> base[4];
+  __device__ __forceinline__ GradAdd() {}
+  __device__ __forceinline__ void fetch(int is_dx, const GradArgs& a, int64_t at, int col) {
+    if (is_dx) {
+#pragma unroll
+      for (int p = 0; p < 2; ++p)
+        if (col + 8 * p < a.K) w[p] = ldg16(reinterpret_cast<const T*>(a.w) + at + col + 8 * p);
+    } else {
+#pragma unroll
+      for (int p = 0; p < 4; ++p)
+        if (col + 4 * p < a.K) base[p] = ldg16(a.base + at + col + 4 * p);
+    }
+  }
+};
+template <typename T>
 struct GradRow {
   float mul, coef;
   bool zero;
   int64_t add_at;   // w's or base's first element of the row, or -1
+  GradAdd<T> add;
 };
 __device__ __forceinline__ int pair_dx(const GradArgs& a, int pair, int P) {
   return a.n_dx / P + (pair < a.n_dx % P ? 1 : 0);
@@ -663,26 +702,22 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
   const int pair = (int)blockIdx.x / 2, P = (int)gridDim.x / 2;
   const int cols1 = min(a.cols, kBN), cols2 = a.cols - cols1;   // of the two MMAs
 
+  const Pipe pipe{a.cols, kGradsBox};
   pair_gemm(
-      smem, Pipe{a.cols}, pair_items(a, pair, P), a.limit,
+      smem, pipe, pair_items(a, pair, P), a.limit,
       [&](int i) { return pair_item(a, pair, P, i); },
       [&](const GradItem& m, int kb, uint8_t* st, uint32_t bar) {
         const int k = ((m.is_dx ? m.split * a.kb_share : 0) + kb) * kBK;
         const CUtensorMap* b = m.is_dx ? &wmap : &xsmap;
-        if (m.is_dx) {
-          tma_load_2d_pair(st, &ekmap, bar, k, m.tile * (2 * kBM) + rank * kBM);
-        } else {
-          const int v = m.tile * (2 * kBM) + rank * kBM;
-          tma_load_2d_pair(st, &emmap, bar, v, k);
-          tma_load_2d_pair(st + kMnBox, &emmap, bar, v + 64, k);
-        }
+        if (m.is_dx) tma_load_3d_pair(st, &ekmap, bar, 0, m.tile * (2 * kBM) + rank * kBM, k / 64);
+        else tma_load_3d_pair(st, &emmap, bar, 0, k, (m.tile * 2 + rank) * 2);   // two panels
         const int c1 = m.ct * a.cols + rank * (cols1 / 2), c2 = m.ct * a.cols + cols1 + rank * (cols2 / 2);
         uint8_t* bs = st + kATile;
         for (int c = 0; c < cols1 / 2; c += 64, bs += kMnBox) tma_load_2d_pair(bs, b, bar, c1 + c, k);
         for (int c = 0; c < cols2 / 2; c += 64, bs += kMnBox) tma_load_2d_pair(bs, b, bar, c2 + c, k);
       },
       [&](const GradItem& m) {
-        const uint32_t s0 = smem_u32(smem);
+        const uint32_t s0 = smem_u32(smem + pipe.ring_at());
         return MmaShape{m.is_dx ? kmajor_sw128(s0) : mnmajor_sw128(s0), mnmajor_sw128(s0 + kATile),
                         m.is_dx ? 32u >> 4 : (16u * 128u) >> 4, (16u * 128u) >> 4,
                         idesc_f16(2 * kBM, cols1, F16 ? 0u : 1u, !m.is_dx, true),
@@ -690,11 +725,18 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
       },
       [&](const GradItem& m) {
         const int row = m.tile * (2 * kBM) + rank * kBM + (warp % 4) * 32 + lane;   // of dx, or the token of dw
-        GradRow r{1.f, 0.f, false, -1};
+        GradRow<T> r;
+        r.mul = 1.f;
+        r.coef = 0.f;
+        r.zero = false;
+        r.add_at = -1;
         if (row >= (m.is_dx ? a.rows : a.V)) return r;
         if (!m.is_dx) {
           r.mul = a.alpha * g_unit(a.g_top);
-          if (a.base && a.start[row] < a.start[row + 1]) r.add_at = (int64_t)row * a.K;
+          if (a.base) {
+            const int k = a.order.key(row);
+            if (a.start[k] < a.start[k + 1]) r.add_at = (int64_t)row * a.K;
+          }
         } else if (!a.dx_part) {
           const int t = a.tgt[row];
           r.mul = a.factor[row];
@@ -702,9 +744,11 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
           r.zero = t == kIgnored;
           if (t >= 0) r.add_at = (int64_t)t * a.K;
         }
+        if (r.add_at >= 0)
+          r.add.fetch(m.is_dx, a, r.add_at, m.ct * a.cols + (warp - kEpiWarp0) / 4 * (a.cols / 2));
         return r;
       },
-      [&](const GradItem& m, const GradRow& r, uint32_t taddr, auto release) {
+      [&](const GradItem& m, const GradRow<T>& r, uint32_t taddr, auto release) {
         const int ew = warp - kEpiWarp0, half = ew / 4, half_n = a.cols / 2;
         const int row0 = m.tile * (2 * kBM) + rank * kBM + (warp % 4) * 32;
         const int col0 = m.ct * a.cols + half * half_n;
@@ -713,64 +757,57 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
         const bool any = row0 < (m.is_dx ? a.rows : a.V);
         const CUtensorMap* map = m.is_dx ? &dxmap : &dwmap;
         const int out_row = m.is_dx ? m.split * (a.n_rt * 2 * kBM) + row0 : row0;
-        uint8_t* box = smem + kRingBytes + ew * kBoxBytes;
-        // 32 columns at a time through the staged box: [32 rows x 32 columns] of fp32 in the 128-byte
-        // swizzle, or of 16 bits in the 64-byte swizzle; the maps clip rows and columns.  The target's
-        // row of w for the next columns is on its way while these are worked on.
-        const T* wt = m.is_dx && r.add_at >= 0 ? reinterpret_cast<const T*>(a.w) + r.add_at + col0 : nullptr;
-        const float* base = !m.is_dx && r.add_at >= 0 ? a.base + r.add_at + col0 : nullptr;
-        Vec16<T> next[4];
-        auto fetch = [&](int j) {
-          if (wt)
-#pragma unroll
-            for (int p = 0; p < 4; ++p)
-              if (col0 + j + 8 * p < a.K) next[p] = ldg16(wt + j + 8 * p);
-        };
-        fetch(0);
+        // 16 columns at a time through the staged box: [32 rows x 16 columns] of fp32 in the 64-byte
+        // swizzle, or of 16 bits in the 32-byte swizzle, two such boxes in turn; the maps clip rows and
+        // columns.  What is to be added to the next columns is on its way while these are worked on.
+        GradAdd<T> add = r.add;
 #pragma unroll 1
-        for (int j = 0; j < half_n; j += 32) {
-          uint32_t q[32];
+        for (int j = 0; j < half_n; j += 16) {
+          uint32_t q[16];
           __syncwarp();
-          tmem_ld32(acc + j, q);
+          tmem_ld16(acc + j, q);
           tmem_wait_ld();
-          if (j + 32 >= half_n) release();
-          float v[32];
+          if (j + 16 >= half_n) release();
+          float v[16];
 #pragma unroll
-          for (int e = 0; e < 32; ++e) v[e] = r.zero ? 0.f : r.mul * __uint_as_float(q[e]);
-          if (wt) {
+          for (int e = 0; e < 16; ++e) v[e] = r.zero ? 0.f : r.mul * __uint_as_float(q[e]);
+          if (r.add_at >= 0) {
+            if (m.is_dx) {
+#pragma unroll
+              for (int p = 0; p < 2; ++p)
+                if (col0 + j + 8 * p < a.K)
+#pragma unroll
+                  for (int e = 0; e < 8; ++e) v[8 * p + e] = fmaf(r.coef, E::load(add.w[p].v[e]), v[8 * p + e]);
+            } else {
+#pragma unroll
+              for (int p = 0; p < 4; ++p)
+                if (col0 + j + 4 * p < a.K)
+#pragma unroll
+                  for (int e = 0; e < 4; ++e) v[4 * p + e] += add.base[p].v[e];
+            }
+            if (j + 16 < half_n) add.fetch(m.is_dx, a, r.add_at, col0 + j + 16);
+          }
+          uint8_t* box = smem + ew * kGradsBox + (!wide && (j & 16) ? kGradsBox / 2 : 0);
+          if (lane == 0) {   // the box's previous content has been read
+            if (wide || j < 32) bulk_wait_read_all();
+            else bulk_wait_read_but_one();
+          }
+          __syncwarp();
+          if (wide) {   // 64-byte rows: the packet index xor bits 1-2 of the row
 #pragma unroll
             for (int p = 0; p < 4; ++p)
-              if (col0 + j + 8 * p < a.K)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) v[8 * p + e] = fmaf(r.coef, E::load(next[p].v[e]), v[8 * p + e]);
-            if (j + 32 < half_n) fetch(j + 32);
-          }
-          if (base) {
-#pragma unroll
-            for (int p = 0; p < 8; ++p)
-              if (col0 + j + 4 * p < a.K) {
-                const float4 b = *reinterpret_cast<const float4*>(base + j + 4 * p);
-                v[4 * p] += b.x; v[4 * p + 1] += b.y; v[4 * p + 2] += b.z; v[4 * p + 3] += b.w;
-              }
-          }
-          if (lane == 0) bulk_wait_read_all();    // the box's previous content has been read
-          __syncwarp();
-          if (wide) {
-#pragma unroll
-            for (int p = 0; p < 8; ++p)
-              *reinterpret_cast<float4*>(box + lane * 128 + ((p ^ (lane & 7)) << 4)) =
+              *reinterpret_cast<float4*>(box + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) =
                   make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
-          } else {
+          } else {      // 32-byte rows: xor bit 2 of the row
 #pragma unroll
-            for (int p = 0; p < 4; ++p) {
+            for (int p = 0; p < 2; ++p) {
               uint32_t o[4];
 #pragma unroll
               for (int h = 0; h < 4; ++h) {
                 const float lo = a.scale * v[8 * p + 2 * h], hi = a.scale * v[8 * p + 2 * h + 1];
                 o[h] = F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
               }
-              // 64-byte rows: the packet index xor bits 1-2 of the row
-              *reinterpret_cast<uint4*>(box + lane * 64 + ((p ^ ((lane >> 1) & 3)) << 4)) =
+              *reinterpret_cast<uint4*>(box + lane * 32 + ((p ^ ((lane >> 2) & 1)) << 4)) =
                   make_uint4(o[0], o[1], o[2], o[3]);
             }
           }
@@ -779,15 +816,16 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
           if (lane == 0 && any && col0 + j < a.K) {
             if (!m.is_dx && a.accumulate) tma_reduce_add_2d(map, box, col0 + j, out_row);
             else tma_store_2d(map, box, col0 + j, out_row);
-            bulk_commit_group();
           }
+          if (lane == 0) bulk_commit_group();   // one group a step, empty where nothing is stored
         }
       });
 }
 
-// dx from the shares of the vocabulary (`share` values apart, added in order): 8 columns per thread.
+// dx from the shares of the vocabulary (`share` values apart, added in order): 4 columns per thread, 8
+// shares' loads in flight.
 template <int DT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(128)
 ce_dx_join_kernel(const float* __restrict__ part, int splits, int64_t share, const int* __restrict__ tgt,
                   const float* __restrict__ factor, const float* __restrict__ coef,
                   const typename Elem<DT>::T* __restrict__ w, void* __restrict__ dx, int rows, int K, float scale,
@@ -795,38 +833,33 @@ ce_dx_join_kernel(const float* __restrict__ part, int splits, int64_t share, con
   pdl_enter();
   using E = Elem<DT>;
   using T = typename E::T;
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  const int packets = K / 8;
-  const int64_t row = i / packets;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x, packets = K / 4;
+  const uint32_t row = i / packets;
   if (row >= rows) return;
-  const int col = (int)(i - row * packets) * 8;
-  const int64_t at = row * K + col;
-  float v[8] = {};
-#pragma unroll 4
-  for (int s = 0; s < splits; ++s) {
-    const float4* p = reinterpret_cast<const float4*>(part + s * share + at);
-    const float4 b0 = p[0], b1 = p[1];
-    v[0] += b0.x; v[1] += b0.y; v[2] += b0.z; v[3] += b0.w;
-    v[4] += b1.x; v[5] += b1.y; v[6] += b1.z; v[7] += b1.w;
-  }
+  const int col = (int)(i - row * packets) * 4;
+  const int64_t at = (int64_t)row * K + col;
   const int t = tgt[row];
   const float f = factor[row], c = coef[row];
+  tokens::Pack<T, 4> q;
+  if (t >= 0) q = *reinterpret_cast<const tokens::Pack<T, 4>*>(w + (int64_t)t * K + col);
+  float v[4] = {};
+#pragma unroll 8
+  for (int s = 0; s < splits; ++s) {
+    const float4 b = __ldg(reinterpret_cast<const float4*>(part + s * share + at));
+    v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+  }
 #pragma unroll
-  for (int e = 0; e < 8; ++e) v[e] = t == kIgnored ? 0.f : f * v[e];
-  if (t >= 0) {
-    const auto q = ldg16(w + (int64_t)t * K + col);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fmaf(c, E::load(q.v[e]), v[e]);
+  for (int e = 0; e < 4; ++e) {
+    v[e] = t == kIgnored ? 0.f : f * v[e];
+    if (t >= 0) v[e] = fmaf(c, E::load(q.v[e]), v[e]);
   }
   if (dx32) {
-    float4* o = reinterpret_cast<float4*>(reinterpret_cast<float*>(dx) + at);
-    o[0] = make_float4(v[0], v[1], v[2], v[3]);
-    o[1] = make_float4(v[4], v[5], v[6], v[7]);
+    *reinterpret_cast<float4*>(reinterpret_cast<float*>(dx) + at) = make_float4(v[0], v[1], v[2], v[3]);
   } else {
-    Vec16<T> o;
+    tokens::Pack<T, 4> o;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) o.v[e] = E::store(scale * v[e]);
-    stg16(reinterpret_cast<T*>(dx) + at, o);
+    for (int e = 0; e < 4; ++e) o.v[e] = E::store(scale * v[e]);
+    *reinterpret_cast<tokens::Pack<T, 4>*>(reinterpret_cast<T*>(dx) + at) = o;
   }
 }
 
@@ -850,21 +883,24 @@ ce_finish_kernel(const float* __restrict__ a, typename Elem<DT>::T* __restrict__
   }
 }
 
-// The weighted sums of x by target token, as rows of dw32 (written, or added where it accumulates).
+// The weighted sums of x by target token, as rows of dw32: written, or added to what is there.
 struct DwRows {
   float* dw32;
   int64_t K;
   int add;
+  // One addition per element and call, so a reduction in L2 (no read to wait for) gives the same bits
+  // every time.
   __device__ __forceinline__ void packet(int v, uint32_t c, const float* s) const {
-    float4* p = reinterpret_cast<float4*>(dw32 + v * K + c * 8);
-    float4 a = make_float4(s[0], s[1], s[2], s[3]), b = make_float4(s[4], s[5], s[6], s[7]);
-    if (add) {
-      const float4 o = p[0], q = p[1];
-      a.x += o.x; a.y += o.y; a.z += o.z; a.w += o.w;
-      b.x += q.x; b.y += q.y; b.z += q.z; b.w += q.w;
+    float* p = dw32 + v * K + c * 8;
+#pragma unroll
+    for (int h = 0; h < 8; h += 4) {
+      if (add)
+        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + h), "f"(s[h]), "f"(s[h + 1]),
+                     "f"(s[h + 2]), "f"(s[h + 3])
+                     : "memory");
+      else
+        *reinterpret_cast<float4*>(p + h) = make_float4(s[h], s[h + 1], s[h + 2], s[h + 3]);
     }
-    p[0] = a;
-    p[1] = b;
   }
   __device__ __forceinline__ void zero(int, uint32_t) const {}
   __device__ __forceinline__ void column(int v, int col, float s) const {
@@ -874,18 +910,18 @@ struct DwRows {
 };
 
 // ---------------------------------------------------------------- host
-// 2-D view of fp32 rows, copied in boxes of 32 x 32 with the 128-byte swizzle; stores skip what is
-// outside.
+// 2-D view of fp32 rows, copied in boxes of 32 rows x 16 columns with the 64-byte swizzle; stores skip
+// what is outside.
 inline bool make_map_f32(CUtensorMap* map, const void* base, int64_t rows, int64_t cols) {
   attn::EncodeTiledFn enc = attn::encode_fn();
   if (!enc) return false;
   memset(map, 0, sizeof(*map));
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)cols * 4};
-  cuuint32_t box[2] = {32, 32};
+  cuuint32_t box[2] = {16, 32};
   cuuint32_t estr[2] = {1, 1};
   return enc(map, CU_TENSOR_MAP_DATA_TYPE_FLOAT32, 2, const_cast<void*>(base), dims, strides, box, estr,
-             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
@@ -948,12 +984,28 @@ cudaError_t launch_pairs(void (*kern)(KArgs...), int pairs, cudaStream_t stream,
 
 inline int64_t ceil_div(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// e, in panels of 64 vocabulary entries, each [rows][64]: what one TMA box takes (64 columns of some
+// rows) is contiguous, where rows of V elements would scatter it over as many DRAM pages as it has rows.
+inline bool make_panel_map(CUtensorMap* map, const void* base, int64_t rows, int64_t panels, bool f16,
+                           uint32_t box_rows, uint32_t box_panels) {
+  attn::EncodeTiledFn enc = attn::encode_fn();
+  if (!enc) return false;
+  memset(map, 0, sizeof(*map));
+  cuuint64_t dims[3] = {64, (cuuint64_t)rows, (cuuint64_t)panels};
+  cuuint64_t strides[2] = {128, (cuuint64_t)rows * 128};
+  cuuint32_t box[3] = {64, box_rows, box_panels};
+  cuuint32_t estr[3] = {1, 1, 1};
+  return enc(map, f16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base),
+             dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Sizes of one call.
 struct Plan {
   int64_t N, V, K;
   bool grads, direct;      // gradients wanted; dw leaves the GEMM in 16 bits
   bool dw_space;           // the workspace holds fp32 rows of dw
-  int64_t n_vt, pitch;     // vocabulary tiles; elements between rows of e
+  int64_t n_vt, panels;    // vocabulary tiles; panels of e
   int64_t chunk, chunks;   // rows per chunk (a multiple of 256)
   int cols, n_ct;
   int64_t splits;          // of dx over the vocabulary
@@ -962,20 +1014,20 @@ struct Plan {
 inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool out32, int pairs) {
   Plan p{N, V, K, grads};
   p.n_vt = ceil_div(V, kBN);
-  p.pitch = ceil_div(V, 64) * 64;
+  p.panels = ceil_div(V, 64);
   // At most 2^28 logits a chunk (512 MB of e), in chunks of equal size; the loss alone keeps none.
-  const int64_t most = std::max<int64_t>(256, ((int64_t)1 << 28) / p.pitch / 256 * 256);
+  const int64_t most = std::max<int64_t>(256, ((int64_t)1 << 28) / (p.panels * 64) / 256 * 256);
   p.chunks = grads ? std::max<int64_t>(1, ceil_div(N, most)) : 1;
   p.chunk = std::max<int64_t>(256, ceil_div(ceil_div(N, p.chunks), 256) * 256);
   p.chunks = std::max<int64_t>(1, ceil_div(N, p.chunk));
-  p.direct = !out32 && N <= kDirectRows && p.chunks == 1;
+  p.direct = !out32 && p.chunks == 1;
   p.dw_space = !out32;
   // Column tiles of K.  Per K block of 64 a pair's tensor cores take 2 cycles a column, and its operands
   // (16 KB of A and 64 B a column of B for each CTA) come from L2 at about 50 bytes a cycle and SM, as
   // measured on the logits' tiles, so wider tiles feed the tensor cores better.  Up to 256 columns two
-  // accumulators alternate and the epilogue is hidden: with few rows (short sums) that counts more.
+  // accumulators alternate and the epilogue is hidden: with short sums (few rows) that counts more.
   int64_t best = INT64_MAX;
-  for (int m = 1; m <= (p.direct ? 2 : 4); ++m) {
+  for (int m = 1; m <= (p.chunk <= 1024 ? 2 : 4); ++m) {
     const int64_t n = ceil_div(K, 128 * m);
     const int64_t cost = n * std::max<int64_t>(256 * m, (16384 + 8192 * m) / 50);
     if (cost <= best) {
@@ -1023,7 +1075,7 @@ inline Space space_at(void* base, const Plan& p) {
     s.factor = reinterpret_cast<float*>(take((size_t)p.N * 4));
     s.ref = reinterpret_cast<float*>(take((size_t)p.N * 4));
     s.g_top = reinterpret_cast<float*>(take(4));
-    s.e = reinterpret_cast<void*>(take((size_t)rows * p.pitch * 2));
+    s.e = reinterpret_cast<void*>(take((size_t)rows * p.panels * 128));
     s.xs = reinterpret_cast<void*>(take((size_t)rows * p.K * 2));
     s.dw32 = reinterpret_cast<float*>(p.dw_space ? take((size_t)p.V * p.K * 4) : 0);
     s.dx_part = reinterpret_cast<float*>(p.splits > 1 ? take((size_t)p.splits * p.chunk * p.K * 4) : 0);
@@ -1085,7 +1137,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   float* dw32 = c.out32 ? static_cast<float*>(c.dw) : s.dw32;
   const DwRows dw_rows{dw32, p.K, p.direct ? 0 : 1};
   CUtensorMap dwm = wm;
-  if (c.dw && !(p.direct ? make_map(&dwm, c.dw, V, K, K, F16, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)
+  if (c.dw && !(p.direct ? make_map(&dwm, c.dw, V, K, K, F16, 16, 32, CU_TENSOR_MAP_SWIZZLE_32B)
                          : make_map_f32(&dwm, dw32, V, K)))
     return KRSI_ERR_CUDA;
   for (int64_t r0 = 0; r0 < p.N; r0 += p.chunk) {
@@ -1094,9 +1146,9 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     CUtensorMap xm, es, ek, em, xs;
     if (!make_map(&xm, xc, rows, K, K, F16, kBK, kBM, sw128)) return KRSI_ERR_CUDA;
     es = xm;
-    if (p.grads && (!make_map(&es, s.e, rows, V, p.pitch, F16, 64, 32, sw128) ||
-                    !make_map(&ek, s.e, rows, V, p.pitch, F16, kBK, kBM, sw128) ||
-                    !make_map(&em, s.e, rows, V, p.pitch, F16, 64, kBK, sw128) ||
+    if (p.grads && (!make_panel_map(&es, s.e, rows, p.panels, F16, 32, 1) ||
+                    !make_panel_map(&ek, s.e, rows, p.panels, F16, kBM, 1) ||
+                    !make_panel_map(&em, s.e, rows, p.panels, F16, kBK, 2) ||
                     !make_map(&xs, s.xs, rows, K, K, F16, 64, kBK, sw128)))
       return KRSI_ERR_CUDA;
     LogitsArgs la{};
@@ -1179,6 +1231,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     ga.accumulate = r0 > 0;
     ga.base = p.direct ? dw32 : nullptr;
     ga.start = s.sorted.start;
+    ga.order = s.sorted.order;
     ga.g_top = g_top;
     ga.alpha = 1.f / e_scale;
     ga.scale = c.scale;
@@ -1188,11 +1241,11 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     const int64_t part_rows = (int64_t)ga.n_rt * 256;
     if (c.dx && !(ga.dx_part  ? make_map_f32(&dxm, s.dx_part, ga.splits * part_rows, K)
                   : c.out32 ? make_map_f32(&dxm, dxc, rows, K)
-                            : make_map(&dxm, dxc, rows, K, K, F16, 32, 32, CU_TENSOR_MAP_SWIZZLE_64B)))
+                            : make_map(&dxm, dxc, rows, K, K, F16, 16, 32, CU_TENSOR_MAP_SWIZZLE_32B)))
       return KRSI_ERR_CUDA;
     KRSI_CUDA_TRY(launch_pairs(ce_grads_kernel<F16>, P, stream, ek, wm, em, xs, dxm, dwm, ga));
     if (ga.dx_part && c.dx)
-      KRSI_CUDA_TRY(launch_pdl(ce_dx_join_kernel<DT>, dim3((unsigned)ceil_div(rows * (K / 8), 256)), dim3(256), 0,
+      KRSI_CUDA_TRY(launch_pdl(ce_dx_join_kernel<DT>, dim3((unsigned)ceil_div(rows * (K / 4), 128)), dim3(128), 0,
                                stream, (const float*)s.dx_part, ga.splits, part_rows * K, ga.tgt, ga.factor, ga.coef, w,
                                dxc, (int)rows, K, c.scale, (int)c.out32));
   }

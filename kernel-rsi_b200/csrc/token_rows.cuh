@@ -18,10 +18,26 @@ constexpr int kChunkRows = 32;
 
 inline int64_t chunks_of(int64_t n) { return (n + kChunkRows - 1) / kChunkRows; }
 
-// The positions of tokens[0, n) sorted by token (equal tokens in position order), those outside [0, V)
-// and those equal to `skip` left out:
-//   start[v] .. start[v + 1]   the sorted entries of token v (start[V] = their number)
-//   pos[i], tok[i]             position and token of sorted entry i
+// The order that tokens are sorted into: by their low bits (the groups), then by the rest.  Low ids are
+// the frequent ones in most vocabularies; the groups spread them over the blocks of the sort.
+struct Order {
+  int bits;    // log2 of the groups
+  int range;   // tokens per group
+  __host__ __device__ __forceinline__ int key(int v) const { return (v & ((1 << bits) - 1)) * range + (v >> bits); }
+};
+constexpr int kMaxRange = 1024;
+inline Order order_of(int64_t V) {
+  Order o{7, 0};   // 128 groups, more where a group would pass kMaxRange tokens
+  while (((V - 1) >> o.bits) + 1 > kMaxRange) ++o.bits;
+  o.range = (int)(((V - 1) >> o.bits) + 1);
+  return o;
+}
+
+// The positions of tokens[0, n) sorted by token (in Order, equal tokens in position order), those outside
+// [0, V) and those equal to `skip` left out:
+//   start[key(v)] .. start[key(v) + 1]   the sorted entries of token v (start[end] = their number, end being
+//                                        groups * range)
+//   pos[i], tok[i]                       position and token of sorted entry i
 // token_bits 32 or 64.  One kernel, no workspace beyond the outputs.
 cudaError_t token_sort(const void* toks, int token_bits, int64_t n, int64_t V, int64_t skip, int* start, int* pos,
                        int* tok, cudaStream_t stream);
@@ -30,6 +46,7 @@ cudaError_t token_sort(const void* toks, int token_bits, int64_t n, int64_t V, i
 struct Space {
   int *start, *pos, *tok;
   float* partial;
+  Order order;
   size_t bytes;
 };
 inline Space space_at(void* base, int64_t n, int64_t V, int64_t d) {
@@ -37,8 +54,9 @@ inline Space space_at(void* base, int64_t n, int64_t V, int64_t d) {
   const uintptr_t p = reinterpret_cast<uintptr_t>(base);
   Space s;
   size_t off = 0;
+  s.order = order_of(V);
   s.start = reinterpret_cast<int*>(p + off);
-  off += up((size_t)(V + 1) * 4);
+  off += up((((size_t)s.order.range << s.order.bits) + 1) * 4);
   s.pos = reinterpret_cast<int*>(p + off);
   off += up((size_t)n * 4);
   s.tok = reinterpret_cast<int*>(p + off);
@@ -66,19 +84,21 @@ template <int DT, int VEC, bool WEIGHTED, typename Out>
 __global__ void __launch_bounds__(256)
 sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restrict__ weight,
                 const int* __restrict__ start, const int* __restrict__ pos, const int* __restrict__ tok,
-                float* __restrict__ partial, const Out out, int chunks, int V, uint32_t packets) {
+                float* __restrict__ partial, const Out out, const Order order, int chunks, int V, uint32_t packets) {
   pdl_enter();
   using E = Elem<DT>;
   using P = Pack<typename E::T, VEC>;
   const uint32_t c = blockIdx.y * blockDim.x + threadIdx.x;
   if ((int)blockIdx.x >= chunks) {
     const int v0 = ((int)blockIdx.x - chunks) * kZeroTokens;
-    for (int v = v0; v < v0 + kZeroTokens && v < V; ++v)
-      if (start[v] == start[v + 1] && c < packets) out.zero(v, c);
+    for (int v = v0; v < v0 + kZeroTokens && v < V; ++v) {
+      const int k = order.key(v);
+      if (start[k] == start[k + 1] && c < packets) out.zero(v, c);
+    }
     return;
   }
   const int chunk = blockIdx.x;
-  const int i0 = chunk * kChunkRows, m = min(kChunkRows, start[V] - i0);   // the entries of this chunk
+  const int i0 = chunk * kChunkRows, m = min(kChunkRows, start[order.range << order.bits] - i0);   // the entries of this chunk
   if (m <= 0) return;
   __shared__ int s_pos[kChunkRows], s_tok[kChunkRows + 1];
   __shared__ float s_weight[kChunkRows];
@@ -91,7 +111,7 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
   if (threadIdx.x == 0) s_tok[m] = -1;   // the chunk's end ends a run
   __syncthreads();
   if (c >= packets) return;
-  const bool from_before = start[s_tok[0]] < i0, goes_on = start[s_tok[m - 1] + 1] > i0 + m;
+  const bool from_before = start[order.key(s_tok[0])] < i0, goes_on = start[order.key(s_tok[m - 1]) + 1] > i0 + m;
   const P* gp = reinterpret_cast<const P*>(g);
   float acc[VEC];
 #pragma unroll
@@ -127,35 +147,71 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
   }
 }
 
-// The rows of runs that cross chunks.  Block (chunk, y) finishes the run that begins in `chunk` and goes
-// on past it, for 32 columns: its warps add contiguous shares of the run's partial rows, in order, then
-// the warps' sums are added in warp order.
+// The rows of runs that cross chunks, for 128 columns a block.  Each of the block's warps looks at one
+// chunk: where a run begins in it and goes on past it, that run's partial rows (one per chunk) are added
+// in chunk order.  Up to kShortRun of them the warp adds alone; a longer run is left to the whole block,
+// whose warps add contiguous shares, in order, and then their sums in warp order.
 constexpr int kJoinWarps = 8;
+constexpr int kShortRun = 32;
 
 template <typename Out>
 __global__ void __launch_bounds__(32 * kJoinWarps)
 join_rows_kernel(const int* __restrict__ start, const int* __restrict__ tok, const float* __restrict__ partial,
-                 const Out out, int V, int d) {
+                 const Out out, const Order order, int d) {
   pdl_enter();
-  const int chunk = blockIdx.x, i0 = chunk * kChunkRows, i1 = i0 + kChunkRows;
-  if (i1 >= start[V]) return;                       // no entries after this chunk
-  const int t = tok[i1 - 1], s = start[t], e = start[t + 1];
-  if (s < i0 || e <= i1) return;
-  const int n = (e - 1) / kChunkRows - chunk + 1;   // partial rows: this chunk's, then one per later chunk
-  const int col = blockIdx.y * 32 + threadIdx.x % 32, warp = threadIdx.x / 32;
-  const int share = (n + kJoinWarps - 1) / kJoinWarps;
-  const int k1 = min(n, (warp + 1) * share);
-  float acc = 0.f;
-  if (col < d)
-#pragma unroll 8
-    for (int k = warp * share; k < k1; ++k) acc += partial[(int64_t)(2 * (chunk + k) + (k == 0 ? 1 : 0)) * d + col];
-  __shared__ float sum[kJoinWarps][32];
-  sum[warp][threadIdx.x % 32] = acc;
-  __syncthreads();
-  if (warp == 0 && col < d) {
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int col0 = blockIdx.y * 128 + lane;         // and 32, 64, 96 further
+  // partial rows [k0, k1) of the run that begins in `chunk`: its tail, then the heads of later chunks
+  auto add = [&](int chunk, int k0, int k1, float* acc) {
 #pragma unroll
-    for (int w = 1; w < kJoinWarps; ++w) acc += sum[w][threadIdx.x];
-    out.column(t, col, acc);
+    for (int j = 0; j < 4; ++j) acc[j] = 0.f;
+#pragma unroll 4
+    for (int k = k0; k < k1; ++k) {
+      const float* row = partial + (int64_t)(2 * (chunk + k) + (k == 0 ? 1 : 0)) * d;
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (col0 + 32 * j < d) acc[j] += row[col0 + 32 * j];
+    }
+  };
+  auto put = [&](int t, const float* acc) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      if (col0 + 32 * j < d) out.column(t, col0 + 32 * j, acc[j]);
+  };
+  const int chunk = blockIdx.x * kJoinWarps + warp, i0 = chunk * kChunkRows, i1 = i0 + kChunkRows;
+  int t = 0, n = 0;                                 // the run's token and partial rows; n = 0: none
+  if (i1 < start[order.range << order.bits]) {
+    t = tok[i1 - 1];
+    const int k = order.key(t), e = start[k + 1];
+    if (start[k] >= i0 && e > i1) n = (e - 1) / kChunkRows - chunk + 1;
+  }
+  float acc[4];
+  if (n > 0 && n <= kShortRun) {
+    add(chunk, 0, n, acc);
+    put(t, acc);
+  }
+  __shared__ int s_n[kJoinWarps], s_t[kJoinWarps];
+  __shared__ float sum[kJoinWarps][4][32];
+  if (lane == 0) {
+    s_n[warp] = n;
+    s_t[warp] = t;
+  }
+  __syncthreads();
+  for (int w = 0; w < kJoinWarps; ++w) {
+    const int m = s_n[w];
+    if (m <= kShortRun) continue;                   // the same for the whole block
+    const int share = (m + kJoinWarps - 1) / kJoinWarps;
+    add(blockIdx.x * kJoinWarps + w, min(m, warp * share), min(m, (warp + 1) * share), acc);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) sum[warp][j][lane] = acc[j];
+    __syncthreads();
+    if (warp == 0) {
+      for (int o = 1; o < kJoinWarps; ++o)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[j] += sum[o][j][lane];
+      put(s_t[w], acc);
+    }
+    __syncthreads();
   }
 }
 
@@ -170,11 +226,11 @@ cudaError_t sum_by_token(const void* g, const float* weight, const Space& s, con
   const int64_t zero_blocks = zeros ? (V + kZeroTokens - 1) / kZeroTokens : 0;
   const dim3 grid((unsigned)(chunks + zero_blocks), (packets + threads - 1) / threads);
   cudaError_t e = launch_pdl(sum_rows_kernel<DT, VEC, WEIGHTED, Out>, grid, dim3(threads), 0, stream, (const T*)g,
-                             weight, (const int*)s.start, (const int*)s.pos, (const int*)s.tok, s.partial, out, chunks,
+                             weight, (const int*)s.start, (const int*)s.pos, (const int*)s.tok, s.partial, out, s.order, chunks,
                              (int)V, packets);
   if (e != cudaSuccess || chunks == 1) return e;
-  return launch_pdl(join_rows_kernel<Out>, dim3(chunks - 1, (unsigned)((d + 31) / 32)), dim3(32 * kJoinWarps), 0,
-                    stream, (const int*)s.start, (const int*)s.tok, (const float*)s.partial, out, (int)V, (int)d);
+  const dim3 join_grid((unsigned)((chunks - 1 + kJoinWarps - 1) / kJoinWarps), (unsigned)((d + 127) / 128));
+  return launch_pdl(join_rows_kernel<Out>, join_grid, dim3(32 * kJoinWarps), 0, stream, (const int*)s.start, (const int*)s.tok, (const float*)s.partial, out, s.order, (int)d);
 }
 
 }  // namespace tokens

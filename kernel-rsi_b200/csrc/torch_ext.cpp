@@ -10,6 +10,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
 #include "../../include/krsi_b200.h"
@@ -473,6 +474,104 @@ at::Tensor linear_ce_finish(const at::Tensor& grad, const at::Tensor& g_in, cons
   return out;
 }
 
+// ---------------------------------------------------------------- eager autograd
+// Autograd nodes of the vocabulary operators and the 8-bit checkpoint, in C++: at small sizes a pass is
+// bound by the host, and a Python autograd.Function costs it 60 us more a step than these do.  (Compiled
+// graphs use the *_fwd operators with the gradients registered in _ext.py.)
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& tokens, const at::Tensor& table, double scale,
+                            int64_t padding_idx) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    ctx->save_for_backward({tokens, table});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["padding_idx"] = padding_idx;
+    return embedding_fwd(tokens, table, scale, padding_idx);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    return {at::Tensor(),
+            embedding_bwd(g[0], saved[0], saved[1], ctx->saved_data["scale"].toDouble(),
+                          ctx->saved_data["padding_idx"].toInt()),
+            at::Tensor(), at::Tensor()};
+  }
+};
+at::Tensor embedding_autograd(const at::Tensor& tokens, const at::Tensor& table, double scale, int64_t padding_idx) {
+  if (at::GradMode::is_enabled() && table.requires_grad())
+    return EmbeddingNode::apply(tokens, table, scale, padding_idx);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return embedding_fwd(tokens, table, scale, padding_idx);
+}
+
+struct GegluQ8Node : public torch::autograd::Function<GegluQ8Node> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& u) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [out, q, ex] = geglu_q8_fwd(u, true);
+    ctx->save_for_backward({q, ex});
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    return {std::get<0>(geglu_q8_bwd(g[0], saved[0], saved[1], false))};
+  }
+};
+at::Tensor geglu_q8_autograd(const at::Tensor& u) {
+  if (at::GradMode::is_enabled() && u.requires_grad()) return GegluQ8Node::apply(u);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return std::get<0>(geglu_q8_fwd(u, false));
+}
+at::Tensor geglu_q8_plain(const at::Tensor& u) { return std::get<0>(geglu_q8_fwd(u, false)); }
+
+// keep: form the gradients in the forward (saved in fp32) instead of saving the operands.
+at::Tensor linear_ce_plain(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, double scale,
+                           int64_t ignore_index, double z_loss, int64_t reduction, bool /*keep*/) {
+  auto [loss, reduced, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction, false, false);
+  return reduction != 0 ? reduced.select(0, 0) : loss;
+}
+struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
+  static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
+                            double scale, int64_t ignore_index, double z_loss, int64_t reduction, bool keep) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [loss, reduced, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction,
+                                                 keep && x.requires_grad(), keep && w.requires_grad());
+    auto out = reduction != 0 ? reduced.select(0, 0) : loss;
+    auto weight = reduced.slice(0, 1);
+    if (keep) ctx->save_for_backward({weight, dx, dw, w});
+    else ctx->save_for_backward({weight, x, w, targets});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["ignore_index"] = ignore_index;
+    ctx->saved_data["z_loss"] = z_loss;
+    ctx->saved_data["keep"] = keep;
+    return out;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    const auto saved = ctx->get_saved_variables();
+    const double scale = ctx->saved_data["scale"].toDouble();
+    const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    at::Tensor dx, dw;
+    if (ctx->saved_data["keep"].toBool()) {
+      if (need_x) dx = linear_ce_finish(saved[1], g[0], saved[0], scale, saved[3]);
+      if (need_w) dw = linear_ce_finish(saved[2], g[0], saved[0], scale, saved[3]);
+    } else {
+      std::tie(dx, dw) = linear_ce_grad(g[0], saved[0], saved[1], saved[2], saved[3], scale,
+                                        ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["z_loss"].toDouble(),
+                                        need_x, need_w);
+      if (!need_x) dx = at::Tensor();
+      if (!need_w) dw = at::Tensor();
+    }
+    return {dx, dw, at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+at::Tensor linear_ce_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, double scale,
+                              int64_t ignore_index, double z_loss, int64_t reduction, bool keep) {
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()))
+    return LinearCeNode::apply(x, w, targets, scale, ignore_index, z_loss, reduction, keep);
+  at::AutoDispatchBelowADInplaceOrView below;
+  return linear_ce_plain(x, w, targets, scale, ignore_index, z_loss, reduction, keep);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(krsi, m) {
@@ -490,6 +589,10 @@ TORCH_LIBRARY(krsi, m) {
   m.def("t5_bias_bwd(Tensor dpd, Tensor table, int S, int num_buckets, int max_distance, bool bidirectional) -> Tensor");
   m.def("embedding_fwd(Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
   m.def("embedding_bwd(Tensor g, Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
+  m.def("embedding(Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
+  m.def("geglu_q8(Tensor u) -> Tensor");
+  m.def("linear_ce(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, int reduction, "
+        "bool keep) -> Tensor");
   m.def("linear_ce_fwd(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, "
         "int reduction, bool want_dx, bool want_dw) -> (Tensor, Tensor, Tensor, Tensor)");
   m.def("linear_ce_grad(Tensor g, Tensor weight, Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, "
@@ -513,9 +616,18 @@ TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
   m.impl("t5_bias_bwd", &t5_bias_bwd);
   m.impl("embedding_fwd", &embedding_fwd);
   m.impl("embedding_bwd", &embedding_bwd);
+  m.impl("embedding", &embedding_fwd);
+  m.impl("geglu_q8", &geglu_q8_plain);
+  m.impl("linear_ce", &linear_ce_plain);
   m.impl("linear_ce_fwd", &linear_ce_fwd);
   m.impl("linear_ce_grad", &linear_ce_grad);
   m.impl("linear_ce_finish", &linear_ce_finish);
   m.impl("geglu_q8_fwd", &geglu_q8_fwd);
   m.impl("geglu_q8_bwd", &geglu_q8_bwd);
+}
+
+TORCH_LIBRARY_IMPL(krsi, AutogradCUDA, m) {
+  m.impl("embedding", &embedding_autograd);
+  m.impl("geglu_q8", &geglu_q8_autograd);
+  m.impl("linear_ce", &linear_ce_autograd);
 }

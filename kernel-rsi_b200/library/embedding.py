@@ -10,6 +10,7 @@ row gets no gradient; it is looked up like any other.
 
 A token outside [0, V) cannot raise without a synchronisation: its row of the output is NaN and it adds
 to no gradient.  The reference has no such op (its models use torch's embedding).
+The autograd node is in csrc/torch_ext.cpp (krsi::embedding).
 Kernels: kernel-rsi_b200/csrc/embedding.cu, token_rows.cu; C ABI: include/krsi_b200.h.
 """
 import sys
@@ -23,21 +24,6 @@ from _compat import compiling  # noqa: E402
 from _ext import ops  # noqa: E402
 
 
-class Embedding(torch.autograd.Function):
-    """Eager path: saves (tokens, table); returns (None, dtable, None, None)."""
-
-    @staticmethod
-    def forward(ctx, tokens, table, scale, padding_idx):
-        ctx.save_for_backward(tokens, table)
-        ctx.args = (scale, padding_idx)
-        return ops.embedding_fwd(tokens, table, scale, padding_idx)
-
-    @staticmethod
-    def backward(ctx, g):
-        tokens, table = ctx.saved_tensors
-        return None, ops.embedding_bwd(g, tokens, table, *ctx.args), None, None
-
-
 def embedding(tokens, table, scale=1.0, padding_idx=None):
     """scale * table[tokens] for integer tokens of any shape and a [V, d] table."""
     if padding_idx is None:
@@ -47,9 +33,9 @@ def embedding(tokens, table, scale=1.0, padding_idx=None):
         if not -V <= padding_idx < V:
             raise ValueError(f"embedding: padding_idx {padding_idx} is outside a table of {V} rows")
         pad = padding_idx % V
-    if compiling() or not (table.requires_grad and torch.is_grad_enabled()):
+    if compiling():
         return ops.embedding_fwd(tokens, table, scale, pad)
-    return Embedding.apply(tokens, table, scale, pad)
+    return ops.embedding(tokens, table, scale, pad)
 
 
 def reference(tokens, table, scale=1.0, padding_idx=None):

@@ -14,6 +14,7 @@ feed_forward_q8(x2d, wi, wo, res) is res + geglu(x2d @ wi.t()) @ wo.t() that kee
 the checkpoint only: the GEGLU output, which the down projection's weight gradient needs, is computed
 again from the checkpoint in the same pass as u's gradient.  Per row 2.06 F bytes stay for the backward
 where feed_forward() keeps 6F (u and the GEGLU output in 16 bits).  The products are cuBLAS.
+geglu_q8's autograd node is in csrc/torch_ext.cpp (krsi::geglu_q8).
 Kernels: kernel-rsi_b200/csrc/geglu_q8.cu; C ABI: include/krsi_b200.h.
 """
 import sys
@@ -29,28 +30,11 @@ from _ext import ops  # noqa: E402
 GROUP = 32
 
 
-class GEGLUQ8(torch.autograd.Function):
-    """Eager path: saves the checkpoint (q, exponents); returns du."""
-
-    @staticmethod
-    def forward(ctx, u):
-        out, q, ex = ops.geglu_q8_fwd(u, True)
-        ctx.save_for_backward(q, ex)
-        return out
-
-    @staticmethod
-    def backward(ctx, g):
-        q, ex = ctx.saved_tensors
-        return ops.geglu_q8_bwd(g, q, ex, False)[0]
-
-
 def geglu_q8(u):
     """gelu_tanh(u[:, :F]) * u[:, F:] for u [rows, 2F], its backward from an 8-bit copy of u."""
     if compiling():
         return ops.geglu_q8_fwd(u, True)[0]
-    if not (u.requires_grad and torch.is_grad_enabled()):
-        return ops.geglu_q8_fwd(u, False)[0]
-    return GEGLUQ8.apply(u)
+    return ops.geglu_q8(u)
 
 
 class FeedForwardQ8(torch.autograd.Function):

@@ -16,7 +16,8 @@ The logits exist one tile at a time, in the GEMM's epilogue.  With "mean" or "su
 or more, the forward also forms both gradients (of the sum of the losses, in fp32) while the
 exponentials are at hand, and the backward only scales and rounds them: one pass over the logits in all,
 for the memory of two fp32 gradients.  Otherwise the backward computes the logits again.
-The reference has no loss op.  Kernels: kernel-rsi_b200/csrc/linear_ce.cu; C ABI: include/krsi_b200.h.
+The reference has no loss op.  The autograd node is in csrc/torch_ext.cpp (krsi::linear_ce).
+Kernels: kernel-rsi_b200/csrc/linear_ce.cu; C ABI: include/krsi_b200.h.
 """
 import sys
 from pathlib import Path
@@ -32,47 +33,18 @@ REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
 KEEP_ROWS = 1024
 
 
-class LinearCrossEntropy(torch.autograd.Function):
-    """Eager path: saves the fp32 gradients, or the operands; returns (dx, dw, None, ...)."""
-
-    @staticmethod
-    def forward(ctx, x2d, w, targets, scale, ignore_index, z_loss, reduction):
-        ctx.args = (scale, ignore_index, z_loss)
-        ctx.kept = reduction != 0 and x2d.shape[0] >= KEEP_ROWS
-        want = ctx.needs_input_grad[:2] if ctx.kept else (False, False)
-        loss, reduced, dx, dw = ops.linear_ce_fwd(x2d, w, targets, scale, ignore_index, z_loss, reduction, *want)
-        if ctx.kept:
-            ctx.save_for_backward(reduced, dx, dw, w)
-        else:
-            ctx.save_for_backward(reduced, x2d, w, targets)
-        return reduced[0] if reduction else loss
-
-    @staticmethod
-    def backward(ctx, g):
-        need = ctx.needs_input_grad[:2]
-        reduced, *saved = ctx.saved_tensors
-        weight = reduced[1:]
-        if ctx.kept:
-            dx, dw, like = saved
-            dx = ops.linear_ce_finish(dx, g, weight, ctx.args[0], like) if need[0] else None
-            dw = ops.linear_ce_finish(dw, g, weight, ctx.args[0], like) if need[1] else None
-        else:
-            dx, dw = ops.linear_ce_grad(g, weight, *saved, *ctx.args, *need)
-        return (dx if need[0] else None), (dw if need[1] else None), None, None, None, None, None
-
-
 def linear_cross_entropy(x2d, w, targets, scale=1.0, ignore_index=-100, z_loss=0.0, reduction="mean"):
     """The cross entropy of softmax(scale * x2d @ w.t()) against targets, for x2d [N, K] and w [V, K]."""
     if reduction not in REDUCTIONS:
         raise ValueError(f"linear_cross_entropy: reduction must be one of {sorted(REDUCTIONS)}, got {reduction!r}")
     kind = REDUCTIONS[reduction]
-    need = torch.is_grad_enabled() and (x2d.requires_grad or w.requires_grad)
-    if compiling() or not need:
-        keep = need and kind != 0 and x2d.shape[0] >= KEEP_ROWS
+    keep = kind != 0 and x2d.shape[0] >= KEEP_ROWS
+    if compiling():
+        keep = keep and torch.is_grad_enabled()
         loss, reduced, _, _ = ops.linear_ce_fwd(x2d, w, targets, scale, ignore_index, z_loss, kind,
                                                 keep and x2d.requires_grad, keep and w.requires_grad)
         return reduced[0] if kind else loss
-    return LinearCrossEntropy.apply(x2d, w, targets, scale, ignore_index, z_loss, kind)
+    return ops.linear_ce(x2d, w, targets, scale, ignore_index, z_loss, kind, keep)
 
 
 def reference(x2d, w, targets, scale=1.0, ignore_index=-100, z_loss=0.0, reduction="mean"):
