@@ -208,7 +208,8 @@ int krsi_embedding_bwd(const void* tokens, int token_bits, const void* g, void* 
 /* ---------------------------------------------------------------- GEGLU with an 8-bit checkpoint
  * krsi_geglu_fwd/bwd with u kept for the backward in 8 bits.  No counterpart in the reference (its
  * backward reads u in full, geglu.py:64-68).
- * The checkpoint: q [rows, 2F] int8 and exponents [rows, ceil(F / 32), 2] uint8 (gate, value); in a
+ * The checkpoint: q [rows, 2F] int8 and exponents [rows, ceil(F / 32), 2] uint8 (gate, value; 2-byte
+ * aligned); in a
  * group of 32 columns of a half-row u is kept as q * 2^(e - 127), with 2^(e - 127) = 2^-6 of the power
  * of two at or below the group's largest magnitude (2^-126 at least) and q rounded to nearest even
  * within [-127, 127].  e = 255 marks a group with a value that is not finite: it reads back as NaN.

@@ -19,9 +19,9 @@ template <int DT>
 __device__ __forceinline__ typename Elem<DT>::T nan_of() { return Elem<DT>::store(__int_as_float(0x7fffffff)); }
 
 // ---------------------------------------------------------------- forward
-// A thread keeps one packet of columns and takes kFwdRows rows of a block's share, their loads in flight
-// together behind the loads of their tokens.
-constexpr int kFwdRows = 8;
+// A thread keeps one packet of columns and takes up to kFwdRows rows, staged in shared memory so that
+// their loads are in flight together (behind those of their tokens).
+constexpr int kFwdRows = 16;
 
 template <int DT, int VEC, typename I>
 __global__ void __launch_bounds__(256)
@@ -32,31 +32,36 @@ embedding_fwd_kernel(const I* __restrict__ toks, const typename Elem<DT>::T* __r
   using P = Pack<typename E::T, VEC>;
   const uint32_t c = blockIdx.y * blockDim.x + threadIdx.x;
   const int row0 = (int)blockIdx.x * rows, m = min(rows, n - row0);
+  __shared__ int s_tok[kFwdRows];    // -1: outside the table
+  if (threadIdx.x < m) {
+    const I v = toks[row0 + threadIdx.x];
+    s_tok[threadIdx.x] = v >= 0 && v < (I)V ? (int)v : -1;
+  }
+  __syncthreads();
   if (c >= packets) return;
+  extern __shared__ __align__(16) unsigned char stage_raw[];
+  P* stage = reinterpret_cast<P*>(stage_raw) + threadIdx.x;   // [rows][blockDim.x]
   const P* tp = reinterpret_cast<const P*>(table) + c;
   P* op = reinterpret_cast<P*>(out) + (int64_t)row0 * packets + c;
-  I t[kFwdRows];
-  P r[kFwdRows];
+  P none;
 #pragma unroll
-  for (int k = 0; k < kFwdRows; ++k) t[k] = k < m ? toks[row0 + k] : (I)0;
-#pragma unroll
-  for (int k = 0; k < kFwdRows; ++k) {
-    if (k >= m) break;
-    if (t[k] >= 0 && t[k] < (I)V) {
-      r[k] = tp[(int64_t)t[k] * packets];
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) r[k].v[e] = nan_of<DT>();
-    }
+  for (int e = 0; e < VEC; ++e) none.v[e] = nan_of<DT>();
+#pragma unroll 4
+  for (int k = 0; k < m; ++k) {
+    const int t = s_tok[k];
+    if (t >= 0) tokens::copy_packet(stage + k * blockDim.x, tp + (int64_t)t * packets);
+    else stage[k * blockDim.x] = none;
   }
-#pragma unroll
-  for (int k = 0; k < kFwdRows; ++k) {
-    if (k >= m) break;
+  tokens::copy_commit();
+  tokens::copy_wait<0>();
+#pragma unroll 4
+  for (int k = 0; k < m; ++k) {
+    P r = stage[k * blockDim.x];
     if (scale != 1.0f) {   // else the row's own bits
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) r[k].v[e] = E::store(scale * E::load(r[k].v[e]));
+      for (int e = 0; e < VEC; ++e) r.v[e] = E::store(scale * E::load(r.v[e]));
     }
-    op[(int64_t)k * packets] = r[k];
+    op[(int64_t)k * packets] = r;
   }
 }
 
@@ -103,13 +108,15 @@ int fwd(const void* toks, int token_bits, const void* table, void* out, int64_t 
   // as many rows a block as still leave a block for every SM
   const int rows = (int)std::max<int64_t>(1, std::min<int64_t>(kFwdRows, n / kNumSMsB200));
   const dim3 grid((unsigned)((n + rows - 1) / rows), (packets + threads - 1) / threads);
-  if (token_bits == 64)
-    KRSI_CUDA_TRY(launch_pdl(embedding_fwd_kernel<DT, VEC, long long>, grid, dim3(threads), 0, stream,
-                             (const long long*)toks, (const T*)table, (T*)out, (int)n, rows, packets, V, scale));
-  else
-    KRSI_CUDA_TRY(launch_pdl(embedding_fwd_kernel<DT, VEC, int>, grid, dim3(threads), 0, stream, (const int*)toks,
-                             (const T*)table, (T*)out, (int)n, rows, packets, V, scale));
-  return KRSI_OK;
+  const size_t smem = (size_t)rows * threads * VEC * sizeof(T);   // at most 64 KB
+  auto launch = [&](auto kern, auto* t) -> int {
+    KRSI_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdRows * 256 * 16));
+    KRSI_CUDA_TRY(launch_pdl(kern, grid, dim3(threads), smem, stream, t, (const T*)table, (T*)out, (int)n, rows,
+                             packets, V, scale));
+    return KRSI_OK;
+  };
+  return token_bits == 64 ? launch(embedding_fwd_kernel<DT, VEC, long long>, (const long long*)toks)
+                          : launch(embedding_fwd_kernel<DT, VEC, int>, (const int*)toks);
 }
 
 template <int DT, int VEC>

@@ -16,12 +16,25 @@
 //
 // Bound by memory: 2F values read, F values and 2F bytes written per row forward; F values and 2F bytes
 // read, 2F values written backward.  A thread holds 8 columns of both halves; a group is 4 lanes.
+//
+// What that takes: the arithmetic has to stay under the memory time, and the conversions alone would not
+// (a quarter-rate instruction per value and direction).  16-bit values are worked on in pairs (f32x2);
+// the largest magnitude is an integer maximum of pairs; a value is rounded to an integer by adding
+// 1.5 * 2^23 (the low byte of the sum is q), and a byte becomes a float as the low byte of 2^23 + 128 + q.
 #include <algorithm>
 
 #include "common.cuh"
+#include "gelu.cuh"
 
 namespace krsi {
 namespace {
+
+using sm100::f2_add;
+using sm100::f2_fma;
+using sm100::f2_mul;
+using sm100::f2_pack;
+using sm100::f2_unpack;
+using gelu::f2c;
 
 constexpr int kGroup = 32;        // columns that share a step
 constexpr int kCols = 8;          // columns of each half per thread
@@ -29,123 +42,215 @@ constexpr int kSlots = kGroup / kCols;
 constexpr float kTwoC = 1.5957691216057308f;                       // 2 sqrt(2 / pi)
 constexpr float kA = 0.044715f;
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kMagic = 12582912.0f;                              // 1.5 * 2^23
 
 template <typename T, int VEC>
 struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-// s = 1 / (1 + exp(-2 z)); exp overflows to inf for a very negative z, and s is then 0.
-__device__ __forceinline__ float gate_sigmoid(float a) {
-  const float z2 = kTwoC * (a + kA * a * a * a);
-  return rcp_approx(1.0f + ex2_approx(-kLog2e * z2));
-}
-__device__ __forceinline__ float gate_slope(float a, float s) {
-  const float dz2 = kTwoC * (1.0f + 3.0f * kA * a * a);
-  return s + a * s * (1.0f - s) * dz2;
+// kCols values of one half-row, as four pairs.
+struct Cols {
+  uint64_t v[4];
+};
+
+// s = 1 / (1 + exp(-2 z)) for a pair; exp overflows to inf for a very negative z, and s is then 0.
+__device__ __forceinline__ uint64_t gate_sigmoid(uint64_t a, uint64_t a2) {
+  const uint64_t x = f2_mul(a, f2_fma(a2, f2c(-kLog2e * kTwoC * kA), f2c(-kLog2e * kTwoC)));
+  float x0, x1, y0, y1;
+  f2_unpack(x, x0, x1);
+  f2_unpack(f2_add(f2_pack(ex2_approx(x0), ex2_approx(x1)), f2c(1.0f)), y0, y1);
+  return f2_pack(rcp_approx(y0), rcp_approx(y1));
 }
 
 // Up to kCols columns from p (the columns from `left` on are zero), VEC at a time: VEC divides F, so an
 // access is inside the row or outside it.
-template <int DT, int VEC>
-__device__ __forceinline__ void load_cols(const typename Elem<DT>::T* p, int left, float* v) {
-  using P = Pack<typename Elem<DT>::T, VEC>;
+template <typename T, int VEC>
+__device__ __forceinline__ void load_raw(const T* p, int left, T* v) {
 #pragma unroll
   for (int k = 0; k < kCols; k += VEC) {
-    if (k < left) {
-      const P r = *reinterpret_cast<const P*>(p + k);
+    Pack<T, VEC> r;
+    memset(&r, 0, sizeof(r));
+    if (k < left) r = *reinterpret_cast<const Pack<T, VEC>*>(p + k);
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) v[k + e] = Elem<DT>::load(r.v[e]);
-    } else {
-#pragma unroll
-      for (int e = 0; e < VEC; ++e) v[k + e] = 0.f;
-    }
+    for (int e = 0; e < VEC; ++e) v[k + e] = r.v[e];
   }
 }
-template <int DT, int VEC>
-__device__ __forceinline__ void store_cols(typename Elem<DT>::T* p, int left, const float* v) {
-  using P = Pack<typename Elem<DT>::T, VEC>;
+template <typename T, int VEC>
+__device__ __forceinline__ void store_raw(T* p, int left, const T* v) {
 #pragma unroll
   for (int k = 0; k < kCols; k += VEC)
     if (k < left) {
-      P r;
+      Pack<T, VEC> r;
 #pragma unroll
-      for (int e = 0; e < VEC; ++e) r.v[e] = Elem<DT>::store(v[k + e]);
-      *reinterpret_cast<P*>(p + k) = r;
+      for (int e = 0; e < VEC; ++e) r.v[e] = v[k + e];
+      *reinterpret_cast<Pack<T, VEC>*>(p + k) = r;
     }
 }
 
-// The group's exponent byte from the magnitudes of its 4 lanes' columns (float bits order as integers;
-// NaN above infinity above every finite value).
-__device__ __forceinline__ uint32_t group_exponent(const float* v) {
-  uint32_t top = 0;
+// One half-row's columns of a storage type: the raw values, widened and narrowed in pairs.
+template <int DT>
+struct alignas(16) Raw {
+  using T = typename Elem<DT>::T;
+  T v[kCols];
+  __device__ __forceinline__ Cols widen() const {
+    Cols c;
 #pragma unroll
-  for (int k = 0; k < kCols; ++k) top = max(top, __float_as_uint(v[k]) & 0x7fffffffu);
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-  top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (DT == KRSI_F32) c.v[k] = f2_pack(v[2 * k], v[2 * k + 1]);
+      else c.v[k] = gelu::widen<DT == KRSI_F16>(reinterpret_cast<const uint32_t*>(v)[k]);
+    }
+    return c;
+  }
+  __device__ __forceinline__ void narrow(const Cols& c) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if constexpr (DT == KRSI_F32) f2_unpack(c.v[k], v[2 * k], v[2 * k + 1]);
+      else reinterpret_cast<uint32_t*>(v)[k] = gelu::narrow<DT == KRSI_F16>(c.v[k]);
+    }
+  }
+  // The largest magnitude as fp32 bits (which order as integers: NaN above infinity above the rest).
+  __device__ __forceinline__ uint32_t top() const {
+    if constexpr (DT == KRSI_F32) {
+      uint32_t t = 0;
+#pragma unroll
+      for (int k = 0; k < kCols; ++k) t = max(t, __float_as_uint(v[k]) & 0x7fffffffu);
+      return t;
+    } else {
+      uint32_t t = 0;
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const uint32_t m = reinterpret_cast<const uint32_t*>(v)[k] & 0x7fff7fffu;
+        asm("max.u16x2 %0, %0, %1;" : "+r"(t) : "r"(m));
+      }
+      const uint32_t h = max(t & 0xffffu, t >> 16);
+      return DT == KRSI_BF16 ? h << 16 : __float_as_uint(__half2float(__ushort_as_half((unsigned short)h)));
+    }
+  }
+};
+
+// The group's largest magnitude over its 4 lanes.
+__device__ __forceinline__ uint32_t group_top(uint32_t t) {
+  t = max(t, __shfl_xor_sync(0xffffffffu, t, 1));
+  return max(t, __shfl_xor_sync(0xffffffffu, t, 2));
+}
+__device__ __forceinline__ uint32_t exponent_of(uint32_t top) {
   return top >= 0x7f800000u ? 255u : max(top >> 23, 7u) - 6u;   // at least 1: a step of 2^-126
 }
 __device__ __forceinline__ float step_of(uint32_t e) { return __uint_as_float(e == 255u ? 0x7fffffffu : e << 23); }
 
 template <int VEC>
-__device__ __forceinline__ void store_q(int8_t* p, int left, const float* v, uint32_t e) {
+__device__ __forceinline__ void store_q(int8_t* p, int left, const Cols& c, uint32_t top, uint32_t e) {
   const float inv = __uint_as_float((254u - min(e, 253u)) << 23);   // 1 / step
-  using P = Pack<int8_t, VEC>;
+  uint32_t w[2];
+  uint32_t y[kCols];
+  if (__uint_as_float(top) * inv < 127.5f) {
 #pragma unroll
-  for (int k = 0; k < kCols; k += VEC)
-    if (k < left) {
-      P r;
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) r.v[i] = (int8_t)max(-127, min(127, __float2int_rn(v[k + i] * inv)));
-      *reinterpret_cast<P*>(p + k) = r;
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t r = f2_fma(c.v[k], f2c(inv), f2c(kMagic));
+      y[2 * k] = (uint32_t)r;
+      y[2 * k + 1] = (uint32_t)(r >> 32);
     }
-}
-template <int VEC>
-__device__ __forceinline__ void load_q(const int8_t* p, int left, uint32_t e, float* v) {
-  const float step = step_of(e);
-  using P = Pack<int8_t, VEC>;
+  } else {   // (or not finite: anything) some value may round to 128: held at 127
 #pragma unroll
-  for (int k = 0; k < kCols; k += VEC) {
-    if (k < left) {
-      const P r = *reinterpret_cast<const P*>(p + k);
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[k + i] = (float)r.v[i] * step;
-    } else {
-#pragma unroll
-      for (int i = 0; i < VEC; ++i) v[k + i] = 0.f;
+    for (int k = 0; k < 4; ++k) {
+      float x0, x1;
+      f2_unpack(f2_mul(c.v[k], f2c(inv)), x0, x1);
+      y[2 * k] = __float_as_uint(fminf(fmaxf(x0, -127.f), 127.f) + kMagic);
+      y[2 * k + 1] = __float_as_uint(fminf(fmaxf(x1, -127.f), 127.f) + kMagic);
     }
   }
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    w[h] = __byte_perm(__byte_perm(y[4 * h], y[4 * h + 1], 0x0040), __byte_perm(y[4 * h + 2], y[4 * h + 3], 0x0040),
+                       0x5410);
+  store_raw<int8_t, VEC>(p, left, reinterpret_cast<const int8_t*>(w));
 }
+struct alignas(8) Bytes {
+  int8_t v[kCols];
+};
+template <int VEC>
+__device__ __forceinline__ Bytes load_q(const int8_t* p, int left) {
+  Bytes b;
+  load_raw<int8_t, VEC>(p, left, b.v);
+  return b;
+}
+__device__ __forceinline__ Cols dequantise(const Bytes& b, uint32_t e) {
+  const uint64_t step = f2c(step_of(e));
+  Cols c;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t w = reinterpret_cast<const uint32_t*>(b.v)[k / 2] ^ 0x80808080u;   // q + 128
+    const uint32_t lo = __byte_perm(w, 0x4B000000u, 0x7440 | (k % 2 * 2));           // 2^23 + q + 128
+    const uint32_t hi = __byte_perm(w, 0x4B000000u, 0x7440 | (k % 2 * 2 + 1));
+    c.v[k] = f2_mul(f2_add((uint64_t)hi << 32 | lo, f2c(-8388736.0f)), step);
+  }
+  return c;
+}
+
+// One item, 8 columns of both halves of a row, per thread, in row order: many short blocks, all of whose
+// loads are issued at once, keep more in flight than fewer blocks that loop (Q8_LAYOUT).
+struct Rows {
+  uint32_t items, slots, mul, shift;   // slots: items per row, divided by as (umulhi(i, mul) + i) >> shift
+  int F;
+};
+struct Place {
+  uint32_t row, slot;
+  int left;             // columns from the item's first to the end of the half-row; 0: no item
+  int64_t at, half;     // offsets in [rows, 2F] (the gate's; the value's is F further) and in [rows, F]
+  __device__ __forceinline__ Place(const Rows& r, uint32_t i) {
+    row = (__umulhi(i, r.mul) + i) >> r.shift;
+    slot = i - row * r.slots;
+    left = i < r.items ? r.F - (int)(slot * kCols) : 0;
+    half = (int64_t)row * r.F + slot * kCols;
+    at = half + (int64_t)row * r.F;
+  }
+};
 
 template <int DT, int VEC>
 __global__ void __launch_bounds__(256)
 geglu_q8_fwd_kernel(const typename Elem<DT>::T* __restrict__ u, typename Elem<DT>::T* __restrict__ out,
-                    int8_t* __restrict__ q, uint8_t* __restrict__ ex, int64_t items, int F, uint32_t slots) {
+                    int8_t* __restrict__ q, uint8_t* __restrict__ ex, const Rows r) {
   pdl_enter();
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  const int64_t base = (int64_t)blockIdx.x * blockDim.x;
-  for (int64_t b0 = base; b0 < items; b0 += stride) {   // uniform per block: every lane meets the shuffles
-    const int64_t i = b0 + threadIdx.x;
-    const bool live = i < items;
-    const int64_t row = live ? i / slots : 0;
-    const int slot = live ? (int)(i - row * slots) : 0, c = slot * kCols;
-    const int left = live ? F - c : 0;
-    const int64_t at = row * 2 * F + c;
-    float a[kCols], b[kCols], o[kCols];
-    load_cols<DT, VEC>(u + at, left, a);
-    load_cols<DT, VEC>(u + at + F, left, b);
-    const uint32_t ea = group_exponent(a), eb = group_exponent(b);
+  using T = typename Elem<DT>::T;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+  const Place p(r, i);
+  Raw<DT> ra, rb, ro;
+  load_raw<T, VEC>(u + p.at, p.left, ra.v);
+  load_raw<T, VEC>(u + p.at + r.F, p.left, rb.v);
+  const Cols a = ra.widen(), b = rb.widen();
+  Cols o;
 #pragma unroll
-    for (int k = 0; k < kCols; ++k) o[k] = a[k] * gate_sigmoid(a[k]) * b[k];
-    store_cols<DT, VEC>(out + row * F + c, left, o);
-    if (q == nullptr) continue;
-    store_q<VEC>(q + at, left, a, ea);
-    store_q<VEC>(q + at + F, left, b, eb);
-    if (live && slot % kSlots == 0) {
-      uint8_t* er = ex + (row * slots + slot) / kSlots * 2;   // [row][group][gate, value]
-      er[0] = (uint8_t)ea;
-      er[1] = (uint8_t)eb;
+  for (int k = 0; k < 4; ++k) o.v[k] = f2_mul(f2_mul(a.v[k], gate_sigmoid(a.v[k], f2_mul(a.v[k], a.v[k]))), b.v[k]);
+  ro.narrow(o);
+  store_raw<T, VEC>(out + p.half, p.left, ro.v);
+  if (q == nullptr) return;
+  const uint32_t ta = group_top(ra.top()), tb = group_top(rb.top());   // every lane meets the shuffles
+  const uint32_t ea = exponent_of(ta), eb = exponent_of(tb);
+  store_q<VEC>(q + p.at, p.left, a, ta, ea);
+  store_q<VEC>(q + p.at + r.F, p.left, b, tb, eb);
+  if (p.left > 0 && i % kSlots == 0)   // [row][group][gate, value]
+    *reinterpret_cast<uint16_t*>(ex + i / kSlots * 2) = (uint16_t)(ea | eb << 8);
+}
+
+// From the checkpoint's gate a and value b and the output's gradient g: d(gate), d(value) and, where OUT,
+// the output again.  HUGE: a^2 may overflow; it is held finite, so that a slope of 0 times it is 0.
+template <bool OUT, bool HUGE>
+__device__ __forceinline__ void grad_cols(Cols& a, Cols& b, const Cols& g, Cols& o) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    uint64_t a2 = f2_mul(a.v[k], a.v[k]);
+    if (HUGE) {
+      float lo, hi;
+      f2_unpack(a2, lo, hi);
+      a2 = f2_pack(fminf(lo, 1e30f), fminf(hi, 1e30f));
     }
+    const uint64_t s = gate_sigmoid(a.v[k], a2), gel = f2_mul(a.v[k], s);
+    const uint64_t rest = f2_fma(s ^ 0x8000000080000000ull, gel, gel);                  // gel (1 - s)
+    const uint64_t slope = f2_fma(rest, f2_fma(a2, f2c(3.0f * kA * kTwoC), f2c(kTwoC)), s);
+    if (OUT) o.v[k] = f2_mul(gel, b.v[k]);
+    a.v[k] = f2_mul(f2_mul(g.v[k], b.v[k]), slope);
+    b.v[k] = f2_mul(g.v[k], gel);
   }
 }
 
@@ -153,52 +258,67 @@ template <int DT, int VEC, bool OUT>
 __global__ void __launch_bounds__(256)
 geglu_q8_bwd_kernel(const typename Elem<DT>::T* __restrict__ g, const int8_t* __restrict__ q,
                     const uint8_t* __restrict__ ex, typename Elem<DT>::T* __restrict__ du,
-                    typename Elem<DT>::T* __restrict__ out, int64_t items, int F, uint32_t slots) {
+                    typename Elem<DT>::T* __restrict__ out, const Rows r) {
   pdl_enter();
-  const int64_t stride = (int64_t)gridDim.x * blockDim.x;
-  for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < items; i += stride) {
-    const int64_t row = i / slots;
-    const int slot = (int)(i - row * slots), c = slot * kCols, left = F - c;
-    const int64_t at = row * 2 * F + c;
-    const uint8_t* er = ex + (row * slots + slot) / kSlots * 2;
-    float a[kCols], b[kCols], gv[kCols], o[kCols];
-    load_q<VEC>(q + at, left, er[0], a);
-    load_q<VEC>(q + at + F, left, er[1], b);
-    load_cols<DT, VEC>(g + row * F + c, left, gv);
-#pragma unroll
-    for (int k = 0; k < kCols; ++k) {
-      const float s = gate_sigmoid(a[k]), gel = a[k] * s;
-      const float slope = gate_slope(a[k], s);
-      if (OUT) o[k] = gel * b[k];
-      a[k] = gv[k] * b[k] * slope;
-      b[k] = gv[k] * gel;
-    }
-    store_cols<DT, VEC>(du + at, left, a);
-    store_cols<DT, VEC>(du + at + F, left, b);
-    if (OUT) store_cols<DT, VEC>(out + row * F + c, left, o);
+  using T = typename Elem<DT>::T;
+  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x;
+  const Place p(r, i);
+  if (p.left <= 0) return;
+  const Bytes qa = load_q<VEC>(q + p.at, p.left), qb = load_q<VEC>(q + p.at + r.F, p.left);
+  Raw<DT> w;
+  load_raw<T, VEC>(g + p.half, p.left, w.v);
+  const uint32_t e = *reinterpret_cast<const uint16_t*>(ex + i / kSlots * 2);
+  Cols a = dequantise(qa, e & 255u), b = dequantise(qb, e >> 8), o;
+  const Cols gv = w.widen();
+  // values of 2^7 2^(e - 127) and less: their squares stay below 2^127 up to e = 183
+  if (DT == KRSI_F16 || (e & 255u) <= 183u) grad_cols<OUT, false>(a, b, gv, o);
+  else grad_cols<OUT, true>(a, b, gv, o);
+  w.narrow(a);
+  store_raw<T, VEC>(du + p.at, p.left, w.v);
+  w.narrow(b);
+  store_raw<T, VEC>(du + p.at + r.F, p.left, w.v);
+  if (OUT) {
+    w.narrow(o);
+    store_raw<T, VEC>(out + p.half, p.left, w.v);
   }
 }
 
 inline uint32_t slots_of(int64_t F) { return (uint32_t)((F + kGroup - 1) / kGroup * kSlots); }
-
-inline dim3 grid_of(int64_t items) { return dim3((unsigned)std::min<int64_t>((items + 255) / 256, 1 << 22)); }
+// A launch takes at most this many rows, so that its items fit 31 bits.
+inline int64_t rows_per_launch(int64_t F) { return ((int64_t)1 << 31) / slots_of(F) - 1; }
+inline Rows rows_of(int64_t rows, int64_t F) {
+  Rows r;
+  r.slots = slots_of(F);
+  r.items = (uint32_t)rows * r.slots;
+  r.F = (int)F;
+  r.shift = 0;
+  while (((uint64_t)1 << r.shift) < r.slots) ++r.shift;
+  r.mul = (uint32_t)((((uint64_t)1 << (32 + r.shift)) + r.slots - 1) / r.slots - ((uint64_t)1 << 32));
+  return r;
+}
 
 template <int DT, int VEC>
 int fwd(const void* u, void* out, void* q, void* ex, int64_t rows, int64_t F, cudaStream_t stream) {
   using T = typename Elem<DT>::T;
-  const int64_t items = rows * slots_of(F);
-  KRSI_CUDA_TRY(launch_pdl(geglu_q8_fwd_kernel<DT, VEC>, grid_of(items), dim3(256), 0, stream, (const T*)u, (T*)out,
-                           (int8_t*)q, (uint8_t*)ex, items, (int)F, slots_of(F)));
+  for (int64_t r0 = 0; r0 < rows; r0 += rows_per_launch(F)) {
+    const Rows r = rows_of(std::min(rows - r0, rows_per_launch(F)), F);
+    KRSI_CUDA_TRY(launch_pdl(geglu_q8_fwd_kernel<DT, VEC>, dim3((r.items + 255) / 256), dim3(256), 0, stream,
+                             (const T*)u + r0 * 2 * F, (T*)out + r0 * F, q ? (int8_t*)q + r0 * 2 * F : nullptr,
+                             (uint8_t*)ex + r0 * (r.slots / kSlots) * 2, r));
+  }
   return KRSI_OK;
 }
 template <int DT, int VEC>
 int bwd(const void* g, const void* q, const void* ex, void* du, void* out, int64_t rows, int64_t F,
         cudaStream_t stream) {
   using T = typename Elem<DT>::T;
-  const int64_t items = rows * slots_of(F);
   auto kern = out ? geglu_q8_bwd_kernel<DT, VEC, true> : geglu_q8_bwd_kernel<DT, VEC, false>;
-  KRSI_CUDA_TRY(launch_pdl(kern, grid_of(items), dim3(256), 0, stream, (const T*)g, (const int8_t*)q,
-                           (const uint8_t*)ex, (T*)du, (T*)out, items, (int)F, slots_of(F)));
+  for (int64_t r0 = 0; r0 < rows; r0 += rows_per_launch(F)) {
+    const Rows r = rows_of(std::min(rows - r0, rows_per_launch(F)), F);
+    KRSI_CUDA_TRY(launch_pdl(kern, dim3((r.items + 255) / 256), dim3(256), 0, stream, (const T*)g + r0 * F,
+                             (const int8_t*)q + r0 * 2 * F, (const uint8_t*)ex + r0 * (r.slots / kSlots) * 2,
+                             (T*)du + r0 * 2 * F, out ? (T*)out + r0 * F : nullptr, r));
+  }
   return KRSI_OK;
 }
 
@@ -244,6 +364,7 @@ extern "C" int krsi_geglu_q8_fwd(const void* u, void* out, void* q, void* expone
   if (rc != KRSI_OK) return rc;
   if (rows == 0 || F == 0) return KRSI_OK;
   KRSI_CHECK_ARG(u && out && (q != nullptr) == (exponents != nullptr));
+  if (bits_of(exponents) % 2 != 0) return KRSI_ERR_MISALIGNED;
   const int es = dtype == KRSI_F32 ? 4 : 2;
   const int vec = access_cols(F, es, bits_of(u) | bits_of(out), bits_of(q));
   KRSI_Q8_DISPATCH(fwd, vec, u, out, q, exponents, rows, F, stream)
@@ -255,6 +376,7 @@ extern "C" int krsi_geglu_q8_bwd(const void* g, const void* q, const void* expon
   if (rc != KRSI_OK) return rc;
   if (rows == 0 || F == 0) return KRSI_OK;
   KRSI_CHECK_ARG(g && q && exponents && du);
+  if (bits_of(exponents) % 2 != 0) return KRSI_ERR_MISALIGNED;
   const int es = dtype == KRSI_F32 ? 4 : 2;
   const int vec = access_cols(F, es, bits_of(g) | bits_of(du) | bits_of(out), bits_of(q));
   KRSI_Q8_DISPATCH(bwd, vec, g, q, exponents, du, out, rows, F, stream)

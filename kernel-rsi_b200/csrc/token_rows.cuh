@@ -2,9 +2,9 @@
 // (embedding.cu) and the targets' part of the vocabulary projection's gradient (linear_ce.cu):
 //   out[v] (+)= sum over the positions i with token v of weight[i] * g[i]
 //
-// The sum of the rows of one token has to be the same on every run, so it is taken in position order:
-// the positions are sorted by token first (token_sort, stable), then cut into chunks of kChunkRows
-// sorted entries, each summed by one block.  A token whose run lies inside one chunk is finished there;
+// The sum of the rows of one token has to be the same on every run, so it is taken in a fixed order: the
+// positions are sorted by token first (token_sort), then cut into chunks of kChunkRows sorted entries,
+// each summed by one block.  A token whose run lies inside one chunk is finished there;
 // a run that crosses chunks leaves one partial row per chunk, which a second kernel adds in chunk order.
 #pragma once
 #include <algorithm>
@@ -14,7 +14,7 @@
 namespace krsi {
 namespace tokens {
 
-constexpr int kChunkRows = 32;
+constexpr int kChunkRows = 16;
 
 inline int64_t chunks_of(int64_t n) { return (n + kChunkRows - 1) / kChunkRows; }
 
@@ -25,7 +25,7 @@ struct Order {
   int range;   // tokens per group
   __host__ __device__ __forceinline__ int key(int v) const { return (v & ((1 << bits) - 1)) * range + (v >> bits); }
 };
-constexpr int kMaxRange = 1024;
+constexpr int kMaxRange = 512;
 inline Order order_of(int64_t V) {
   Order o{7, 0};   // 128 groups, more where a group would pass kMaxRange tokens
   while (((V - 1) >> o.bits) + 1 > kMaxRange) ++o.bits;
@@ -33,8 +33,8 @@ inline Order order_of(int64_t V) {
   return o;
 }
 
-// The positions of tokens[0, n) sorted by token (in Order, equal tokens in position order), those outside
-// [0, V) and those equal to `skip` left out:
+// The positions of tokens[0, n) sorted by token (in Order; equal tokens in an order that depends on n
+// alone), those outside [0, V) and those equal to `skip` left out:
 //   start[key(v)] .. start[key(v) + 1]   the sorted entries of token v (start[end] = their number, end being
 //                                        groups * range)
 //   pos[i], tok[i]                       position and token of sorted entry i
@@ -73,12 +73,33 @@ struct alignas(sizeof(T) * VEC) Pack {
   T v[VEC];
 };
 
-// Blocks [0, chunks) sum one chunk of sorted entries each, one packet of columns per thread; the blocks
-// after them (if the grid has any) write the rows of tokens that do not occur, kZeroTokens tokens each.
+// A thread's own packet from global to shared memory, asynchronously where the copy instruction exists
+// for its width (4 bytes and more).  Only the thread that copied a packet reads it back, so waiting for
+// its own copies is all the synchronisation there is.
+template <typename P>
+__device__ __forceinline__ void copy_packet(P* dst, const P* src) {
+  if constexpr (sizeof(P) == 16)
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                 : "memory");
+  else if constexpr (sizeof(P) >= 4)
+    asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                 "n"(sizeof(P))
+                 : "memory");
+  else
+    *dst = *src;
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
+
+// The first blocks (if `chunks` is less than the grid) write the rows of tokens that do not occur,
+// kZeroTokens tokens each; the last `chunks` blocks sum one chunk of sorted entries each, one packet of
+// columns per thread.  A chunk's rows are staged in shared memory, all of its loads in flight at once: held
+// in registers they cost so many that a third as much was in flight (measured: SUM_STAGED).
 // Out: packet(v, c, sums) takes the VEC finished sums of token v's packet c, zero(v, c) an absent one,
 // column(v, col, sum) one finished column.
-constexpr int kRowsAhead = 8;     // rows of a chunk whose loads are in flight together
-constexpr int kZeroTokens = 64;
+constexpr int kZeroTokens = 32;
+constexpr int kGroupRows = 4;     // rows per group of copies
 
 template <int DT, int VEC, bool WEIGHTED, typename Out>
 __global__ void __launch_bounds__(256)
@@ -89,19 +110,20 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
   using E = Elem<DT>;
   using P = Pack<typename E::T, VEC>;
   const uint32_t c = blockIdx.y * blockDim.x + threadIdx.x;
-  if ((int)blockIdx.x >= chunks) {
-    const int v0 = ((int)blockIdx.x - chunks) * kZeroTokens;
-    for (int v = v0; v < v0 + kZeroTokens && v < V; ++v) {
-      const int k = order.key(v);
-      if (start[k] == start[k + 1] && c < packets) out.zero(v, c);
-    }
+  const int chunk = (int)blockIdx.x - ((int)gridDim.x - chunks);
+  if (chunk < 0) {
+    const int v0 = (int)blockIdx.x * kZeroTokens, v = v0 + (int)(threadIdx.x % 32);
+    const int k = v < V ? order.key(v) : 0;
+    unsigned absent = __ballot_sync(0xffffffffu, v < V && start[k] == start[k + 1]);
+    if (c < packets)
+      for (; absent != 0; absent &= absent - 1) out.zero(v0 + __ffs(absent) - 1, c);
     return;
   }
-  const int chunk = blockIdx.x;
-  const int i0 = chunk * kChunkRows, m = min(kChunkRows, start[order.range << order.bits] - i0);   // the entries of this chunk
-  if (m <= 0) return;
+  const int i0 = chunk * kChunkRows;
   __shared__ int s_pos[kChunkRows], s_tok[kChunkRows + 1];
   __shared__ float s_weight[kChunkRows];
+  const int m = min(kChunkRows, start[order.range << order.bits] - i0);   // the entries of this chunk
+  if (m <= 0) return;
   if (threadIdx.x < m) {
     const int p = pos[i0 + threadIdx.x];
     s_pos[threadIdx.x] = p;
@@ -111,24 +133,25 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
   if (threadIdx.x == 0) s_tok[m] = -1;   // the chunk's end ends a run
   __syncthreads();
   if (c >= packets) return;
+  extern __shared__ __align__(16) unsigned char stage_raw[];
+  P* stage = reinterpret_cast<P*>(stage_raw) + threadIdx.x;   // [kChunkRows][blockDim.x]
+  const P* gp = reinterpret_cast<const P*>(g) + c;
+#pragma unroll
+  for (int j = 0; j < kChunkRows; ++j) {
+    if (j < m) copy_packet(stage + j * blockDim.x, gp + (int64_t)s_pos[j] * packets);
+    if (j % kGroupRows == kGroupRows - 1) copy_commit();
+  }
   const bool from_before = start[order.key(s_tok[0])] < i0, goes_on = start[order.key(s_tok[m - 1]) + 1] > i0 + m;
-  const P* gp = reinterpret_cast<const P*>(g);
   float acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
   bool first_run = true;
-  for (int j0 = 0; j0 < m; j0 += kRowsAhead) {
-    P r[kRowsAhead];
-#pragma unroll
-    for (int k = 0; k < kRowsAhead; ++k)
-      if (j0 + k < m) r[k] = gp[(int64_t)s_pos[j0 + k] * packets + c];
-#pragma unroll
-    for (int k = 0; k < kRowsAhead; ++k) {
-      const int j = j0 + k;
-      if (j >= m) break;
+  auto add_group = [&](int j0) {
+    for (int j = j0; j < j0 + kGroupRows && j < m; ++j) {
+      const P r = stage[j * blockDim.x];
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
-        acc[e] = WEIGHTED ? fmaf(s_weight[j], E::load(r[k].v[e]), acc[e]) : acc[e] + E::load(r[k].v[e]);
+        acc[e] = WEIGHTED ? fmaf(s_weight[j], E::load(r.v[e]), acc[e]) : acc[e] + E::load(r.v[e]);
       if (s_tok[j + 1] == s_tok[j]) continue;
       // the run of s_tok[j] ends here (or goes on in the next chunk): a run that began in an earlier
       // chunk is that chunk's to finish (partial row 2 chunk), one that goes on is this chunk's
@@ -144,7 +167,16 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
 #pragma unroll
       for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
     }
-  }
+  };
+  static_assert(kChunkRows == 4 * kGroupRows, "four groups of copies");
+  copy_wait<3>();
+  add_group(0);
+  copy_wait<2>();
+  add_group(kGroupRows);
+  copy_wait<1>();
+  add_group(2 * kGroupRows);
+  copy_wait<0>();
+  add_group(3 * kGroupRows);
 }
 
 // The rows of runs that cross chunks, for 128 columns a block.  Each of the block's warps looks at one
@@ -152,7 +184,7 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
 // in chunk order.  Up to kShortRun of them the warp adds alone; a longer run is left to the whole block,
 // whose warps add contiguous shares, in order, and then their sums in warp order.
 constexpr int kJoinWarps = 8;
-constexpr int kShortRun = 32;
+constexpr int kShortRun = 16;
 
 template <typename Out>
 __global__ void __launch_bounds__(32 * kJoinWarps)
@@ -165,7 +197,7 @@ join_rows_kernel(const int* __restrict__ start, const int* __restrict__ tok, con
   auto add = [&](int chunk, int k0, int k1, float* acc) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) acc[j] = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int k = k0; k < k1; ++k) {
       const float* row = partial + (int64_t)(2 * (chunk + k) + (k == 0 ? 1 : 0)) * d;
 #pragma unroll
@@ -225,8 +257,12 @@ cudaError_t sum_by_token(const void* g, const float* weight, const Space& s, con
   const int chunks = (int)chunks_of(n);
   const int64_t zero_blocks = zeros ? (V + kZeroTokens - 1) / kZeroTokens : 0;
   const dim3 grid((unsigned)(chunks + zero_blocks), (packets + threads - 1) / threads);
-  cudaError_t e = launch_pdl(sum_rows_kernel<DT, VEC, WEIGHTED, Out>, grid, dim3(threads), 0, stream, (const T*)g,
-                             weight, (const int*)s.start, (const int*)s.pos, (const int*)s.tok, s.partial, out, s.order, chunks,
+  const size_t smem = (size_t)kChunkRows * threads * VEC * sizeof(T);   // at most 64 KB
+  auto kern = sum_rows_kernel<DT, VEC, WEIGHTED, Out>;
+  cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kChunkRows * 256 * 16);
+  if (e != cudaSuccess) return e;
+  e = launch_pdl(kern, grid, dim3(threads), smem, stream, (const T*)g, weight,
+                 (const int*)s.start, (const int*)s.pos, (const int*)s.tok, s.partial, out, s.order, chunks,
                              (int)V, packets);
   if (e != cudaSuccess || chunks == 1) return e;
   const dim3 join_grid((unsigned)((chunks - 1 + kJoinWarps - 1) / kJoinWarps), (unsigned)((d + 127) / 128));

@@ -120,6 +120,18 @@ def test_large_gates_saturate():
     assert out[5] == u[0, 5].cpu() and out[6] == 0
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_gradient_of_huge_gates(dtype):
+    """Gates whose square overflows fp32: the slope is 1 or 0 there, not 0 times infinity."""
+    F = 32
+    u = torch.ones(4, 2 * F)
+    for r, big in enumerate((3e19, -3e19, 3e38, -3e38)):
+        u[r, :F] = big
+    x = u.to(dev, dtype).requires_grad_(True)
+    (du,) = torch.autograd.grad(geglu_q8(x), x, torch.ones(4, F, device=dev, dtype=dtype))
+    assert torch.equal(du[:, :F].cpu(), torch.tensor([1.0, 0, 1, 0], dtype=dtype)[:, None].expand(4, F))
+
+
 def test_autograd_and_compile():
     u, g = inputs(40, 96, torch.bfloat16, 3)
     x = u.to(dev).requires_grad_(True)
