@@ -239,18 +239,20 @@ int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, int mode, siz
 
 /* loss: [N] fp32.  reduced: two floats or null: the sum of the losses (mean: divided by the number of
  * rows that are not ignored, at least 1) and the weight of one row in it (1, or one over that number).
+ * stats: [N, 2] fp32 for krsi_linear_ce_grad (8-byte aligned), or null.
  * dx, dw: null, or fp32 gradients of the sum of the losses without the factor `scale`, for
  * krsi_linear_ce_finish: the logits are computed once for loss and gradients. */
 int krsi_linear_ce_fwd(const void* x, const void* w, const void* targets, int target_bits, float* loss,
-                       float* reduced, float* dx, float* dw, void* workspace, size_t workspace_bytes, int64_t N,
-                       int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss, int mean,
+                       float* reduced, float* stats, float* dx, float* dw, void* workspace,
+                       size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss, int mean,
                        int dtype, cudaStream_t stream);
 
 /* Gradients for the upstream gradient g of each row's loss (fp32, stride 1, or 0: one for all rows), times
- * *weight where that is not null.  dx, dw: of `dtype`, one of them may be null. */
+ * *weight where that is not null, from the stats of krsi_linear_ce_fwd on the same operands (the logits
+ * are computed again).  dx, dw: of `dtype`, one of them may be null. */
 int krsi_linear_ce_grad(const void* x, const void* w, const void* targets, int target_bits, const float* g,
-                        int64_t g_stride, const float* weight, void* dx, void* dw, void* workspace,
-                        size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index,
+                        int64_t g_stride, const float* weight, const float* stats, void* dx, void* dw,
+                        void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index,
                         float z_loss, int dtype, cudaStream_t stream);
 
 /* out = scale * *g * *weight * grad, rounded once (g, weight: device scalars or null); n a multiple of 8. */

@@ -252,6 +252,11 @@ __device__ __forceinline__ uint8_t* aligned_smem(uint8_t* raw) {
   return reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~uintptr_t(1023));
 }
 
+template <typename I>
+__device__ __forceinline__ int target_code(I t, long long ignore, int V) {
+  return (long long)t == ignore ? kIgnored : (t >= 0 && t < (I)V) ? (int)t : kInvalid;
+}
+
 // ---------------------------------------------------------------- 1: targets
 // One warp per row: t_i (kIgnored, kInvalid or the token) and the target's logit in log2 units.  An
 // invalid target makes the row's loss and gradients NaN (an error that cannot be raised without a
@@ -268,7 +273,7 @@ ce_target_kernel(const typename Elem<DT>::T* __restrict__ x, const typename Elem
   if (row >= n) return;
   if (row % (2 * kBM) == 0 && lane == 0) marked[row / (2 * kBM)] = 0;
   const long long t = (long long)targets[row];
-  const int code = t == ignore ? kIgnored : (t >= 0 && t < V) ? (int)t : kInvalid;
+  const int code = target_code(t, ignore, V);
   float dot = 0.f;
   if (code >= 0) {
     const T* xr = x + (int64_t)row * K;
@@ -445,12 +450,9 @@ struct JoinArgs {
   const int* tgt;
   const float* l2t;
   const float* l2t_low;    // the exact target's logit less l2t
-  const float* g;          // gradient of each row's loss (stride g_stride), null: 1
-  int64_t g_stride;
-  const float* weight;     // a factor of g for all rows, null: 1
-  const float* g_top;      // f16: the largest |g| in use, null: 1
-  float* loss;             // [rows], or null
-  float* coef;             // [rows]: the target's term of dl; null: loss alone
+  float* loss;             // [rows]
+  float2* stats;           // [rows]: (log2-sum-exp, 1 - p_t) for ce_rows_kernel, or null
+  float* coef;             // [rows]: the target's term of dl; null: no gradients
   float* factor;           // [rows]: of the row's softmax part of dx
   float* ref;              // [rows]: the second pass's reference
   int* marked;
@@ -461,11 +463,82 @@ struct JoinArgs {
   float e_scale, z;
 };
 
-// The power of two above the largest |g|: row factors are divided by it before they meet 16 bits.
-__device__ __forceinline__ float g_unit(const float* g_top) {
-  if (g_top == nullptr) return 1.f;
-  const uint32_t e = __float_as_uint(*g_top) & 0x7f800000u;
-  return e == 0u || e >= 0x7f000000u ? 1.f : 2.f * __uint_as_float(e);
+// The upstream gradient of the rows' losses.
+struct Upstream {
+  const float* g;          // per row (stride 1) or one (stride 0); null: 1
+  int64_t stride;
+  const float* weight;     // a factor of g for all rows, or null
+  const float* top;        // f16 and one g per row: the largest |g weight|
+  int scaled;              // f16: row factors are divided by unit() before they meet 16 bits
+  __device__ __forceinline__ float of(int64_t row) const { return g ? g[row * stride] * (weight ? *weight : 1.f) : 1.f; }
+  // The power of two above the largest |g weight|.
+  __device__ __forceinline__ float unit() const {
+    if (!scaled || g == nullptr) return 1.f;
+    const uint32_t e = __float_as_uint(top ? *top : of(0)) & 0x7f800000u;
+    return e == 0u || e >= 0x7f000000u ? 1.f : 2.f * __uint_as_float(e);
+  }
+};
+
+// A row's x times a factor, in 16 bits (zeros where `dead`): `ahead` holds the first packets.
+constexpr int kAhead = 5;
+template <int DT>
+struct RowCopy {
+  using T = typename Elem<DT>::T;
+  Vec16<T> ahead[kAhead];
+  __device__ __forceinline__ void fetch(const T* x, int K, int lane) {
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (lane * 8 + j * 256 < K) ahead[j] = ldg16(x + lane * 8 + j * 256);
+  }
+  __device__ __forceinline__ void write(const T* x, T* out, int K, int lane, float f, bool dead) const {
+    auto put = [&](int k, Vec16<T> v) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v.v[e] = Elem<DT>::store(dead ? 0.f : f * Elem<DT>::load(v.v[e]));
+      stg16(out + k, v);
+    };
+#pragma unroll
+    for (int j = 0; j < kAhead; ++j)
+      if (lane * 8 + j * 256 < K) put(lane * 8 + j * 256, ahead[j]);
+    for (int k = lane * 8 + kAhead * 256; k < K; k += 256) put(k, ldg16(x + k));
+  }
+};
+
+// What the gradients need of each row where its log-sum-exp is known from the forward (one warp per row):
+// the target, the factors and x'; e will be e_scale p.
+struct RowsArgs {
+  const void* targets;
+  const float2* stats;     // (log2-sum-exp, 1 - p_t)
+  Upstream up;
+  int64_t row0;            // of the chunk, for g
+  int* tgt;
+  float *coef, *factor, *ref;
+  const void* x;
+  void* xs;
+  int rows, V, K;
+  long long ignore;
+  float e_scale, z;
+};
+template <int DT, typename I>
+__global__ void __launch_bounds__(256)
+ce_rows_kernel(const RowsArgs a) {
+  pdl_enter();
+  using T = typename Elem<DT>::T;
+  const int row = (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32), lane = threadIdx.x % 32;
+  if (row >= a.rows) return;
+  RowCopy<DT> copy;
+  const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.K;
+  copy.fetch(xr, a.K, lane);
+  const int t = target_code(reinterpret_cast<const I*>(a.targets)[row], a.ignore, a.V);
+  const bool dead = t == kIgnored;
+  const float2 st = a.stats[row];
+  const float r = a.up.of(a.row0 + row), zl = 2.f * a.z * st.x * kLn2, soft = r * (1.f + zl);
+  if (lane == 0) {
+    a.tgt[row] = t;
+    a.coef[row] = dead ? 0.f : r * (zl * (1.f - st.y) - st.y);
+    a.factor[row] = dead ? 0.f : soft / a.e_scale;
+    a.ref[row] = st.x;
+  }
+  copy.write(xr, reinterpret_cast<T*>(a.xs) + (int64_t)row * a.K, a.K, lane, soft / a.up.unit(), dead);
 }
 
 template <int DT>
@@ -480,13 +553,8 @@ ce_join_kernel(const JoinArgs a) {
   const float l2t = a.l2t[row];
   const float2* pr = a.part + (int64_t)row * a.n_part;
   const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.K;
-  constexpr int kAhead = 5;   // packets of the row on their way while the sums are added
-  Vec16<T> xv[kAhead];
-  if (a.coef != nullptr) {
-#pragma unroll
-    for (int j = 0; j < kAhead; ++j)
-      if (lane * 8 + j * 256 < a.K) xv[j] = ldg16(xr + lane * 8 + j * 256);
-  }
+  RowCopy<DT> copy;        // on its way while the sums are added
+  if (a.coef != nullptr) copy.fetch(xr, a.K, lane);
   float s = 0.f, top = l2t;
   bool lifted = !(l2t == l2t);
 #pragma unroll 8
@@ -517,34 +585,21 @@ ce_join_kernel(const JoinArgs a) {
     rest = 1.f - pt;
   }
   const float lse = lse2 * kLn2;
-  if (lane == 0 && a.loss != nullptr) {
+  if (lane == 0) {
     const float nll = t == kIgnored ? 0.f : lifted ? (lse2 - l2t) * kLn2 : log1pf(s);
     a.loss[row] = t == kIgnored ? 0.f : nll + a.z * lse * lse;
+    if (a.stats != nullptr) a.stats[row] = make_float2(lse2, rest);
   }
   if (a.coef == nullptr) return;
-  float r = a.g ? a.g[row * a.g_stride] : 1.f;
-  if (a.weight) r *= *a.weight;
-  const bool second = a.all_second != 0 || lifted;
-  const float soft = r * (1.f + 2.f * a.z * lse) * (second ? 1.f : pt);
-  const float unit = g_unit(a.g_top);
-  const bool dead = t == kIgnored;
+  const bool second = a.all_second != 0 || lifted, dead = t == kIgnored;
+  const float soft = (1.f + 2.f * a.z * lse) * (second ? 1.f : pt);
   if (lane == 0) {
-    a.coef[row] = dead ? 0.f : r * (2.f * a.z * lse * pt - rest);
+    a.coef[row] = dead ? 0.f : 2.f * a.z * lse * pt - rest;
     a.factor[row] = dead ? 0.f : soft / a.e_scale;
     a.ref[row] = second ? lse2 : l2t;
     if (lifted && !dead) a.marked[row / (2 * kBM)] = 1;   // every writer writes the same
   }
-  const float f = soft / unit;
-  T* xo = reinterpret_cast<T*>(a.xs) + (int64_t)row * a.K;
-  auto put = [&](int k, Vec16<T> v) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v.v[e] = E::store(dead ? 0.f : f * E::load(v.v[e]));
-    stg16(xo + k, v);
-  };
-#pragma unroll
-  for (int j = 0; j < kAhead; ++j)
-    if (lane * 8 + j * 256 < a.K) put(lane * 8 + j * 256, xv[j]);
-  for (int k = lane * 8 + kAhead * 256; k < a.K; k += 256) put(k, ldg16(xr + k));
+  copy.write(xr, reinterpret_cast<T*>(a.xs) + (int64_t)row * a.K, a.K, lane, soft, dead);
 }
 
 // The reduced loss and the weight of each row in it, one block, in a fixed order.
@@ -584,15 +639,16 @@ ce_reduce_kernel(const float* __restrict__ loss, const int* __restrict__ tgt, fl
 }
 
 // The largest |g weight| over the rows that are not ignored (a fixed result whatever the order).
+template <typename I>
 __global__ void __launch_bounds__(1024)
-ce_gtop_kernel(const float* __restrict__ g, int64_t g_stride, const float* __restrict__ weight,
-               const int* __restrict__ tgt, float* __restrict__ out, int n) {
+ce_gtop_kernel(const float* __restrict__ g, const float* __restrict__ weight, const I* __restrict__ targets,
+               long long ignore, float* __restrict__ out, int n) {
   pdl_enter();
   __shared__ float tops[32];
   float m = 0.f;
 #pragma unroll 8
   for (int i = threadIdx.x; i < n; i += 1024)
-    if (tgt[i] != kIgnored) m = fmaxf(m, fabsf(g[i * g_stride]));
+    if ((long long)targets[i] != ignore) m = fmaxf(m, fabsf(g[i]));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = m;
@@ -625,8 +681,8 @@ struct GradArgs {
   const float* base;
   const int* start;
   tokens::Order order;
-  const float* g_top;
-  float alpha;             // of the dw sums
+  Upstream up;
+  float alpha;             // of the dw sums, times up.unit()
   float scale;
   uint32_t limit;
 };
@@ -732,7 +788,7 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
         r.add_at = -1;
         if (row >= (m.is_dx ? a.rows : a.V)) return r;
         if (!m.is_dx) {
-          r.mul = a.alpha * g_unit(a.g_top);
+          r.mul = a.alpha * a.up.unit();
           if (a.base) {
             const int k = a.order.key(row);
             if (a.start[k] < a.start[k + 1]) r.add_at = (int64_t)row * a.K;
@@ -1003,16 +1059,16 @@ inline bool make_panel_map(CUtensorMap* map, const void* base, int64_t rows, int
 // Sizes of one call.
 struct Plan {
   int64_t N, V, K;
-  bool grads, direct;      // gradients wanted; dw leaves the GEMM in 16 bits
-  bool dw_space;           // the workspace holds fp32 rows of dw
+  bool grads, known;       // gradients wanted; from known log-sum-exps (krsi_linear_ce_grad)
+  bool direct;             // dw leaves the GEMM in 16 bits
   int64_t n_vt, panels;    // vocabulary tiles; panels of e
   int64_t chunk, chunks;   // rows per chunk (a multiple of 256)
   int cols, n_ct;
   int64_t splits;          // of dx over the vocabulary
 };
 
-inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool out32, int pairs) {
-  Plan p{N, V, K, grads};
+inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool known, int pairs) {
+  Plan p{N, V, K, grads, known};
   p.n_vt = ceil_div(V, kBN);
   p.panels = ceil_div(V, 64);
   // At most 2^28 logits a chunk (512 MB of e), in chunks of equal size; the loss alone keeps none.
@@ -1020,8 +1076,7 @@ inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool out32, i
   p.chunks = grads ? std::max<int64_t>(1, ceil_div(N, most)) : 1;
   p.chunk = std::max<int64_t>(256, ceil_div(ceil_div(N, p.chunks), 256) * 256);
   p.chunks = std::max<int64_t>(1, ceil_div(N, p.chunk));
-  p.direct = !out32 && p.chunks == 1;
-  p.dw_space = !out32;
+  p.direct = known && p.chunks == 1;
   // Column tiles of K.  Per K block of 64 a pair's tensor cores take 2 cycles a column, and its operands
   // (16 KB of A and 64 B a column of B for each CTA) come from L2 at about 50 bytes a cycle and SM, as
   // measured on the logits' tiles, so wider tiles feed the tensor cores better.  Up to 256 columns two
@@ -1069,7 +1124,7 @@ inline Space space_at(void* base, const Plan& p) {
   s.l2t = reinterpret_cast<float*>(take((size_t)p.N * 4));
   s.l2t_low = reinterpret_cast<float*>(take((size_t)p.N * 4));
   s.marked = reinterpret_cast<int*>(take((size_t)(p.N / 256 + 1) * 4));
-  s.part = reinterpret_cast<float2*>(take((size_t)rows * 2 * p.n_vt * 8));
+  s.part = reinterpret_cast<float2*>(p.known ? 0 : take((size_t)rows * 2 * p.n_vt * 8));
   if (p.grads) {
     s.coef = reinterpret_cast<float*>(take((size_t)p.N * 4));
     s.factor = reinterpret_cast<float*>(take((size_t)p.N * 4));
@@ -1077,7 +1132,7 @@ inline Space space_at(void* base, const Plan& p) {
     s.g_top = reinterpret_cast<float*>(take(4));
     s.e = reinterpret_cast<void*>(take((size_t)rows * p.panels * 128));
     s.xs = reinterpret_cast<void*>(take((size_t)rows * p.K * 2));
-    s.dw32 = reinterpret_cast<float*>(p.dw_space ? take((size_t)p.V * p.K * 4) : 0);
+    s.dw32 = reinterpret_cast<float*>(p.known ? take((size_t)p.V * p.K * 4) : 0);
     s.dx_part = reinterpret_cast<float*>(p.splits > 1 ? take((size_t)p.splits * p.chunk * p.K * 4) : 0);
     const size_t sort_off = off;
     s.sorted = tokens::space_at(reinterpret_cast<void*>(at + sort_off), p.N, p.V, p.K);
@@ -1090,15 +1145,15 @@ inline Space space_at(void* base, const Plan& p) {
 struct Call {
   const void *x, *w, *targets;
   int target_bits;
-  float* loss;             // [N] rows
+  float* loss;             // [N] rows: the forward; null: gradients from stats
   float* reduced;          // (loss, weight) or null
   int mean;
+  float2* stats;           // [N]: written by the forward (or null), read by the gradients
   const float* g;
   int64_t g_stride;
   const float* weight;
   void* dx;                // null: no gradients
   void* dw;
-  bool out32;              // dx and dw are fp32, without `scale`
   float scale, z;
   int64_t ignore;
 };
@@ -1111,22 +1166,29 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   const T* x = static_cast<const T*>(c.x);
   const T* w = static_cast<const T*>(c.w);
   const int N = (int)p.N, V = (int)p.V, K = (int)p.K;
+  const bool known = c.loss == nullptr;   // the rows' log-sum-exps
+  const bool wide = c.target_bits == 64;
   const dim3 row_grid((unsigned)ceil_div(N, 8));
-  if (c.target_bits == 64)
-    KRSI_CUDA_TRY(launch_pdl(ce_target_kernel<DT, long long>, row_grid, dim3(256), 0, stream, x, w,
-                             (const long long*)c.targets, s.tgt, s.l2t, s.l2t_low, s.marked, N, V, K, (long long)c.ignore, c2));
-  else
-    KRSI_CUDA_TRY(launch_pdl(ce_target_kernel<DT, int>, row_grid, dim3(256), 0, stream, x, w, (const int*)c.targets,
-                             s.tgt, s.l2t, s.l2t_low, s.marked, N, V, K, (long long)c.ignore, c2));
-  const float* g_top = nullptr;
-  if (F16 && p.grads && c.g) {
-    KRSI_CUDA_TRY(launch_pdl(ce_gtop_kernel, dim3(1), dim3(1024), 0, stream, c.g, c.g_stride, c.weight,
-                             (const int*)s.tgt, s.g_top, N));
-    g_top = s.g_top;
+  Upstream up{c.g, c.g_stride, c.weight, nullptr, F16};
+  if (!known) {
+    auto kern = [&](auto k, auto* t) {
+      return launch_pdl(k, row_grid, dim3(256), 0, stream, x, w, t, s.tgt, s.l2t, s.l2t_low, s.marked, N, V, K,
+                        (long long)c.ignore, c2);
+    };
+    KRSI_CUDA_TRY(wide ? kern(ce_target_kernel<DT, long long>, (const long long*)c.targets)
+                       : kern(ce_target_kernel<DT, int>, (const int*)c.targets));
+  } else if (F16 && c.g_stride == 1) {
+    auto kern = [&](auto k, auto* t) {
+      return launch_pdl(k, dim3(1), dim3(1024), 0, stream, c.g, c.weight, t, (long long)c.ignore, s.g_top, N);
+    };
+    KRSI_CUDA_TRY(wide ? kern(ce_gtop_kernel<long long>, (const long long*)c.targets)
+                       : kern(ce_gtop_kernel<int>, (const int*)c.targets));
+    up.top = s.g_top;
   }
   const float e_scale = F16 ? kHalfScale : 1.f;
   if (p.grads && c.dw)
-    KRSI_CUDA_TRY(tokens::token_sort(s.tgt, 32, N, V, -1, s.sorted.start, s.sorted.pos, s.sorted.tok, stream));
+    KRSI_CUDA_TRY(tokens::token_sort(c.targets, c.target_bits, N, V, c.ignore, s.sorted.start, s.sorted.pos,
+                                     s.sorted.tok, stream));
 
   CUtensorMap wk, wm;
   const auto sw128 = CU_TENSOR_MAP_SWIZZLE_128B;
@@ -1134,7 +1196,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     return KRSI_ERR_CUDA;
   // The targets' part of dw: with a direct dw first, as fp32 rows of the tokens that occur, which the
   // GEMM's epilogue adds; otherwise after the chunks, added to the fp32 dw.
-  float* dw32 = c.out32 ? static_cast<float*>(c.dw) : s.dw32;
+  float* dw32 = known ? s.dw32 : static_cast<float*>(c.dw);
   const DwRows dw_rows{dw32, p.K, p.direct ? 0 : 1};
   CUtensorMap dwm = wm;
   if (c.dw && !(p.direct ? make_map(&dwm, c.dw, V, K, K, F16, 16, 32, CU_TENSOR_MAP_SWIZZLE_32B)
@@ -1165,38 +1227,56 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     la.store = p.grads && !F16;
     la.limit = kSpinLimit;
     const int logit_pairs = (int)std::min<int64_t>(pairs, (int64_t)la.n_rt * la.n_vt);
-    KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, logit_pairs, stream, xm, wk, es, la));
-
-    JoinArgs ja{};
-    ja.part = s.part;
-    ja.n_part = 2 * (int)p.n_vt;
-    ja.tgt = s.tgt + r0;
-    ja.l2t = s.l2t + r0;
-    ja.l2t_low = s.l2t_low + r0;
-    ja.g = c.g ? c.g + r0 * c.g_stride : nullptr;
-    ja.g_stride = c.g_stride;
-    ja.weight = c.weight;
-    ja.g_top = g_top;
-    ja.loss = c.loss ? c.loss + r0 : nullptr;
-    ja.rows = (int)rows;
-    ja.K = K;
-    ja.all_second = F16;
-    ja.e_scale = e_scale;
-    ja.z = c.z;
-    if (p.grads) {
-      ja.coef = s.coef + r0;
-      ja.factor = s.factor + r0;
-      ja.ref = s.ref + r0;
-      ja.marked = s.marked + r0 / 256;
-      ja.xs = s.xs;
-      ja.x = xc;
+    if (known) {
+      RowsArgs ra{};
+      ra.targets = static_cast<const char*>(c.targets) + r0 * (c.target_bits / 8);
+      ra.stats = c.stats + r0;
+      ra.up = up;
+      ra.row0 = r0;
+      ra.tgt = s.tgt + r0;
+      ra.coef = s.coef + r0;
+      ra.factor = s.factor + r0;
+      ra.ref = s.ref + r0;
+      ra.x = xc;
+      ra.xs = s.xs;
+      ra.rows = (int)rows;
+      ra.V = V;
+      ra.K = K;
+      ra.ignore = (long long)c.ignore;
+      ra.e_scale = e_scale;
+      ra.z = c.z;
+      KRSI_CUDA_TRY(launch_pdl(wide ? ce_rows_kernel<DT, long long> : ce_rows_kernel<DT, int>,
+                               dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ra));
+    } else {
+      KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, logit_pairs, stream, xm, wk, es, la));
+      JoinArgs ja{};
+      ja.part = s.part;
+      ja.n_part = 2 * (int)p.n_vt;
+      ja.tgt = s.tgt + r0;
+      ja.l2t = s.l2t + r0;
+      ja.l2t_low = s.l2t_low + r0;
+      ja.loss = c.loss + r0;
+      ja.stats = c.stats ? c.stats + r0 : nullptr;
+      ja.rows = (int)rows;
+      ja.K = K;
+      ja.all_second = F16;
+      ja.e_scale = e_scale;
+      ja.z = c.z;
+      if (p.grads) {
+        ja.coef = s.coef + r0;
+        ja.factor = s.factor + r0;
+        ja.ref = s.ref + r0;
+        ja.marked = s.marked + r0 / 256;
+        ja.xs = s.xs;
+        ja.x = xc;
+      }
+      KRSI_CUDA_TRY(launch_pdl(ce_join_kernel<DT>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ja));
+      if (!p.grads) continue;
     }
-    KRSI_CUDA_TRY(launch_pdl(ce_join_kernel<DT>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ja));
-    if (!p.grads) continue;
 
     la.ref = s.ref + r0;
     la.part = nullptr;
-    la.marked = F16 ? nullptr : s.marked + r0 / 256;
+    la.marked = F16 || known ? nullptr : s.marked + r0 / 256;
     la.e_scale = e_scale;
     la.store = 1;
     KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, logit_pairs, stream, xm, wk, es, la));
@@ -1222,7 +1302,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     if (ga.n_dx % P != 0)   // pairs with one dx item less than the others take dw items for it
       ga.low_first = std::min((ga.kb_share + ga.kb_rows / 2) / ga.kb_rows, ga.n_dw / (P - ga.n_dx % P));
     ga.dx_part = ga.splits > 1;
-    ga.dx32 = ga.dx_part || c.out32;
+    ga.dx32 = ga.dx_part || !known;
     ga.tgt = s.tgt + r0;
     ga.factor = s.factor + r0;
     ga.coef = s.coef + r0;
@@ -1232,26 +1312,26 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     ga.base = p.direct ? dw32 : nullptr;
     ga.start = s.sorted.start;
     ga.order = s.sorted.order;
-    ga.g_top = g_top;
+    ga.up = up;
     ga.alpha = 1.f / e_scale;
     ga.scale = c.scale;
     ga.limit = kSpinLimit;
-    void* dxc = c.dx ? static_cast<char*>(c.dx) + (size_t)r0 * K * (c.out32 ? 4 : 2) : nullptr;
+    void* dxc = c.dx ? static_cast<char*>(c.dx) + (size_t)r0 * K * (known ? 2 : 4) : nullptr;
     CUtensorMap dxm = wm;
     const int64_t part_rows = (int64_t)ga.n_rt * 256;
     if (c.dx && !(ga.dx_part  ? make_map_f32(&dxm, s.dx_part, ga.splits * part_rows, K)
-                  : c.out32 ? make_map_f32(&dxm, dxc, rows, K)
+                  : !known ? make_map_f32(&dxm, dxc, rows, K)
                             : make_map(&dxm, dxc, rows, K, K, F16, 16, 32, CU_TENSOR_MAP_SWIZZLE_32B)))
       return KRSI_ERR_CUDA;
     KRSI_CUDA_TRY(launch_pairs(ce_grads_kernel<F16>, P, stream, ek, wm, em, xs, dxm, dwm, ga));
     if (ga.dx_part && c.dx)
       KRSI_CUDA_TRY(launch_pdl(ce_dx_join_kernel<DT>, dim3((unsigned)ceil_div(rows * (K / 4), 128)), dim3(128), 0,
                                stream, (const float*)s.dx_part, ga.splits, part_rows * K, ga.tgt, ga.factor, ga.coef, w,
-                               dxc, (int)rows, K, c.scale, (int)c.out32));
+                               dxc, (int)rows, K, c.scale, known ? 0 : 1));
   }
   if (p.grads && !p.direct && c.dw) {
     KRSI_CUDA_TRY((tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, dw_rows, false, N, V, K, stream)));
-    if (!c.out32) {
+    if (known) {
       const int64_t n = p.V * p.K;
       KRSI_CUDA_TRY(launch_pdl(ce_finish_kernel<DT>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 2048), 148 * 64)),
                                dim3(256), 0, stream, (const float*)dw32, (T*)c.dw, n, c.scale, (const float*)nullptr,
@@ -1279,7 +1359,7 @@ inline int run_checked(const Call& c, int64_t N, int64_t V, int64_t K, void* wor
   if (!aligned16(c.x) || !aligned16(c.w) || !aligned16(c.dx) || !aligned16(c.dw)) return KRSI_ERR_MISALIGNED;
   const int pairs = device_pairs();
   if (pairs <= 0) return KRSI_ERR_UNSUPPORTED;   // a device partition without clusters of two
-  const Plan p = make_plan(N, V, K, c.dx != nullptr || c.dw != nullptr, c.out32, pairs);
+  const Plan p = make_plan(N, V, K, c.dx != nullptr || c.dw != nullptr, c.loss == nullptr, pairs);
   const Space s = space_at(workspace, p);
   if (!workspace || workspace_bytes < s.bytes) return KRSI_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return KRSI_ERR_MISALIGNED;
@@ -1295,13 +1375,13 @@ extern "C" int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, in
   KRSI_CHECK_ARG(bytes && N >= 0 && V > 0 && K > 0 && mode >= 0 && mode <= 2);
   const int pairs = device_pairs();
   if (pairs <= 0) return KRSI_ERR_UNSUPPORTED;
-  *bytes = space_at(nullptr, make_plan(N, V, K, mode > 0, mode == 1, pairs)).bytes;
+  *bytes = space_at(nullptr, make_plan(N, V, K, mode > 0, mode == 2, pairs)).bytes;
   return KRSI_OK;
 }
 
 extern "C" int krsi_linear_ce_fwd(const void* x, const void* w, const void* targets, int target_bits, float* loss,
-                                  float* reduced, float* dx, float* dw, void* workspace, size_t workspace_bytes,
-                                  int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss,
+                                  float* reduced, float* stats, float* dx, float* dw, void* workspace,
+                                  size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss,
                                   int mean, int dtype, cudaStream_t stream) {
   const int rc = check(N, V, K, target_bits, dtype);
   if (rc != KRSI_OK) return rc;
@@ -1312,13 +1392,14 @@ extern "C" int krsi_linear_ce_fwd(const void* x, const void* w, const void* targ
     return KRSI_OK;
   }
   KRSI_CHECK_ARG(x && w && targets && loss);
-  const Call c{x, w, targets, target_bits, loss, reduced, mean, nullptr, 0, nullptr, dx, dw, true, scale, z_loss,
+  if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) return KRSI_ERR_MISALIGNED;
+  const Call c{x, w, targets, target_bits, loss, reduced, mean, reinterpret_cast<float2*>(stats), nullptr, 0, nullptr, dx, dw, scale, z_loss,
                ignore_index};
   return run_checked(c, N, V, K, workspace, workspace_bytes, dtype, stream);
 }
 
 extern "C" int krsi_linear_ce_grad(const void* x, const void* w, const void* targets, int target_bits, const float* g,
-                                   int64_t g_stride, const float* weight, void* dx, void* dw,
+                                   int64_t g_stride, const float* weight, const float* stats, void* dx, void* dw,
                                    void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t K,
                                    float scale, int64_t ignore_index, float z_loss, int dtype, cudaStream_t stream) {
   const int rc = check(N, V, K, target_bits, dtype);
@@ -1328,8 +1409,10 @@ extern "C" int krsi_linear_ce_grad(const void* x, const void* w, const void* tar
     if (dw) KRSI_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)V * K * 2, stream));
     return KRSI_OK;
   }
-  KRSI_CHECK_ARG(x && w && targets && g);
-  const Call c{x, w, targets, target_bits, nullptr, nullptr, 0, g, g_stride, weight, dx, dw, false, scale, z_loss,
+  KRSI_CHECK_ARG(x && w && targets && g && stats);
+  if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) return KRSI_ERR_MISALIGNED;
+  const Call c{x, w, targets, target_bits, nullptr, nullptr, 0,
+               const_cast<float2*>(reinterpret_cast<const float2*>(stats)), g, g_stride, weight, dx, dw, scale, z_loss,
                ignore_index};
   return run_checked(c, N, V, K, workspace, workspace_bytes, dtype, stream);
 }

@@ -409,9 +409,9 @@ CeCall ce_call(const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor&
   return c;
 }
 
-// (loss rows, [loss, row weight], dx, dw): the gradients are fp32, of the sum of the losses and without
+// (loss rows, [loss, row weight], stats, dx, dw): stats is for linear_ce_grad; the gradients are fp32, of the sum of the losses and without
 // `scale`, or empty.  reduction 0 none, 1 mean, 2 sum.
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(
     const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor& targets_in, double scale, int64_t ignore_index,
     double z_loss, int64_t reduction, bool want_dx, bool want_dw) {
   TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
@@ -420,21 +420,23 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(
   auto f32 = c.x.options().dtype(at::kFloat);
   auto loss = at::empty({c.N}, f32);
   auto reduced = at::empty({reduction != 0 ? 2 : 0}, f32);
+  auto stats = at::empty({c.N, 2}, f32);
   auto dx = at::empty({want_dx ? c.N : 0, c.K}, f32);
   auto dw = at::empty({want_dw ? c.V : 0, c.K}, f32);
   check_rc(krsi_linear_ce_fwd(c.x.data_ptr(), c.w.data_ptr(), c.targets.data_ptr(), c.bits, loss.data_ptr<float>(),
-                              reduction != 0 ? reduced.data_ptr<float>() : nullptr,
+                              reduction != 0 ? reduced.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
                               want_dx ? dx.data_ptr<float>() : nullptr, want_dw ? dw.data_ptr<float>() : nullptr,
                               c.ws.data_ptr(), (size_t)c.ws.numel(), c.N, c.V, c.K, (float)scale, ignore_index,
                               (float)z_loss, reduction == 1, c.dtype, at::cuda::getCurrentCUDAStream()),
            "krsi_linear_ce_fwd");
-  return {loss, reduced, dx, dw};
+  return {loss, reduced, stats, dx, dw};
 }
 
 // Gradients in x2d's dtype for g, the upstream gradient of each row's loss ([N], or one for all), times
-// weight (one value, or empty).
+// weight (one value, or empty); stats: linear_ce_fwd's.
 std::tuple<at::Tensor, at::Tensor> linear_ce_grad(const at::Tensor& g_in, const at::Tensor& weight_in,
-                                                  const at::Tensor& x_in, const at::Tensor& w_in,
+                                                  const at::Tensor& stats, const at::Tensor& x_in,
+                                                  const at::Tensor& w_in,
                                                   const at::Tensor& targets_in, double scale, int64_t ignore_index,
                                                   double z_loss, bool want_dx, bool want_dw) {
   TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
@@ -442,6 +444,11 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_grad(const at::Tensor& g_in, const 
   const CeCall c = ce_call(x_in, w_in, targets_in, 2);
   TORCH_CHECK(g_in.numel() == c.N || g_in.numel() == 1, "linear_ce_grad: g must have ", c.N, " values or one");
   TORCH_CHECK(weight_in.numel() <= 1, "linear_ce_grad: weight must be one value or empty");
+  TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * c.N,
+              "linear_ce_grad: stats must be linear_ce_fwd's");
+  check_cuda(g_in, "g");
+  check_same_device(g_in, x_in, "linear_ce_grad");
+  check_same_device(stats, x_in, "linear_ce_grad");
   auto g = g_in.to(at::kFloat).contiguous();
   auto weight = weight_in.to(at::kFloat).contiguous();
   auto dx = at::empty({want_dx ? c.N : 0, c.K}, c.x.options());
@@ -449,7 +456,7 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_grad(const at::Tensor& g_in, const 
   if (!want_dx && !want_dw) return {dx, dw};
   check_rc(krsi_linear_ce_grad(c.x.data_ptr(), c.w.data_ptr(), c.targets.data_ptr(), c.bits, g.data_ptr<float>(),
                                g.numel() == 1 ? 0 : 1, weight.numel() == 1 ? weight.data_ptr<float>() : nullptr,
-                               want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, c.ws.data_ptr(),
+                               stats.data_ptr<float>(), want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, c.ws.data_ptr(),
                                (size_t)c.ws.numel(), c.N, c.V, c.K, (float)scale, ignore_index, (float)z_loss, c.dtype,
                                at::cuda::getCurrentCUDAStream()),
            "krsi_linear_ce_grad");
@@ -527,19 +534,19 @@ at::Tensor geglu_q8_plain(const at::Tensor& u) { return std::get<0>(geglu_q8_fwd
 // keep: form the gradients in the forward (saved in fp32) instead of saving the operands.
 at::Tensor linear_ce_plain(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, double scale,
                            int64_t ignore_index, double z_loss, int64_t reduction, bool /*keep*/) {
-  auto [loss, reduced, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction, false, false);
+  auto [loss, reduced, stats, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction, false, false);
   return reduction != 0 ? reduced.select(0, 0) : loss;
 }
 struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
                             double scale, int64_t ignore_index, double z_loss, int64_t reduction, bool keep) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [loss, reduced, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction,
+    auto [loss, reduced, stats, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction,
                                                  keep && x.requires_grad(), keep && w.requires_grad());
     auto out = reduction != 0 ? reduced.select(0, 0) : loss;
     auto weight = reduced.slice(0, 1);
     if (keep) ctx->save_for_backward({weight, dx, dw, w});
-    else ctx->save_for_backward({weight, x, w, targets});
+    else ctx->save_for_backward({weight, stats, x, w, targets});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["z_loss"] = z_loss;
@@ -555,7 +562,7 @@ struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
       if (need_x) dx = linear_ce_finish(saved[1], g[0], saved[0], scale, saved[3]);
       if (need_w) dw = linear_ce_finish(saved[2], g[0], saved[0], scale, saved[3]);
     } else {
-      std::tie(dx, dw) = linear_ce_grad(g[0], saved[0], saved[1], saved[2], saved[3], scale,
+      std::tie(dx, dw) = linear_ce_grad(g[0], saved[0], saved[1], saved[2], saved[3], saved[4], scale,
                                         ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["z_loss"].toDouble(),
                                         need_x, need_w);
       if (!need_x) dx = at::Tensor();
@@ -594,9 +601,9 @@ TORCH_LIBRARY(krsi, m) {
   m.def("linear_ce(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, int reduction, "
         "bool keep) -> Tensor");
   m.def("linear_ce_fwd(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, "
-        "int reduction, bool want_dx, bool want_dw) -> (Tensor, Tensor, Tensor, Tensor)");
-  m.def("linear_ce_grad(Tensor g, Tensor weight, Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, "
-        "float z_loss, bool want_dx, bool want_dw) -> (Tensor, Tensor)");
+        "int reduction, bool want_dx, bool want_dw) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+  m.def("linear_ce_grad(Tensor g, Tensor weight, Tensor stats, Tensor x2d, Tensor w, Tensor targets, float scale, "
+        "int ignore_index, float z_loss, bool want_dx, bool want_dw) -> (Tensor, Tensor)");
   m.def("linear_ce_finish(Tensor grad, Tensor g, Tensor weight, float scale, Tensor like) -> Tensor");
   m.def("geglu_q8_fwd(Tensor u, bool keep) -> (Tensor, Tensor, Tensor)");
   m.def("geglu_q8_bwd(Tensor g, Tensor q, Tensor exponents, bool want_out) -> (Tensor, Tensor)");

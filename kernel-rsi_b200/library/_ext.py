@@ -134,11 +134,12 @@ def _register_compile_support() -> None:
     def _(x2d, w, targets, scale, ignore_index, z_loss, reduction, want_dx, want_dw):
         f32 = torch.float32
         return (x2d.new_empty((x2d.shape[0],), dtype=f32), x2d.new_empty((2 if reduction else 0,), dtype=f32),
+                x2d.new_empty((x2d.shape[0], 2), dtype=f32),
                 x2d.new_empty((x2d.shape[0] if want_dx else 0, x2d.shape[1]), dtype=f32),
                 x2d.new_empty((w.shape[0] if want_dw else 0, w.shape[1]), dtype=f32))
 
     @reg_fake("krsi::linear_ce_grad")
-    def _(g, weight, x2d, w, targets, scale, ignore_index, z_loss, want_dx, want_dw):
+    def _(g, weight, stats, x2d, w, targets, scale, ignore_index, z_loss, want_dx, want_dw):
         return (x2d.new_empty((x2d.shape[0] if want_dx else 0, x2d.shape[1])),
                 x2d.new_empty((w.shape[0] if want_dw else 0, w.shape[1])))
 
@@ -226,16 +227,16 @@ def _register_compile_support() -> None:
 
     def ce_setup(ctx, inputs, output):
         x2d, w, targets, scale, ignore_index, z_loss, reduction, want_dx, want_dw = inputs
-        loss, reduced, dx, dw = output
+        loss, reduced, stats, dx, dw = output
         ctx.args = (scale, ignore_index, z_loss)
         ctx.reduction, ctx.kept, ctx.wanted = reduction, want_dx or want_dw, (want_dx, want_dw)
         ctx.set_materialize_grads(False)
         if ctx.kept:
             ctx.save_for_backward(reduced, dx, dw, w)
         else:
-            ctx.save_for_backward(reduced, x2d, w, targets)
+            ctx.save_for_backward(reduced, stats, x2d, w, targets)
 
-    def ce_backward(ctx, gloss, greduced, _gdx, _gdw):
+    def ce_backward(ctx, gloss, greduced, _gstats, _gdx, _gdw):
         g = gloss if ctx.reduction == 0 else greduced[0] if greduced is not None else None
         none = (None,) * 7
         if g is None:

@@ -368,6 +368,6 @@ def test_refusals():
     vp, i64, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
     loss = torch.empty(10, device=dev)
     call = lambda ws, size: capi().krsi_linear_ce_fwd(  # noqa: E731
-        vp(x.data_ptr()), vp(w.data_ptr()), vp(t.data_ptr()), 64, vp(loss.data_ptr()), vp(0), vp(0), vp(0), vp(ws),
+        vp(x.data_ptr()), vp(w.data_ptr()), vp(t.data_ptr()), 64, vp(loss.data_ptr()), vp(0), vp(0), vp(0), vp(0), vp(ws),
         ctypes.c_size_t(size), i64(10), i64(20), i64(64), f32(1.0), i64(-100), f32(0.0), 0, 1, vp(0))
     assert call(0, 1 << 20) == 4 and call(t.data_ptr(), 16) == 4
