@@ -57,9 +57,9 @@ constexpr int kBM = 128;                            // rows of A per CTA (256 pe
 constexpr int kBN = 256;                            // columns of one MMA (at most)
 constexpr int kBK = 64;
 constexpr int kMaxStages = 6;
-constexpr int kThreads = 384;
-constexpr int kEpiWarp0 = 4;
-constexpr int kEpiWarps = 8;
+constexpr int kEpiWarp0 = 4;                        // the epilogue's first warp
+constexpr int kLogitsEpi = 8, kGradsEpi = 12;       // epilogue warps
+constexpr int kLogitsThreads = 32 * (kEpiWarp0 + kLogitsEpi), kGradsThreads = 32 * (kEpiWarp0 + kGradsEpi);
 constexpr uint32_t kATile = kBM * kBK * 2;          // 16 KB
 constexpr uint32_t kMnBox = 64 * kBK * 2;           // one [64 K-rows x 64 columns] MN-major box: 8 KB
 // Shared memory: the epilogue warps' staged boxes, the barriers, then the operand ring.
@@ -81,12 +81,13 @@ __device__ __forceinline__ uint64_t mnmajor_sw128(uint32_t addr) { return smem_d
 // of B (8 KB per 64 columns), the second MMA's 16 KB after the first's.
 struct Pipe {
   int cols;
+  int epi_warps;
   uint32_t box_bytes;   // one epilogue warp's staged box
-  __device__ __forceinline__ uint32_t bars_at() const { return kEpiWarps * box_bytes; }
+  __device__ __forceinline__ uint32_t bars_at() const { return epi_warps * box_bytes; }
   __device__ __forceinline__ uint32_t ring_at() const { return bars_at() + 1024; }
   __device__ __forceinline__ uint32_t stage_bytes() const { return kATile + (cols / 128) * kMnBox; }
   __device__ __forceinline__ int stages() const {
-    return min((int)((kUsable - kEpiWarps * box_bytes) / stage_bytes()), kMaxStages);
+    return min((int)((kUsable - epi_warps * box_bytes) / stage_bytes()), kMaxStages);
   }
   __device__ __forceinline__ int accs() const { return cols <= kBN ? 2 : 1; }
 };
@@ -98,8 +99,8 @@ struct MmaShape {
 };
 
 // The roles of one CTA of a pair over `n_items` items (the same list in both CTAs): warp 0 loads the K
-// blocks of each item into the ring, the even CTA's warp 1 issues the MMAs, warps 4-11 of both CTAs run
-// the epilogue on their CTA's 128 rows.
+// blocks of each item into the ring, the even CTA's warp 1 issues the MMAs, the warps from 4 on of both
+// CTAs run the epilogue on their CTA's 128 rows.
 //   item(i)                      item i of the list; its n_kb is the number of K blocks (at least 1)
 //   load(item, kb, stage, bar)   issues this CTA's TMA loads of a K block (stage_bytes() in all)
 //   shape(item)                  the descriptors of its MMAs
@@ -130,7 +131,7 @@ __device__ __forceinline__ void pair_gemm(uint8_t* smem, const Pipe pipe, int n_
     }
     for (int b = 0; b < 2; ++b) {
       mbar_init(&acc_full[b], 1);                // the even CTA's tcgen05.commit
-      mbar_init(&acc_empty[b], 2 * kEpiWarps);   // one arrival per epilogue warp of both CTAs
+      mbar_init(&acc_empty[b], 2 * pipe.epi_warps);   // one arrival per epilogue warp of both CTAs
     }
     mbar_init(drain, 1);
     *abort_flag = 0;
@@ -309,7 +310,7 @@ struct LogitsArgs {
 };
 
 template <bool F16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kLogitsThreads, 1)
 ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                  const __grid_constant__ CUtensorMap emap, const LogitsArgs a) {
   pdl_enter();   // before any global access and before claiming TMEM
@@ -333,7 +334,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
     int rt, vt, n_kb;
   };
 
-  const Pipe pipe{kBN, kLogitsBox};
+  const Pipe pipe{kBN, kLogitsEpi, kLogitsBox};
   pair_gemm(
       smem, pipe, pair < n_tiles ? (n_tiles - 1 - pair) / n_pairs + 1 : 0, a.limit,
       [&](int i) {
@@ -675,10 +676,10 @@ struct GradArgs {
   const float* factor;
   const float* coef;
   const void* w;
-  // dw: fp32 sums, stored or added; or, scaled and rounded, with the rows of `base` added for the tokens
-  // that occur (token_rows.cuh's start)
+  // dw: fp32 sums, stored or added; or scaled and rounded, and for the tokens that occur (token_rows.cuh's
+  // start) the fp32 sums as well, rows of `sums`
   int dw32, accumulate;
-  const float* base;
+  float* sums;
   const int* start;
   tokens::Order order;
   Upstream up;
@@ -692,31 +693,12 @@ struct GradArgs {
 struct GradItem {
   int is_dx, tile, ct, split, n_kb;
 };
-// One epilogue thread's row of an item: out = mul * sum + add, add being coef * w_t (16 bits) or the row
-// of base (fp32); `add` holds the 16 columns that come next.
-template <typename T>
-union GradAdd {
-  Vec16<T> w[2];
-  Vec16<float> base[4];
-  __device__ __forceinline__ GradAdd() {}
-  __device__ __forceinline__ void fetch(int is_dx, const GradArgs& a, int64_t at, int col) {
-    if (is_dx) {
-#pragma unroll
-      for (int p = 0; p < 2; ++p)
-        if (col + 8 * p < a.K) w[p] = ldg16(reinterpret_cast<const T*>(a.w) + at + col + 8 * p);
-    } else {
-#pragma unroll
-      for (int p = 0; p < 4; ++p)
-        if (col + 4 * p < a.K) base[p] = ldg16(a.base + at + col + 4 * p);
-    }
-  }
-};
-template <typename T>
+// One epilogue thread's row of an item.
 struct GradRow {
   float mul, coef;
   bool zero;
-  int64_t add_at;   // w's or base's first element of the row, or -1
-  GradAdd<T> add;
+  int64_t w_at;     // dx: w_t's first element, which coef times is added; or -1
+  float* sums;      // dw in 16 bits: where the token's row of fp32 sums goes; or null
 };
 __device__ __forceinline__ int pair_dx(const GradArgs& a, int pair, int P) {
   return a.n_dx / P + (pair < a.n_dx % P ? 1 : 0);
@@ -742,7 +724,7 @@ __device__ __forceinline__ GradItem pair_item(const GradArgs& a, int pair, int P
 }
 
 template <bool F16>
-__global__ void __launch_bounds__(kThreads, 1)
+__global__ void __launch_bounds__(kGradsThreads, 1)
 ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant__ CUtensorMap wmap,
                 const __grid_constant__ CUtensorMap emmap, const __grid_constant__ CUtensorMap xsmap,
                 const __grid_constant__ CUtensorMap dxmap, const __grid_constant__ CUtensorMap dwmap,
@@ -758,7 +740,7 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
   const int pair = (int)blockIdx.x / 2, P = (int)gridDim.x / 2;
   const int cols1 = min(a.cols, kBN), cols2 = a.cols - cols1;   // of the two MMAs
 
-  const Pipe pipe{a.cols, kGradsBox};
+  const Pipe pipe{a.cols, kGradsEpi, kGradsBox};
   pair_gemm(
       smem, pipe, pair_items(a, pair, P), a.limit,
       [&](int i) { return pair_item(a, pair, P, i); },
@@ -781,71 +763,73 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
       },
       [&](const GradItem& m) {
         const int row = m.tile * (2 * kBM) + rank * kBM + (warp % 4) * 32 + lane;   // of dx, or the token of dw
-        GradRow<T> r;
-        r.mul = 1.f;
-        r.coef = 0.f;
-        r.zero = false;
-        r.add_at = -1;
+        GradRow r{1.f, 0.f, false, -1, nullptr};
         if (row >= (m.is_dx ? a.rows : a.V)) return r;
         if (!m.is_dx) {
           r.mul = a.alpha * a.up.unit();
-          if (a.base) {
+          if (a.sums) {
             const int k = a.order.key(row);
-            if (a.start[k] < a.start[k + 1]) r.add_at = (int64_t)row * a.K;
+            if (a.start[k] < a.start[k + 1]) r.sums = a.sums + (int64_t)row * a.K;
           }
         } else if (!a.dx_part) {
           const int t = a.tgt[row];
           r.mul = a.factor[row];
           r.coef = a.coef[row];
           r.zero = t == kIgnored;
-          if (t >= 0) r.add_at = (int64_t)t * a.K;
+          if (t >= 0) r.w_at = (int64_t)t * a.K;
         }
-        if (r.add_at >= 0)
-          r.add.fetch(m.is_dx, a, r.add_at, m.ct * a.cols + (warp - kEpiWarp0) / 4 * (a.cols / 2));
         return r;
       },
-      [&](const GradItem& m, const GradRow<T>& r, uint32_t taddr, auto release) {
-        const int ew = warp - kEpiWarp0, half = ew / 4, half_n = a.cols / 2;
+      [&](const GradItem& m, const GradRow& r, uint32_t taddr, auto release) {
+        const int ew = warp - kEpiWarp0, third = ew / 4;
         const int row0 = m.tile * (2 * kBM) + rank * kBM + (warp % 4) * 32;
-        const int col0 = m.ct * a.cols + half * half_n;
-        const uint32_t acc = taddr + half * half_n;
         const bool wide = m.is_dx ? a.dx32 : a.dw32;      // fp32 out
         const bool any = row0 < (m.is_dx ? a.rows : a.V);
         const CUtensorMap* map = m.is_dx ? &dxmap : &dwmap;
         const int out_row = m.is_dx ? m.split * (a.n_rt * 2 * kBM) + row0 : row0;
-        // 16 columns at a time through the staged box: [32 rows x 16 columns] of fp32 in the 64-byte
-        // swizzle, or of 16 bits in the 32-byte swizzle, two such boxes in turn; the maps clip rows and
-        // columns.  What is to be added to the next columns is on its way while these are worked on.
-        GradAdd<T> add = r.add;
+        // 16 columns at a time (every third 16 of the tile) through the staged box: [32 rows x 16 columns]
+        // of fp32 in the 64-byte swizzle, or of 16 bits in the 32-byte swizzle, two such boxes in turn; the
+        // maps clip rows and columns.  The target's row of w for the next columns is on its way while these
+        // are worked on.
+        Vec16<T> wt[2];
+        auto fetch = [&](int col) {
+          if (r.w_at >= 0)
+#pragma unroll
+            for (int p = 0; p < 2; ++p)
+              if (col + 8 * p < a.K) wt[p] = ldg16(reinterpret_cast<const T*>(a.w) + r.w_at + col + 8 * p);
+        };
+        fetch(m.ct * a.cols + third * 16);
+        constexpr int kStep = 16 * (kGradsEpi / 4);
+        int turn = 0;
 #pragma unroll 1
-        for (int j = 0; j < half_n; j += 16) {
+        for (int j = third * 16; j < a.cols; j += kStep, ++turn) {
+          const int col = m.ct * a.cols + j;
           uint32_t q[16];
           __syncwarp();
-          tmem_ld16(acc + j, q);
+          tmem_ld16(taddr + j, q);
           tmem_wait_ld();
-          if (j + 16 >= half_n) release();
+          if (j + kStep >= a.cols) release();
           float v[16];
 #pragma unroll
           for (int e = 0; e < 16; ++e) v[e] = r.zero ? 0.f : r.mul * __uint_as_float(q[e]);
-          if (r.add_at >= 0) {
-            if (m.is_dx) {
+          if (r.w_at >= 0) {
 #pragma unroll
-              for (int p = 0; p < 2; ++p)
-                if (col0 + j + 8 * p < a.K)
+            for (int p = 0; p < 2; ++p)
+              if (col + 8 * p < a.K)
 #pragma unroll
-                  for (int e = 0; e < 8; ++e) v[8 * p + e] = fmaf(r.coef, E::load(add.w[p].v[e]), v[8 * p + e]);
-            } else {
-#pragma unroll
-              for (int p = 0; p < 4; ++p)
-                if (col0 + j + 4 * p < a.K)
-#pragma unroll
-                  for (int e = 0; e < 4; ++e) v[4 * p + e] += add.base[p].v[e];
-            }
-            if (j + 16 < half_n) add.fetch(m.is_dx, a, r.add_at, col0 + j + 16);
+                for (int e = 0; e < 8; ++e) v[8 * p + e] = fmaf(r.coef, E::load(wt[p].v[e]), v[8 * p + e]);
+            if (j + kStep < a.cols) fetch(col + kStep);
           }
-          uint8_t* box = smem + ew * kGradsBox + (!wide && (j & 16) ? kGradsBox / 2 : 0);
+          if (r.sums != nullptr) {   // (the 16-bit row is written again from these)
+#pragma unroll
+            for (int p = 0; p < 4; ++p)
+              if (col + 4 * p < a.K)
+                *reinterpret_cast<float4*>(r.sums + col + 4 * p) =
+                    make_float4(v[4 * p], v[4 * p + 1], v[4 * p + 2], v[4 * p + 3]);
+          }
+          uint8_t* box = smem + ew * kGradsBox + (!wide && (turn & 1) ? kGradsBox / 2 : 0);
           if (lane == 0) {   // the box's previous content has been read
-            if (wide || j < 32) bulk_wait_read_all();
+            if (wide || turn < 2) bulk_wait_read_all();
             else bulk_wait_read_but_one();
           }
           __syncwarp();
@@ -869,9 +853,9 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
           }
           fence_async_shared();
           __syncwarp();
-          if (lane == 0 && any && col0 + j < a.K) {
-            if (!m.is_dx && a.accumulate) tma_reduce_add_2d(map, box, col0 + j, out_row);
-            else tma_store_2d(map, box, col0 + j, out_row);
+          if (lane == 0 && any && col < a.K) {
+            if (!m.is_dx && a.accumulate) tma_reduce_add_2d(map, box, col, out_row);
+            else tma_store_2d(map, box, col, out_row);
           }
           if (lane == 0) bulk_commit_group();   // one group a step, empty where nothing is stored
         }
@@ -939,29 +923,45 @@ ce_finish_kernel(const float* __restrict__ a, typename Elem<DT>::T* __restrict__
   }
 }
 
-// The weighted sums of x by target token, as rows of dw32: written, or added to what is there.
-struct DwRows {
+// The weighted sums of x by target token, added to rows of fp32 sums: in place, or (16-bit dw) into the
+// finished rows.
+struct DwSums {
   float* dw32;
   int64_t K;
-  int add;
   // One addition per element and call, so a reduction in L2 (no read to wait for) gives the same bits
   // every time.
   __device__ __forceinline__ void packet(int v, uint32_t c, const float* s) const {
     float* p = dw32 + v * K + c * 8;
 #pragma unroll
-    for (int h = 0; h < 8; h += 4) {
-      if (add)
-        asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + h), "f"(s[h]), "f"(s[h + 1]),
-                     "f"(s[h + 2]), "f"(s[h + 3])
-                     : "memory");
-      else
-        *reinterpret_cast<float4*>(p + h) = make_float4(s[h], s[h + 1], s[h + 2], s[h + 3]);
+    for (int h = 0; h < 8; h += 4)
+      asm volatile("red.global.add.v4.f32 [%0], {%1, %2, %3, %4};" ::"l"(p + h), "f"(s[h]), "f"(s[h + 1]),
+                   "f"(s[h + 2]), "f"(s[h + 3])
+                   : "memory");
+  }
+  __device__ __forceinline__ void zero(int, uint32_t) const {}
+  __device__ __forceinline__ void column(int v, int col, float s) const { dw32[v * K + col] += s; }
+};
+template <int DT>
+struct DwRows {
+  using T = typename Elem<DT>::T;
+  const float* sums;
+  T* dw;
+  int64_t K;
+  float scale;
+  __device__ __forceinline__ void packet(int v, uint32_t c, const float* s) const {
+    const int64_t at = v * K + c * 8;
+    const auto a = ldg16(sums + at), b = ldg16(sums + at + 4);
+    Vec16<T> o;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      o.v[e] = Elem<DT>::store(scale * (a.v[e] + s[e]));
+      o.v[4 + e] = Elem<DT>::store(scale * (b.v[e] + s[4 + e]));
     }
+    stg16(dw + at, o);
   }
   __device__ __forceinline__ void zero(int, uint32_t) const {}
   __device__ __forceinline__ void column(int v, int col, float s) const {
-    float* p = dw32 + v * K + col;
-    *p = add ? *p + s : s;
+    dw[v * K + col] = Elem<DT>::store(scale * (sums[v * K + col] + s));
   }
 };
 
@@ -982,14 +982,14 @@ inline bool make_map_f32(CUtensorMap* map, const void* base, int64_t rows, int64
 }
 
 template <typename Kern>
-int max_pairs(Kern kern) {   // clusters of two of `kern` that fit on the device at once; 0: none
+int max_pairs(Kern kern, int threads) {   // clusters of two of `kern` that fit on the device at once; 0: none
   if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmem) != cudaSuccess) {
     cudaGetLastError();
     return 0;
   }
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * (device_sm_count() / 2));
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = kSmem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -1012,18 +1012,20 @@ inline int device_pairs() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   int v = cached[dev].load(std::memory_order_relaxed);
   if (v == 0) {
-    v = std::min(std::min(max_pairs(ce_logits_kernel<false>), max_pairs(ce_logits_kernel<true>)),
-                 std::min(max_pairs(ce_grads_kernel<false>), max_pairs(ce_grads_kernel<true>))) + 1;
+    v = std::min(std::min(max_pairs(ce_logits_kernel<false>, kLogitsThreads),
+                          max_pairs(ce_logits_kernel<true>, kLogitsThreads)),
+                 std::min(max_pairs(ce_grads_kernel<false>, kGradsThreads),
+                          max_pairs(ce_grads_kernel<true>, kGradsThreads))) + 1;
     cached[dev].store(v, std::memory_order_relaxed);
   }
   return v - 1;
 }
 
 template <typename... KArgs, typename... Args>
-cudaError_t launch_pairs(void (*kern)(KArgs...), int pairs, cudaStream_t stream, Args&&... args) {
+cudaError_t launch_pairs(void (*kern)(KArgs...), int threads, int pairs, cudaStream_t stream, Args&&... args) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(2 * pairs);
-  cfg.blockDim = dim3(kThreads);
+  cfg.blockDim = dim3(threads);
   cfg.dynamicSmemBytes = kSmem;
   cfg.stream = stream;
   cudaLaunchAttribute attr[2];
@@ -1091,10 +1093,11 @@ inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool known, i
       p.n_ct = (int)n;
     }
   }
-  // dx has few, long sums: shares of the vocabulary until every pair has one (at least 8 K blocks each).
+  // dx has few, long sums: shares of the vocabulary where one sum is longer than a pair's part of all the
+  // work (at least 8 K blocks each).
   const int64_t tiles = p.chunk / 256 * p.n_ct, kb = ceil_div(V, kBK);
-  p.splits = 1;
-  if (tiles < pairs) p.splits = std::max<int64_t>(1, std::min(ceil_div(pairs, tiles), kb / 8));
+  const int64_t work = tiles * kb + p.n_vt * p.n_ct * ceil_div(std::min(N, p.chunk), kBK);
+  p.splits = std::max<int64_t>(1, std::min(ceil_div(kb * pairs, work), kb / 8));
   p.splits = ceil_div(kb, ceil_div(kb, p.splits));   // no empty share
   return p;
 }
@@ -1194,10 +1197,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   const auto sw128 = CU_TENSOR_MAP_SWIZZLE_128B;
   if (!make_map(&wk, w, V, K, K, F16, kBK, kBM, sw128) || !make_map(&wm, w, V, K, K, F16, 64, kBK, sw128))
     return KRSI_ERR_CUDA;
-  // The targets' part of dw: with a direct dw first, as fp32 rows of the tokens that occur, which the
-  // GEMM's epilogue adds; otherwise after the chunks, added to the fp32 dw.
   float* dw32 = known ? s.dw32 : static_cast<float*>(c.dw);
-  const DwRows dw_rows{dw32, p.K, p.direct ? 0 : 1};
   CUtensorMap dwm = wm;
   if (c.dw && !(p.direct ? make_map(&dwm, c.dw, V, K, K, F16, 16, 32, CU_TENSOR_MAP_SWIZZLE_32B)
                          : make_map_f32(&dwm, dw32, V, K)))
@@ -1248,7 +1248,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       KRSI_CUDA_TRY(launch_pdl(wide ? ce_rows_kernel<DT, long long> : ce_rows_kernel<DT, int>,
                                dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ra));
     } else {
-      KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, logit_pairs, stream, xm, wk, es, la));
+      KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
       JoinArgs ja{};
       ja.part = s.part;
       ja.n_part = 2 * (int)p.n_vt;
@@ -1279,10 +1279,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     la.marked = F16 || known ? nullptr : s.marked + r0 / 256;
     la.e_scale = e_scale;
     la.store = 1;
-    KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, logit_pairs, stream, xm, wk, es, la));
-
-    if (p.direct && c.dw)
-      KRSI_CUDA_TRY((tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, dw_rows, false, N, V, K, stream)));
+    KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
 
     GradArgs ga{};
     ga.rows = (int)rows;
@@ -1309,7 +1306,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     ga.w = w;
     ga.dw32 = !p.direct;
     ga.accumulate = r0 > 0;
-    ga.base = p.direct ? dw32 : nullptr;
+    ga.sums = p.direct ? dw32 : nullptr;
     ga.start = s.sorted.start;
     ga.order = s.sorted.order;
     ga.up = up;
@@ -1323,19 +1320,25 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
                   : !known ? make_map_f32(&dxm, dxc, rows, K)
                             : make_map(&dxm, dxc, rows, K, K, F16, 16, 32, CU_TENSOR_MAP_SWIZZLE_32B)))
       return KRSI_ERR_CUDA;
-    KRSI_CUDA_TRY(launch_pairs(ce_grads_kernel<F16>, P, stream, ek, wm, em, xs, dxm, dwm, ga));
+    KRSI_CUDA_TRY(launch_pairs(ce_grads_kernel<F16>, kGradsThreads, P, stream, ek, wm, em, xs, dxm, dwm, ga));
     if (ga.dx_part && c.dx)
       KRSI_CUDA_TRY(launch_pdl(ce_dx_join_kernel<DT>, dim3((unsigned)ceil_div(rows * (K / 4), 128)), dim3(128), 0,
                                stream, (const float*)s.dx_part, ga.splits, part_rows * K, ga.tgt, ga.factor, ga.coef, w,
                                dxc, (int)rows, K, c.scale, known ? 0 : 1));
   }
-  if (p.grads && !p.direct && c.dw) {
-    KRSI_CUDA_TRY((tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, dw_rows, false, N, V, K, stream)));
-    if (known) {
-      const int64_t n = p.V * p.K;
-      KRSI_CUDA_TRY(launch_pdl(ce_finish_kernel<DT>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 2048), 148 * 64)),
-                               dim3(256), 0, stream, (const float*)dw32, (T*)c.dw, n, c.scale, (const float*)nullptr,
-                               (const float*)nullptr));
+  if (p.grads && c.dw) {   // the targets' part of dw
+    if (p.direct) {
+      const DwRows<DT> out{dw32, (T*)c.dw, p.K, c.scale};
+      KRSI_CUDA_TRY((tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
+    } else {
+      const DwSums out{dw32, p.K};
+      KRSI_CUDA_TRY((tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
+      if (known) {
+        const int64_t n = p.V * p.K;
+        KRSI_CUDA_TRY(launch_pdl(ce_finish_kernel<DT>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 2048), 148 * 64)),
+                                 dim3(256), 0, stream, (const float*)dw32, (T*)c.dw, n, c.scale, (const float*)nullptr,
+                                 (const float*)nullptr));
+      }
     }
   }
   if (c.reduced)
