@@ -119,7 +119,10 @@ def main():
     ap = argparse.ArgumentParser()
     ap.add_argument("--out", required=True)
     a = ap.parse_args()
+    import embedding
     import geglu
+    import geglu_q8
+    import linear_cross_entropy as ce
     import linear_geglu
     import relpos_attention as ra
     import rmsnorm
@@ -146,6 +149,17 @@ def main():
     cases["linear_geglu"] = (linear_geglu.linear_geglu, linear_geglu.reference, [xl, wl])
     table = 0.1 * torch.randn(32, 12, device=dev)
     cases["t5_bias"] = (lambda t: t5_bias.t5_relpos_bias(t, 512), lambda t: t5_bias.reference(t, 512), [table])
+    tok = torch.randint(0, 32768, (4, 1024), device=dev)
+    emb = torch.randn(32768, 768, device=dev, dtype=torch.bfloat16)
+    cases["embedding"] = (lambda t: embedding.embedding(tok, t, 0.5), lambda t: embedding.reference(tok, t, 0.5), [emb])
+    xc = torch.randn(2048, 768, device=dev, dtype=torch.bfloat16)
+    wc = (torch.randn(32768, 768, device=dev) * 768 ** -0.5).to(torch.bfloat16)
+    tgt = torch.randint(0, 32768, (2048,), device=dev)
+    cases["linear_cross_entropy"] = (lambda x, w: ce.linear_cross_entropy(x, w, tgt), lambda x, w: ce.reference(x, w, tgt),
+                                     [xc, wc])
+    uq = (torch.randn(2048, 2 * 2048, device=dev).clamp(-4, 4) * 16).round() / 16
+    uq[:, ::geglu_q8.GROUP] = 4.0
+    cases["geglu_q8"] = (geglu_q8.geglu_q8, geglu_q8.reference, [uq.to(torch.bfloat16)])
     out = {"versions": info, "library": {}, "regions": {},
            "note": "recorded by tests/make_replay_record.py (this repository's restatement of tools/replay.py "
                    "and selftest_autograd; the reference's tools are not present on this host)"}
