@@ -6,6 +6,7 @@
 //
 // A token id outside [0, V) reads nothing: its row of out is NaN and it adds to no gradient.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.cuh"
 #include "token_rows.cuh"
@@ -109,20 +110,30 @@ int fwd(const void* toks, int token_bits, const void* table, void* out, int64_t 
   const int rows = (int)std::max<int64_t>(1, std::min<int64_t>(kFwdRows, n / kNumSMsB200));
   const dim3 grid((unsigned)((n + rows - 1) / rows), (packets + threads - 1) / threads);
   const size_t smem = (size_t)rows * threads * VEC * sizeof(T);   // at most 64 KB
-  auto launch = [&](auto kern, auto* t) -> int {
-    KRSI_CUDA_TRY(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kFwdRows * 256 * 16));
+  auto launch = [&](auto* t) -> int {
+    using I = std::remove_const_t<std::remove_pointer_t<decltype(t)>>;
+    constexpr auto kern = embedding_fwd_kernel<DT, VEC, I>;
+    KRSI_CUDA_TRY(allow_smem<kern>(kFwdRows * 256 * 16));
     KRSI_CUDA_TRY(launch_pdl(kern, grid, dim3(threads), smem, stream, t, (const T*)table, (T*)out, (int)n, rows,
                              packets, V, scale));
     return KRSI_OK;
   };
-  return token_bits == 64 ? launch(embedding_fwd_kernel<DT, VEC, long long>, (const long long*)toks)
-                          : launch(embedding_fwd_kernel<DT, VEC, int>, (const int*)toks);
+  return token_bits == 64 ? launch((const long long*)toks) : launch((const int*)toks);
 }
 
 template <int DT, int VEC>
-int bwd(const void* g, const tokens::Space& s, void* dtable, int64_t n, int64_t V, int64_t d, float scale,
-        cudaStream_t stream) {
+int bwd(const void* toks, int token_bits, const void* g, const tokens::Space& s, void* dtable, int64_t n, int64_t V,
+        int64_t d, float scale, int64_t padding_idx, cudaStream_t stream) {
   const TableRows<DT, VEC> rows{(typename Elem<DT>::T*)dtable, d, scale};
+  if (n <= tokens::kFewRows) {
+    KRSI_CUDA_TRY(token_bits == 64
+                      ? (tokens::sum_few<DT, VEC, false>(g, nullptr, (const long long*)toks, rows, true, n, V,
+                                                         padding_idx, d, stream))
+                      : (tokens::sum_few<DT, VEC, false>(g, nullptr, (const int*)toks, rows, true, n, V, padding_idx, d,
+                                                         stream)));
+    return KRSI_OK;
+  }
+  KRSI_CUDA_TRY(tokens::token_sort(toks, token_bits, n, V, padding_idx, s.start, s.pos, s.tok, stream));
   KRSI_CUDA_TRY((tokens::sum_by_token<DT, VEC, false>(g, nullptr, s, rows, true, n, V, d, stream)));
   return KRSI_OK;
 }
@@ -185,6 +196,5 @@ extern "C" int krsi_embedding_bwd(const void* toks, int token_bits, const void* 
   const tokens::Space s = tokens::space_at(workspace, n, V, d);
   if (!workspace || workspace_bytes < s.bytes) return KRSI_ERR_WORKSPACE;
   if (!aligned16(workspace)) return KRSI_ERR_MISALIGNED;
-  KRSI_CUDA_TRY(tokens::token_sort(toks, token_bits, n, V, padding_idx, s.start, s.pos, s.tok, stream));
-  KRSI_EMB_DISPATCH(bwd, g, dtable, g, s, dtable, n, V, d, scale, stream)
+  KRSI_EMB_DISPATCH(bwd, g, dtable, toks, token_bits, g, s, dtable, n, V, d, scale, padding_idx, stream)
 }

@@ -189,7 +189,9 @@ __device__ __forceinline__ Cols dequantise(const Bytes& b, uint32_t e) {
 }
 
 // One item, 8 columns of both halves of a row, per thread, in row order: many short blocks, all of whose
-// loads are issued at once, keep more in flight than fewer blocks that loop (Q8_LAYOUT).
+// loads are issued at once, keep more in flight than fewer blocks that loop over the rows
+// (measured at 32,768 rows of F = 4,608 in bf16: 212 and 203 us forward and backward, against 277 and 290 with 8
+// looping blocks per SM, and 228 and 261 with two items per thread).
 struct Rows {
   uint32_t items, slots, mul, shift;   // slots: items per row, divided by as (umulhi(i, mul) + i) >> shift
   int F;

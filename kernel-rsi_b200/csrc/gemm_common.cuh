@@ -25,6 +25,27 @@ __device__ __forceinline__ void drain_loads(uint64_t* full, int issued, uint32_t
 // 16 elements inside the swizzle row advances the start address by 32 B.
 __device__ __forceinline__ uint64_t kmajor_sw128(uint32_t addr) { return smem_desc(addr, 16, 1024, kSw128); }
 
+// The tensor maps are made by the driver API, which wants a context current to the calling thread; a
+// thread that has made no runtime call yet (an autograd worker) may have none.  Gives it the primary one
+// then (cudaSetDevice, which stream capture allows), and leaves a context that is there alone.
+inline cudaError_t bind_context() {
+  using GetCurrent = CUresult (*)(CUcontext*);
+  static GetCurrent get = nullptr;
+  if (!get) {
+    cudaDriverEntryPointQueryResult q;
+    void* p = nullptr;
+    const cudaError_t e = cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q);
+    if (e != cudaSuccess) return e;
+    if (q != cudaDriverEntryPointSuccess) return cudaErrorNotSupported;
+    get = reinterpret_cast<GetCurrent>(p);
+  }
+  CUcontext ctx = nullptr;
+  if (get(&ctx) == CUDA_SUCCESS && ctx != nullptr) return cudaSuccess;
+  int dev = 0;
+  const cudaError_t e = cudaGetDevice(&dev);
+  return e != cudaSuccess ? e : cudaSetDevice(dev);
+}
+
 // 2-D view (cols, rows) of a row-major 16-bit matrix with `pitch` elements between rows, copied in
 // boxes of box_cols x box_rows with the given swizzle.  Loads read elements past cols or rows as
 // zero; stores skip them.

@@ -266,13 +266,14 @@ template <int DT, typename I>
 __global__ void __launch_bounds__(256)
 ce_target_kernel(const typename Elem<DT>::T* __restrict__ x, const typename Elem<DT>::T* __restrict__ w,
                  const I* __restrict__ targets, int* __restrict__ tgt, float* __restrict__ l2t,
-                 float* __restrict__ l2t_low, int* __restrict__ marked, int n, int V, int K, long long ignore, float c) {
+                 float* __restrict__ l2t_low, int* __restrict__ marked, int* __restrict__ ticket, int n, int V, int K, long long ignore, float c) {
   pdl_enter();
   using E = Elem<DT>;
   using T = typename E::T;
   const int row = (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32), lane = threadIdx.x % 32;
   if (row >= n) return;
   if (row % (2 * kBM) == 0 && lane == 0) marked[row / (2 * kBM)] = 0;
+  if (row == 0 && lane == 0) *ticket = 0;
   const long long t = (long long)targets[row];
   const int code = target_code(t, ignore, V);
   float dot = 0.f;
@@ -445,7 +446,50 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
 }
 
 // ---------------------------------------------------------------- 3: rows
+// The reduced loss and the weight of each row in it, by one block, in a fixed order.
+template <int NT>
+__device__ __forceinline__ void reduce_rows(const float* loss, const int* tgt, float* out, int n, int mean) {
+  __shared__ double sums[NT / 32];
+  __shared__ int counts[NT / 32];
+  double s = 0.0;
+  int c = 0;
+#pragma unroll 8
+  for (int i = threadIdx.x; i < n; i += NT) {
+    s += (double)__ldcg(loss + i);
+    c += __ldcg(tgt + i) != kIgnored;
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    c += __shfl_xor_sync(0xffffffffu, c, o);
+  }
+  if (threadIdx.x % 32 == 0) {
+    sums[threadIdx.x / 32] = s;
+    counts[threadIdx.x / 32] = c;
+  }
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    s = 0.0;
+    c = 0;
+    for (int w = 0; w < NT / 32; ++w) {
+      s += sums[w];
+      c += counts[w];
+    }
+    const int m = mean ? (c > 1 ? c : 1) : 1;
+    out[0] = (float)(s / m);
+    out[1] = (float)(1.0 / m);
+  }
+}
+__global__ void __launch_bounds__(1024)
+ce_reduce_kernel(const float* __restrict__ loss, const int* __restrict__ tgt, float* __restrict__ out, int n, int mean) {
+  pdl_enter();
+  reduce_rows<1024>(loss, tgt, out, n, mean);
+}
+
 struct JoinArgs {
+  float* reduced;          // with few rows the last block to finish reduces the losses itself; or null
+  int* ticket;             // blocks that have finished (zeroed by ce_target_kernel)
+  int mean;
   const float2* part;      // [rows][n_part]
   int n_part;
   const int* tgt;
@@ -543,13 +587,8 @@ ce_rows_kernel(const RowsArgs a) {
 }
 
 template <int DT>
-__global__ void __launch_bounds__(256)
-ce_join_kernel(const JoinArgs a) {
-  pdl_enter();
-  using E = Elem<DT>;
-  using T = typename E::T;
-  const int row = (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32), lane = threadIdx.x % 32;
-  if (row >= a.rows) return;
+__device__ __forceinline__ void join_row(const JoinArgs& a, int row, int lane) {
+  using T = typename Elem<DT>::T;
   const int t = a.tgt[row];
   const float l2t = a.l2t[row];
   const float2* pr = a.part + (int64_t)row * a.n_part;
@@ -602,41 +641,21 @@ ce_join_kernel(const JoinArgs a) {
   }
   copy.write(xr, reinterpret_cast<T*>(a.xs) + (int64_t)row * a.K, a.K, lane, soft, dead);
 }
-
-// The reduced loss and the weight of each row in it, one block, in a fixed order.
-__global__ void __launch_bounds__(1024)
-ce_reduce_kernel(const float* __restrict__ loss, const int* __restrict__ tgt, float* __restrict__ out, int n, int mean) {
+template <int DT>
+__global__ void __launch_bounds__(256)
+ce_join_kernel(const JoinArgs a) {
   pdl_enter();
-  __shared__ double sums[32];
-  __shared__ int counts[32];
-  double s = 0.0;
-  int c = 0;
-#pragma unroll 8
-  for (int i = threadIdx.x; i < n; i += 1024) {
-    s += (double)loss[i];
-    c += tgt[i] != kIgnored;
-  }
-#pragma unroll
-  for (int o = 16; o > 0; o >>= 1) {
-    s += __shfl_xor_sync(0xffffffffu, s, o);
-    c += __shfl_xor_sync(0xffffffffu, c, o);
-  }
-  if (threadIdx.x % 32 == 0) {
-    sums[threadIdx.x / 32] = s;
-    counts[threadIdx.x / 32] = c;
-  }
+  const int row = (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32);
+  if (row < a.rows) join_row<DT>(a, row, threadIdx.x % 32);
+  if (a.reduced == nullptr) return;
+  __shared__ bool last;
+  __threadfence();    // this block's losses before its ticket
   __syncthreads();
-  if (threadIdx.x == 0) {
-    s = 0.0;
-    c = 0;
-    for (int w = 0; w < 32; ++w) {
-      s += sums[w];
-      c += counts[w];
-    }
-    const int m = mean ? (c > 1 ? c : 1) : 1;
-    out[0] = (float)(s / m);
-    out[1] = (float)(1.0 / m);
-  }
+  if (threadIdx.x == 0) last = atomicAdd(a.ticket, 1) == (int)gridDim.x - 1;
+  __syncthreads();
+  if (!last) return;
+  __threadfence();
+  reduce_rows<256>(a.loss, a.tgt, a.reduced, a.rows, a.mean);
 }
 
 // The largest |g weight| over the rows that are not ignored (a fixed result whatever the order).
@@ -676,9 +695,9 @@ struct GradArgs {
   const float* factor;
   const float* coef;
   const void* w;
-  // dw: fp32 sums, stored or added; or scaled and rounded, and for the tokens that occur (token_rows.cuh's
-  // start) the fp32 sums as well, rows of `sums`
-  int dw32, accumulate;
+  // dw: fp32 sums, stored or added; or scaled and rounded, and for the tokens that occur (by token_rows.cuh's
+  // start, or with few rows by tgt itself) the fp32 sums as well, rows of `sums`
+  int dw32, accumulate, few;
   float* sums;
   const int* start;
   tokens::Order order;
@@ -764,10 +783,14 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
       [&](const GradItem& m) {
         const int row = m.tile * (2 * kBM) + rank * kBM + (warp % 4) * 32 + lane;   // of dx, or the token of dw
         GradRow r{1.f, 0.f, false, -1, nullptr};
+        const bool few = !m.is_dx && a.sums && a.few;
+        const unsigned near = few ? tokens::tokens_near(a.tgt, a.rows, row - lane) : 0;
         if (row >= (m.is_dx ? a.rows : a.V)) return r;
         if (!m.is_dx) {
           r.mul = a.alpha * a.up.unit();
-          if (a.sums) {
+          if (few) {
+            if (near >> lane & 1) r.sums = a.sums + (int64_t)row * a.K;
+          } else if (a.sums) {
             const int k = a.order.key(row);
             if (a.start[k] < a.start[k + 1]) r.sums = a.sums + (int64_t)row * a.K;
           }
@@ -1109,7 +1132,7 @@ struct Space {
   float *dw32, *dx_part;
   int* tgt;
   float *l2t, *l2t_low, *coef, *factor, *ref, *g_top;
-  int* marked;
+  int *marked, *ticket;
   tokens::Space sorted;
   size_t bytes;
 };
@@ -1127,6 +1150,7 @@ inline Space space_at(void* base, const Plan& p) {
   s.l2t = reinterpret_cast<float*>(take((size_t)p.N * 4));
   s.l2t_low = reinterpret_cast<float*>(take((size_t)p.N * 4));
   s.marked = reinterpret_cast<int*>(take((size_t)(p.N / 256 + 1) * 4));
+  s.ticket = reinterpret_cast<int*>(take(4));
   s.part = reinterpret_cast<float2*>(p.known ? 0 : take((size_t)rows * 2 * p.n_vt * 8));
   if (p.grads) {
     s.coef = reinterpret_cast<float*>(take((size_t)p.N * 4));
@@ -1175,7 +1199,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   Upstream up{c.g, c.g_stride, c.weight, nullptr, F16};
   if (!known) {
     auto kern = [&](auto k, auto* t) {
-      return launch_pdl(k, row_grid, dim3(256), 0, stream, x, w, t, s.tgt, s.l2t, s.l2t_low, s.marked, N, V, K,
+      return launch_pdl(k, row_grid, dim3(256), 0, stream, x, w, t, s.tgt, s.l2t, s.l2t_low, s.marked, s.ticket, N, V, K,
                         (long long)c.ignore, c2);
     };
     KRSI_CUDA_TRY(wide ? kern(ce_target_kernel<DT, long long>, (const long long*)c.targets)
@@ -1189,7 +1213,10 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     up.top = s.g_top;
   }
   const float e_scale = F16 ? kHalfScale : 1.f;
-  if (p.grads && c.dw)
+  const bool few = p.N <= tokens::kFewRows;
+  // Up to 4096 rows the join's last block reduces the losses (16 a thread); above, a block of 1024 threads.
+  const bool joined = p.chunks == 1 && p.N <= 4096;
+  if (p.grads && c.dw && !few)
     KRSI_CUDA_TRY(tokens::token_sort(c.targets, c.target_bits, N, V, c.ignore, s.sorted.start, s.sorted.pos,
                                      s.sorted.tok, stream));
 
@@ -1250,6 +1277,9 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     } else {
       KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
       JoinArgs ja{};
+      ja.reduced = joined ? c.reduced : nullptr;
+      ja.ticket = s.ticket;
+      ja.mean = c.mean;
       ja.part = s.part;
       ja.n_part = 2 * (int)p.n_vt;
       ja.tgt = s.tgt + r0;
@@ -1307,6 +1337,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     ga.dw32 = !p.direct;
     ga.accumulate = r0 > 0;
     ga.sums = p.direct ? dw32 : nullptr;
+    ga.few = few;
     ga.start = s.sorted.start;
     ga.order = s.sorted.order;
     ga.up = up;
@@ -1329,10 +1360,12 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   if (p.grads && c.dw) {   // the targets' part of dw
     if (p.direct) {
       const DwRows<DT> out{dw32, (T*)c.dw, p.K, c.scale};
-      KRSI_CUDA_TRY((tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
+      KRSI_CUDA_TRY(few ? (tokens::sum_few<DT, 8, true>(x, s.coef, (const int*)s.tgt, out, false, N, V, -1, K, stream))
+                        : (tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
     } else {
       const DwSums out{dw32, p.K};
-      KRSI_CUDA_TRY((tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
+      KRSI_CUDA_TRY(few ? (tokens::sum_few<DT, 8, true>(x, s.coef, (const int*)s.tgt, out, false, N, V, -1, K, stream))
+                        : (tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
       if (known) {
         const int64_t n = p.V * p.K;
         KRSI_CUDA_TRY(launch_pdl(ce_finish_kernel<DT>, dim3((unsigned)std::min<int64_t>(ceil_div(n, 2048), 148 * 64)),
@@ -1341,7 +1374,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       }
     }
   }
-  if (c.reduced)
+  if (c.reduced && !joined)
     KRSI_CUDA_TRY(launch_pdl(ce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)c.loss,
                              (const int*)s.tgt, c.reduced, N, c.mean));
   return KRSI_OK;
@@ -1366,6 +1399,7 @@ inline int run_checked(const Call& c, int64_t N, int64_t V, int64_t K, void* wor
   const Space s = space_at(workspace, p);
   if (!workspace || workspace_bytes < s.bytes) return KRSI_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return KRSI_ERR_MISALIGNED;
+  KRSI_CUDA_TRY(gemm::bind_context());
   return dtype == KRSI_F16 ? run<true>(c, p, s, pairs, stream) : run<false>(c, p, s, pairs, stream);
 }
 

@@ -14,6 +14,9 @@
 //   4. place: each warp walks its list again and writes the entries.
 // Lists hold a tile of kTile positions; more positions take the steps tile by tile, and 1 again before 4.
 // The order is fixed: by group, token, warp, tile and position.
+// Measured at 32,768 tokens of a vocabulary of 32,768, ids as frequent as one over their rank: 12 us. (With
+// contiguous ranges in place of the interleaved groups one block had half of the tokens: 41 us; with every
+// step counted and ranked at once, without lists: 24 us.)
 #include "token_rows.cuh"
 
 namespace krsi {
@@ -156,8 +159,7 @@ cudaError_t launch(const void* toks, int64_t n, int64_t V, int64_t skip, int* st
   const int share = (int)((tile + 32 * kWarps - 1) / (32 * kWarps) * 32);
   const size_t smem = (size_t)kWarps * (order.range + share) * sizeof(int);
   static_assert(kWarps * (kMaxRange + kShare) * sizeof(int) <= 232448 - 1024, "shared memory budget");
-  cudaError_t e = cudaFuncSetAttribute(token_sort_kernel<T>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)(kWarps * (kMaxRange + kShare) * sizeof(int)));
+  const cudaError_t e = allow_smem<token_sort_kernel<T>>((int)(kWarps * (kMaxRange + kShare) * sizeof(int)));
   if (e != cudaSuccess) return e;
   return launch_pdl(token_sort_kernel<T>, dim3(1u << order.bits), dim3(kThreads), smem, stream, (const T*)toks, (int)n,
                     (int)V, (int)skip, order, share, start, pos, tok);
