@@ -237,13 +237,14 @@ int krsi_geglu_q8_bwd(const void* g, const void* q, const void* exponents, void*
 /* Bytes of workspace: mode 0 krsi_linear_ce_fwd without gradients, 1 with, 2 krsi_linear_ce_grad. */
 int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, int mode, size_t* bytes);
 
-/* loss: [N] fp32.  reduced: two floats or null: the sum of the losses (mean: divided by the number of
- * rows that are not ignored, at least 1) and the weight of one row in it (1, or one over that number).
+/* loss: [N] fp32.  total, weight: one float each, or both null: the sum of the losses (mean: divided by
+ * the number of rows that are not ignored, at least 1), and the weight of one row in it (1, or one over
+ * that number).
  * stats: [N, 2] fp32 for krsi_linear_ce_grad (8-byte aligned), or null.
  * dx, dw: null, or fp32 gradients of the sum of the losses without the factor `scale`, for
  * krsi_linear_ce_finish: the logits are computed once for loss and gradients. */
 int krsi_linear_ce_fwd(const void* x, const void* w, const void* targets, int target_bits, float* loss,
-                       float* reduced, float* stats, float* dx, float* dw, void* workspace,
+                       float* total, float* weight, float* stats, float* dx, float* dw, void* workspace,
                        size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss, int mean,
                        int dtype, cudaStream_t stream);
 

@@ -448,7 +448,8 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
 // ---------------------------------------------------------------- 3: rows
 // The reduced loss and the weight of each row in it, by one block, in a fixed order.
 template <int NT>
-__device__ __forceinline__ void reduce_rows(const float* loss, const int* tgt, float* out, int n, int mean) {
+__device__ __forceinline__ void reduce_rows(const float* loss, const int* tgt, float* total, float* weight, int n,
+                                            int mean) {
   __shared__ double sums[NT / 32];
   __shared__ int counts[NT / 32];
   double s = 0.0;
@@ -476,18 +477,19 @@ __device__ __forceinline__ void reduce_rows(const float* loss, const int* tgt, f
       c += counts[w];
     }
     const int m = mean ? (c > 1 ? c : 1) : 1;
-    out[0] = (float)(s / m);
-    out[1] = (float)(1.0 / m);
+    *total = (float)(s / m);
+    *weight = (float)(1.0 / m);
   }
 }
 __global__ void __launch_bounds__(1024)
-ce_reduce_kernel(const float* __restrict__ loss, const int* __restrict__ tgt, float* __restrict__ out, int n, int mean) {
+ce_reduce_kernel(const float* __restrict__ loss, const int* __restrict__ tgt, float* __restrict__ total,
+                 float* __restrict__ weight, int n, int mean) {
   pdl_enter();
-  reduce_rows<1024>(loss, tgt, out, n, mean);
+  reduce_rows<1024>(loss, tgt, total, weight, n, mean);
 }
 
 struct JoinArgs {
-  float* reduced;          // with few rows the last block to finish reduces the losses itself; or null
+  float *total, *weight;   // with few rows the last block to finish reduces the losses itself; or null
   int* ticket;             // blocks that have finished (zeroed by ce_target_kernel)
   int mean;
   const float2* part;      // [rows][n_part]
@@ -647,7 +649,7 @@ ce_join_kernel(const JoinArgs a) {
   pdl_enter();
   const int row = (int)(blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32);
   if (row < a.rows) join_row<DT>(a, row, threadIdx.x % 32);
-  if (a.reduced == nullptr) return;
+  if (a.total == nullptr) return;
   __shared__ bool last;
   __threadfence();    // this block's losses before its ticket
   __syncthreads();
@@ -655,7 +657,7 @@ ce_join_kernel(const JoinArgs a) {
   __syncthreads();
   if (!last) return;
   __threadfence();
-  reduce_rows<256>(a.loss, a.tgt, a.reduced, a.rows, a.mean);
+  reduce_rows<256>(a.loss, a.tgt, a.total, a.weight, a.rows, a.mean);
 }
 
 // The largest |g weight| over the rows that are not ignored (a fixed result whatever the order).
@@ -1173,7 +1175,7 @@ struct Call {
   const void *x, *w, *targets;
   int target_bits;
   float* loss;             // [N] rows: the forward; null: gradients from stats
-  float* reduced;          // (loss, weight) or null
+  float *total, *row_weight;   // the reduced loss and the weight of a row in it, or null
   int mean;
   float2* stats;           // [N]: written by the forward (or null), read by the gradients
   const float* g;
@@ -1277,7 +1279,8 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     } else {
       KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
       JoinArgs ja{};
-      ja.reduced = joined ? c.reduced : nullptr;
+      ja.total = joined ? c.total : nullptr;
+      ja.weight = c.row_weight;
       ja.ticket = s.ticket;
       ja.mean = c.mean;
       ja.part = s.part;
@@ -1374,9 +1377,9 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       }
     }
   }
-  if (c.reduced && !joined)
+  if (c.total && !joined)
     KRSI_CUDA_TRY(launch_pdl(ce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)c.loss,
-                             (const int*)s.tgt, c.reduced, N, c.mean));
+                             (const int*)s.tgt, c.total, c.row_weight, N, c.mean));
   return KRSI_OK;
 }
 
@@ -1417,20 +1420,21 @@ extern "C" int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, in
 }
 
 extern "C" int krsi_linear_ce_fwd(const void* x, const void* w, const void* targets, int target_bits, float* loss,
-                                  float* reduced, float* stats, float* dx, float* dw, void* workspace,
-                                  size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss,
+                                  float* total, float* weight, float* stats, float* dx, float* dw,
+                                  void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss,
                                   int mean, int dtype, cudaStream_t stream) {
   const int rc = check(N, V, K, target_bits, dtype);
   if (rc != KRSI_OK) return rc;
+  KRSI_CHECK_ARG((total != nullptr) == (weight != nullptr));
   if (N == 0) {
     if (dw) KRSI_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)V * K * 4, stream));
-    if (reduced) KRSI_CUDA_TRY(launch_pdl(ce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)nullptr,
-                                          (const int*)nullptr, reduced, 0, mean));
+    if (total) KRSI_CUDA_TRY(launch_pdl(ce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)nullptr,
+                                        (const int*)nullptr, total, weight, 0, mean));
     return KRSI_OK;
   }
   KRSI_CHECK_ARG(x && w && targets && loss);
   if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) return KRSI_ERR_MISALIGNED;
-  const Call c{x, w, targets, target_bits, loss, reduced, mean, reinterpret_cast<float2*>(stats), nullptr, 0, nullptr, dx, dw, scale, z_loss,
+  const Call c{x, w, targets, target_bits, loss, total, weight, mean, reinterpret_cast<float2*>(stats), nullptr, 0, nullptr, dx, dw, scale, z_loss,
                ignore_index};
   return run_checked(c, N, V, K, workspace, workspace_bytes, dtype, stream);
 }
@@ -1448,7 +1452,7 @@ extern "C" int krsi_linear_ce_grad(const void* x, const void* w, const void* tar
   }
   KRSI_CHECK_ARG(x && w && targets && g && stats);
   if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) return KRSI_ERR_MISALIGNED;
-  const Call c{x, w, targets, target_bits, nullptr, nullptr, 0,
+  const Call c{x, w, targets, target_bits, nullptr, nullptr, nullptr, 0,
                const_cast<float2*>(reinterpret_cast<const float2*>(stats)), g, g_stride, weight, dx, dw, scale, z_loss,
                ignore_index};
   return run_checked(c, N, V, K, workspace, workspace_bytes, dtype, stream);

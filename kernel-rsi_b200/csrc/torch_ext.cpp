@@ -409,9 +409,9 @@ CeCall ce_call(const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor&
   return c;
 }
 
-// (loss rows, [loss, row weight], stats, dx, dw): stats is for linear_ce_grad; the gradients are fp32, of the sum of the losses and without
+// (loss rows, loss, row weight, stats, dx, dw): stats is for linear_ce_grad; the gradients are fp32, of the sum of the losses and without
 // `scale`, or empty.  reduction 0 none, 1 mean, 2 sum.
-std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(
+std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(
     const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor& targets_in, double scale, int64_t ignore_index,
     double z_loss, int64_t reduction, bool want_dx, bool want_dw) {
   TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
@@ -419,17 +419,20 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce
   const CeCall c = ce_call(x_in, w_in, targets_in, want_dx || want_dw ? 1 : 0);
   auto f32 = c.x.options().dtype(at::kFloat);
   auto loss = at::empty({c.N}, f32);
-  auto reduced = at::empty({reduction != 0 ? 2 : 0}, f32);
+  // (tensors of their own: the weight is saved, and a caller may change the loss in place)
+  auto total = reduction != 0 ? at::empty({}, f32) : at::empty({0}, f32);
+  auto weight = at::empty({reduction != 0 ? 1 : 0}, f32);
   auto stats = at::empty({c.N, 2}, f32);
   auto dx = at::empty({want_dx ? c.N : 0, c.K}, f32);
   auto dw = at::empty({want_dw ? c.V : 0, c.K}, f32);
   check_rc(krsi_linear_ce_fwd(c.x.data_ptr(), c.w.data_ptr(), c.targets.data_ptr(), c.bits, loss.data_ptr<float>(),
-                              reduction != 0 ? reduced.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
+                              reduction != 0 ? total.data_ptr<float>() : nullptr,
+                              reduction != 0 ? weight.data_ptr<float>() : nullptr, stats.data_ptr<float>(),
                               want_dx ? dx.data_ptr<float>() : nullptr, want_dw ? dw.data_ptr<float>() : nullptr,
                               c.ws.data_ptr(), (size_t)c.ws.numel(), c.N, c.V, c.K, (float)scale, ignore_index,
                               (float)z_loss, reduction == 1, c.dtype, at::cuda::getCurrentCUDAStream()),
            "krsi_linear_ce_fwd");
-  return {loss, reduced, stats, dx, dw};
+  return {loss, total, weight, stats, dx, dw};
 }
 
 // Gradients in x2d's dtype for g, the upstream gradient of each row's loss ([N], or one for all), times
@@ -488,6 +491,11 @@ at::Tensor linear_ce_finish(const at::Tensor& grad, const at::Tensor& g_in, cons
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
+// A gradient of the gradient is not built: it would come back as zero, so it is refused.
+void check_once(const char* what) {
+  TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the backward has no gradient of its own (create_graph)");
+}
+
 struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& tokens, const at::Tensor& table, double scale,
                             int64_t padding_idx) {
@@ -498,6 +506,7 @@ struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
     return embedding_fwd(tokens, table, scale, padding_idx);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once("embedding");
     const auto saved = ctx->get_saved_variables();
     return {at::Tensor(),
             embedding_bwd(g[0], saved[0], saved[1], ctx->saved_data["scale"].toDouble(),
@@ -520,6 +529,7 @@ struct GegluQ8Node : public torch::autograd::Function<GegluQ8Node> {
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once("geglu_q8");
     const auto saved = ctx->get_saved_variables();
     return {std::get<0>(geglu_q8_bwd(g[0], saved[0], saved[1], false))};
   }
@@ -534,26 +544,26 @@ at::Tensor geglu_q8_plain(const at::Tensor& u) { return std::get<0>(geglu_q8_fwd
 // keep: form the gradients in the forward (saved in fp32) instead of saving the operands.
 at::Tensor linear_ce_plain(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, double scale,
                            int64_t ignore_index, double z_loss, int64_t reduction, bool /*keep*/) {
-  auto [loss, reduced, stats, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction, false, false);
-  return reduction != 0 ? reduced.select(0, 0) : loss;
+  auto [loss, total, weight, stats, dx, dw] =
+      linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction, false, false);
+  return reduction != 0 ? total : loss;
 }
 struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
                             double scale, int64_t ignore_index, double z_loss, int64_t reduction, bool keep) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [loss, reduced, stats, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction,
-                                                 keep && x.requires_grad(), keep && w.requires_grad());
-    auto out = reduction != 0 ? reduced.select(0, 0) : loss;
-    auto weight = reduced.slice(0, 1);
+    auto [loss, total, weight, stats, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction,
+                                                              keep && x.requires_grad(), keep && w.requires_grad());
     if (keep) ctx->save_for_backward({weight, dx, dw, w});
     else ctx->save_for_backward({weight, stats, x, w, targets});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["ignore_index"] = ignore_index;
     ctx->saved_data["z_loss"] = z_loss;
     ctx->saved_data["keep"] = keep;
-    return out;
+    return reduction != 0 ? total : loss;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once("linear_cross_entropy");
     const auto saved = ctx->get_saved_variables();
     const double scale = ctx->saved_data["scale"].toDouble();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
@@ -601,7 +611,7 @@ TORCH_LIBRARY(krsi, m) {
   m.def("linear_ce(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, int reduction, "
         "bool keep) -> Tensor");
   m.def("linear_ce_fwd(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, "
-        "int reduction, bool want_dx, bool want_dw) -> (Tensor, Tensor, Tensor, Tensor, Tensor)");
+        "int reduction, bool want_dx, bool want_dw) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)");
   m.def("linear_ce_grad(Tensor g, Tensor weight, Tensor stats, Tensor x2d, Tensor w, Tensor targets, float scale, "
         "int ignore_index, float z_loss, bool want_dx, bool want_dw) -> (Tensor, Tensor)");
   m.def("linear_ce_finish(Tensor grad, Tensor g, Tensor weight, float scale, Tensor like) -> Tensor");

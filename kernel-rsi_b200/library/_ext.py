@@ -133,8 +133,8 @@ def _register_compile_support() -> None:
     @reg_fake("krsi::linear_ce_fwd")
     def _(x2d, w, targets, scale, ignore_index, z_loss, reduction, want_dx, want_dw):
         f32 = torch.float32
-        return (x2d.new_empty((x2d.shape[0],), dtype=f32), x2d.new_empty((2 if reduction else 0,), dtype=f32),
-                x2d.new_empty((x2d.shape[0], 2), dtype=f32),
+        return (x2d.new_empty((x2d.shape[0],), dtype=f32), x2d.new_empty(() if reduction else (0,), dtype=f32),
+                x2d.new_empty((1 if reduction else 0,), dtype=f32), x2d.new_empty((x2d.shape[0], 2), dtype=f32),
                 x2d.new_empty((x2d.shape[0] if want_dx else 0, x2d.shape[1]), dtype=f32),
                 x2d.new_empty((w.shape[0] if want_dw else 0, w.shape[1]), dtype=f32))
 
@@ -227,27 +227,27 @@ def _register_compile_support() -> None:
 
     def ce_setup(ctx, inputs, output):
         x2d, w, targets, scale, ignore_index, z_loss, reduction, want_dx, want_dw = inputs
-        loss, reduced, stats, dx, dw = output
+        loss, total, weight, stats, dx, dw = output
         ctx.args = (scale, ignore_index, z_loss)
         ctx.reduction, ctx.kept, ctx.wanted = reduction, want_dx or want_dw, (want_dx, want_dw)
         ctx.set_materialize_grads(False)
         if ctx.kept:
-            ctx.save_for_backward(reduced, dx, dw, w)
+            ctx.save_for_backward(weight, dx, dw, w)
         else:
-            ctx.save_for_backward(reduced, stats, x2d, w, targets)
+            ctx.save_for_backward(weight, stats, x2d, w, targets)
 
-    def ce_backward(ctx, gloss, greduced, _gstats, _gdx, _gdw):
-        g = gloss if ctx.reduction == 0 else greduced[0] if greduced is not None else None
+    def ce_backward(ctx, gloss, gtotal, _gweight, _gstats, _gdx, _gdw):
+        g = gloss if ctx.reduction == 0 else gtotal
         none = (None,) * 7
         if g is None:
             return (None, None) + none
-        reduced, *saved = ctx.saved_tensors
+        weight, *saved = ctx.saved_tensors
         if ctx.kept:
             dx, dw, like = saved
-            return (ops.linear_ce_finish(dx, g, reduced[1:], ctx.args[0], like) if ctx.wanted[0] else None,
-                    ops.linear_ce_finish(dw, g, reduced[1:], ctx.args[0], like) if ctx.wanted[1] else None) + none
+            return (ops.linear_ce_finish(dx, g, weight, ctx.args[0], like) if ctx.wanted[0] else None,
+                    ops.linear_ce_finish(dw, g, weight, ctx.args[0], like) if ctx.wanted[1] else None) + none
         need = ctx.needs_input_grad[:2]
-        dx, dw = ops.linear_ce_grad(g, reduced[1:], *saved, *ctx.args, *need)
+        dx, dw = ops.linear_ce_grad(g, weight, *saved, *ctx.args, *need)
         return (dx if need[0] else None, dw if need[1] else None) + none
 
     torch.library.register_autograd("krsi::linear_ce_fwd", ce_backward, setup_context=ce_setup)

@@ -41,9 +41,9 @@ def linear_cross_entropy(x2d, w, targets, scale=1.0, ignore_index=-100, z_loss=0
     keep = kind != 0 and x2d.shape[0] >= KEEP_ROWS
     if compiling():
         keep = keep and torch.is_grad_enabled()
-        loss, reduced, _, _, _ = ops.linear_ce_fwd(x2d, w, targets, scale, ignore_index, z_loss, kind,
+        loss, total, *_ = ops.linear_ce_fwd(x2d, w, targets, scale, ignore_index, z_loss, kind,
                                                 keep and x2d.requires_grad, keep and w.requires_grad)
-        return reduced[0] if kind else loss
+        return total if kind else loss
     return ops.linear_ce(x2d, w, targets, scale, ignore_index, z_loss, kind, keep)
 
 

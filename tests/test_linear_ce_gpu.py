@@ -296,6 +296,20 @@ def test_gradient_against_differences():
         assert abs((dx.double() * d.double()).sum() - quot) <= truncation + noise
 
 
+def test_a_loss_changed_in_place_and_no_gradient_of_the_gradient():
+    for N in (64, KEEP_ROWS):
+        x, w, t = inputs(N, 300, 64, torch.bfloat16, 15)
+        want = run(x, w, t, torch.tensor(0.25, device=dev))
+        a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+        loss = linear_cross_entropy(a, b, t)
+        loss /= 4
+        assert torch.allclose(loss, want[0] / 4)
+        for g, h in zip(torch.autograd.grad(loss, (a, b)), want[1:]):
+            assert torch.equal(g, h)
+        with pytest.raises(RuntimeError, match="create_graph"):
+            torch.autograd.grad(linear_cross_entropy(a, b, t), a, create_graph=True)
+
+
 def test_compiled_matches_eager():
     for N in (100, KEEP_ROWS):
         x, w, t = inputs(N, 600, 64, torch.bfloat16, 12)
@@ -368,6 +382,6 @@ def test_refusals():
     vp, i64, f32 = ctypes.c_void_p, ctypes.c_int64, ctypes.c_float
     loss = torch.empty(10, device=dev)
     call = lambda ws, size: capi().krsi_linear_ce_fwd(  # noqa: E731
-        vp(x.data_ptr()), vp(w.data_ptr()), vp(t.data_ptr()), 64, vp(loss.data_ptr()), vp(0), vp(0), vp(0), vp(0), vp(ws),
+        vp(x.data_ptr()), vp(w.data_ptr()), vp(t.data_ptr()), 64, vp(loss.data_ptr()), vp(0), vp(0), vp(0), vp(0), vp(0), vp(ws),
         ctypes.c_size_t(size), i64(10), i64(20), i64(64), f32(1.0), i64(-100), f32(0.0), 0, 1, vp(0))
     assert call(0, 1 << 20) == 4 and call(t.data_ptr(), 16) == 4

@@ -46,12 +46,12 @@ def test_fake_impls_give_the_shapes():
     du, again = ops.geglu_q8_bwd(m(4, 40), q, ex, True)
     assert du.shape == (4, 80) and again.shape == (4, 40)
     x, w, t = m(7, 24), m(100, 24), m(7, dtype=torch.long)
-    loss, red, stats, dx, dw = ops.linear_ce_fwd(x, w, t, 1.0, -100, 0.0, 1, True, False)
-    assert loss.shape == (7,) and red.shape == (2,) and stats.shape == (7, 2) and loss.dtype == torch.float32
+    loss, total, weight, stats, dx, dw = ops.linear_ce_fwd(x, w, t, 1.0, -100, 0.0, 1, True, False)
+    assert loss.shape == (7,) and total.shape == () and weight.shape == (1,) and stats.shape == (7, 2) and loss.dtype == torch.float32
     assert dx.shape == (7, 24) and dx.dtype == torch.float32 and dw.shape == (0, 24)
-    dx, dw = ops.linear_ce_grad(loss, red[1:], stats, x, w, t, 1.0, -100, 0.0, False, True)
+    dx, dw = ops.linear_ce_grad(loss, weight, stats, x, w, t, 1.0, -100, 0.0, False, True)
     assert dx.shape == (0, 24) and dw.shape == (100, 24) and dw.dtype == torch.bfloat16
-    assert ops.linear_ce_finish(m(7, 24, dtype=torch.float32), red[:1], red[1:], 1.0, x).dtype == torch.bfloat16
+    assert ops.linear_ce_finish(m(7, 24, dtype=torch.float32), total, weight, 1.0, x).dtype == torch.bfloat16
 
 
 def test_cpu_tensors_are_rejected():
@@ -99,7 +99,7 @@ def test_geglu_q8_argument_checks(lib):
 
 def test_linear_ce_argument_checks(lib):
     def fwd(x=16, w=16, t=16, bits=64, loss=16, n=4, V=10, K=64, dtype=1, stats=0):
-        return lib.krsi_linear_ce_fwd(vp(x), vp(w), vp(t), bits, vp(loss), vp(0), vp(stats), vp(0), vp(0), vp(256),
+        return lib.krsi_linear_ce_fwd(vp(x), vp(w), vp(t), bits, vp(loss), vp(0), vp(0), vp(stats), vp(0), vp(0), vp(256),
                                       size(1 << 30), i64(n), i64(V), i64(K), f32(1), i64(-100), f32(0), 0, dtype, vp(0))
 
     assert fwd(x=0) == 1 and fwd(loss=0) == 1 and fwd(bits=8) == 1 and fwd(n=-1) == 1 and fwd(V=0) == 1
