@@ -107,7 +107,8 @@ template <int DT, int VEC, bool WEIGHTED, typename Out>
 __global__ void __launch_bounds__(256)
 sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restrict__ weight,
                 const int* __restrict__ start, const int* __restrict__ pos, const int* __restrict__ tok,
-                float* __restrict__ partial, const Out out, const Order order, int chunks, int V, uint32_t packets) {
+                float* __restrict__ partial, const Out out, const Order order, int n, int chunks, int V,
+                uint32_t packets) {
   pdl_enter();
   using E = Elem<DT>;
   using P = Pack<typename E::T, VEC>;
@@ -124,12 +125,14 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
   const int i0 = chunk * kChunkRows;
   __shared__ int s_pos[kChunkRows], s_tok[kChunkRows + 1];
   __shared__ float s_weight[kChunkRows];
-  const int m = min(kChunkRows, start[order.range << order.bits] - i0);   // the entries of this chunk
+  // the chunk's entries, read beside the number that says how many of them there are
+  const bool mine = threadIdx.x < kChunkRows && i0 + (int)threadIdx.x < n;
+  const int p = mine ? pos[i0 + threadIdx.x] : 0, t = mine ? tok[i0 + threadIdx.x] : 0;
+  const int m = min(kChunkRows, start[order.range << order.bits] - i0);
   if (m <= 0) return;
   if (threadIdx.x < m) {
-    const int p = pos[i0 + threadIdx.x];
     s_pos[threadIdx.x] = p;
-    s_tok[threadIdx.x] = tok[i0 + threadIdx.x];
+    s_tok[threadIdx.x] = t;
     if (WEIGHTED) s_weight[threadIdx.x] = weight[p];
   }
   if (threadIdx.x == 0) s_tok[m] = -1;   // the chunk's end ends a run
@@ -352,12 +355,12 @@ cudaError_t sum_by_token(const void* g, const float* weight, const Space& s, con
   constexpr auto kern = sum_rows_kernel<DT, VEC, WEIGHTED, Out>;
   cudaError_t e = allow_smem<kern>(kChunkRows * 256 * 16);
   if (e != cudaSuccess) return e;
-  e = launch_pdl(kern, grid, dim3(threads), smem, stream, (const T*)g, weight,
-                 (const int*)s.start, (const int*)s.pos, (const int*)s.tok, s.partial, out, s.order, chunks,
-                             (int)V, packets);
+  e = launch_pdl(kern, grid, dim3(threads), smem, stream, (const T*)g, weight, (const int*)s.start,
+                 (const int*)s.pos, (const int*)s.tok, s.partial, out, s.order, (int)n, chunks, (int)V, packets);
   if (e != cudaSuccess || chunks == 1) return e;
   const dim3 join_grid((unsigned)((chunks - 1 + kJoinWarps - 1) / kJoinWarps), (unsigned)((d + 127) / 128));
-  return launch_pdl(join_rows_kernel<Out>, join_grid, dim3(32 * kJoinWarps), 0, stream, (const int*)s.start, (const int*)s.tok, (const float*)s.partial, out, s.order, (int)d);
+  return launch_pdl(join_rows_kernel<Out>, join_grid, dim3(32 * kJoinWarps), 0, stream, (const int*)s.start,
+                    (const int*)s.tok, (const float*)s.partial, out, s.order, (int)d);
 }
 
 }  // namespace tokens
