@@ -4,6 +4,10 @@
 // Both are bound by memory: the forward reads the looked-up rows and writes out; the backward reads g
 // once and writes every row of dtable once (zeros for tokens that do not occur).
 //
+// Measured at 32768 rows of 1152 bf16 values, vocabulary 32768 (B200): lookup 22 us (15 us at the copy rate), gradient
+// 50 us (24): the sort 12 us, which waits on L2, the sums 33, the long runs 6.  The lookup's rows are staged by
+// asynchronous copies; held in registers it took 34 us, too little being in flight.
+//
 // A token id outside [0, V) reads nothing: its row of out is NaN and it adds to no gradient.
 #include <algorithm>
 #include <type_traits>

@@ -96,8 +96,8 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 // The first blocks (if `chunks` is less than the grid) write the rows of tokens that do not occur,
 // kZeroTokens tokens each; the last `chunks` blocks sum one chunk of sorted entries each, one packet of
 // columns per thread.  A chunk's rows are staged in shared memory, all of its loads in flight at once: held
-// in registers they cost so many that a third as much was in flight (measured at 32,768 rows of 1,152 16-bit values: 34
-// us against 39).
+// in registers they cost so many that a third as much was in flight (measured at 32768 rows of 1152 16-bit
+// values: 33 us against 39).
 // Out: packet(v, c, sums) takes the VEC finished sums of token v's packet c, zero(v, c) an absent one,
 // column(v, col, sum) one finished column.
 constexpr int kZeroTokens = 32;
