@@ -78,7 +78,9 @@ struct TableRows {
   T* dtable;
   int64_t d;
   float scale;
-  __device__ __forceinline__ void packet(int v, uint32_t c, const float* sums) const {
+  using Base = tokens::NoBase;
+  __device__ __forceinline__ Base fetch(int, uint32_t) const { return {}; }
+  __device__ __forceinline__ void packet(int v, uint32_t c, const float* sums, Base) const {
     Pack<T, VEC> o;
 #pragma unroll
     for (int e = 0; e < VEC; ++e) o.v[e] = Elem<DT>::store(scale * sums[e]);

@@ -601,7 +601,7 @@ template <int DT>
 __device__ __forceinline__ void join_row(const JoinArgs& a, int row, int lane) {
   using T = typename Elem<DT>::T;
   const int t = a.tgt[row];
-  const float l2t = a.l2t[row];
+  const float l2t = a.l2t[row], l2t_low = a.l2t_low[row];
   const float2* pr = a.part + (int64_t)row * a.n_part;
   const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.K;
   RowCopy<DT> copy;        // on its way while the sums are added
@@ -621,7 +621,7 @@ __device__ __forceinline__ void join_row(const JoinArgs& a, int row, int lane) {
     lse2 = rest = pt = 0.f;
     lifted = false;
   } else if (!lifted) {
-    s = warp_sum(s) * exp2f(-a.l2t_low[row]);   // relative to the logit itself: a large one's rounding shows in s
+    s = warp_sum(s) * exp2f(-l2t_low);   // relative to the logit itself: a large one's rounding shows in s
     pt = 1.f / (1.f + s);
     rest = s * pt;
     lse2 = l2t + kLog2e * log1pf(s);
@@ -902,8 +902,9 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
       });
 }
 
-// dx from the shares of the vocabulary (`share` values apart, added in order): 4 columns per thread, 8
-// shares' loads in flight.
+// dx from the shares of the vocabulary (`share` values apart, added in order): 4 columns of kJoinRows rows
+// per thread, their loads in flight together.
+constexpr int kJoinRows = 4;
 template <int DT>
 __global__ void __launch_bounds__(128)
 ce_dx_join_kernel(const float* __restrict__ part, int splits, int64_t share, const int* __restrict__ tgt,
@@ -913,33 +914,44 @@ ce_dx_join_kernel(const float* __restrict__ part, int splits, int64_t share, con
   pdl_enter();
   using E = Elem<DT>;
   using T = typename E::T;
-  const uint32_t i = blockIdx.x * blockDim.x + threadIdx.x, packets = K / 4;
-  const uint32_t row = i / packets;
-  if (row >= rows) return;
-  const int col = (int)(i - row * packets) * 4;
-  const int64_t at = (int64_t)row * K + col;
-  const int t = tgt[row];
-  const float f = factor[row], c = coef[row];
-  tokens::Pack<T, 4> q;
-  if (t >= 0) q = *reinterpret_cast<const tokens::Pack<T, 4>*>(w + (int64_t)t * K + col);
-  float v[4] = {};
-#pragma unroll 8
+  const int col = (int)(blockIdx.x * blockDim.x + threadIdx.x) * 4;
+  if (col >= K) return;
+  const int row0 = blockIdx.y * kJoinRows;
+  int t[kJoinRows];
+  float v[kJoinRows][4] = {};
+#pragma unroll
+  for (int r = 0; r < kJoinRows; ++r) t[r] = row0 + r < rows ? tgt[row0 + r] : kIgnored;
+#pragma unroll 2
   for (int s = 0; s < splits; ++s) {
-    const float4 b = __ldg(reinterpret_cast<const float4*>(part + s * share + at));
-    v[0] += b.x; v[1] += b.y; v[2] += b.z; v[3] += b.w;
+#pragma unroll
+    for (int r = 0; r < kJoinRows; ++r) {
+      if (t[r] == kIgnored) continue;
+      const float4 b = __ldg(reinterpret_cast<const float4*>(part + s * share + (int64_t)(row0 + r) * K + col));
+      v[r][0] += b.x; v[r][1] += b.y; v[r][2] += b.z; v[r][3] += b.w;
+    }
   }
 #pragma unroll
-  for (int e = 0; e < 4; ++e) {
-    v[e] = t == kIgnored ? 0.f : f * v[e];
-    if (t >= 0) v[e] = fmaf(c, E::load(q.v[e]), v[e]);
-  }
-  if (dx32) {
-    *reinterpret_cast<float4*>(reinterpret_cast<float*>(dx) + at) = make_float4(v[0], v[1], v[2], v[3]);
-  } else {
-    tokens::Pack<T, 4> o;
+  for (int r = 0; r < kJoinRows; ++r) {
+    const int row = row0 + r;
+    if (row >= rows) break;
+    const int64_t at = (int64_t)row * K + col;
+    const float f = t[r] == kIgnored ? 0.f : factor[row];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o.v[e] = E::store(scale * v[e]);
-    *reinterpret_cast<tokens::Pack<T, 4>*>(reinterpret_cast<T*>(dx) + at) = o;
+    for (int e = 0; e < 4; ++e) v[r][e] *= f;
+    if (t[r] >= 0) {
+      const auto q = *reinterpret_cast<const tokens::Pack<T, 4>*>(w + (int64_t)t[r] * K + col);
+      const float c = coef[row];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[r][e] = fmaf(c, E::load(q.v[e]), v[r][e]);
+    }
+    if (dx32) {
+      *reinterpret_cast<float4*>(reinterpret_cast<float*>(dx) + at) = make_float4(v[r][0], v[r][1], v[r][2], v[r][3]);
+    } else {
+      tokens::Pack<T, 4> o;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o.v[e] = E::store(scale * v[r][e]);
+      *reinterpret_cast<tokens::Pack<T, 4>*>(reinterpret_cast<T*>(dx) + at) = o;
+    }
   }
 }
 
@@ -970,7 +982,9 @@ struct DwSums {
   int64_t K;
   // One addition per element and call, so a reduction in L2 (no read to wait for) gives the same bits
   // every time.
-  __device__ __forceinline__ void packet(int v, uint32_t c, const float* s) const {
+  using Base = tokens::NoBase;
+  __device__ __forceinline__ Base fetch(int, uint32_t) const { return {}; }
+  __device__ __forceinline__ void packet(int v, uint32_t c, const float* s, Base) const {
     float* p = dw32 + v * K + c * 8;
 #pragma unroll
     for (int h = 0; h < 8; h += 4)
@@ -988,16 +1002,21 @@ struct DwRows {
   T* dw;
   int64_t K;
   float scale;
-  __device__ __forceinline__ void packet(int v, uint32_t c, const float* s) const {
-    const int64_t at = v * K + c * 8;
-    const auto a = ldg16(sums + at), b = ldg16(sums + at + 4);
+  struct Base {
+    Vec16<float> a, b;
+  };
+  __device__ __forceinline__ Base fetch(int v, uint32_t c) const {
+    const float* p = sums + v * K + c * 8;
+    return {ldg16(p), ldg16(p + 4)};
+  }
+  __device__ __forceinline__ void packet(int v, uint32_t c, const float* s, const Base& base) const {
     Vec16<T> o;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      o.v[e] = Elem<DT>::store(scale * (a.v[e] + s[e]));
-      o.v[4 + e] = Elem<DT>::store(scale * (b.v[e] + s[4 + e]));
+      o.v[e] = Elem<DT>::store(scale * (base.a.v[e] + s[e]));
+      o.v[4 + e] = Elem<DT>::store(scale * (base.b.v[e] + s[4 + e]));
     }
-    stg16(dw + at, o);
+    stg16(dw + v * K + c * 8, o);
   }
   __device__ __forceinline__ void zero(int, uint32_t) const {}
   __device__ __forceinline__ void column(int v, int col, float s) const {
@@ -1114,7 +1133,7 @@ inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool known, i
   p.n_vt = ceil_div(V, kBN);
   p.panels = ceil_div(V, 64);
   // At most 2^28 logits a chunk (512 MB of e), in chunks of equal size; the loss alone keeps none.
-  const int64_t most = std::max<int64_t>(256, ((int64_t)1 << 28) / (p.panels * 64) / 256 * 256);
+  const int64_t most = std::max<int64_t>(256, std::min<int64_t>(1 << 17, ((int64_t)1 << 28) / (p.panels * 64) / 256 * 256));
   p.chunks = grads ? std::max<int64_t>(1, ceil_div(N, most)) : 1;
   p.chunk = std::max<int64_t>(256, ceil_div(ceil_div(N, p.chunks), 256) * 256);
   p.chunks = std::max<int64_t>(1, ceil_div(N, p.chunk));
@@ -1231,8 +1250,8 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   }
   const float e_scale = F16 ? kHalfScale : 1.f;
   const bool few = p.N <= tokens::kFewRows;
-  // Up to 4096 rows the join's last block reduces the losses (16 a thread); above, a block of 1024 threads.
-  const bool joined = p.chunks == 1 && p.N <= 4096;
+  // Up to 8192 rows the join's last block reduces the losses (32 a thread); above, a block of 1024 threads.
+  const bool joined = p.chunks == 1 && p.N <= 8192;
   if (p.grads && c.dw && !few)
     KRSI_CUDA_TRY(tokens::token_sort(c.targets, c.target_bits, N, V, c.ignore, s.sorted.start, s.sorted.pos,
                                      s.sorted.tok, stream));
@@ -1371,7 +1390,8 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       return KRSI_ERR_CUDA;
     KRSI_CUDA_TRY(launch_pairs(ce_grads_kernel<F16>, kGradsThreads, P, stream, ek, wm, em, xs, dxm, dwm, ga));
     if (ga.dx_part && c.dx)
-      KRSI_CUDA_TRY(launch_pdl(ce_dx_join_kernel<DT>, dim3((unsigned)ceil_div(rows * (K / 4), 128)), dim3(128), 0,
+      KRSI_CUDA_TRY(launch_pdl(ce_dx_join_kernel<DT>,
+                               dim3((unsigned)ceil_div(K / 4, 128), (unsigned)ceil_div(rows, kJoinRows)), dim3(128), 0,
                                stream, (const float*)s.dx_part, ga.splits, part_rows * K, ga.tgt, ga.factor, ga.coef, w,
                                dxc, (int)rows, K, c.scale, known ? 0 : 1));
   }

@@ -98,10 +98,13 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 // columns per thread.  A chunk's rows are staged in shared memory, all of its loads in flight at once: held
 // in registers they cost so many that a third as much was in flight (measured at 32768 rows of 1152 16-bit
 // values: 33 us against 39).
-// Out: packet(v, c, sums) takes the VEC finished sums of token v's packet c, zero(v, c) an absent one,
-// column(v, col, sum) one finished column.
+// Out: packet(v, c, sums, base) takes the VEC finished sums of token v's packet c with what fetch(v, c) read
+// for it (a group's reads are in flight together), zero(v, c) an absent one, column(v, col, sum) one finished
+// column.
 constexpr int kZeroTokens = 32;
 constexpr int kGroupRows = 4;     // rows per group of copies
+
+struct NoBase {};   // of an Out that reads nothing
 
 template <int DT, int VEC, bool WEIGHTED, typename Out>
 __global__ void __launch_bounds__(256)
@@ -151,22 +154,28 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
   bool first_run = true;
+  // a run that began in an earlier chunk is that chunk's to finish (partial row 2 chunk), one that goes on
+  // in the next is this chunk's (partial row 2 chunk + 1)
   auto add_group = [&](int j0) {
-    for (int j = j0; j < j0 + kGroupRows && j < m; ++j) {
+    typename Out::Base base[kGroupRows];
+#pragma unroll
+    for (int k = 0; k < kGroupRows; ++k)
+      if (j0 + k < m && s_tok[j0 + k + 1] != s_tok[j0 + k]) base[k] = out.fetch(s_tok[j0 + k], c);
+#pragma unroll
+    for (int k = 0; k < kGroupRows; ++k) {
+      const int j = j0 + k;
+      if (j >= m) break;
       const P r = stage[j * blockDim.x];
 #pragma unroll
       for (int e = 0; e < VEC; ++e)
         acc[e] = WEIGHTED ? fmaf(s_weight[j], E::load(r.v[e]), acc[e]) : acc[e] + E::load(r.v[e]);
       if (s_tok[j + 1] == s_tok[j]) continue;
-      // the run of s_tok[j] ends here (or goes on in the next chunk): a run that began in an earlier
-      // chunk is that chunk's to finish (partial row 2 chunk), one that goes on is this chunk's
-      // (partial row 2 chunk + 1)
       if ((first_run && from_before) || (j == m - 1 && goes_on)) {
         float* to = partial + ((int64_t)(2 * chunk + (first_run && from_before ? 0 : 1)) * packets + c) * VEC;
 #pragma unroll
         for (int e = 0; e < VEC; ++e) to[e] = acc[e];
       } else {
-        out.packet(s_tok[j], c, acc);
+        out.packet(s_tok[j], c, acc, base[k]);
       }
       first_run = false;
 #pragma unroll
@@ -306,6 +315,7 @@ sum_few_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restri
   extern __shared__ __align__(16) unsigned char stage_raw[];
   P* stage = reinterpret_cast<P*>(stage_raw) + threadIdx.x;   // [kChunkRows][blockDim.x]
   const P* gp = reinterpret_cast<const P*>(g) + c;
+  const typename Out::Base base = out.fetch((int)mine, c);
   float acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;
@@ -322,7 +332,7 @@ sum_few_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restri
       for (int e = 0; e < VEC; ++e) acc[e] = WEIGHTED ? fmaf(w, E::load(r.v[e]), acc[e]) : acc[e] + E::load(r.v[e]);
     }
   }
-  out.packet((int)mine, c, acc);
+  out.packet((int)mine, c, acc, base);
 }
 
 template <int DT, int VEC, bool WEIGHTED, typename Out, typename I>
