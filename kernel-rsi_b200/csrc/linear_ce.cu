@@ -22,6 +22,10 @@
 // gradient differs from row to row, or there are few rows), the logits are computed again, with the rows'
 // log-sum-exps from the forward as reference (ce_rows_kernel in place of 1 to 3): 8 N V K.
 //
+// The loss alone of few rows needs no ce_target_kernel: the logits' epilogue keeps a running maximum per
+// half tile as reference, and the tile that holds a row's target writes l_t (22.1 us became 20.8 for 16 rows of 768 over
+// 32768).
+//
 // The reference l_t is known before the GEMM, so no tile waits for another.  It is a poor one only where
 // some logit is far above the target's: past 2^kMaxLift the tile's sum is taken relative to the tile's
 // maximum instead, and the row is marked; marked rows' blocks are computed once more by the same kernel
@@ -57,6 +61,9 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr float kMaxLift = 64.f;                    // log2: e <= 2^64 in bf16, sums far below fp32's range
 constexpr float kHalfScale = 1024.f;                // f16: e = 2^10 p
 constexpr int kIgnored = -2, kInvalid = -1;         // targets: ignored, outside [0, V)
+// Fewer rows than this without gradients take the running reference. (From as many rows on "mean" and "sum"
+// form gradients in the forward, with l_t as reference; the loss is to have the same bits either way.)
+constexpr int64_t kRunningRows = 1024;
 
 // ---------------------------------------------------------------- CTA-pair GEMM pipeline
 constexpr int kBM = 128;                            // rows of A per CTA (256 per pair)
@@ -263,6 +270,10 @@ template <typename I>
 __device__ __forceinline__ int target_code(I t, long long ignore, int V) {
   return (long long)t == ignore ? kIgnored : (t >= 0 && t < (I)V) ? (int)t : kInvalid;
 }
+__device__ __forceinline__ int target_of(const void* targets, int bits, int row, long long ignore, int V) {
+  return bits == 64 ? target_code(reinterpret_cast<const long long*>(targets)[row], ignore, V)
+                    : target_code(reinterpret_cast<const int*>(targets)[row], ignore, V);
+}
 
 // ---------------------------------------------------------------- 1: targets
 // One warp per row: t_i (kIgnored, kInvalid or the token) and the target's logit in log2 units.  An
@@ -313,13 +324,21 @@ struct LogitsArgs {
   float c;                 // scale * log2(e)
   float e_scale;           // second pass: e is multiplied by it
   int store;               // e goes to memory
+  // the loss alone, few rows: the targets themselves, and where the targets' logits go (else null)
+  const void* targets;
+  int target_bits;
+  long long ignore;
+  float *l2t_out, *l2t_low_out;
+  int* ticket;
   uint32_t limit;
 };
 
 // Measured at 8192 x 32768 x 1152 (bf16, e stored): 420 us, 1,474 TFLOP/s, tensor pipe 81% active at 1.51 GHz;
 // at 768 columns 300 us (1,370): the tiles' operands and e together come to 50 bytes a cycle and SM through
 // L2, which is what it gives.  An epilogue of 8 warps (exponential, sum, store) stays behind the MMAs.
-template <bool F16>
+// RUNNING: the loss alone of few rows (see the top); a variant of its own, because its epilogue's few more
+// instructions cost the others 0.8%.
+template <bool F16, bool RUNNING>
 __global__ void __launch_bounds__(kLogitsThreads, 1)
 ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
                  const __grid_constant__ CUtensorMap emap, const LogitsArgs a) {
@@ -374,8 +393,9 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
         const int row = row0 + lane;
         const int col0 = m.vt * kBN + half * 128;
         const bool in = row < a.rows;
-        const int t = in ? a.tgt[row] : kIgnored;
-        float ref = in ? a.ref[row] : 0.f;
+        const int t = !in ? kIgnored : RUNNING ? target_of(a.targets, a.target_bits, row, a.ignore, a.V) : a.tgt[row];
+        float ref = RUNNING ? -INFINITY : in ? a.ref[row] : 0.f;   // RUNNING: the largest logit so far
+        if (RUNNING && pair == 0 && rank == 0 && threadIdx.x == 32 * kEpiWarp0) *a.ticket = 0;
         const bool live = t != kIgnored;
         const uint32_t keep = live ? 0xffffffffu : 0u;   // an ignored row's e is 0 whatever its logits are
         uint8_t* box = smem + ew * kLogitsBox;
@@ -398,19 +418,35 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
             const int c0 = col0 + j * 32;
             float y[32];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) y[e] = fmaf(__uint_as_float(r[e]), a.c, -ref);
+            for (int e = 0; e < 32; ++e) y[e] = fmaf(__uint_as_float(r[e]), a.c, RUNNING ? 0.f : -ref);
             if (c0 + 32 > a.V) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
                 if (c0 + e >= a.V) y[e] = -INFINITY;
             }
             if ((unsigned)(t - c0) < 32u) {
+              float lt = 0.f;
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (t == c0 + e) y[e] = -INFINITY;
+                if (t == c0 + e) {
+                  lt = __uint_as_float(r[e]);
+                  y[e] = -INFINITY;
+                }
+              if (RUNNING) {
+                a.l2t_out[row] = a.c * lt;
+                a.l2t_low_out[row] = fmaf(a.c, lt, -(a.c * lt));
+              }
             }
 #pragma unroll
             for (int e = 0; e < 32; e += 2) top = max3(top, y[e], y[e + 1]);
+            if (RUNNING && top > ref) {   // (while every logit so far is -inf the reference stays, and e is 0)
+              sum *= ex2_approx(ref - top);
+              ref = top;
+            }
+            if (RUNNING) {
+#pragma unroll
+              for (int e = 0; e < 32; ++e) y[e] = ref == -INFINITY ? y[e] : y[e] - ref;
+            }
 #pragma unroll
             for (int e = 0; e < 32; ++e) y[e] = ex2_approx(y[e]);
 #pragma unroll
@@ -444,7 +480,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
               }
             }
           }
-          if (second || again || !__any_sync(0xffffffffu, live && top > kMaxLift)) break;
+          if (RUNNING || second || again || !__any_sync(0xffffffffu, live && top > kMaxLift)) break;
           if (live && top > kMaxLift) ref += top;
           store = false;
         }
@@ -503,7 +539,10 @@ struct JoinArgs {
   int mean;
   const float2* part;      // [rows][n_part]
   int n_part;
-  const int* tgt;
+  int* tgt;                // of ce_target_kernel, or to be written from `targets`
+  const void* targets;
+  int target_bits, V;
+  long long ignore;
   const float* l2t;
   const float* l2t_low;    // the exact target's logit less l2t
   float* loss;             // [rows]
@@ -600,37 +639,51 @@ ce_rows_kernel(const RowsArgs a) {
 template <int DT>
 __device__ __forceinline__ void join_row(const JoinArgs& a, int row, int lane) {
   using T = typename Elem<DT>::T;
-  const int t = a.tgt[row];
-  const float l2t = a.l2t[row], l2t_low = a.l2t_low[row];
+  const int t = a.targets ? target_of(a.targets, a.target_bits, row, a.ignore, a.V) : a.tgt[row];
+  if (a.targets != nullptr && lane == 0) a.tgt[row] = t;
+  const float l2t = t == kInvalid ? __int_as_float(0x7fffffff) : a.l2t[row], l2t_low = a.l2t_low[row];
   const float2* pr = a.part + (int64_t)row * a.n_part;
   const T* xr = reinterpret_cast<const T*>(a.x) + (int64_t)row * a.K;
   RowCopy<DT> copy;        // on its way while the sums are added
   if (a.coef != nullptr) copy.fetch(xr, a.K, lane);
+  // The parts' sums relative to l_t, which most parts' already are, unless some part's reference is too far
+  // above it for that.
   float s = 0.f, top = l2t;
-  bool lifted = !(l2t == l2t);
+  bool moved = false;
 #pragma unroll 8
   for (int k = lane; k < a.n_part; k += 32) {
     const float2 p = pr[k];
-    lifted |= p.x != l2t;
+    moved |= p.x != l2t;
     top = fmaxf(top, p.x);
     s += p.y;
   }
-  lifted = __any_sync(0xffffffffu, lifted);
+  bool lifted = false;
+  if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    lifted = !(top - l2t <= kMaxLift);   // or NaN
+    const float from = lifted ? top : l2t;
+    s = 0.f;
+#pragma unroll 8
+    for (int k = lane; k < a.n_part; k += 32) {
+      const float2 p = pr[k];
+      if (p.y != 0.f) s += p.y * exp2f(p.x - from);   // (an empty part's reference may be -inf)
+    }
+  } else {
+    lifted = !(l2t == l2t);              // no part at all: NaN
+  }
+  s = warp_sum(s);
   float lse2, rest, pt;        // log2-sum-exp; 1 - p_t; p_t
   if (t == kIgnored) {
     lse2 = rest = pt = 0.f;
     lifted = false;
   } else if (!lifted) {
-    s = warp_sum(s) * exp2f(-l2t_low);   // relative to the logit itself: a large one's rounding shows in s
+    s *= exp2f(-l2t_low);      // relative to the logit itself: a large one's rounding shows in s
     pt = 1.f / (1.f + s);
     rest = s * pt;
     lse2 = l2t + kLog2e * log1pf(s);
   } else {
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    s = 0.f;
-    for (int k = lane; k < a.n_part; k += 32) s += pr[k].y * exp2f(pr[k].x - top);
-    s = warp_sum(s) + exp2f(l2t - top);
+    s += exp2f(l2t - top);
     lse2 = top + log2f(s);
     pt = exp2f(l2t - lse2);
     rest = 1.f - pt;
@@ -1071,8 +1124,10 @@ inline int device_pairs() {
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   int v = cached[dev].load(std::memory_order_relaxed);
   if (v == 0) {
-    v = std::min(std::min(max_pairs(ce_logits_kernel<false>, kLogitsThreads),
-                          max_pairs(ce_logits_kernel<true>, kLogitsThreads)),
+    v = std::min(std::min(std::min(max_pairs(ce_logits_kernel<false, false>, kLogitsThreads),
+                                   max_pairs(ce_logits_kernel<true, false>, kLogitsThreads)),
+                          std::min(max_pairs(ce_logits_kernel<false, true>, kLogitsThreads),
+                                   max_pairs(ce_logits_kernel<true, true>, kLogitsThreads))),
                  std::min(max_pairs(ce_grads_kernel<false>, kGradsThreads),
                           max_pairs(ce_grads_kernel<true>, kGradsThreads))) + 1;
     cached[dev].store(v, std::memory_order_relaxed);
@@ -1233,14 +1288,15 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   const bool wide = c.target_bits == 64;
   const dim3 row_grid((unsigned)ceil_div(N, 8));
   Upstream up{c.g, c.g_stride, c.weight, nullptr, F16};
-  if (!known) {
+  const bool running = !known && !p.grads && p.N < kRunningRows;
+  if (!known && !running) {
     auto kern = [&](auto k, auto* t) {
       return launch_pdl(k, row_grid, dim3(256), 0, stream, x, w, t, s.tgt, s.l2t, s.l2t_low, s.marked, s.ticket, N, V, K,
                         (long long)c.ignore, c2);
     };
     KRSI_CUDA_TRY(wide ? kern(ce_target_kernel<DT, long long>, (const long long*)c.targets)
                        : kern(ce_target_kernel<DT, int>, (const int*)c.targets));
-  } else if (F16 && c.g_stride == 1) {
+  } else if (known && F16 && c.g_stride == 1) {
     auto kern = [&](auto k, auto* t) {
       return launch_pdl(k, dim3(1), dim3(1024), 0, stream, c.g, c.weight, t, (long long)c.ignore, s.g_top, N);
     };
@@ -1289,6 +1345,14 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     la.e_scale = 1.f;
     la.store = p.grads && !F16;
     la.limit = kSpinLimit;
+    if (running) {
+      la.targets = c.targets;
+      la.target_bits = c.target_bits;
+      la.ignore = (long long)c.ignore;
+      la.l2t_out = s.l2t;
+      la.l2t_low_out = s.l2t_low;
+      la.ticket = s.ticket;
+    }
     const int logit_pairs = (int)std::min<int64_t>(pairs, (int64_t)la.n_rt * la.n_vt);
     if (known) {
       RowsArgs ra{};
@@ -1311,7 +1375,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       KRSI_CUDA_TRY(launch_pdl(wide ? ce_rows_kernel<DT, long long> : ce_rows_kernel<DT, int>,
                                dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ra));
     } else {
-      KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
+      KRSI_CUDA_TRY(launch_pairs(running ? ce_logits_kernel<F16, true> : ce_logits_kernel<F16, false>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
       JoinArgs ja{};
       ja.total = joined ? c.total : nullptr;
       ja.weight = c.row_weight;
@@ -1320,6 +1384,10 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       ja.part = s.part;
       ja.n_part = 2 * (int)p.n_vt;
       ja.tgt = s.tgt + r0;
+      ja.targets = running ? c.targets : nullptr;
+      ja.target_bits = c.target_bits;
+      ja.V = V;
+      ja.ignore = (long long)c.ignore;
       ja.l2t = s.l2t + r0;
       ja.l2t_low = s.l2t_low + r0;
       ja.loss = c.loss + r0;
@@ -1346,7 +1414,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     la.marked = F16 || known ? nullptr : s.marked + r0 / 256;
     la.e_scale = e_scale;
     la.store = 1;
-    KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
+    KRSI_CUDA_TRY(launch_pairs(ce_logits_kernel<F16, false>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
 
     GradArgs ga{};
     ga.rows = (int)rows;
