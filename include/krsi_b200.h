@@ -245,16 +245,16 @@ int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, int mode, siz
  * krsi_linear_ce_finish: the logits are computed once for loss and gradients. */
 int krsi_linear_ce_fwd(const void* x, const void* w, const void* targets, int target_bits, float* loss,
                        float* total, float* weight, float* stats, float* dx, float* dw, void* workspace,
-                       size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss, int mean,
-                       int dtype, cudaStream_t stream);
+                       size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index,
+                       float z_loss, int mean, int dtype, cudaStream_t stream);
 
 /* Gradients for the upstream gradient g of each row's loss (fp32, stride 1, or 0: one for all rows), times
  * *weight where that is not null, from the stats of krsi_linear_ce_fwd on the same operands (the logits
  * are computed again).  dx, dw: of `dtype`, one of them may be null. */
 int krsi_linear_ce_grad(const void* x, const void* w, const void* targets, int target_bits, const float* g,
                         int64_t g_stride, const float* weight, const float* stats, void* dx, void* dw,
-                        void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index,
-                        float z_loss, int dtype, cudaStream_t stream);
+                        void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale,
+                        int64_t ignore_index, float z_loss, int dtype, cudaStream_t stream);
 
 /* out = scale * *g * *weight * grad, rounded once (g, weight: device scalars or null); n a multiple of 8. */
 int krsi_linear_ce_finish(const float* grad, const float* g, const float* weight, void* out, int64_t n,

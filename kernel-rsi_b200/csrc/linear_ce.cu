@@ -23,8 +23,8 @@
 // log-sum-exps from the forward as reference (ce_rows_kernel in place of 1 to 3): 8 N V K.
 //
 // The loss alone of few rows needs no ce_target_kernel: the logits' epilogue keeps a running maximum per
-// half tile as reference, and the tile that holds a row's target writes l_t (22.1 us became 20.8 for 16 rows of 768 over
-// 32768).
+// half tile as reference, and the tile that holds a row's target writes l_t (22.1 us became 20.8 for 16 rows
+// of 768 over 32768).
 //
 // The reference l_t is known before the GEMM, so no tile waits for another.  It is a poor one only where
 // some logit is far above the target's: past 2^kMaxLift the tile's sum is taken relative to the tile's
@@ -283,7 +283,8 @@ template <int DT, typename I>
 __global__ void __launch_bounds__(256)
 ce_target_kernel(const typename Elem<DT>::T* __restrict__ x, const typename Elem<DT>::T* __restrict__ w,
                  const I* __restrict__ targets, int* __restrict__ tgt, float* __restrict__ l2t,
-                 float* __restrict__ l2t_low, int* __restrict__ marked, int* __restrict__ ticket, int n, int V, int K, long long ignore, float c) {
+                 float* __restrict__ l2t_low, int* __restrict__ marked, int* __restrict__ ticket, int n, int V, int K,
+                 long long ignore, float c) {
   pdl_enter();
   using E = Elem<DT>;
   using T = typename E::T;
@@ -1375,7 +1376,8 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       KRSI_CUDA_TRY(launch_pdl(wide ? ce_rows_kernel<DT, long long> : ce_rows_kernel<DT, int>,
                                dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ra));
     } else {
-      KRSI_CUDA_TRY(launch_pairs(running ? ce_logits_kernel<F16, true> : ce_logits_kernel<F16, false>, kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
+      KRSI_CUDA_TRY(launch_pairs(running ? ce_logits_kernel<F16, true> : ce_logits_kernel<F16, false>,
+                                 kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
       JoinArgs ja{};
       ja.total = joined ? c.total : nullptr;
       ja.weight = c.row_weight;
@@ -1524,8 +1526,9 @@ extern "C" int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, in
 
 extern "C" int krsi_linear_ce_fwd(const void* x, const void* w, const void* targets, int target_bits, float* loss,
                                   float* total, float* weight, float* stats, float* dx, float* dw,
-                                  void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t K, float scale, int64_t ignore_index, float z_loss,
-                                  int mean, int dtype, cudaStream_t stream) {
+                                  void* workspace, size_t workspace_bytes, int64_t N, int64_t V, int64_t K,
+                                  float scale, int64_t ignore_index, float z_loss, int mean, int dtype,
+                                  cudaStream_t stream) {
   const int rc = check(N, V, K, target_bits, dtype);
   if (rc != KRSI_OK) return rc;
   KRSI_CHECK_ARG((total != nullptr) == (weight != nullptr));
@@ -1537,8 +1540,8 @@ extern "C" int krsi_linear_ce_fwd(const void* x, const void* w, const void* targ
   }
   KRSI_CHECK_ARG(x && w && targets && loss);
   if (reinterpret_cast<uintptr_t>(stats) % 8 != 0) return KRSI_ERR_MISALIGNED;
-  const Call c{x, w, targets, target_bits, loss, total, weight, mean, reinterpret_cast<float2*>(stats), nullptr, 0, nullptr, dx, dw, scale, z_loss,
-               ignore_index};
+  const Call c{x, w, targets, target_bits, loss, total, weight, mean, reinterpret_cast<float2*>(stats), nullptr, 0,
+               nullptr, dx, dw, scale, z_loss, ignore_index};
   return run_checked(c, N, V, K, workspace, workspace_bytes, dtype, stream);
 }
 

@@ -409,8 +409,8 @@ CeCall ce_call(const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor&
   return c;
 }
 
-// (loss rows, loss, row weight, stats, dx, dw): stats is for linear_ce_grad; the gradients are fp32, of the sum of the losses and without
-// `scale`, or empty.  reduction 0 none, 1 mean, 2 sum.
+// (loss rows, loss, row weight, stats, dx, dw): stats is for linear_ce_grad; the gradients are fp32, of the sum
+// of the losses and without `scale`, or empty.  reduction 0 none, 1 mean, 2 sum.
 std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor> linear_ce_fwd(
     const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor& targets_in, double scale, int64_t ignore_index,
     double z_loss, int64_t reduction, bool want_dx, bool want_dw) {
@@ -459,8 +459,9 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_grad(const at::Tensor& g_in, const 
   if (!want_dx && !want_dw) return {dx, dw};
   check_rc(krsi_linear_ce_grad(c.x.data_ptr(), c.w.data_ptr(), c.targets.data_ptr(), c.bits, g.data_ptr<float>(),
                                g.numel() == 1 ? 0 : 1, weight.numel() == 1 ? weight.data_ptr<float>() : nullptr,
-                               stats.data_ptr<float>(), want_dx ? dx.data_ptr() : nullptr, want_dw ? dw.data_ptr() : nullptr, c.ws.data_ptr(),
-                               (size_t)c.ws.numel(), c.N, c.V, c.K, (float)scale, ignore_index, (float)z_loss, c.dtype,
+                               stats.data_ptr<float>(), want_dx ? dx.data_ptr() : nullptr,
+                               want_dw ? dw.data_ptr() : nullptr, c.ws.data_ptr(), (size_t)c.ws.numel(), c.N, c.V,
+                               c.K, (float)scale, ignore_index, (float)z_loss, c.dtype,
                                at::cuda::getCurrentCUDAStream()),
            "krsi_linear_ce_grad");
   return {dx, dw};
