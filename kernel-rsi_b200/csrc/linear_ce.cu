@@ -83,6 +83,10 @@ constexpr uint32_t kSmem = 232448;
 constexpr uint32_t kUsable = kSmem - 1024 - 1024;   // less the 1024-byte alignment and the barriers' KB
 static_assert(kNumBars * 8 + 16 <= 1024, "barriers");
 constexpr uint32_t kTmemCols = 512;
+// What an item's epilogue costs in K blocks where a single accumulator leaves it exposed, for dealing the items
+// out: 10 as read from the launch's ends, which spread over 83 of 395 us when it was left out (2001 x 1152 over
+// 50021: 844 us a step without it, 817 to 825 with 10, 833 with 14, 839 with 20).
+constexpr int kEpilogueBlocks = 10;
 
 // MN-major operand in the 128-byte swizzle: 64-column atoms of 8 K-rows x 128 B (SBO = 1024 B), the next
 // 64 columns one box further; the K step of 16 rows advances the start by 2 KB.
@@ -1433,8 +1437,11 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     ga.n_dx = c.dx ? ga.n_rt * ga.n_ct * ga.splits : 0;
     ga.n_dw = c.dw ? ga.n_vt * ga.n_ct : 0;
     const int P = (int)std::min<int64_t>(pairs, (int64_t)ga.n_dx + ga.n_dw);
-    if (ga.n_dx % P != 0)   // pairs with one dx item less than the others take dw items for it
-      ga.low_first = std::min((ga.kb_share + ga.kb_rows / 2) / ga.kb_rows, ga.n_dw / (P - ga.n_dx % P));
+    // Pairs with one dx item less than the others take dw items for it, as many as fit into its time. In K
+    // blocks an item costs its own and, with one accumulator, its epilogue's.
+    const int epilogue = p.cols > kBN ? kEpilogueBlocks : 0;
+    if (ga.n_dx % P != 0)
+      ga.low_first = std::min((ga.kb_share + epilogue) / (ga.kb_rows + epilogue), ga.n_dw / (P - ga.n_dx % P));
     ga.dx_part = ga.splits > 1;
     ga.dx32 = ga.dx_part || !known;
     ga.tgt = s.tgt + r0;
