@@ -85,7 +85,7 @@ static_assert(kNumBars * 8 + 16 <= 1024, "barriers");
 constexpr uint32_t kTmemCols = 512;
 // What an item's epilogue costs in K blocks where a single accumulator leaves it exposed, for dealing the items
 // out: 10 as read from the launch's ends, which spread over 83 of 395 us when it was left out (2001 x 1152 over
-// 50021: 844 us a step without it, 817 to 825 with 10, 833 with 14, 839 with 20).
+// 50021: 857 us a step without it, 830 with 10, 833 to 841 with 14 and 20; long sums do not notice).
 constexpr int kEpilogueBlocks = 10;
 
 // MN-major operand in the 128-byte swizzle: 64-column atoms of 8 K-rows x 128 B (SBO = 1024 B), the next
