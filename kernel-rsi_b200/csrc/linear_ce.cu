@@ -37,7 +37,7 @@
 // of dw; the alternative is to compute the logits twice); everything else is fp32 until the result.
 //
 // What bounds it (B200, 32768 x 1152 over 32768 entries, bf16, loss and gradients: 7.42 PFLOP): the tensor
-// cores under the power cap.  Each GEMM below runs at 1.5 GHz by itself; the step takes 6.15 to 6.35 ms, of
+// cores under the power cap.  Each GEMM below runs at 1.5 GHz by itself; the step takes 6.15 to 6.45 ms, of
 // which 0.2 ms are the other kernels.  cuBLAS takes 5.84 ms for the three bare products in the same loop.
 #include <algorithm>
 #include <atomic>
