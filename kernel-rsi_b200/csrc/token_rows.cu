@@ -126,7 +126,7 @@ token_sort_kernel(const T* __restrict__ toks, int n, int V, int skip, const Orde
   int first = base + before + incl - total;
   if (b < range) {
     start[group * range + b] = first;
-    if (group == mask && b == range - 1) start[(group + 1) * range] = first + total;
+    if (group == mask && b == range - 1) start[order.end()] = first + total;
     if (total > 0) {
 #pragma unroll 8
       for (int w = 0; w < kWarps; ++w) {

@@ -25,8 +25,11 @@ struct Order {
   int bits;    // log2 of the groups
   int range;   // tokens per group
   __host__ __device__ __forceinline__ int key(int v) const { return (v & ((1 << bits) - 1)) * range + (v >> bits); }
+  // One past the last key: 2^31 for the largest vocabularies, whose keys still fit an int.
+  __host__ __device__ constexpr int64_t end() const { return (int64_t)range << bits; }
 };
 constexpr int kMaxRange = 512;
+static_assert(Order{22, kMaxRange}.end() == (int64_t)1 << 31, "end() of the largest order");
 inline Order order_of(int64_t V) {
   Order o{7, 0};   // 128 groups, more where a group would pass kMaxRange tokens
   while (((V - 1) >> o.bits) + 1 > kMaxRange) ++o.bits;
@@ -36,8 +39,7 @@ inline Order order_of(int64_t V) {
 
 // The positions of tokens[0, n) sorted by token (in Order; equal tokens in an order that depends on n
 // alone), those outside [0, V) and those equal to `skip` left out:
-//   start[key(v)] .. start[key(v) + 1]   the sorted entries of token v (start[end] = their number, end being
-//                                        groups * range)
+//   start[key(v)] .. start[key(v) + 1]   the sorted entries of token v (start[order.end()] = their number)
 //   pos[i], tok[i]                       position and token of sorted entry i
 // token_bits 32 or 64.  One kernel, no workspace beyond the outputs.
 cudaError_t token_sort(const void* toks, int token_bits, int64_t n, int64_t V, int64_t skip, int* start, int* pos,
@@ -57,7 +59,7 @@ inline Space space_at(void* base, int64_t n, int64_t V, int64_t d) {
   size_t off = 0;
   s.order = order_of(V);
   s.start = reinterpret_cast<int*>(p + off);
-  off += up((((size_t)s.order.range << s.order.bits) + 1) * 4);
+  off += up(((size_t)s.order.end() + 1) * 4);
   s.pos = reinterpret_cast<int*>(p + off);
   off += up((size_t)n * 4);
   s.tok = reinterpret_cast<int*>(p + off);
@@ -131,7 +133,7 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
   // the chunk's entries, read beside the number that says how many of them there are
   const bool mine = threadIdx.x < kChunkRows && i0 + (int)threadIdx.x < n;
   const int p = mine ? pos[i0 + threadIdx.x] : 0, t = mine ? tok[i0 + threadIdx.x] : 0;
-  const int m = min(kChunkRows, start[order.range << order.bits] - i0);
+  const int m = min(kChunkRows, start[order.end()] - i0);
   if (m <= 0) return;
   if (threadIdx.x < m) {
     s_pos[threadIdx.x] = p;
@@ -226,7 +228,7 @@ join_rows_kernel(const int* __restrict__ start, const int* __restrict__ tok, con
   };
   const int chunk = blockIdx.x * kJoinWarps + warp, i0 = chunk * kChunkRows, i1 = i0 + kChunkRows;
   int t = 0, n = 0;                                 // the run's token and partial rows; n = 0: none
-  if (i1 < start[order.range << order.bits]) {
+  if (i1 < start[order.end()]) {
     t = tok[i1 - 1];
     const int k = order.key(t), e = start[k + 1];
     if (start[k] >= i0 && e > i1) n = (e - 1) / kChunkRows - chunk + 1;
