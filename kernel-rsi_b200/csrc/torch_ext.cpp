@@ -497,6 +497,13 @@ void check_once(const char* what) {
   TORCH_CHECK(!at::GradMode::is_enabled(), what, ": the backward has no gradient of its own (create_graph)");
 }
 
+// Nor is a forward-mode derivative: a dual tensor's tangent would be dropped, with a derivative of zero, on the way
+// below the autograd keys.
+void check_no_tangent(std::initializer_list<const at::Tensor*> inputs, const char* what) {
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK(!t->_fw_grad(/*level=*/0).defined(), what, ": forward-mode differentiation is not supported");
+}
+
 struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& tokens, const at::Tensor& table, double scale,
                             int64_t padding_idx) {
@@ -516,6 +523,7 @@ struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
   }
 };
 at::Tensor embedding_autograd(const at::Tensor& tokens, const at::Tensor& table, double scale, int64_t padding_idx) {
+  check_no_tangent({&table}, "embedding");
   if (at::GradMode::is_enabled() && table.requires_grad())
     return EmbeddingNode::apply(tokens, table, scale, padding_idx);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -536,6 +544,7 @@ struct GegluQ8Node : public torch::autograd::Function<GegluQ8Node> {
   }
 };
 at::Tensor geglu_q8_autograd(const at::Tensor& u) {
+  check_no_tangent({&u}, "geglu_q8");
   if (at::GradMode::is_enabled() && u.requires_grad()) return GegluQ8Node::apply(u);
   at::AutoDispatchBelowADInplaceOrView below;
   return std::get<0>(geglu_q8_fwd(u, false));
@@ -584,6 +593,7 @@ struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
 };
 at::Tensor linear_ce_autograd(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, double scale,
                               int64_t ignore_index, double z_loss, int64_t reduction, bool keep) {
+  check_no_tangent({&x, &w}, "linear_cross_entropy");
   if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad()))
     return LinearCeNode::apply(x, w, targets, scale, ignore_index, z_loss, reduction, keep);
   at::AutoDispatchBelowADInplaceOrView below;
