@@ -31,7 +31,9 @@
 // maximum instead, and the row is marked; marked rows' blocks are computed once more by the same kernel
 // with lse as reference ("second pass", skipped tile by tile elsewhere).  bf16 holds e over fp32's whole
 // range.  f16 does not, so for f16 the second pass writes e = 2^10 p for every row and the first stores
-// none: 8 N V K, the price of f16's range.
+// none: 8 N V K, the price of f16's range. x' in f16 is divided by a power of two above the largest row
+// factor, which the products' fp32 sums are multiplied by again: with a z-loss the factors 1 + 2 z lse are known
+// after the join only, and ce_rows_kernel then writes x' in the forward too.
 //
 // Rounding: e and x' are rounded to the operands' 16 bits (x' costs a second rounding in the softmax part
 // of dw; the alternative is to compute the logits twice); everything else is fp32 until the result.
@@ -568,12 +570,12 @@ struct Upstream {
   const float* g;          // per row (stride 1) or one (stride 0); null: 1
   int64_t stride;
   const float* weight;     // a factor of g for all rows, or null
-  const float* top;        // f16 and one g per row: the largest |g weight|
+  const float* top;        // f16, where row factors differ (g, or z's): their largest magnitude
   int scaled;              // f16: row factors are divided by unit() before they meet 16 bits
   __device__ __forceinline__ float of(int64_t row) const { return g ? g[row * stride] * (weight ? *weight : 1.f) : 1.f; }
-  // The power of two above the largest |g weight|.
+  // The power of two above the largest |g weight (1 + 2 z lse)|.
   __device__ __forceinline__ float unit() const {
-    if (!scaled || g == nullptr) return 1.f;
+    if (!scaled || (top == nullptr && g == nullptr)) return 1.f;
     const uint32_t e = __float_as_uint(top ? *top : of(0)) & 0x7f800000u;
     return e == 0u || e >= 0x7f000000u ? 1.f : 2.f * __uint_as_float(e);
   }
@@ -727,23 +729,27 @@ ce_join_kernel(const JoinArgs a) {
   reduce_rows<256>(a.loss, a.tgt, a.total, a.weight, a.rows, a.mean);
 }
 
-// The largest |g weight| over the rows that are not ignored (a fixed result whatever the order).
+// The largest |g weight (1 + 2 z lse)| over the rows that are not ignored (a fixed result whatever the order);
+// g: one per row, or null for what all rows have in common (`common`, or 1); stats: null where z is 0.
 template <typename I>
 __global__ void __launch_bounds__(1024)
-ce_gtop_kernel(const float* __restrict__ g, const float* __restrict__ weight, const I* __restrict__ targets,
-               long long ignore, float* __restrict__ out, int n) {
+ce_top_kernel(const float* __restrict__ g, const float* __restrict__ common, const float* __restrict__ weight,
+              const float2* __restrict__ stats, const I* __restrict__ targets, long long ignore, float z,
+              float* __restrict__ out, int n) {
   pdl_enter();
   __shared__ float tops[32];
   float m = 0.f;
 #pragma unroll 8
   for (int i = threadIdx.x; i < n; i += 1024)
-    if ((long long)targets[i] != ignore) m = fmaxf(m, fabsf(g[i]));
+    if ((long long)targets[i] != ignore)
+      m = fmaxf(m, fabsf((g ? g[i] : 1.f) * (stats ? 1.f + 2.f * z * stats[i].x * kLn2 : 1.f)));
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
   if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = m;
   __syncthreads();
   if (threadIdx.x == 0) {
     for (int w = 1; w < 32; ++w) m = fmaxf(m, tops[w]);
+    if (common) m *= fabsf(*common);
     *out = weight ? m * fabsf(*weight) : m;
   }
 }
@@ -1224,17 +1230,17 @@ inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool known, i
 struct Space {
   void* e;
   void* xs;
-  float2* part;
+  float2 *part, *stats;
   float *dw32, *dx_part;
   int* tgt;
-  float *l2t, *l2t_low, *coef, *factor, *ref, *g_top;
+  float *l2t, *l2t_low, *coef, *factor, *ref, *top;
   int *marked, *ticket;
   tokens::Space sorted;
   size_t bytes;
 };
 inline Space space_at(void* base, const Plan& p) {
   const uintptr_t at = reinterpret_cast<uintptr_t>(base);
-  Space s;
+  Space s{};
   size_t off = 0;
   auto take = [&](size_t bytes) {
     const uintptr_t r = at + off;
@@ -1252,7 +1258,8 @@ inline Space space_at(void* base, const Plan& p) {
     s.coef = reinterpret_cast<float*>(take((size_t)p.N * 4));
     s.factor = reinterpret_cast<float*>(take((size_t)p.N * 4));
     s.ref = reinterpret_cast<float*>(take((size_t)p.N * 4));
-    s.g_top = reinterpret_cast<float*>(take(4));
+    s.top = reinterpret_cast<float*>(take(4));
+    s.stats = reinterpret_cast<float2*>(p.known ? 0 : take((size_t)p.N * 8));
     s.e = reinterpret_cast<void*>(take((size_t)rows * p.panels * 128));
     s.xs = reinterpret_cast<void*>(take((size_t)rows * p.K * 2));
     s.dw32 = reinterpret_cast<float*>(p.known ? take((size_t)p.V * p.K * 4) : 0);
@@ -1301,14 +1308,23 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     };
     KRSI_CUDA_TRY(wide ? kern(ce_target_kernel<DT, long long>, (const long long*)c.targets)
                        : kern(ce_target_kernel<DT, int>, (const int*)c.targets));
-  } else if (known && F16 && c.g_stride == 1) {
-    auto kern = [&](auto k, auto* t) {
-      return launch_pdl(k, dim3(1), dim3(1024), 0, stream, c.g, c.weight, t, (long long)c.ignore, s.g_top, N);
-    };
-    KRSI_CUDA_TRY(wide ? kern(ce_gtop_kernel<long long>, (const long long*)c.targets)
-                       : kern(ce_gtop_kernel<int>, (const int*)c.targets));
-    up.top = s.g_top;
   }
+  // f16 holds x' only where the row factors leave its magnitude near x's, so they are divided by a power of two
+  // above the largest.  The factors differ between rows with one g per row, and with a z-loss: its 1 + 2 z lse is
+  // known after the join, so the forward then forms x' as the gradients from known log-sum-exps do.
+  const bool tops = F16 && p.grads && (c.z != 0.f || c.g_stride == 1);
+  const bool rows_after_join = tops && !known;
+  float2* stats = c.stats ? c.stats : s.stats;
+  if (tops) up.top = s.top;
+  auto find_top = [&](int64_t r0, int64_t rows) -> cudaError_t {
+    auto kern = [&](auto k, auto* t) {
+      return launch_pdl(k, dim3(1), dim3(1024), 0, stream, c.g_stride == 1 ? c.g + r0 : nullptr,
+                        c.g_stride == 1 ? nullptr : c.g, c.weight, c.z != 0.f ? (const float2*)stats + r0 : nullptr, t + r0,
+                        (long long)c.ignore, c.z, s.top, (int)rows);
+    };
+    return wide ? kern(ce_top_kernel<long long>, (const long long*)c.targets)
+                : kern(ce_top_kernel<int>, (const int*)c.targets);
+  };
   const float e_scale = F16 ? kHalfScale : 1.f;
   const bool few = p.N <= tokens::kFewRows;
   // Up to 8192 rows the join's last block reduces the losses (32 a thread); above, a block of 1024 threads.
@@ -1359,27 +1375,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       la.ticket = s.ticket;
     }
     const int logit_pairs = (int)std::min<int64_t>(pairs, (int64_t)la.n_rt * la.n_vt);
-    if (known) {
-      RowsArgs ra{};
-      ra.targets = static_cast<const char*>(c.targets) + r0 * (c.target_bits / 8);
-      ra.stats = c.stats + r0;
-      ra.up = up;
-      ra.row0 = r0;
-      ra.tgt = s.tgt + r0;
-      ra.coef = s.coef + r0;
-      ra.factor = s.factor + r0;
-      ra.ref = s.ref + r0;
-      ra.x = xc;
-      ra.xs = s.xs;
-      ra.rows = (int)rows;
-      ra.V = V;
-      ra.K = K;
-      ra.ignore = (long long)c.ignore;
-      ra.e_scale = e_scale;
-      ra.z = c.z;
-      KRSI_CUDA_TRY(launch_pdl(wide ? ce_rows_kernel<DT, long long> : ce_rows_kernel<DT, int>,
-                               dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ra));
-    } else {
+    if (!known) {
       KRSI_CUDA_TRY(launch_pairs(running ? ce_logits_kernel<F16, true> : ce_logits_kernel<F16, false>,
                                  kLogitsThreads, logit_pairs, stream, xm, wk, es, la));
       JoinArgs ja{};
@@ -1397,13 +1393,13 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       ja.l2t = s.l2t + r0;
       ja.l2t_low = s.l2t_low + r0;
       ja.loss = c.loss + r0;
-      ja.stats = c.stats ? c.stats + r0 : nullptr;
+      ja.stats = stats ? stats + r0 : nullptr;
       ja.rows = (int)rows;
       ja.K = K;
       ja.all_second = F16;
       ja.e_scale = e_scale;
       ja.z = c.z;
-      if (p.grads) {
+      if (p.grads && !rows_after_join) {
         ja.coef = s.coef + r0;
         ja.factor = s.factor + r0;
         ja.ref = s.ref + r0;
@@ -1413,6 +1409,28 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       }
       KRSI_CUDA_TRY(launch_pdl(ce_join_kernel<DT>, dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ja));
       if (!p.grads) continue;
+    }
+    if (known || rows_after_join) {
+      if (tops) KRSI_CUDA_TRY(find_top(r0, rows));
+      RowsArgs ra{};
+      ra.targets = static_cast<const char*>(c.targets) + r0 * (c.target_bits / 8);
+      ra.stats = stats + r0;
+      ra.up = up;
+      ra.row0 = r0;
+      ra.tgt = s.tgt + r0;
+      ra.coef = s.coef + r0;
+      ra.factor = s.factor + r0;
+      ra.ref = s.ref + r0;
+      ra.x = xc;
+      ra.xs = s.xs;
+      ra.rows = (int)rows;
+      ra.V = V;
+      ra.K = K;
+      ra.ignore = (long long)c.ignore;
+      ra.e_scale = e_scale;
+      ra.z = c.z;
+      KRSI_CUDA_TRY(launch_pdl(wide ? ce_rows_kernel<DT, long long> : ce_rows_kernel<DT, int>,
+                               dim3((unsigned)ceil_div(rows, 8)), dim3(256), 0, stream, ra));
     }
 
     la.ref = s.ref + r0;

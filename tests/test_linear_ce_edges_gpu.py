@@ -1,0 +1,47 @@
+"""The vocabulary cross entropy (B200) at the limits of its types and paths, against float64."""
+import pytest
+import torch
+
+import _ext
+from linear_cross_entropy import KEEP_ROWS
+from test_linear_ce_gpu import UNIT, exact, inputs, run
+
+pytestmark = pytest.mark.gpu
+dev = "cuda"
+
+
+@pytest.mark.parametrize("N,reduction", [(40, "mean"), (300, "none"), (KEEP_ROWS + 60, "mean"), (KEEP_ROWS + 60, "none")])
+def test_f16_rows_scaled_far_up_by_the_z_loss(N, reduction):
+    """x up to 1e4 and log-sum-exps in the hundreds with z = 0.1: x (1 + 2 z lse) is far above f16's 65504, the
+    gradients are not.  Row 5 is four times smaller, so that the factors differ from row to row."""
+    V, K, z, scale, dtype = 700, 64, 0.1, 0.1, torch.float16
+    x, w, t = inputs(N, V, K, dtype, 21, ignored=0.1, lift=0.0)
+    x = (x.float() * 1000).clamp(-1e4, 1e4).half()
+    x[5] *= 0.25
+    t[5] = 3
+    kept = int((t != -100).sum())
+    up = torch.rand(N, device=dev) / kept if reduction == "none" else None
+    e = exact(x, w, t, scale, z, up if up is not None else torch.tensor(1.0 / kept, device=dev))
+    loss, dx, dw = run(x, w, t, up, scale=scale, z_loss=z, reduction=reduction)
+    live = t != -100
+    L = torch.where(live[:, None], x.double(), 0.0) @ w.double().t() * scale
+    lse = torch.logsumexp(L, 1)
+    p = torch.exp(L - lse[:, None]) * live[:, None]
+    soft = (e["up"] * (1 + 2 * z * lse)).abs()
+    assert (x.double().abs().amax(1) * (1 + 2 * z * lse)).max() > 2 * 65504
+    # the row's own |p - 1| 2 z lse term: the loss moves by 1 + 2 z lse for an error of lse
+    tol = (4 * e["lerr"] + 2.0 ** -20 * (1 + lse)) * (1 + 2 * z * lse) + 2.0 ** -20 * e["loss"].abs()
+    if reduction == "none":
+        assert torch.all((loss.double() - e["loss"]).abs() <= tol)
+    else:
+        assert abs(loss.double() - e["loss"].sum() / kept) <= tol.sum() / kept
+    # as in test_linear_ce_gpu: the result's rounding; the exponentials' and the scaled rows' (dw) and the logits'
+    # errors on the magnitudes; e's smallest step (p off by 2^-35) and the scaled rows' (2^-24 of the largest factor)
+    U, le = UNIT[dtype], e["lerr"].max() * 4 + 2.0 ** -14
+    bdx = 1.01 * U * e["dx"].abs() + (U + le) * e["mdx"] + 2.0 ** -25 + 1.1 * 2.0 ** -35 * soft[:, None] * e["wsum"]
+    bdw = (1.01 * U * e["dw"].abs() + (2 * U + le) * e["mdw"] + 2.0 ** -25
+           + soft.max() * (1.1 * 2.0 ** -35 * e["xsum"] + 2.0 ** -24 * scale * p.sum(0)[:, None]))
+    assert torch.isfinite(dw).all() and torch.isfinite(dx).all()
+    assert torch.all((dx.double() - e["dx"]).abs() <= bdx)
+    assert torch.all((dw.double() - e["dw"]).abs() <= bdw)
+    assert _ext.device_status() == 0
