@@ -489,6 +489,13 @@ at::Tensor linear_ce_finish(const at::Tensor& grad, const at::Tensor& g_in, cons
 // Autograd nodes of the vocabulary operators and the 8-bit checkpoint, in C++: at small sizes a pass is
 // bound by the host, and a Python autograd.Function costs it 60 us more a step than these do.  (Compiled
 // graphs use the *_fwd operators with the gradients registered in _ext.py.)
+// They call the operators through the dispatcher, below autograd: dispatch modes and fake tensors see them there.
+#define KRSI_OP(NAME)                                                                                    \
+  ([]() -> const auto& {                                                                                 \
+    static const auto handle =                                                                           \
+        c10::Dispatcher::singleton().findSchemaOrThrow("krsi::" #NAME, "").typed<decltype(NAME)>();      \
+    return handle;                                                                                       \
+  }())
 using torch::autograd::AutogradContext;
 using torch::autograd::variable_list;
 
@@ -511,14 +518,15 @@ struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
     ctx->save_for_backward({tokens, table});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding_idx"] = padding_idx;
-    return embedding_fwd(tokens, table, scale, padding_idx);
+    return KRSI_OP(embedding_fwd).call(tokens, table, scale, padding_idx);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_once("embedding");
     const auto saved = ctx->get_saved_variables();
+    at::AutoDispatchBelowADInplaceOrView below;
     return {at::Tensor(),
-            embedding_bwd(g[0], saved[0], saved[1], ctx->saved_data["scale"].toDouble(),
-                          ctx->saved_data["padding_idx"].toInt()),
+            KRSI_OP(embedding_bwd).call(g[0], saved[0], saved[1], ctx->saved_data["scale"].toDouble(),
+                                        ctx->saved_data["padding_idx"].toInt()),
             at::Tensor(), at::Tensor()};
   }
 };
@@ -527,27 +535,28 @@ at::Tensor embedding_autograd(const at::Tensor& tokens, const at::Tensor& table,
   if (at::GradMode::is_enabled() && table.requires_grad())
     return EmbeddingNode::apply(tokens, table, scale, padding_idx);
   at::AutoDispatchBelowADInplaceOrView below;
-  return embedding_fwd(tokens, table, scale, padding_idx);
+  return KRSI_OP(embedding_fwd).call(tokens, table, scale, padding_idx);
 }
 
 struct GegluQ8Node : public torch::autograd::Function<GegluQ8Node> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& u) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [out, q, ex] = geglu_q8_fwd(u, true);
+    auto [out, q, ex] = KRSI_OP(geglu_q8_fwd).call(u, true);
     ctx->save_for_backward({q, ex});
     return out;
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_once("geglu_q8");
     const auto saved = ctx->get_saved_variables();
-    return {std::get<0>(geglu_q8_bwd(g[0], saved[0], saved[1], false))};
+    at::AutoDispatchBelowADInplaceOrView below;
+    return {std::get<0>(KRSI_OP(geglu_q8_bwd).call(g[0], saved[0], saved[1], false))};
   }
 };
 at::Tensor geglu_q8_autograd(const at::Tensor& u) {
   check_no_tangent({&u}, "geglu_q8");
   if (at::GradMode::is_enabled() && u.requires_grad()) return GegluQ8Node::apply(u);
   at::AutoDispatchBelowADInplaceOrView below;
-  return std::get<0>(geglu_q8_fwd(u, false));
+  return std::get<0>(KRSI_OP(geglu_q8_fwd).call(u, false));
 }
 at::Tensor geglu_q8_plain(const at::Tensor& u) { return std::get<0>(geglu_q8_fwd(u, false)); }
 
@@ -555,15 +564,16 @@ at::Tensor geglu_q8_plain(const at::Tensor& u) { return std::get<0>(geglu_q8_fwd
 at::Tensor linear_ce_plain(const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets, double scale,
                            int64_t ignore_index, double z_loss, int64_t reduction, bool /*keep*/) {
   auto [loss, total, weight, stats, dx, dw] =
-      linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction, false, false);
+      KRSI_OP(linear_ce_fwd).call(x, w, targets, scale, ignore_index, z_loss, reduction, false, false);
   return reduction != 0 ? total : loss;
 }
 struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& w, const at::Tensor& targets,
                             double scale, int64_t ignore_index, double z_loss, int64_t reduction, bool keep) {
     at::AutoDispatchBelowADInplaceOrView below;
-    auto [loss, total, weight, stats, dx, dw] = linear_ce_fwd(x, w, targets, scale, ignore_index, z_loss, reduction,
-                                                              keep && x.requires_grad(), keep && w.requires_grad());
+    auto [loss, total, weight, stats, dx, dw] =
+        KRSI_OP(linear_ce_fwd).call(x, w, targets, scale, ignore_index, z_loss, reduction, keep && x.requires_grad(),
+                                    keep && w.requires_grad());
     if (keep) ctx->save_for_backward({weight, dx, dw, w});
     else ctx->save_for_backward({weight, stats, x, w, targets});
     ctx->saved_data["scale"] = scale;
@@ -577,14 +587,16 @@ struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
     const auto saved = ctx->get_saved_variables();
     const double scale = ctx->saved_data["scale"].toDouble();
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1);
+    at::AutoDispatchBelowADInplaceOrView below;
     at::Tensor dx, dw;
     if (ctx->saved_data["keep"].toBool()) {
-      if (need_x) dx = linear_ce_finish(saved[1], g[0], saved[0], scale, saved[3]);
-      if (need_w) dw = linear_ce_finish(saved[2], g[0], saved[0], scale, saved[3]);
+      if (need_x) dx = KRSI_OP(linear_ce_finish).call(saved[1], g[0], saved[0], scale, saved[3]);
+      if (need_w) dw = KRSI_OP(linear_ce_finish).call(saved[2], g[0], saved[0], scale, saved[3]);
     } else {
-      std::tie(dx, dw) = linear_ce_grad(g[0], saved[0], saved[1], saved[2], saved[3], saved[4], scale,
-                                        ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["z_loss"].toDouble(),
-                                        need_x, need_w);
+      std::tie(dx, dw) = KRSI_OP(linear_ce_grad)
+                             .call(g[0], saved[0], saved[1], saved[2], saved[3], saved[4], scale,
+                                   ctx->saved_data["ignore_index"].toInt(), ctx->saved_data["z_loss"].toDouble(),
+                                   need_x, need_w);
       if (!need_x) dx = at::Tensor();
       if (!need_w) dw = at::Tensor();
     }

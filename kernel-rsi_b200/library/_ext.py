@@ -159,6 +159,19 @@ def _register_compile_support() -> None:
         rows, F = q.shape[0], q.shape[1] // 2
         return g.new_empty((rows, 2 * F)), g.new_empty((rows if want_out else 0, F))
 
+    # The operators of eager autograd (torch_ext.cpp), as inference mode reaches them.
+    @reg_fake("krsi::embedding")
+    def _(tokens, table, scale, padding_idx):
+        return table.new_empty((*tokens.shape, table.shape[1]))
+
+    @reg_fake("krsi::geglu_q8")
+    def _(u):
+        return u.new_empty((u.shape[0], u.shape[1] // 2))
+
+    @reg_fake("krsi::linear_ce")
+    def _(x2d, w, targets, scale, ignore_index, z_loss, reduction, keep):
+        return x2d.new_empty(() if reduction else (x2d.shape[0],), dtype=torch.float32)
+
     # Autograd of the forward ops, used when a compiled graph contains them (the eager path
     # uses the autograd.Function classes of each module instead).
     def rms_setup(ctx, inputs, output):

@@ -3,6 +3,8 @@ differentiation, dispatch modes, fake tensors, in-place changes and gradients of
 import pytest
 import torch
 import torch.autograd.forward_ad as fwd_ad
+from torch._subclasses.fake_tensor import FakeTensorMode
+from torch.utils._python_dispatch import TorchDispatchMode
 
 from embedding import embedding
 from geglu_q8 import feed_forward_q8, geglu_q8
@@ -46,3 +48,56 @@ def test_forward_mode_is_refused(name, requires_grad):
         with pytest.raises((RuntimeError, NotImplementedError), match="forward|jvp"):
             torch.func.jvp(fn, tuple(args), tuple(torch.ones_like(a) for a in args))
     fn(*args)   # and plain tensors still pass
+
+
+OPS = {   # the operators of a step of each function, forward and backward
+    "embedding": {"embedding_fwd", "embedding_bwd"},
+    "cross entropy": {"linear_ce_fwd", "linear_ce_grad"},
+    "cross entropy rows": {"linear_ce_fwd", "linear_ce_grad"},
+    "geglu": {"geglu_q8_fwd", "geglu_q8_bwd"},
+    "feed forward": {"geglu_q8_fwd", "geglu_q8_bwd"},
+}
+
+
+class Seen(TorchDispatchMode):
+    """The krsi operators that pass, and the calls themselves."""
+
+    def __init__(self):
+        super().__init__()
+        self.ops = set()
+
+    def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+        if func.namespace == "krsi":
+            self.ops.add(func._opname)
+        return func(*args, **(kwargs or {}))
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_dispatch_mode_sees_the_operators(name):
+    fn, args = calls()[name]
+    args = [a.requires_grad_(True) for a in args]
+    with Seen() as seen:
+        out = fn(*args)
+        torch.autograd.grad(out, args, torch.ones_like(out))
+    assert OPS[name] <= seen.ops, seen.ops
+    for mode in (torch.no_grad, torch.inference_mode):
+        with Seen() as seen, mode():
+            plain = fn(*args)
+        assert len(seen.ops) == 1 and torch.equal(plain, out), seen.ops
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_fake_tensors_get_shapes(name):
+    """Under a fake-tensor mode no kernel runs; outputs and gradients have the real ones' shapes and types."""
+    fn, args = calls()[name]
+    args = [a.requires_grad_(True) for a in args]
+    out = fn(*args)
+    grads = torch.autograd.grad(out, args, torch.ones_like(out))
+    with FakeTensorMode(allow_non_fake_inputs=True) as mode:   # (the integer inputs are real)
+        fakes = [mode.from_tensor(a.detach()).requires_grad_(True) for a in args]
+        fake = fn(*fakes)
+        fake_grads = torch.autograd.grad(fake, fakes, torch.ones_like(fake))
+        with torch.inference_mode():
+            again = fn(*[f.detach() for f in fakes])
+    for got, want in zip((fake, again, *fake_grads), (out, out, *grads)):
+        assert got.shape == want.shape and got.dtype == want.dtype and got.device == want.device

@@ -134,3 +134,22 @@ def test_perf_cases_are_well_formed():
     for _ in range(200):
         w = ops.work(ops.draw(rng))
         assert 0 < max(w["bytes"] * 300, w["flops"]) <= most
+
+
+def test_fake_tensors_pass_the_eager_operators():
+    """Shapes of fake CUDA tensors through the public functions, where no kernel can run."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    from embedding import embedding
+    from geglu_q8 import geglu_q8
+    from linear_cross_entropy import linear_cross_entropy
+
+    with FakeTensorMode():
+        f = lambda *s, dtype=torch.bfloat16: torch.empty(*s, device="cuda", dtype=dtype)  # noqa: E731
+        t, x, tok = f(50, 64), f(24, 64), f(24, dtype=torch.long)
+        for need in (False, True):
+            a, b = x.clone().requires_grad_(need), t.clone().requires_grad_(need)
+            for y, shape in ((embedding(tok, b), (24, 64)), (geglu_q8(a), (24, 32)),
+                             (linear_cross_entropy(a, b, tok), ()),
+                             (linear_cross_entropy(a, b, tok, reduction="none"), (24,))):
+                assert y.shape == shape and y.device.type == "cuda" and y.requires_grad == need
