@@ -306,31 +306,41 @@ at::Tensor embedding_fwd(const at::Tensor& tokens_in, const at::Tensor& table_in
   return out;
 }
 
-at::Tensor embedding_bwd(const at::Tensor& g_in, const at::Tensor& tokens_in, const at::Tensor& table, double scale,
-                         int64_t padding_idx) {
+// The gradient of a table of V rows in g's type.  It needs nothing of the table itself, so the autograd node does
+// not keep it: a table that is changed in place between forward and backward is none of its business.
+at::Tensor embedding_grad(const at::Tensor& g_in, const at::Tensor& tokens_in, int64_t V, double scale,
+                          int64_t padding_idx) {
   check_cuda(g_in, "g");
   check_cuda(tokens_in, "tokens");
-  check_cuda(table, "table");
-  check_same_device(tokens_in, table, "embedding_bwd");
-  check_same_device(g_in, table, "embedding_bwd");
-  TORCH_CHECK(table.dim() == 2 && g_in.dim() > 0 && g_in.size(-1) == table.size(1) &&
-                  g_in.numel() == tokens_in.numel() * table.size(1),
-              "embedding_bwd: g must be [*tokens.shape, d]");
-  TORCH_CHECK(padding_idx >= -1 && padding_idx < table.size(0), "embedding_bwd: padding_idx out of range");
-  const int bits = token_bits_of(tokens_in, "embedding_bwd: tokens");
-  c10::cuda::CUDAGuard guard(table.device());
+  check_same_device(g_in, tokens_in, "embedding_grad");
+  TORCH_CHECK(g_in.dim() > 0 && g_in.size(-1) > 0 && g_in.numel() == tokens_in.numel() * g_in.size(-1),
+              "embedding_grad: g must be [*tokens.shape, d]");
+  TORCH_CHECK(V > 0 && padding_idx >= -1 && padding_idx < V, "embedding_grad: padding_idx out of range");
+  const int bits = token_bits_of(tokens_in, "embedding_grad: tokens");
+  c10::cuda::CUDAGuard guard(g_in.device());
   auto tokens = tokens_in.contiguous();
-  auto g = g_in.to(table.scalar_type()).contiguous();
-  auto dtable = at::empty(table.sizes(), table.options().memory_format(at::MemoryFormat::Contiguous));
-  const int64_t n = tokens.numel(), V = table.size(0), d = table.size(1);
+  auto g = g_in.contiguous();
+  const int64_t n = tokens.numel(), d = g.size(-1);
+  auto dtable = at::empty({V, d}, g.options());
   size_t ws = 0;
   check_rc(krsi_embedding_bwd_workspace_size(n, V, d, &ws), "krsi_embedding_bwd_workspace_size");
   auto wsp = workspace(g, ws);
   check_rc(krsi_embedding_bwd(tokens.data_ptr(), bits, g.data_ptr(), dtable.data_ptr(), wsp.data_ptr(),
-                              (size_t)wsp.numel(), n, V, d, (float)scale, padding_idx, krsi_dtype_of(table),
+                              (size_t)wsp.numel(), n, V, d, (float)scale, padding_idx, krsi_dtype_of(g),
                               at::cuda::getCurrentCUDAStream()),
            "krsi_embedding_bwd");
   return dtable;
+}
+
+// The same for a table at hand, whose shape and type the gradient takes.
+at::Tensor embedding_bwd(const at::Tensor& g_in, const at::Tensor& tokens_in, const at::Tensor& table, double scale,
+                         int64_t padding_idx) {
+  check_cuda(table, "table");
+  check_same_device(g_in, table, "embedding_bwd");
+  TORCH_CHECK(table.dim() == 2 && g_in.dim() > 0 && g_in.size(-1) == table.size(1) &&
+                  g_in.numel() == tokens_in.numel() * table.size(1),
+              "embedding_bwd: g must be [*tokens.shape, d]");
+  return embedding_grad(g_in.to(table.scalar_type()), tokens_in, table.size(0), scale, padding_idx);
 }
 
 // ---------------------------------------------------------------- GEGLU with an 8-bit checkpoint
@@ -515,7 +525,8 @@ struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& tokens, const at::Tensor& table, double scale,
                             int64_t padding_idx) {
     at::AutoDispatchBelowADInplaceOrView below;
-    ctx->save_for_backward({tokens, table});
+    ctx->save_for_backward({tokens});
+    ctx->saved_data["rows"] = table.dim() > 0 ? table.size(0) : 0;
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["padding_idx"] = padding_idx;
     return KRSI_OP(embedding_fwd).call(tokens, table, scale, padding_idx);
@@ -525,8 +536,9 @@ struct EmbeddingNode : public torch::autograd::Function<EmbeddingNode> {
     const auto saved = ctx->get_saved_variables();
     at::AutoDispatchBelowADInplaceOrView below;
     return {at::Tensor(),
-            KRSI_OP(embedding_bwd).call(g[0], saved[0], saved[1], ctx->saved_data["scale"].toDouble(),
-                                        ctx->saved_data["padding_idx"].toInt()),
+            KRSI_OP(embedding_grad)
+                .call(g[0], saved[0], ctx->saved_data["rows"].toInt(), ctx->saved_data["scale"].toDouble(),
+                      ctx->saved_data["padding_idx"].toInt()),
             at::Tensor(), at::Tensor()};
   }
 };
@@ -629,6 +641,7 @@ TORCH_LIBRARY(krsi, m) {
   m.def("t5_bias_bwd(Tensor dpd, Tensor table, int S, int num_buckets, int max_distance, bool bidirectional) -> Tensor");
   m.def("embedding_fwd(Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
   m.def("embedding_bwd(Tensor g, Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
+  m.def("embedding_grad(Tensor g, Tensor tokens, SymInt rows, float scale, int padding_idx) -> Tensor");
   m.def("embedding(Tensor tokens, Tensor table, float scale, int padding_idx) -> Tensor");
   m.def("geglu_q8(Tensor u) -> Tensor");
   m.def("linear_ce(Tensor x2d, Tensor w, Tensor targets, float scale, int ignore_index, float z_loss, int reduction, "
@@ -656,6 +669,7 @@ TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
   m.impl("t5_bias_bwd", &t5_bias_bwd);
   m.impl("embedding_fwd", &embedding_fwd);
   m.impl("embedding_bwd", &embedding_bwd);
+  m.impl("embedding_grad", &embedding_grad);
   m.impl("embedding", &embedding_fwd);
   m.impl("geglu_q8", &geglu_q8_plain);
   m.impl("linear_ce", &linear_ce_plain);

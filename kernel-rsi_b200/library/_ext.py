@@ -130,6 +130,10 @@ def _register_compile_support() -> None:
     def _(g, tokens, table, scale, padding_idx):
         return table.new_empty(table.shape)
 
+    @reg_fake("krsi::embedding_grad")
+    def _(g, tokens, rows, scale, padding_idx):
+        return g.new_empty((rows, g.shape[-1]))
+
     @reg_fake("krsi::linear_ce_fwd")
     def _(x2d, w, targets, scale, ignore_index, z_loss, reduction, want_dx, want_dw):
         f32 = torch.float32
@@ -229,12 +233,12 @@ def _register_compile_support() -> None:
 
     def emb_setup(ctx, inputs, output):
         tokens, table, scale, padding_idx = inputs
-        ctx.save_for_backward(tokens, table)
-        ctx.args = (scale, padding_idx)
+        ctx.save_for_backward(tokens)
+        ctx.args = (table.shape[0], scale, padding_idx)
 
     def emb_backward(ctx, g):
-        tokens, table = ctx.saved_tensors
-        return None, ops.embedding_bwd(g, tokens, table, *ctx.args), None, None
+        (tokens,) = ctx.saved_tensors
+        return None, ops.embedding_grad(g, tokens, *ctx.args), None, None
 
     torch.library.register_autograd("krsi::embedding_fwd", emb_backward, setup_context=emb_setup)
 

@@ -51,7 +51,7 @@ def test_forward_mode_is_refused(name, requires_grad):
 
 
 OPS = {   # the operators of a step of each function, forward and backward
-    "embedding": {"embedding_fwd", "embedding_bwd"},
+    "embedding": {"embedding_fwd", "embedding_grad"},
     "cross entropy": {"linear_ce_fwd", "linear_ce_grad"},
     "cross entropy rows": {"linear_ce_fwd", "linear_ce_grad"},
     "geglu": {"geglu_q8_fwd", "geglu_q8_bwd"},
@@ -101,3 +101,27 @@ def test_fake_tensors_get_shapes(name):
             again = fn(*[f.detach() for f in fakes])
     for got, want in zip((fake, again, *fake_grads), (out, out, *grads)):
         assert got.shape == want.shape and got.dtype == want.dtype and got.device == want.device
+
+
+def test_a_table_changed_in_place_before_the_backward():
+    """As with torch's embedding: the gradient needs the table's shape alone, and the table is not kept alive."""
+    tokens = torch.randint(0, V, (600,), device=dev)
+    g = torch.randn(600, K, device=dev)
+    for fn in (embedding, torch.compile(embedding, fullgraph=True)):
+        table = torch.randn(V, K, device=dev, requires_grad=True)
+        (want,) = torch.autograd.grad(fn(tokens, table), table, g)
+        out = fn(tokens, table)
+        with torch.no_grad():
+            table.mul_(0.5)
+        (got,) = torch.autograd.grad(out, table, g)
+        assert torch.equal(got, want)
+
+
+def test_embedding_grad_refusals():
+    op = torch.ops.krsi.embedding_grad
+    tokens, g = torch.zeros(4, dtype=torch.long, device=dev), torch.zeros(4, 8, device=dev)
+    assert op(g, tokens, 5, 1.0, -1).shape == (5, 8)
+    for bad in (lambda: op(g[:3], tokens, 5, 1.0, -1), lambda: op(g, tokens, 5, 1.0, 5), lambda: op(g, tokens, 0, 1.0, -1),
+                lambda: op(g, tokens.float(), 5, 1.0, -1), lambda: op(g.double(), tokens, 5, 1.0, -1)):
+        with pytest.raises(RuntimeError):
+            bad()
