@@ -586,7 +586,7 @@ struct LinearCeNode : public torch::autograd::Function<LinearCeNode> {
     auto [loss, total, weight, stats, dx, dw] =
         KRSI_OP(linear_ce_fwd).call(x, w, targets, scale, ignore_index, z_loss, reduction, keep && x.requires_grad(),
                                     keep && w.requires_grad());
-    if (keep) ctx->save_for_backward({weight, dx, dw, w});
+    if (keep) ctx->save_for_backward({weight, dx, dw, at::empty({0}, x.options())});   // (the gradients' type)
     else ctx->save_for_backward({weight, stats, x, w, targets});
     ctx->saved_data["scale"] = scale;
     ctx->saved_data["ignore_index"] = ignore_index;

@@ -249,7 +249,8 @@ def _register_compile_support() -> None:
         ctx.reduction, ctx.kept, ctx.wanted = reduction, want_dx or want_dw, (want_dx, want_dw)
         ctx.set_materialize_grads(False)
         if ctx.kept:
-            ctx.save_for_backward(weight, dx, dw, w)
+            ctx.save_for_backward(weight, dx, dw)
+            ctx.like = x2d.new_empty(0)   # the gradients' type: the operands themselves are not needed
         else:
             ctx.save_for_backward(weight, stats, x2d, w, targets)
 
@@ -260,9 +261,9 @@ def _register_compile_support() -> None:
             return (None, None) + none
         weight, *saved = ctx.saved_tensors
         if ctx.kept:
-            dx, dw, like = saved
-            return (ops.linear_ce_finish(dx, g, weight, ctx.args[0], like) if ctx.wanted[0] else None,
-                    ops.linear_ce_finish(dw, g, weight, ctx.args[0], like) if ctx.wanted[1] else None) + none
+            dx, dw = saved
+            return (ops.linear_ce_finish(dx, g, weight, ctx.args[0], ctx.like) if ctx.wanted[0] else None,
+                    ops.linear_ce_finish(dw, g, weight, ctx.args[0], ctx.like) if ctx.wanted[1] else None) + none
         need = ctx.needs_input_grad[:2]
         dx, dw = ops.linear_ce_grad(g, weight, *saved, *ctx.args, *need)
         return (dx if need[0] else None, dw if need[1] else None) + none

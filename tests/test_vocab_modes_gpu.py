@@ -8,7 +8,7 @@ from torch.utils._python_dispatch import TorchDispatchMode
 
 from embedding import embedding
 from geglu_q8 import feed_forward_q8, geglu_q8
-from linear_cross_entropy import linear_cross_entropy
+from linear_cross_entropy import KEEP_ROWS, linear_cross_entropy
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -125,3 +125,25 @@ def test_embedding_grad_refusals():
                 lambda: op(g, tokens.float(), 5, 1.0, -1), lambda: op(g.double(), tokens, 5, 1.0, -1)):
         with pytest.raises(RuntimeError):
             bad()
+
+
+def test_operands_changed_in_place_after_their_gradients_were_formed():
+    """From KEEP_ROWS rows on the forward of a reduced loss forms both gradients; what they were formed from may
+    then change or be freed.  (Gradients formed later need their operands and refuse a change.)"""
+    rows = KEEP_ROWS
+    t = torch.randint(0, V, (rows,), device=dev)
+    x0, w0 = torch.randn(rows, K, device=dev).bfloat16(), torch.randn(V, K, device=dev).bfloat16()
+    for fn in (linear_cross_entropy, torch.compile(linear_cross_entropy, fullgraph=True)):
+        x, w = x0.clone().requires_grad_(True), w0.clone().requires_grad_(True)
+        want = torch.autograd.grad(fn(x, w, t), (x, w))
+        loss = fn(x, w, t)
+        with torch.no_grad():
+            w.mul_(0.5)
+            x.zero_()
+        assert all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(loss, (x, w)), want))
+    x, w = x0[:100].clone().requires_grad_(True), w0.clone().requires_grad_(True)
+    loss = linear_cross_entropy(x, w, t[:100])
+    with torch.no_grad():
+        w.mul_(0.5)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        torch.autograd.grad(loss, x)
