@@ -49,6 +49,8 @@ class FeedForwardQ8(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gy):
+        if torch.is_grad_enabled():   # it would miss what du owes to gy and the operands
+            raise RuntimeError("feed_forward_q8: the backward has no gradient of its own (create_graph)")
         x2d, wi, wo, q, ex = ctx.saved_tensors
         gy = gy.contiguous()
         du, g = ops.geglu_q8_bwd(gy @ wo, q, ex, ctx.needs_input_grad[2])

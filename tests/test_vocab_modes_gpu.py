@@ -147,3 +147,12 @@ def test_operands_changed_in_place_after_their_gradients_were_formed():
         w.mul_(0.5)
     with pytest.raises(RuntimeError, match="modified by an inplace operation"):
         torch.autograd.grad(loss, x)
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_a_gradient_of_the_gradient_is_refused(name):
+    fn, args = calls()[name]
+    args = [a.requires_grad_(True) for a in args]
+    out = fn(*args)
+    with pytest.raises(RuntimeError, match="create_graph"):
+        torch.autograd.grad(out, args, torch.ones_like(out), create_graph=True)
