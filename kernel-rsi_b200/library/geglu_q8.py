@@ -33,17 +33,19 @@ GROUP = 32
 def geglu_q8(u):
     """gelu_tanh(u[:, :F]) * u[:, F:] for u [rows, 2F], its backward from an 8-bit copy of u."""
     if compiling():
-        return ops.geglu_q8_fwd(u, True)[0]
+        return ops.geglu_q8_fwd(u, torch.is_grad_enabled() and u.requires_grad)[0]
     return ops.geglu_q8(u)
 
 
 class FeedForwardQ8(torch.autograd.Function):
-    """res + geglu(x2d @ wi^T) @ wo^T; saves (x2d, wi, wo, q, exponents); returns (dx, dwi, dwo, dres)."""
+    """res + geglu(x2d @ wi^T) @ wo^T; saves (x2d, wi, wo, q, exponents); returns (dx, dwi, dwo, dres).
+    keep: whether a gradient but res's can be asked for; else there is no checkpoint."""
 
     @staticmethod
-    def forward(ctx, x2d, wi, wo, res):
-        g, q, ex = ops.geglu_q8_fwd(x2d @ wi.t(), True)
-        ctx.save_for_backward(x2d, wi, wo, q, ex)
+    def forward(ctx, x2d, wi, wo, res, keep):
+        g, q, ex = ops.geglu_q8_fwd(x2d @ wi.t(), keep)
+        if keep:
+            ctx.save_for_backward(x2d, wi, wo, q, ex)
         ctx.has_res = res is not None
         return torch.addmm(res, g, wo.t()) if res is not None else g @ wo.t()
 
@@ -51,13 +53,15 @@ class FeedForwardQ8(torch.autograd.Function):
     def backward(ctx, gy):
         if torch.is_grad_enabled():   # it would miss what du owes to gy and the operands
             raise RuntimeError("feed_forward_q8: the backward has no gradient of its own (create_graph)")
+        if not any(ctx.needs_input_grad[:3]):
+            return None, None, None, gy, None
         x2d, wi, wo, q, ex = ctx.saved_tensors
         gy = gy.contiguous()
         du, g = ops.geglu_q8_bwd(gy @ wo, q, ex, ctx.needs_input_grad[2])
         dx = du @ wi if ctx.needs_input_grad[0] else None
         dwi = du.t() @ x2d if ctx.needs_input_grad[1] else None
         dwo = gy.t() @ g if ctx.needs_input_grad[2] else None
-        return dx, dwi, dwo, (gy if ctx.has_res else None)
+        return dx, dwi, dwo, (gy if ctx.has_res else None), None
 
 
 def feed_forward_q8(x2d, wi, wo, res=None):
@@ -66,7 +70,8 @@ def feed_forward_q8(x2d, wi, wo, res=None):
     if compiling():
         y = geglu_q8(x2d @ wi.t()) @ wo.t()
         return y if res is None else y + res
-    return FeedForwardQ8.apply(x2d, wi, wo, res)
+    keep = torch.is_grad_enabled() and (x2d.requires_grad or wi.requires_grad or wo.requires_grad)
+    return FeedForwardQ8.apply(x2d, wi, wo, res, keep)
 
 
 def dequantise(q, exponents):
