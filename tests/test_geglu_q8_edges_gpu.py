@@ -69,3 +69,23 @@ def test_only_the_gradients_that_are_asked_for(which):
     need = [t for t in some if t.requires_grad]
     got = torch.autograd.grad(out, need, torch.ones_like(out))
     assert all(torch.equal(a, b) for a, b in zip(got, [w for w, n in zip(want, which) if n]))
+
+
+@pytest.mark.parametrize("residual", [True, False])
+def test_compiled_feed_forward_keeps_the_checkpoint_alone(residual):
+    """What is held between forward and backward besides the output: 2.0625 F bytes a row, compiled and not (the
+    rows' count makes the allocator's 512-byte rounding small); and the same bits of outputs and gradients."""
+    torch._dynamo.reset()
+    rows, d, F = 4096, 128, 1024
+    args = operands(rows, d, F)[:4 if residual else 3]
+    gy = torch.randn(rows, d, device=dev).bfloat16()
+    results = []
+    for fn in (feed_forward_q8, torch.compile(feed_forward_q8, fullgraph=True)):
+        fn(*args)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        out = fn(*args)
+        held = torch.cuda.memory_allocated() - before - out.numel() * 2
+        assert abs(held - 2.0625 * F * rows) <= 0.02 * F * rows, held / (F * rows)
+        results.append((out, *torch.autograd.grad(out, args, gy)))
+    assert all(torch.equal(a, b) for a, b in zip(*results))
