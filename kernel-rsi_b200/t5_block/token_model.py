@@ -93,12 +93,15 @@ def build(vocab, layers=2, checkpoint8=True, seed=0):
 
 
 def batch(vocab, B, S, seed, device="cuda"):
-    """Sequences in which each token follows from the one before (t -> 5 t + 3 mod the vocabulary less its
-    mask token, from a start below 64), 15% of them masked; the masked ones are the targets."""
+    """Sequences in which each token follows from the one before (t -> 5 t + 3 mod 64, or mod the vocabulary
+    less its mask token where that is smaller), 15% of them masked; the masked ones are the targets."""
+    if vocab < 2:
+        raise ValueError(f"a vocabulary of {vocab} has no token beside the mask token")
+    used = min(64, vocab - 1)
     g = torch.Generator().manual_seed(seed)
-    t = [torch.randint(0, 64, (B,), generator=g)]
+    t = [torch.randint(0, used, (B,), generator=g)]
     for _ in range(S - 1):
-        t.append((5 * t[-1] + 3) % 64)
+        t.append((5 * t[-1] + 3) % used)
     tokens = torch.stack(t, 1)
     masked = torch.rand(B, S, generator=g) < 0.15
     targets = torch.where(masked, tokens, IGNORE)

@@ -153,3 +153,23 @@ def test_fake_tensors_pass_the_eager_operators():
                              (linear_cross_entropy(a, b, tok), ()),
                              (linear_cross_entropy(a, b, tok, reduction="none"), (24,))):
                 assert y.shape == shape and y.device.type == "cuda" and y.requires_grad == need
+
+
+@pytest.mark.parametrize("vocab", [2, 3, 40, 64, 65, 66, 8192])
+def test_token_model_batches_stay_in_the_vocabulary(vocab):
+    """The synthetic sequences of any vocabulary: tokens and targets below its mask token, which stands for the
+    masked positions; the step from token to token holds.  From 65 on the sequences are the same ones."""
+    import importlib.util
+
+    spec = importlib.util.spec_from_file_location("krsi_token_model_cpu", PKG / "t5_block" / "token_model.py")
+    tm = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(tm)
+    tokens, targets = tm.batch(vocab, 4, 100, 3, device="cpu")
+    masked = targets != tm.IGNORE
+    assert masked.any() and torch.equal(masked, tokens == vocab - 1)
+    text = torch.where(masked, targets, tokens)
+    used = min(64, vocab - 1)
+    assert text.min() >= 0 and text.max() < vocab - 1
+    assert torch.equal(text[:, 1:], (5 * text[:, :-1] + 3) % used)
+    with pytest.raises(ValueError, match="mask token"):
+        tm.batch(1, 4, 100, 3, device="cpu")
