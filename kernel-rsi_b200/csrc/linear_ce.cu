@@ -426,10 +426,15 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
             float y[32];
 #pragma unroll
             for (int e = 0; e < 32; ++e) y[e] = fmaf(__uint_as_float(r[e]), a.c, RUNNING ? 0.f : -ref);
+            // what is left out: y, and for RUNNING the accumulator that it is made of again below
+            auto leave_out = [&](int e) {
+              y[e] = -INFINITY;
+              if (RUNNING) r[e] = a.c < 0.f ? 0x7f800000u : 0xff800000u;
+            };
             if (c0 + 32 > a.V) {
 #pragma unroll
               for (int e = 0; e < 32; ++e)
-                if (c0 + e >= a.V) y[e] = -INFINITY;
+                if (c0 + e >= a.V) leave_out(e);
             }
             if ((unsigned)(t - c0) < 32u) {
               float lt = 0.f;
@@ -437,7 +442,7 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
               for (int e = 0; e < 32; ++e)
                 if (t == c0 + e) {
                   lt = __uint_as_float(r[e]);
-                  y[e] = -INFINITY;
+                  leave_out(e);
                 }
               if (RUNNING) {
                 a.l2t_out[row] = a.c * lt;
@@ -450,9 +455,9 @@ ce_logits_kernel(const __grid_constant__ CUtensorMap xmap, const __grid_constant
               sum *= ex2_approx(ref - top);
               ref = top;
             }
-            if (RUNNING) {
+            if (RUNNING && ref != -INFINITY && a.c != 0.f) {   // l - ref in one rounding (of 0 there is none)
 #pragma unroll
-              for (int e = 0; e < 32; ++e) y[e] = ref == -INFINITY ? y[e] : y[e] - ref;
+              for (int e = 0; e < 32; ++e) y[e] = fmaf(__uint_as_float(r[e]), a.c, -ref);
             }
 #pragma unroll
             for (int e = 0; e < 32; ++e) y[e] = ex2_approx(y[e]);

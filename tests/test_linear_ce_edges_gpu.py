@@ -3,8 +3,8 @@ import pytest
 import torch
 
 import _ext
-from linear_cross_entropy import KEEP_ROWS
-from test_linear_ce_gpu import UNIT, exact, inputs, run
+from linear_cross_entropy import KEEP_ROWS, linear_cross_entropy
+from test_linear_ce_gpu import UNIT, check_grads, check_loss, exact, inputs, run
 
 pytestmark = pytest.mark.gpu
 dev = "cuda"
@@ -45,3 +45,32 @@ def test_f16_rows_scaled_far_up_by_the_z_loss(N, reduction):
     assert torch.all((dx.double() - e["dx"]).abs() <= bdx)
     assert torch.all((dw.double() - e["dw"]).abs() <= bdw)
     assert _ext.device_status() == 0
+
+
+@pytest.mark.parametrize("N", [64, KEEP_ROWS])
+def test_logits_far_from_zero_lose_nothing(N):
+    """Two entries whose logits are 1024 and 1024 + k / 64, both exact in fp32: the loss log1p(exp(k / 64)) is right
+    to what its exponential and logarithm cost, with no rounding of a logit's own size (2^-14 in log2 units here:
+    4e-5 of the exponential) in between."""
+    x, w = torch.zeros(N, 64), torch.zeros(2, 64)
+    k = (torch.arange(N) * 37 % 509 - 254).float()
+    x[:, 0], w[:, 0] = 64.0, 16.0
+    x[:, 1], w[1, 1] = k / 64, 1.0
+    t = torch.zeros(N, dtype=torch.long)
+    x, w, t = x.bfloat16().to(dev), w.bfloat16().to(dev), t.to(dev)
+    want = torch.log1p(torch.exp(x[:, 1].double()))
+    with torch.no_grad():
+        loss = linear_cross_entropy(x, w, t, reduction="none")
+    # l - ref: one rounding at up to 4 log2(e) = 5.8; 2 units each of the exponentials, factors and logarithm
+    assert torch.all((loss.double() - want).abs() <= 2.0 ** -19 * want), ((loss.double() - want).abs() / want).max()
+
+
+@pytest.mark.parametrize("N", [60, KEEP_ROWS])
+@pytest.mark.parametrize("scale", [0.0, -0.5])
+def test_scales_of_zero_and_below(N, scale):
+    """A scale of 0 (every logit 0: the loss is log V) and a negative one, with a ragged vocabulary."""
+    x, w, t = inputs(N, 333, 64, torch.bfloat16, 8, ignored=0.1)
+    e = exact(x, w, t, scale, up=torch.ones(N, device=dev))
+    loss, dx, dw = run(x, w, t, torch.ones(N, device=dev), scale=scale, reduction="none")
+    check_loss(loss, e)
+    check_grads(dx, dw, e, torch.bfloat16)
