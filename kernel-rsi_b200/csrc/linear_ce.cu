@@ -538,12 +538,16 @@ __device__ __forceinline__ void reduce_rows(const float* loss, const int* tgt, f
     *weight = (float)(1.0 / m);
   }
 }
-__global__ void __launch_bounds__(1024)
+template <int NT>
+__global__ void __launch_bounds__(NT)
 ce_reduce_kernel(const float* __restrict__ loss, const int* __restrict__ tgt, float* __restrict__ total,
                  float* __restrict__ weight, int n, int mean) {
   pdl_enter();
-  reduce_rows<1024>(loss, tgt, total, weight, n, mean);
+  reduce_rows<NT>(loss, tgt, total, weight, n, mean);
 }
+// Rows up to which 256 threads reduce (32 rows a thread; the join's last block where one join has all rows), above
+// 1024: by the rows alone, since the loss is to have the same bits whatever the chunks.
+constexpr int64_t kJoinReduceRows = 8192;
 
 struct JoinArgs {
   float *total, *weight;   // with few rows the last block to finish reduces the losses itself; or null
@@ -1332,8 +1336,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   };
   const float e_scale = F16 ? kHalfScale : 1.f;
   const bool few = p.N <= tokens::kFewRows;
-  // Up to 8192 rows the join's last block reduces the losses (32 a thread); above, a block of 1024 threads.
-  const bool joined = p.chunks == 1 && p.N <= 8192;
+  const bool joined = p.chunks == 1 && p.N <= kJoinReduceRows;
   if (p.grads && c.dw && !few)
     KRSI_CUDA_TRY(tokens::token_sort(c.targets, c.target_bits, N, V, c.ignore, s.sorted.start, s.sorted.pos,
                                      s.sorted.tok, stream));
@@ -1512,9 +1515,11 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       }
     }
   }
-  if (c.total && !joined)
-    KRSI_CUDA_TRY(launch_pdl(ce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)c.loss,
-                             (const int*)s.tgt, c.total, c.row_weight, N, c.mean));
+  if (c.total && !joined) {
+    const bool small = p.N <= kJoinReduceRows;
+    KRSI_CUDA_TRY(launch_pdl(small ? ce_reduce_kernel<256> : ce_reduce_kernel<1024>, dim3(1), dim3(small ? 256 : 1024), 0,
+                             stream, (const float*)c.loss, (const int*)s.tgt, c.total, c.row_weight, N, c.mean));
+  }
   return KRSI_OK;
 }
 
@@ -1564,7 +1569,7 @@ extern "C" int krsi_linear_ce_fwd(const void* x, const void* w, const void* targ
   KRSI_CHECK_ARG((total != nullptr) == (weight != nullptr));
   if (N == 0) {
     if (dw) KRSI_CUDA_TRY(cudaMemsetAsync(dw, 0, (size_t)V * K * 4, stream));
-    if (total) KRSI_CUDA_TRY(launch_pdl(ce_reduce_kernel, dim3(1), dim3(1024), 0, stream, (const float*)nullptr,
+    if (total) KRSI_CUDA_TRY(launch_pdl(ce_reduce_kernel<256>, dim3(1), dim3(256), 0, stream, (const float*)nullptr,
                                         (const int*)nullptr, total, weight, 0, mean));
     return KRSI_OK;
   }

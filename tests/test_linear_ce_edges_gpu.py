@@ -74,3 +74,17 @@ def test_scales_of_zero_and_below(N, scale):
     loss, dx, dw = run(x, w, t, torch.ones(N, device=dev), scale=scale, reduction="none")
     check_loss(loss, e)
     check_grads(dx, dw, e, torch.bfloat16)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum"])
+@pytest.mark.parametrize("N,V", [(1100, 300_001), (8192, 500), (8193, 500), (8300, 40_000)])
+def test_the_loss_has_the_same_bits_with_and_without_gradients(N, V, reduction):
+    """Rows on both sides of the reductions' border, and chunks with gradients where there are none without."""
+    x, w, t = inputs(N, V, 64, torch.bfloat16, 17, ignored=0.1)
+    loss = run(x, w, t, reduction=reduction)[0]
+    with torch.no_grad():
+        rows = linear_cross_entropy(x, w, t, reduction="none")
+        assert torch.equal(linear_cross_entropy(x, w, t, reduction=reduction), loss)
+    count = int((t != -100).sum()) if reduction == "mean" else 1
+    # rows added in float64, one rounding
+    assert abs(loss.double() - rows.double().sum() / count) <= 2.0 ** -23 * loss.double()
