@@ -1207,9 +1207,11 @@ inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool known, i
   Plan p{N, V, K, grads, known};
   p.n_vt = ceil_div(V, kBN);
   p.panels = ceil_div(V, 64);
-  // At most 2^28 logits a chunk (512 MB of e), in chunks of equal size; the loss alone keeps none.
-  const int64_t most = std::max<int64_t>(256, std::min<int64_t>(1 << 17, ((int64_t)1 << 28) / (p.panels * 64) / 256 * 256));
-  p.chunks = grads ? std::max<int64_t>(1, ceil_div(N, most)) : 1;
+  // Chunks of equal size, of at least 256 rows: with gradients of at most 2^28 logits (512 MB of e); the loss alone
+  // keeps the half tiles' sums only, at most 256 MB of them (2^17 rows of up to 32768 entries).
+  const int64_t kept = grads ? ((int64_t)1 << 28) / (p.panels * 64) : ((int64_t)1 << 28) / (2 * p.n_vt * 8);
+  const int64_t most = std::max<int64_t>(256, std::min<int64_t>(1 << 17, kept / 256 * 256));
+  p.chunks = std::max<int64_t>(1, ceil_div(N, most));
   p.chunk = std::max<int64_t>(256, ceil_div(ceil_div(N, p.chunks), 256) * 256);
   p.chunks = std::max<int64_t>(1, ceil_div(N, p.chunk));
   p.direct = known && p.chunks == 1;
@@ -1352,6 +1354,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     return KRSI_ERR_CUDA;
   for (int64_t r0 = 0; r0 < p.N; r0 += p.chunk) {
     const int64_t rows = std::min(p.chunk, p.N - r0);
+    const void* targets = static_cast<const char*>(c.targets) + r0 * (c.target_bits / 8);
     const T* xc = x + r0 * K;
     CUtensorMap xm, es, ek, em, xs;
     if (!make_map(&xm, xc, rows, K, K, F16, kBK, kBM, sw128)) return KRSI_ERR_CUDA;
@@ -1375,11 +1378,11 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     la.store = p.grads && !F16;
     la.limit = kSpinLimit;
     if (running) {
-      la.targets = c.targets;
+      la.targets = targets;
       la.target_bits = c.target_bits;
       la.ignore = (long long)c.ignore;
-      la.l2t_out = s.l2t;
-      la.l2t_low_out = s.l2t_low;
+      la.l2t_out = s.l2t + r0;
+      la.l2t_low_out = s.l2t_low + r0;
       la.ticket = s.ticket;
     }
     const int logit_pairs = (int)std::min<int64_t>(pairs, (int64_t)la.n_rt * la.n_vt);
@@ -1394,7 +1397,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
       ja.part = s.part;
       ja.n_part = 2 * (int)p.n_vt;
       ja.tgt = s.tgt + r0;
-      ja.targets = running ? c.targets : nullptr;
+      ja.targets = running ? targets : nullptr;
       ja.target_bits = c.target_bits;
       ja.V = V;
       ja.ignore = (long long)c.ignore;
@@ -1421,7 +1424,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     if (known || rows_after_join) {
       if (tops) KRSI_CUDA_TRY(find_top(r0, rows));
       RowsArgs ra{};
-      ra.targets = static_cast<const char*>(c.targets) + r0 * (c.target_bits / 8);
+      ra.targets = targets;
       ra.stats = stats + r0;
       ra.up = up;
       ra.row0 = r0;
@@ -1527,9 +1530,8 @@ inline int check(int64_t N, int64_t V, int64_t K, int target_bits, int dtype) {
   KRSI_CHECK_ARG(N >= 0 && V > 0 && K > 0);
   KRSI_CHECK_ARG(target_bits == 32 || target_bits == 64);
   if (dtype != KRSI_BF16 && dtype != KRSI_F16) return KRSI_ERR_UNSUPPORTED;
-  // TMA row strides and 16-byte packets (K % 8); 32-bit tile and row indices
+  // TMA row strides and 16-byte packets (K % 8); 32-bit tile and row indices (a chunk has at most 2^22 tiles)
   if (K % 8 != 0 || N > (1 << 30) || V > (1 << 30) || K > (1 << 20)) return KRSI_ERR_UNSUPPORTED;
-  if (ceil_div(std::min<int64_t>(N, (1 << 28)), 256) * ceil_div(V, kBN) > INT32_MAX / 2) return KRSI_ERR_UNSUPPORTED;
   return KRSI_OK;
 }
 

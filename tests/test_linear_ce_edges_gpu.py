@@ -1,8 +1,11 @@
 """The vocabulary cross entropy (B200) at the limits of its types and paths, against float64."""
+import ctypes
+
 import pytest
 import torch
 
 import _ext
+from gpu_util import capi
 from linear_cross_entropy import KEEP_ROWS, linear_cross_entropy
 from test_linear_ce_gpu import UNIT, check_grads, check_loss, exact, inputs, run
 
@@ -88,3 +91,44 @@ def test_the_loss_has_the_same_bits_with_and_without_gradients(N, V, reduction):
     count = int((t != -100).sum()) if reduction == "mean" else 1
     # rows added in float64, one rounding
     assert abs(loss.double() - rows.double().sum() / count) <= 2.0 ** -23 * loss.double()
+
+
+def workspace(N, V, K, mode):
+    size = ctypes.c_size_t(0)
+    rc = capi().krsi_linear_ce_workspace_size(ctypes.c_int64(N), ctypes.c_int64(V), ctypes.c_int64(K), mode, ctypes.byref(size))
+    assert rc == 0
+    return size.value
+
+
+def test_the_losses_workspace_is_bounded():
+    """The loss alone holds a chunk's partial sums (256 MB at most, or 256 rows') and under 32 bytes a row."""
+    for N, V in ((1, 100), (4096, 131072), (32768, 131072), (1 << 20, 131072), (1 << 24, 32768), (1 << 20, 1 << 26)):
+        part = max(1 << 28, 256 * 16 * ((V + 255) // 256))
+        assert workspace(N, V, 64, 0) <= part + 32 * N + 4096
+
+
+@pytest.mark.parametrize("bits", [32, 64])
+@pytest.mark.parametrize("N", [600, KEEP_ROWS + 276])
+def test_losses_of_several_chunks(N, bits):
+    """A vocabulary of 8.4 million entries cuts the rows of the loss alone into chunks of 256."""
+    V, K = 8_400_003, 8
+    g = torch.Generator(device=dev).manual_seed(2)
+    w = torch.randn(V, K, generator=g, device=dev).bfloat16()
+    x = torch.randn(N, K, generator=g, device=dev).bfloat16()
+    t = torch.randint(0, V, (N,), generator=g, device=dev)
+    t[3::11] = -100
+    with torch.no_grad():
+        rows = linear_cross_entropy(x, w, t if bits == 64 else t.int(), reduction="none")
+        total = linear_cross_entropy(x, w, t if bits == 64 else t.int(), reduction="sum")
+    W = w.double()
+    want = torch.zeros(N, dtype=torch.float64, device=dev)
+    for i in range(0, N, 64):
+        L = x[i:i + 64].double() @ W.t()
+        want[i:i + 64] = torch.logsumexp(L, 1) - L.gather(1, t[i:i + 64].clamp(min=0)[:, None])[:, 0]
+        del L
+    want = torch.where(t != -100, want, 0.0)
+    # sums of exponentials: 128 of a half tile, 2 V / 256 / 32 half tiles a lane, 8 more; the logits' own 2^-20
+    bound = (128 + V // 4096 + 8) * 2.0 ** -24 + 2.0 ** -20 * (1 + want)
+    assert torch.all((rows.double() - want).abs() <= bound), (rows.double() - want).abs().max()
+    assert torch.equal(total, rows.double().sum().float())
+    assert _ext.device_status() == 0
