@@ -234,7 +234,15 @@ int krsi_geglu_q8_bwd(const void* g, const void* q, const void* exponents, void*
  * gradients NaN.  workspace: 256-byte aligned.  Needs clusters of two CTAs (KRSI_ERR_UNSUPPORTED where
  * the device has none). */
 
-/* Bytes of workspace: mode 0 krsi_linear_ce_fwd without gradients, 1 with, 2 krsi_linear_ce_grad. */
+/* Bytes of workspace: mode 0 krsi_linear_ce_fwd without gradients, 1 with, 2 krsi_linear_ce_grad; 1 and 2 less what
+ * one gradient takes with KRSI_CE_NO_DX or KRSI_CE_NO_DW added, for calls where that pointer is null.
+ * A call works on chunks of rows: R rows, of at least 256.  In bytes, each part rounded up to 256:
+ *   always     16 N; mode 0 and 1: 16 R ceil(V / 256), at most 2^28 for the loss alone (or 256 rows')
+ *   gradients  20 N + R (128 ceil(V / 64) + 2 K), R so that the first product is at most 2^29 (or 256 rows')
+ *   dx         4 R K for each share of the vocabulary that its sums are cut into (none where R is large)
+ *   dw         with more than 512 rows the sorted targets, about 4 V + 8 N + N K / 2; mode 2: 4 V K */
+#define KRSI_CE_NO_DX 4
+#define KRSI_CE_NO_DW 8
 int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, int mode, size_t* bytes);
 
 /* loss: [N] fp32.  total, weight: one float each, or both null: the sum of the losses (mean: divided by

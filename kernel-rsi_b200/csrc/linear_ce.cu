@@ -1195,7 +1195,8 @@ inline bool make_panel_map(CUtensorMap* map, const void* base, int64_t rows, int
 // Sizes of one call.
 struct Plan {
   int64_t N, V, K;
-  bool grads, known;       // gradients wanted; from known log-sum-exps (krsi_linear_ce_grad)
+  bool dx, dw, known;      // gradients wanted; from known log-sum-exps (krsi_linear_ce_grad)
+  bool grads;              // either
   bool direct;             // dw leaves the GEMM in 16 bits
   int64_t n_vt, panels;    // vocabulary tiles; panels of e
   int64_t chunk, chunks;   // rows per chunk (a multiple of 256)
@@ -1203,8 +1204,11 @@ struct Plan {
   int64_t splits;          // of dx over the vocabulary
 };
 
-inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool grads, bool known, int pairs) {
-  Plan p{N, V, K, grads, known};
+// (The tiles and shares do not depend on which gradients are wanted: one alone has the bits that it has with the
+// other.)
+inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool dx, bool dw, bool known, int pairs) {
+  const bool grads = dx || dw;
+  Plan p{N, V, K, dx, dw, known, grads};
   p.n_vt = ceil_div(V, kBN);
   p.panels = ceil_div(V, 64);
   // Chunks of equal size, of at least 256 rows: with gradients of at most 2^28 logits (512 MB of e); the loss alone
@@ -1273,11 +1277,15 @@ inline Space space_at(void* base, const Plan& p) {
     s.stats = reinterpret_cast<float2*>(p.known ? 0 : take((size_t)p.N * 8));
     s.e = reinterpret_cast<void*>(take((size_t)rows * p.panels * 128));
     s.xs = reinterpret_cast<void*>(take((size_t)rows * p.K * 2));
-    s.dw32 = reinterpret_cast<float*>(p.known ? take((size_t)p.V * p.K * 4) : 0);
-    s.dx_part = reinterpret_cast<float*>(p.splits > 1 ? take((size_t)p.splits * p.chunk * p.K * 4) : 0);
-    const size_t sort_off = off;
-    s.sorted = tokens::space_at(reinterpret_cast<void*>(at + sort_off), p.N, p.V, p.K);
-    off += s.sorted.bytes;
+    s.dx_part = reinterpret_cast<float*>(p.dx && p.splits > 1 ? take((size_t)p.splits * p.chunk * p.K * 4) : 0);
+    if (p.dw) {
+      s.dw32 = reinterpret_cast<float*>(p.known ? take((size_t)p.V * p.K * 4) : 0);
+      if (p.N > tokens::kFewRows) {
+        const size_t sort_off = off;
+        s.sorted = tokens::space_at(reinterpret_cast<void*>(at + sort_off), p.N, p.V, p.K);
+        off += s.sorted.bytes;
+      }
+    }
   }
   s.bytes = off;
   return s;
@@ -1540,7 +1548,7 @@ inline int run_checked(const Call& c, int64_t N, int64_t V, int64_t K, void* wor
   if (!aligned16(c.x) || !aligned16(c.w) || !aligned16(c.dx) || !aligned16(c.dw)) return KRSI_ERR_MISALIGNED;
   const int pairs = device_pairs();
   if (pairs <= 0) return KRSI_ERR_UNSUPPORTED;   // a device partition without clusters of two
-  const Plan p = make_plan(N, V, K, c.dx != nullptr || c.dw != nullptr, c.loss == nullptr, pairs);
+  const Plan p = make_plan(N, V, K, c.dx != nullptr, c.dw != nullptr, c.loss == nullptr, pairs);
   const Space s = space_at(workspace, p);
   if (!workspace || workspace_bytes < s.bytes) return KRSI_ERR_WORKSPACE;
   if (reinterpret_cast<uintptr_t>(workspace) % 256 != 0) return KRSI_ERR_MISALIGNED;
@@ -1554,10 +1562,13 @@ inline int run_checked(const Call& c, int64_t N, int64_t V, int64_t K, void* wor
 using namespace krsi;
 
 extern "C" int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, int mode, size_t* bytes) {
-  KRSI_CHECK_ARG(bytes && N >= 0 && V > 0 && K > 0 && mode >= 0 && mode <= 2);
+  const int kind = mode & 3;
+  KRSI_CHECK_ARG(bytes && N >= 0 && V > 0 && K > 0 && mode >= 0 && kind <= 2);
+  KRSI_CHECK_ARG(mode == kind || (kind > 0 && (mode == kind + KRSI_CE_NO_DX || mode == kind + KRSI_CE_NO_DW)));
   const int pairs = device_pairs();
   if (pairs <= 0) return KRSI_ERR_UNSUPPORTED;
-  *bytes = space_at(nullptr, make_plan(N, V, K, mode > 0, mode == 2, pairs)).bytes;
+  *bytes = space_at(nullptr, make_plan(N, V, K, kind > 0 && !(mode & KRSI_CE_NO_DX),
+                                          kind > 0 && !(mode & KRSI_CE_NO_DW), kind == 2, pairs)).bytes;
   return KRSI_OK;
 }
 

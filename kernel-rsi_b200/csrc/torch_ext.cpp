@@ -393,6 +393,10 @@ struct CeCall {
   int bits, dtype;
   int64_t N, V, K;
 };
+int ce_mode(int kind, bool want_dx, bool want_dw) {
+  if (!want_dx && !want_dw) return 0;
+  return kind + (want_dx ? 0 : KRSI_CE_NO_DX) + (want_dw ? 0 : KRSI_CE_NO_DW);
+}
 CeCall ce_call(const at::Tensor& x_in, const at::Tensor& w_in, const at::Tensor& targets_in, int mode) {
   check_cuda(x_in, "x2d");
   check_cuda(w_in, "w");
@@ -426,7 +430,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tensor, at::Tenso
     double z_loss, int64_t reduction, bool want_dx, bool want_dw) {
   TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(x_in.device());
-  const CeCall c = ce_call(x_in, w_in, targets_in, want_dx || want_dw ? 1 : 0);
+  const CeCall c = ce_call(x_in, w_in, targets_in, ce_mode(1, want_dx, want_dw));
   auto f32 = c.x.options().dtype(at::kFloat);
   auto loss = at::empty({c.N}, f32);
   // (tensors of their own: the weight is saved, and a caller may change the loss in place)
@@ -454,7 +458,7 @@ std::tuple<at::Tensor, at::Tensor> linear_ce_grad(const at::Tensor& g_in, const 
                                                   double z_loss, bool want_dx, bool want_dw) {
   TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
   c10::cuda::CUDAGuard guard(x_in.device());
-  const CeCall c = ce_call(x_in, w_in, targets_in, 2);
+  const CeCall c = ce_call(x_in, w_in, targets_in, ce_mode(2, want_dx, want_dw));
   TORCH_CHECK(g_in.numel() == c.N || g_in.numel() == 1, "linear_ce_grad: g must have ", c.N, " values or one");
   TORCH_CHECK(weight_in.numel() <= 1, "linear_ce_grad: weight must be one value or empty");
   TORCH_CHECK(stats.scalar_type() == at::kFloat && stats.is_contiguous() && stats.numel() == 2 * c.N,

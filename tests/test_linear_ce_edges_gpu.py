@@ -132,3 +132,25 @@ def test_losses_of_several_chunks(N, bits):
     assert torch.all((rows.double() - want).abs() <= bound), (rows.double() - want).abs().max()
     assert torch.equal(total, rows.double().sum().float())
     assert _ext.device_status() == 0
+
+
+@pytest.mark.parametrize("N", [1, 600])
+def test_one_gradient_takes_its_own_workspace_alone(N):
+    """The weight's fp32 rows and sorted targets are held for dw only, dx's shares for dx only; and each gradient alone
+    has the bits that it has beside the other, on every path."""
+    V, K = 20_000, 512
+    both, no_dw, no_dx = (workspace(N, V, K, 2 + f) for f in (0, 8, 4))
+    assert no_dw < both - 4 * min(N, V) * K + 4096 and no_dx <= both
+    chunk = 256 * ((N + 255) // 256)      # e and x' of a chunk, and at most one share of dx per 8 blocks of 64 entries
+    assert no_dw <= 64 * N + chunk * (2 * (V + 64) + 2 * K) + 4 * chunk * K * (V // 512 + 1) + 8192
+    assert workspace(N, V, K, 1 + 8) <= workspace(N, V, K, 1) and workspace(N, V, K, 1 + 4) <= workspace(N, V, K, 1)
+    x, w, t = inputs(N, V, K, torch.bfloat16, 3)
+    up = torch.rand(N, device=dev)
+    loss, dx, dw = run(x, w, t, up, reduction="none")
+    a, b = x.detach().requires_grad_(True), w.detach().requires_grad_(True)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    held = torch.cuda.memory_allocated()
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(a, w, t, reduction="none"), a, up)[0], dx)
+    assert torch.cuda.max_memory_allocated() - held <= no_dw + 4 * N * K + (1 << 21)
+    assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, b, t, reduction="none"), b, up)[0], dw)

@@ -173,3 +173,11 @@ def test_token_model_batches_stay_in_the_vocabulary(vocab):
     assert torch.equal(text[:, 1:], (5 * text[:, :-1] + 3) % used)
     with pytest.raises(ValueError, match="mask token"):
         tm.batch(1, 4, 100, 3, device="cpu")
+
+
+def test_linear_ce_workspace_modes(lib):
+    """Kinds 0 to 2, and with gradients at most one of the two flags; refused before the device is asked."""
+    for mode in (-1, 3, 4, 8, 7, 11, 13, 14, 16, 17):
+        assert lib.krsi_linear_ce_workspace_size(i64(4), i64(10), i64(64), mode, ctypes.byref(size(0))) == 1, mode
+    for mode in (0, 1, 2, 5, 6, 9, 10):
+        assert lib.krsi_linear_ce_workspace_size(i64(4), i64(10), i64(64), mode, ctypes.byref(size(0))) != 1, mode
