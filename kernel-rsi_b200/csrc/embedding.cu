@@ -78,8 +78,9 @@ struct TableRows {
   T* dtable;
   int64_t d;
   float scale;
+  static constexpr bool kUsesFirst = false;
   using Base = tokens::NoBase;
-  __device__ __forceinline__ Base fetch(int, uint32_t) const { return {}; }
+  __device__ __forceinline__ Base fetch(int, int, uint32_t) const { return {}; }
   __device__ __forceinline__ void packet(int v, uint32_t c, const float* sums, Base) const {
     Pack<T, VEC> o;
 #pragma unroll
@@ -92,7 +93,7 @@ struct TableRows {
     for (int e = 0; e < VEC; ++e) o.v[e] = Elem<DT>::store(0.f);
     *reinterpret_cast<Pack<T, VEC>*>(dtable + v * d + c * VEC) = o;
   }
-  __device__ __forceinline__ void column(int v, int col, float sum) const {
+  __device__ __forceinline__ void column(int v, int, int col, float sum) const {
     dtable[v * d + col] = Elem<DT>::store(scale * sum);
   }
 };

@@ -780,8 +780,9 @@ struct GradArgs {
   const float* coef;
   const void* w;
   // dw: fp32 sums, stored or added; or scaled and rounded, and for the tokens that occur (by token_rows.cuh's
-  // start, or with few rows by tgt itself) the fp32 sums as well, rows of `sums`
-  int dw32, accumulate, few;
+  // start, or with few rows by tgt itself) the fp32 sums as well: rows of `sums`, by token, or (by_entry, where
+  // there are fewer rows than tokens) by the token's first entry
+  int dw32, accumulate, few, by_entry;
   float* sums;
   const int* start;
   tokens::Order order;
@@ -874,15 +875,15 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
         const int row = m.tile * (2 * kBM) + rank * kBM + (warp % 4) * 32 + lane;   // of dx, or the token of dw
         GradRow r{1.f, 0.f, false, -1, nullptr};
         const bool few = !m.is_dx && a.sums && a.few;
-        const unsigned near = few ? tokens::tokens_near(a.tgt, a.rows, row - lane) : 0;
+        const int first = few ? tokens::first_near(a.tgt, a.rows, row - lane) : 0;
         if (row >= (m.is_dx ? a.rows : a.V)) return r;
         if (!m.is_dx) {
           r.mul = a.alpha * a.up.unit();
           if (few) {
-            if (near >> lane & 1) r.sums = a.sums + (int64_t)row * a.K;
+            if (first >= 0) r.sums = a.sums + (int64_t)(a.by_entry ? first : row) * a.K;
           } else if (a.sums) {
-            const int k = a.order.key(row);
-            if (a.start[k] < a.start[k + 1]) r.sums = a.sums + (int64_t)row * a.K;
+            const int k = a.order.key(row), at = a.start[k];
+            if (at < a.start[k + 1]) r.sums = a.sums + (int64_t)(a.by_entry ? at : row) * a.K;
           }
         } else if (!a.dx_part) {
           const int t = a.tgt[row];
@@ -1055,8 +1056,9 @@ struct DwSums {
   int64_t K;
   // One addition per element and call, so a reduction in L2 (no read to wait for) gives the same bits
   // every time.
+  static constexpr bool kUsesFirst = false;
   using Base = tokens::NoBase;
-  __device__ __forceinline__ Base fetch(int, uint32_t) const { return {}; }
+  __device__ __forceinline__ Base fetch(int, int, uint32_t) const { return {}; }
   __device__ __forceinline__ void packet(int v, uint32_t c, const float* s, Base) const {
     float* p = dw32 + v * K + c * 8;
 #pragma unroll
@@ -1066,20 +1068,22 @@ struct DwSums {
                    : "memory");
   }
   __device__ __forceinline__ void zero(int, uint32_t) const {}
-  __device__ __forceinline__ void column(int v, int col, float s) const { dw32[v * K + col] += s; }
+  __device__ __forceinline__ void column(int v, int, int col, float s) const { dw32[v * K + col] += s; }
 };
 template <int DT>
 struct DwRows {
   using T = typename Elem<DT>::T;
-  const float* sums;
+  const float* sums;       // rows by token, or by the token's first entry
   T* dw;
   int64_t K;
   float scale;
+  bool by_entry;
+  static constexpr bool kUsesFirst = true;
   struct Base {
     Vec16<float> a, b;
   };
-  __device__ __forceinline__ Base fetch(int v, uint32_t c) const {
-    const float* p = sums + v * K + c * 8;
+  __device__ __forceinline__ Base fetch(int v, int first, uint32_t c) const {
+    const float* p = sums + (by_entry ? first : v) * K + c * 8;
     return {ldg16(p), ldg16(p + 4)};
   }
   __device__ __forceinline__ void packet(int v, uint32_t c, const float* s, const Base& base) const {
@@ -1092,8 +1096,8 @@ struct DwRows {
     stg16(dw + v * K + c * 8, o);
   }
   __device__ __forceinline__ void zero(int, uint32_t) const {}
-  __device__ __forceinline__ void column(int v, int col, float s) const {
-    dw[v * K + col] = Elem<DT>::store(scale * (sums[v * K + col] + s));
+  __device__ __forceinline__ void column(int v, int first, int col, float s) const {
+    dw[v * K + col] = Elem<DT>::store(scale * (sums[(by_entry ? first : v) * K + col] + s));
   }
 };
 
@@ -1279,7 +1283,9 @@ inline Space space_at(void* base, const Plan& p) {
     s.xs = reinterpret_cast<void*>(take((size_t)rows * p.K * 2));
     s.dx_part = reinterpret_cast<float*>(p.dx && p.splits > 1 ? take((size_t)p.splits * p.chunk * p.K * 4) : 0);
     if (p.dw) {
-      s.dw32 = reinterpret_cast<float*>(p.known ? take((size_t)p.V * p.K * 4) : 0);
+      // 16-bit dw in one chunk needs the sums of the tokens that occur only
+      const int64_t sum_rows = p.direct ? std::min(p.N, p.V) : p.V;
+      s.dw32 = reinterpret_cast<float*>(p.known ? take((size_t)sum_rows * p.K * 4) : 0);
       if (p.N > tokens::kFewRows) {
         const size_t sort_off = off;
         s.sorted = tokens::space_at(reinterpret_cast<void*>(at + sort_off), p.N, p.V, p.K);
@@ -1489,6 +1495,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     ga.accumulate = r0 > 0;
     ga.sums = p.direct ? dw32 : nullptr;
     ga.few = few;
+    ga.by_entry = p.N < p.V;
     ga.start = s.sorted.start;
     ga.order = s.sorted.order;
     ga.up = up;
@@ -1511,7 +1518,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   }
   if (p.grads && c.dw) {   // the targets' part of dw
     if (p.direct) {
-      const DwRows<DT> out{dw32, (T*)c.dw, p.K, c.scale};
+      const DwRows<DT> out{dw32, (T*)c.dw, p.K, c.scale, p.N < p.V};
       KRSI_CUDA_TRY(few ? (tokens::sum_few<DT, 8, true>(x, s.coef, (const int*)s.tgt, out, false, N, V, -1, K, stream))
                         : (tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
     } else {

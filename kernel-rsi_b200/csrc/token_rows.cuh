@@ -100,9 +100,10 @@ __device__ __forceinline__ void copy_wait() { asm volatile("cp.async.wait_group 
 // columns per thread.  A chunk's rows are staged in shared memory, all of its loads in flight at once: held
 // in registers they cost so many that a third as much was in flight (measured at 32768 rows of 1152 16-bit
 // values: 33 us against 39).
-// Out: packet(v, c, sums, base) takes the VEC finished sums of token v's packet c with what fetch(v, c) read
-// for it (a group's reads are in flight together), zero(v, c) an absent one, column(v, col, sum) one finished
-// column.
+// Out: packet(v, c, sums, base) takes the VEC finished sums of token v's packet c with what fetch(v, first, c)
+// read for it (a group's reads are in flight together), zero(v, c) an absent one, column(v, first, col, sum) one
+// finished column.  first: the place of v's first entry among the sorted ones, a number below n that is v's own
+// (kUsesFirst; else anything).
 constexpr int kZeroTokens = 32;
 constexpr int kGroupRows = 4;     // rows per group of copies
 
@@ -128,7 +129,7 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
     return;
   }
   const int i0 = chunk * kChunkRows;
-  __shared__ int s_pos[kChunkRows], s_tok[kChunkRows + 1];
+  __shared__ int s_pos[kChunkRows], s_tok[kChunkRows + 1], s_first[kChunkRows];
   __shared__ float s_weight[kChunkRows];
   // the chunk's entries, read beside the number that says how many of them there are
   const bool mine = threadIdx.x < kChunkRows && i0 + (int)threadIdx.x < n;
@@ -138,6 +139,7 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
   if (threadIdx.x < m) {
     s_pos[threadIdx.x] = p;
     s_tok[threadIdx.x] = t;
+    if (Out::kUsesFirst) s_first[threadIdx.x] = start[order.key(t)];
     if (WEIGHTED) s_weight[threadIdx.x] = weight[p];
   }
   if (threadIdx.x == 0) s_tok[m] = -1;   // the chunk's end ends a run
@@ -162,7 +164,8 @@ sum_rows_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restr
     typename Out::Base base[kGroupRows];
 #pragma unroll
     for (int k = 0; k < kGroupRows; ++k)
-      if (j0 + k < m && s_tok[j0 + k + 1] != s_tok[j0 + k]) base[k] = out.fetch(s_tok[j0 + k], c);
+      if (j0 + k < m && s_tok[j0 + k + 1] != s_tok[j0 + k]) 
+        base[k] = out.fetch(s_tok[j0 + k], Out::kUsesFirst ? s_first[j0 + k] : 0, c);
 #pragma unroll
     for (int k = 0; k < kGroupRows; ++k) {
       const int j = j0 + k;
@@ -222,9 +225,10 @@ join_rows_kernel(const int* __restrict__ start, const int* __restrict__ tok, con
     }
   };
   auto put = [&](int t, const float* acc) {
+    const int first = Out::kUsesFirst ? start[order.key(t)] : 0;
 #pragma unroll
     for (int j = 0; j < 4; ++j)
-      if (col0 + 32 * j < d) out.column(t, col0 + 32 * j, acc[j]);
+      if (col0 + 32 * j < d) out.column(t, first, col0 + 32 * j, acc[j]);
   };
   const int chunk = blockIdx.x * kJoinWarps + warp, i0 = chunk * kChunkRows, i1 = i0 + kChunkRows;
   int t = 0, n = 0;                                 // the run's token and partial rows; n = 0: none
@@ -281,6 +285,35 @@ __device__ __forceinline__ unsigned tokens_near(const I* tokens, int n, int v0) 
   return __reduce_or_sync(0xffffffffu, mask);
 }
 
+// The lane's token v0 + lane among tokens[0, n), n up to kFewRows: its first position, or -1.  Which lanes hold a
+// lane's token follows from five ballots a step, one per bit of the difference (a loop over the hits cost the steps
+// of 257 rows 5 us).
+template <typename I>
+__device__ __forceinline__ int first_near(const I* tokens, int n, int v0) {
+  constexpr int kSteps = kFewRows / 32;
+  const int lane = threadIdx.x % 32;
+  unsigned d[kSteps];
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {   // all loads in flight together
+    const int i = k * 32 + lane;
+    const auto far = i < n ? (std::make_unsigned_t<I>)tokens[i] - (std::make_unsigned_t<I>)v0 : (std::make_unsigned_t<I>)32;
+    d[k] = far < 32 ? (unsigned)far : 32u;
+  }
+  int first = -1;
+#pragma unroll
+  for (int k = 0; k < kSteps; ++k) {
+    unsigned same = __ballot_sync(0xffffffffu, d[k] < 32);
+    if (same == 0) continue;           // the same in every lane
+#pragma unroll
+    for (int b = 0; b < 5; ++b) {
+      const unsigned set = __ballot_sync(0xffffffffu, d[k] >> b & 1);
+      same &= lane >> b & 1 ? set : ~set;
+    }
+    if (same != 0 && first < 0) first = k * 32 + __ffs(same) - 1;
+  }
+  return first;
+}
+
 template <int DT, int VEC, bool WEIGHTED, typename Out, typename I>
 __global__ void __launch_bounds__(256)
 sum_few_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restrict__ weight,
@@ -317,7 +350,7 @@ sum_few_kernel(const typename Elem<DT>::T* __restrict__ g, const float* __restri
   extern __shared__ __align__(16) unsigned char stage_raw[];
   P* stage = reinterpret_cast<P*>(stage_raw) + threadIdx.x;   // [kChunkRows][blockDim.x]
   const P* gp = reinterpret_cast<const P*>(g) + c;
-  const typename Out::Base base = out.fetch((int)mine, c);
+  const typename Out::Base base = out.fetch((int)mine, i, c);
   float acc[VEC];
 #pragma unroll
   for (int e = 0; e < VEC; ++e) acc[e] = 0.f;

@@ -154,3 +154,25 @@ def test_one_gradient_takes_its_own_workspace_alone(N):
     assert torch.equal(torch.autograd.grad(linear_cross_entropy(a, w, t, reduction="none"), a, up)[0], dx)
     assert torch.cuda.max_memory_allocated() - held <= no_dw + 4 * N * K + (1 << 21)
     assert torch.equal(torch.autograd.grad(linear_cross_entropy(x, b, t, reduction="none"), b, up)[0], dw)
+
+
+def test_the_weights_sums_go_by_the_rows_where_those_are_fewer():
+    """One row over a large vocabulary used to hold fp32 sums for every entry of w (604 MB here)."""
+    assert workspace(1, 131072, 1152, 2) < 256 * 131072 * 2 + (16 << 20)   # the exponentials of 256 rows, and little else
+    assert workspace(3000, 1000, 512, 2) < workspace(3000, 3001, 512, 2)
+
+
+@pytest.mark.parametrize("N,V", [(40, 5000), (512, 5000), (513, 5000), (700, 701), (700, 700), (700, 699), (500, 33)])
+def test_tokens_that_occur_often(N, V):
+    """A few tokens that hold most of the rows (runs over many chunks of the sorted sum) among single ones, with more
+    tokens than rows and fewer; the sums' rows are those of the tokens that occur."""
+    x, w, t = inputs(N, V, 136, torch.bfloat16, 31)
+    often = torch.randint(0, 3, (N,), generator=torch.Generator().manual_seed(4)).to(dev) * (V // 3 + 1) % V
+    t = torch.where(torch.arange(N, device=dev) % 4 == 0, t, often)
+    t[1::13] = -100
+    up = torch.rand(N, device=dev)
+    e = exact(x, w, t, up=up)
+    loss, dx, dw = run(x, w, t, up, reduction="none")
+    check_loss(loss, e)
+    check_grads(dx, dw, e, torch.bfloat16)
+    assert _ext.device_status() == 0
