@@ -176,3 +176,74 @@ def test_tokens_that_occur_often(N, V):
     check_loss(loss, e)
     check_grads(dx, dw, e, torch.bfloat16)
     assert _ext.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("reduction,z", [("mean", 0.0), ("sum", 1e-3), ("none", 0.0)])
+def test_gradients_over_several_chunks(reduction, z, dtype):
+    """A vocabulary that cuts 1100 rows into chunks of 768: gradients formed in the forward (mean, sum) and later
+    (none), ignored rows in both chunks, and rows of both whose target lies far below another logit."""
+    N, V, K = 1100, 300_001, 64
+    x, w, t = inputs(N, V, K, dtype, 6, ignored=0.1, lift=0.0)
+    x = x.clone()
+    for r in (5, 700, 768, 900, N - 1):
+        x[r] *= 40
+        t[r] = r
+    kept = int((t != -100).sum())
+    up = torch.rand(N, device=dev) if reduction == "none" else None
+    weight = up if reduction == "none" else torch.tensor(1.0 / kept if reduction == "mean" else 1.0, device=dev)
+    e = exact(x, w, t, 1.0, z, weight)
+    assert e["loss"][[5, 900]].max() > 60
+    loss, dx, dw = run(x, w, t, up, z_loss=z, reduction=reduction)
+    if reduction == "none":
+        check_loss(loss, e)
+    else:
+        want = e["loss"].sum() / (kept if reduction == "mean" else 1)
+        # (z: an error of lse counts 1 + 2 z lse times; lse is below 150 here)
+        assert abs(loss.double() - want) <= 1.3 * check_loss(loss, e, False).sum() / (kept if reduction == "mean" else 1)
+    check_grads(dx, dw, e, dtype)
+    assert _ext.device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("K", [1272, 1280, 1288, 2048, 4104])
+@pytest.mark.parametrize("N,reduction", [(70, "none"), (530, "mean"), (KEEP_ROWS + 3, "mean")])
+def test_wide_rows(N, reduction, K, dtype):
+    """Rows around and past the 1280 columns that a warp has under way at once, on all three gradient paths."""
+    V = 601
+    x, w, t = inputs(N, V, K, dtype, K, ignored=0.1)
+    kept = int((t != -100).sum())
+    up = torch.rand(N, device=dev) if reduction == "none" else None
+    e = exact(x, w, t, up=up if up is not None else torch.tensor(1.0 / kept, device=dev))
+    loss, dx, dw = run(x, w, t, up, reduction=reduction)
+    if reduction == "none":
+        check_loss(loss, e)
+    else:
+        assert abs(loss.double() - e["loss"].sum() / kept) <= check_loss(loss, e, False).sum() / kept
+    check_grads(dx, dw, e, dtype)
+
+
+@pytest.mark.parametrize("reduction", ["mean", "sum", "none"])
+def test_more_rows_than_the_joins_block_reduces(reduction):
+    N, V, K = 8300, 300, 64
+    x, w, t = inputs(N, V, K, torch.bfloat16, 12, ignored=0.2)
+    kept = int((t != -100).sum())
+    up = torch.rand(N, device=dev) if reduction == "none" else None
+    weight = up if reduction == "none" else torch.tensor(1.0 / kept if reduction == "mean" else 1.0, device=dev)
+    e = exact(x, w, t, up=weight)
+    loss, dx, dw = run(x, w, t, up, reduction=reduction)
+    bound = check_loss(loss, e, rows=reduction == "none")
+    if reduction != "none":
+        k = kept if reduction == "mean" else 1
+        assert abs(loss.double() - e["loss"].sum() / k) <= bound.sum() / k
+    check_grads(dx, dw, e, torch.bfloat16)
+
+
+@pytest.mark.parametrize("N", [511, 512, 513])
+def test_both_sides_of_the_one_launch_sum(N):
+    x, w, t = inputs(N, 1500, 72, torch.bfloat16, N, ignored=0.1)
+    up = torch.rand(N, device=dev)
+    e = exact(x, w, t, up=up)
+    loss, dx, dw = run(x, w, t, up, reduction="none")
+    check_loss(loss, e)
+    check_grads(dx, dw, e, torch.bfloat16)
