@@ -241,7 +241,7 @@ int krsi_geglu_q8_bwd(const void* g, const void* q, const void* exponents, void*
  *   gradients  20 N + R (128 ceil(V / 64) + 2 K), R so that the first product is at most 2^29 (or 256 rows')
  *   dx         4 R K for each share of the vocabulary that its sums are cut into (none where R is large)
  *   dw         with more than 512 rows the sorted targets, about 4 V + 8 N + N K / 2; mode 2: 4 K for each
- *              token of w, or in one chunk for each row of x where those are fewer */
+ *              row of w, or in one chunk for each row of x where those are fewer and w's take over 32 MB */
 #define KRSI_CE_NO_DX 4
 #define KRSI_CE_NO_DW 8
 int krsi_linear_ce_workspace_size(int64_t N, int64_t V, int64_t K, int mode, size_t* bytes);

@@ -780,8 +780,8 @@ struct GradArgs {
   const float* coef;
   const void* w;
   // dw: fp32 sums, stored or added; or scaled and rounded, and for the tokens that occur (by token_rows.cuh's
-  // start, or with few rows by tgt itself) the fp32 sums as well: rows of `sums`, by token, or (by_entry, where
-  // there are fewer rows than tokens) by the token's first entry
+  // start, or with few rows by tgt itself) the fp32 sums as well: rows of `sums`, by token, or (by_entry) by the
+  // token's first entry
   int dw32, accumulate, few, by_entry;
   float* sums;
   const int* start;
@@ -875,12 +875,16 @@ ce_grads_kernel(const __grid_constant__ CUtensorMap ekmap, const __grid_constant
         const int row = m.tile * (2 * kBM) + rank * kBM + (warp % 4) * 32 + lane;   // of dx, or the token of dw
         GradRow r{1.f, 0.f, false, -1, nullptr};
         const bool few = !m.is_dx && a.sums && a.few;
-        const int first = few ? tokens::first_near(a.tgt, a.rows, row - lane) : 0;
+        int first = -1;
+        if (few) {
+          if (a.by_entry) first = tokens::first_near(a.tgt, a.rows, row - lane);
+          else if (tokens::tokens_near(a.tgt, a.rows, row - lane) >> lane & 1) first = row;
+        }
         if (row >= (m.is_dx ? a.rows : a.V)) return r;
         if (!m.is_dx) {
           r.mul = a.alpha * a.up.unit();
           if (few) {
-            if (first >= 0) r.sums = a.sums + (int64_t)(a.by_entry ? first : row) * a.K;
+            if (first >= 0) r.sums = a.sums + (int64_t)first * a.K;
           } else if (a.sums) {
             const int k = a.order.key(row), at = a.start[k];
             if (at < a.start[k + 1]) r.sums = a.sums + (int64_t)(a.by_entry ? at : row) * a.K;
@@ -1202,6 +1206,7 @@ struct Plan {
   bool dx, dw, known;      // gradients wanted; from known log-sum-exps (krsi_linear_ce_grad)
   bool grads;              // either
   bool direct;             // dw leaves the GEMM in 16 bits
+  bool by_entry;           // then the fp32 sums of the tokens that occur stand by first entry, not by token
   int64_t n_vt, panels;    // vocabulary tiles; panels of e
   int64_t chunk, chunks;   // rows per chunk (a multiple of 256)
   int cols, n_ct;
@@ -1223,6 +1228,10 @@ inline Plan make_plan(int64_t N, int64_t V, int64_t K, bool dx, bool dw, bool kn
   p.chunk = std::max<int64_t>(256, ceil_div(ceil_div(N, p.chunks), 256) * 256);
   p.chunks = std::max<int64_t>(1, ceil_div(N, p.chunk));
   p.direct = known && p.chunks == 1;
+  // V K floats of sums would be mostly empty with few rows: 604 MB for one row over 131072 x 1152.  By entry, N K
+  // do, but a tile's epilogue then looks up first positions and not presence: 72.4 us against 71.6 for 257 rows of
+  // 512 over 10007 (20 MB), which is taken from 32 MB on only.
+  p.by_entry = p.direct && N < V && V * K > ((int64_t)1 << 23);
   // Column tiles of K.  Per K block of 64 a pair's tensor cores take 2 cycles a column, and its operands
   // (16 KB of A and 64 B a column of B for each CTA) come from L2 at about 50 bytes a cycle and SM, as
   // measured on the logits' tiles, so wider tiles feed the tensor cores better.  Up to 256 columns two
@@ -1283,8 +1292,7 @@ inline Space space_at(void* base, const Plan& p) {
     s.xs = reinterpret_cast<void*>(take((size_t)rows * p.K * 2));
     s.dx_part = reinterpret_cast<float*>(p.dx && p.splits > 1 ? take((size_t)p.splits * p.chunk * p.K * 4) : 0);
     if (p.dw) {
-      // 16-bit dw in one chunk needs the sums of the tokens that occur only
-      const int64_t sum_rows = p.direct ? std::min(p.N, p.V) : p.V;
+      const int64_t sum_rows = p.by_entry ? p.N : p.V;
       s.dw32 = reinterpret_cast<float*>(p.known ? take((size_t)sum_rows * p.K * 4) : 0);
       if (p.N > tokens::kFewRows) {
         const size_t sort_off = off;
@@ -1495,7 +1503,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
     ga.accumulate = r0 > 0;
     ga.sums = p.direct ? dw32 : nullptr;
     ga.few = few;
-    ga.by_entry = p.N < p.V;
+    ga.by_entry = p.by_entry;
     ga.start = s.sorted.start;
     ga.order = s.sorted.order;
     ga.up = up;
@@ -1518,7 +1526,7 @@ int run(const Call& c, const Plan& p, const Space& s, int pairs, cudaStream_t st
   }
   if (p.grads && c.dw) {   // the targets' part of dw
     if (p.direct) {
-      const DwRows<DT> out{dw32, (T*)c.dw, p.K, c.scale, p.N < p.V};
+      const DwRows<DT> out{dw32, (T*)c.dw, p.K, c.scale, p.by_entry};
       KRSI_CUDA_TRY(few ? (tokens::sum_few<DT, 8, true>(x, s.coef, (const int*)s.tgt, out, false, N, V, -1, K, stream))
                         : (tokens::sum_by_token<DT, 8, true>(x, s.coef, s.sorted, out, false, N, V, K, stream)));
     } else {

@@ -162,7 +162,8 @@ def test_the_weights_sums_go_by_the_rows_where_those_are_fewer():
     assert workspace(3000, 1000, 512, 2) < workspace(3000, 3001, 512, 2)
 
 
-@pytest.mark.parametrize("N,V", [(40, 5000), (512, 5000), (513, 5000), (700, 701), (700, 700), (700, 699), (500, 33)])
+@pytest.mark.parametrize("N,V", [(40, 5000), (512, 5000), (513, 5000), (700, 701), (700, 700), (700, 699), (500, 33),
+                                 (40, 70_001), (512, 70_001), (513, 70_001), (2000, 70_001)])
 def test_tokens_that_occur_often(N, V):
     """A few tokens that hold most of the rows (runs over many chunks of the sorted sum) among single ones, with more
     tokens than rows and fewer; the sums' rows are those of the tokens that occur."""
