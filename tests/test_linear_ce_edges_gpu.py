@@ -248,3 +248,16 @@ def test_both_sides_of_the_one_launch_sum(N):
     loss, dx, dw = run(x, w, t, up, reduction="none")
     check_loss(loss, e)
     check_grads(dx, dw, e, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_few_rows_in_several_chunks(dtype):
+    """Up to 512 rows, so that the targets' sums need no sort, over a vocabulary that leaves 256 to a chunk."""
+    N, V, K = 300, 1_000_003, 64
+    x, w, t = inputs(N, V, K, dtype, 14, ignored=0.1)
+    t[7::20] = t[0]
+    up = torch.rand(N, device=dev)
+    e = exact(x, w, t, up=up)
+    loss, dx, dw = run(x, w, t, up, reduction="none")
+    check_loss(loss, e)
+    check_grads(dx, dw, e, dtype)
