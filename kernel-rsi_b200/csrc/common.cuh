@@ -69,7 +69,7 @@ inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, siz
 }
 
 // Lets a kernel use `bytes` of dynamic shared memory, once per device and kernel (the attribute call costs
-// as much as a third of a launch; a device reset undoes neither the attribute nor this note of it).
+// as much as a third of a launch; the note is the process's, and assumes that its context is not reset).
 template <auto Kern>
 inline cudaError_t allow_smem(int bytes) {
   static std::atomic<uint64_t> done{0};

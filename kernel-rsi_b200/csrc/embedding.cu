@@ -1,6 +1,7 @@
 // embedding.cu - the embedding lookup with scaling, and the table's gradient by sorted tokens.
 //   forward:  out[i] = scale * table[tokens[i]]                       (a gather)
-//   backward: dtable[v] = scale * sum over i with tokens[i] = v of g[i], in position order
+//   backward: dtable[v] = scale * sum over i with tokens[i] = v of g[i], in a fixed order (that of token_rows.cu's
+//             sort; the positions' own up to 512 of them)
 // Both are bound by memory: the forward reads the looked-up rows and writes out; the backward reads g
 // once and writes every row of dtable once (zeros for tokens that do not occur).
 //

@@ -5,7 +5,7 @@
 //   dx = scale dl w,  dw = scale dl^T x
 // r_i is the gradient of loss_i (0 for an ignored row).  2 N V K flops for the loss; dx and dw take 4 more.
 //
-// Rows are worked on in chunks (at most 2^28 logits each).  For a chunk:
+// Rows are worked on in chunks (of at most 2^28 logits with gradients).  For a chunk:
 //   1. ce_target_kernel (once for all rows): the target's logit l_t from x and its row of w.
 //   2. ce_logits_kernel: a tcgen05 GEMM over tiles of 256 rows x 256 vocabulary entries on CTA pairs,
 //      whose epilogue turns each logit into e = exp(l - l_t) while it is in registers, sums e per row and
@@ -36,10 +36,13 @@
 // after the join only, and ce_rows_kernel then writes x' in the forward too.
 //
 // Rounding: e and x' are rounded to the operands' 16 bits (x' costs a second rounding in the softmax part
-// of dw; the alternative is to compute the logits twice); everything else is fp32 until the result.
+// of dw; the alternative is to compute the logits twice); everything else is fp32 until the result.  In dw's
+// rows of tokens that are no row's target, which are these sums alone, that comes to 2.1e-3 to 2.3e-3 of their
+// norm (2.8e-3 where another entry than the target leads) against 1.5e-3 to 1.7e-3 for the result's own rounding
+// to bf16; where targets are, their fp32 term dominates.
 //
-// What bounds it (B200, 32768 x 1152 over 32768 entries, bf16, loss and gradients: 7.42 PFLOP): the tensor
-// cores under the power cap.  Each GEMM below runs at 1.5 GHz by itself; the step takes 6.15 to 6.45 ms, of
+// What bounds it (B200, 32768 x 1152 over 32768 entries, bf16, loss and gradients: 7.42 TFLOP): the tensor
+// cores under the power cap.  Each GEMM below runs at 1.5 GHz by itself; the step takes 6.15 to 6.55 ms, of
 // which 0.2 ms are the other kernels.  cuBLAS takes 5.84 ms for the three bare products in the same loop.
 #include <algorithm>
 #include <atomic>
@@ -87,7 +90,8 @@ static_assert(kNumBars * 8 + 16 <= 1024, "barriers");
 constexpr uint32_t kTmemCols = 512;
 // What an item's epilogue costs in K blocks where a single accumulator leaves it exposed, for dealing the items
 // out: 10 as read from the launch's ends, which spread over 83 of 395 us when it was left out (2001 x 1152 over
-// 50021: 857 us a step without it, 830 with 10, 833 to 841 with 14 and 20; long sums do not notice).
+// 50021: 857 us a step without it, 830 with 10, 833 to 841 with 14 and 20).  Elsewhere it gives 2% (3000 x 1024 over
+// 50021: 983 us without, 946 to 964 with 5 to 20) or nothing (1100 x 512, 1500 x 768, 2001 x 2048; long sums).
 constexpr int kEpilogueBlocks = 10;
 
 // MN-major operand in the 128-byte swizzle: 64-column atoms of 8 K-rows x 128 B (SBO = 1024 B), the next
@@ -590,7 +594,8 @@ struct Upstream {
   }
 };
 
-// A row's x times a factor, in 16 bits (zeros where `dead`): `ahead` holds the first packets.
+// A row's x times a factor, in 16 bits (zeros where `dead`): `ahead` holds the first packets, 1280 columns of the
+// row under way at once (3 and 8 packets take the same time at 512 to 4096 columns).
 constexpr int kAhead = 5;
 template <int DT>
 struct RowCopy {

@@ -16,6 +16,9 @@ The logits exist one tile at a time, in the GEMM's epilogue.  With "mean" or "su
 or more, the forward also forms both gradients (of the sum of the losses, in fp32) while the
 exponentials are at hand, and the backward only scales and rounds them: one pass over the logits in all,
 for the memory of two fp32 gradients.  Otherwise the backward computes the logits again.
+Sums, statistics and the targets' own terms are fp32; the exponentials and the scaled rows of x that the
+gradient products multiply are in the operands' 16 bits, so a row of dw whose token is no row's target
+carries up to two roundings more than its result's own.
 The reference has no loss op.  The autograd node is in csrc/torch_ext.cpp (krsi::linear_ce).
 Kernels: kernel-rsi_b200/csrc/linear_ce.cu; C ABI: include/krsi_b200.h.
 """
