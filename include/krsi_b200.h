@@ -269,6 +269,61 @@ int krsi_linear_ce_grad(const void* x, const void* w, const void* targets, int t
 int krsi_linear_ce_finish(const float* grad, const float* g, const float* weight, void* out, int64_t n,
                           float scale, int dtype, cudaStream_t stream);
 
+/* ---------------------------------------------------------------- residual addition and RMSNorm
+ * z = (x + res) rounded to x_dtype, then krsi_rmsnorm_fwd's norm of z: y and rstd as there.  The reference has no
+ * such op (its models add, then call library/rmsnorm.py:22-31).  The backward is krsi_rmsnorm_bwd_add on z.
+ * x, res, z, y: [rows, n] of x_dtype; w: [n] of w_dtype; contiguous; dtypes and widths as krsi_rmsnorm_fwd's.
+ * res null: z is x, and is not written. */
+int krsi_add_rmsnorm_fwd(const void* x, const void* res, const void* w, void* z, void* y, float* rstd,
+                         int64_t rows, int64_t n, float eps, int x_dtype, int w_dtype, cudaStream_t stream);
+
+/* The same with y in 8 bits: q [rows, n] e4m3, row i at q + i * q_stride bytes, and scale [rows] fp32;
+ * y = q * scale, q = e4m3(z * w * (448 / m)) and scale = m * rstd / 448 for the row's largest |z * w| m.
+ * A row with a value that is not finite has a scale that is not finite. */
+int krsi_add_rmsnorm_q8_fwd(const void* x, const void* res, const void* w, void* z, void* q, int64_t q_stride,
+                            float* scale, int64_t rows, int64_t n, float eps, int x_dtype, int w_dtype,
+                            cudaStream_t stream);
+
+/* Rows in 8 bits: q = e4m3(x * (448 / m)), scale = m / 448 for the row's largest |x| m. */
+int krsi_quantise_rows(const void* x, void* q, int64_t q_stride, float* scale, int64_t rows, int64_t n, int x_dtype,
+                       cudaStream_t stream);
+
+/* ---------------------------------------------------------------- product of rows and a weight in 8 bits
+ * out[i, j] = (sum over k of q[i, k] * wq[j, k]) * scale[i] * wscale[j], summed in fp32, rounded once.
+ * q: rows of K e4m3, q_stride bytes apart; wq: M rows of K e4m3, w_stride bytes apart (both strides multiples of
+ * 16, both bases 16-byte aligned); out: [rows, M] of out_dtype, contiguous.  No counterpart in the reference. */
+int krsi_linear_q8(const void* q, int64_t q_stride, const float* scale, const void* wq, int64_t w_stride,
+                   const float* wscale, void* out, int64_t rows, int64_t K, int64_t M, int out_dtype,
+                   cudaStream_t stream);
+
+/* ---------------------------------------------------------------- AdamW over many tensors
+ * One step for every tensor of the list, in place; no counterpart in the reference (its models leave the
+ * optimizer to torch).  With g' = g * min(1, max_norm / (|all g| + 1e-6)), or g where max_norm is 0:
+ *   t = t + 1,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,
+ *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * A norm that is not finite leaves everything as it is, the step included. */
+typedef struct {
+  void* p;            /* [n] of p_dtype */
+  const void* g;      /* [n] of g_dtype: p_dtype or F32 */
+  void* m;            /* state_bits 32: fp32 m and v; 8: e4m3 codes of m and of sqrt(v) */
+  void* v;
+  float* master;      /* fp32 copy of a 16-bit p that is updated in its place (p: its rounding), or null */
+  uint8_t* exponents; /* state_bits 8: [ceil(n / 256), 2]: a group of 256 codes stands for code * 2^(e - 127),
+                         e of m and of sqrt(v); 255 marks a group that is not finite (it reads back as NaN).
+                         2-byte aligned */
+  int64_t n;
+  int p_dtype, g_dtype, state_bits, reserved;
+} krsi_adamw_tensor;
+
+int krsi_adamw_workspace_size(int64_t count, size_t* bytes);
+
+/* tensors: host memory, read during the call only; no two of them may overlap.  step: device, the steps taken so
+ * far.  lr_dev: a device float that is read in place of lr, or null.  norm_out: device, the norm of all gradients
+ * (max_norm > 0 only).  workspace: 16-byte aligned. */
+int krsi_adamw_step(const krsi_adamw_tensor* tensors, int64_t count, int64_t* step, const float* lr_dev, double lr,
+                    double beta1, double beta2, double eps, double weight_decay, double max_norm, float* norm_out,
+                    void* workspace, size_t workspace_bytes, cudaStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

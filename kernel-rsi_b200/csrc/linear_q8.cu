@@ -1,0 +1,564 @@
+// linear_q8.cu - the product of rows and a weight in 8 bits, for B200 (sm_100a):
+//   out[i, j] = (sum_k q[i, k] * wq[j, k]) * scale[i] * wscale[j]
+// q [rows, K] and wq [M, K] in e4m3 (nn.Linear's layout), one fp32 scale for each row of both, out [rows, M] in
+// bf16, f16 or fp32.  The products of two e4m3 are exact in fp32; the sums are the tensor cores' fp32, the scales
+// are applied to them in fp32 and the result is rounded once.
+//
+// Structure (as linear_geglu.cu): a persistent grid, 12 warps a CTA: warp 0 the TMA producer (128-byte swizzled
+// K-major tiles of 128 values), warp 1 the TMEM owner and issuer of tcgen05.mma kind::f8f6f4 (32 values of K an
+// instruction), warps 4-11 the epilogue.  Two accumulators alternate, so a tile's epilogue runs beside the next
+// tile's MMAs.
+//   more than 128 rows   linear_q8_pair_kernel: CTA pairs (cta_group::2) on tiles of 256 rows x 256 columns
+//   up to 128 rows       linear_q8_kernel: one CTA on tiles of 128 rows x 64 columns (the weight's read bounds it:
+//                        narrow tiles spread it over the SMs)
+// Every wait is bounded (watchdog.cuh); a stalled pipeline ends the CTA with an error word.
+#include <atomic>
+
+#include "common.cuh"
+#include "gemm_common.cuh"
+#include "watchdog.cuh"
+
+KRSI_DEFINE_WATCHDOG(q8)
+
+namespace krsi {
+namespace {
+
+using namespace sm100;
+using gemm::drain_loads;
+using gemm::kmajor_sw128;
+
+constexpr int kBM = 128;                    // rows of q per CTA
+constexpr int kBK = 128;                    // values of K per stage: one 128-byte swizzle row
+constexpr int kThreads = 384;
+constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
+constexpr uint32_t kATile = kBM * kBK;      // 16 KB
+constexpr uint32_t kBoxBytes = 32 * 64;     // one warp's staged [32 rows x 64 bytes] of the output
+
+struct Q8Args {
+  const float* scale;
+  const float* wscale;
+  void* out;
+  int rows, M;
+  int n_ctiles;       // column tiles
+  int n_tiles;        // row tiles x column tiles
+  int n_kb;           // K blocks
+  uint32_t spin_limit;
+};
+
+// kind::f8f6f4, both operands e4m3 (format 0), K-major, fp32 sums: the bit layout is idesc_f16's.
+__host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t M, uint32_t N) { return idesc_f16(M, N, 0, false, false); }
+
+__device__ __forceinline__ void mma_q8_e(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                         uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+__device__ __forceinline__ void mma_q8_pair_e(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                              uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+// The epilogue of one warp: 32 rows (TMEM lanes) x `cols` columns of each of the CTA's tiles, one output box of
+// 64 bytes a row at a time.  `row_of(i)`, `col_of(i)`: the tile's first row and column for this CTA.
+// TMA: boxes leave by TMA stores; else (rows of out that do not start on 16 bytes) by coalesced stores.
+template <int DT, bool TMA, typename RowOf, typename ColOf, typename Release>
+__device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int acc_cols, int cols, int warp, int lane,
+                                            int my_tiles, uint64_t* acc_full, volatile int* abort_flag,
+                                            const CUtensorMap* omap, const Q8Args& a, RowOf row_of, ColOf col_of,
+                                            Release release) {
+  using E = Elem<DT>;
+  using T = typename E::T;
+  constexpr int kCols = 64 / (int)sizeof(T);   // columns of a box: 32, or 16 in fp32
+  const int ew = warp - kEpiWarp0;
+  const int quarter = ew % 4, part = ew / 4;   // TMEM lane quarter; which `cols` of the tile's columns
+  const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
+  uint8_t* box = boxes + ew * kBoxBytes;
+  // 16-byte packet p of row r in the 64-byte swizzle
+  auto packet = [&](int r, int p) { return box + r * 64 + ((p ^ ((r >> 1) & 3)) << 4); };
+  bool ok = true;
+  for (int i = 0; i < my_tiles; ++i) {
+    const int acc = i & 1;
+    const int row0 = row_of(i) + quarter * 32;
+    const int c_base = col_of(i) + part * cols;
+    const float s = row0 + lane < a.rows ? __ldg(a.scale + row0 + lane) : 0.f;
+    if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], (i >> 1) & 1, abort_flag, a.spin_limit))) {
+      ok = false;
+      break;
+    }
+    tc_fence_after();
+    const uint32_t acc_addr = tmem + lane_addr + acc * acc_cols + part * cols;
+#pragma unroll 1
+    for (int c0 = 0; c0 < cols; c0 += kCols) {
+      uint32_t v[kCols];
+      if constexpr (kCols == 32) tmem_ld32(acc_addr + c0, v);
+      else tmem_ld16(acc_addr + c0, v);
+      const int col = c_base + c0;
+      float ws[kCols];
+      if (col + kCols <= a.M) {
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) ws[e] = __ldg(a.wscale + col + e);
+      } else {
+#pragma unroll
+        for (int e = 0; e < kCols; ++e) ws[e] = col + e < a.M ? __ldg(a.wscale + col + e) : 0.f;
+      }
+      tmem_wait_ld();
+      if (c0 + kCols >= cols) {                  // the accumulator has been read: the MMA may reuse it
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) release(acc);
+      }
+      if (TMA) {
+        if (lane == 0) bulk_wait_read_all();     // the previous box has been read
+        __syncwarp();
+      }
+#pragma unroll
+      for (int p = 0; p < 4; ++p) {
+        uint32_t u[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          if constexpr (DT == KRSI_F32) {
+            const int e = 4 * p + k;
+            u[k] = __float_as_uint(__uint_as_float(v[e]) * s * ws[e]);
+          } else {
+            const int e = 8 * p + 2 * k;
+            const float lo = __uint_as_float(v[e]) * s * ws[e], hi = __uint_as_float(v[e + 1]) * s * ws[e + 1];
+            u[k] = DT == KRSI_F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+          }
+        }
+        *reinterpret_cast<uint4*>(packet(lane, p)) = make_uint4(u[0], u[1], u[2], u[3]);
+      }
+      if constexpr (TMA) {
+        fence_async_shared();
+        __syncwarp();
+        if (lane == 0 && col < a.M && row0 < a.rows) {   // the map clips rows >= rows and columns >= M
+          tma_store_2d(omap, box, col, row0);
+          bulk_commit_group();
+        }
+      } else {
+        __syncwarp();
+        constexpr int kRowsAtOnce = 32 / kCols;
+        const int r_lane = lane / kCols, e = lane % kCols;
+        for (int r = r_lane; r < 32; r += kRowsAtOnce) {
+          if (row0 + r < a.rows && col + e < a.M) {
+            constexpr int kPer = 16 / (int)sizeof(T);
+            const T val = reinterpret_cast<const T*>(packet(r, e / kPer))[e % kPer];
+            static_cast<T*>(a.out)[(int64_t)(row0 + r) * a.M + col + e] = val;
+          }
+        }
+        __syncwarp();
+      }
+    }
+  }
+  if (TMA && lane == 0) bulk_wait_all();   // every store has completed before the CTA exits
+  return ok;
+}
+
+// ---------------------------------------------------------------- up to 128 rows: one CTA, narrow tiles
+constexpr int kOneBN = 64;
+constexpr int kOneStages = 8;
+constexpr uint32_t kOneStageBytes = kATile + kOneBN * kBK;           // 24 KB
+constexpr uint32_t kOneBoxOff = kOneStages * kOneStageBytes;
+constexpr uint32_t kOneBarOff = kOneBoxOff + kEpiWarps * kBoxBytes;
+constexpr uint32_t kOneMiscOff = kOneBarOff + (2 * kOneStages + 2 + 2 + 1) * 8;
+constexpr uint32_t kOneSmem = kOneMiscOff + 16 + 1024;               // + slack for the 1024-byte alignment
+constexpr uint32_t kOneTmemCols = 2 * kOneBN;
+static_assert(kOneSmem <= 232448, "shared memory budget");
+
+template <int DT, bool TMA>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap,
+                 const __grid_constant__ CUtensorMap omap, const Q8Args a) {
+  pdl_enter();   // before any global access and before claiming TMEM
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOneBarOff);
+  uint64_t* empty = full + kOneStages;
+  uint64_t* acc_full = empty + kOneStages;
+  uint64_t* acc_empty = acc_full + 2;
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOneMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kOneMiscOff + 4);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int my_tiles = (int)blockIdx.x < a.n_tiles ? (a.n_tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
+  auto tile_of = [&](int i) { return (int)blockIdx.x + i * (int)gridDim.x; };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kOneStages; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], kEpiWarps);
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&wmap);
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, kOneTmemCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer
+    bool ok = true;
+    int it = 0;
+    for (int i = 0; i < my_tiles && ok; ++i) {
+      const int t = tile_of(i);
+      const int m0 = (t / a.n_ctiles) * kBM, n0 = (t % a.n_ctiles) * kOneBN;
+      for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
+        const int s = it % kOneStages;
+        if (it >= kOneStages && !__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((it / kOneStages) - 1) & 1,
+                                                                           abort_flag, a.spin_limit))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* st = smem + s * kOneStageBytes;
+          mbar_arrive_expect_tx(&full[s], kOneStageBytes);
+          tma_load_2d(st, &qmap, &full[s], kb * kBK, m0);
+          tma_load_2d(st + kATile, &wmap, &full[s], kb * kBK, n0);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      watchdog_fire(kWdQ8Load);
+      drain_loads<kOneStages>(full, it, a.spin_limit);
+    }
+  } else if (warp == 1) {
+    // ------------------------------------------------------------ MMA issuer (whole warp, elected lane)
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit));
+    };
+    constexpr uint32_t idesc = idesc_e4m3(kBM, kOneBN);
+    const uint64_t desc0 = kmajor_sw128(smem_u32(smem));
+    bool ok = true;
+    int it = 0;
+    for (int i = 0; i < my_tiles && ok; ++i) {
+      const int acc = i & 1;
+      if (i >= 2 && !wait(&acc_empty[acc], ((i >> 1) - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
+        const int s = it % kOneStages;
+        if (!wait(&full[s], (it / kOneStages) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t ad = desc0 + (uint64_t)s * (kOneStageBytes >> 4), bd = ad + (kATile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kBK / 32; ++kk)
+          mma_q8_e(tmem + acc * kOneBN, ad + kk * 2, bd + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+        mma_commit_e(&empty[s]);
+      }
+      if (!ok) break;
+      mma_commit_e(&acc_full[acc]);
+    }
+    if (!ok && my_tiles > 0) watchdog_fire(kWdQ8Mma);
+    mma_commit_e(drain);   // every MMA issued above has completed before TMEM is released
+    for (uint32_t i = 0; i < a.spin_limit && !mbar_try_wait(drain, 0); ++i) {
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ------------------------------------------------------------ epilogue
+    const bool ok = q8_epilogue<DT, TMA>(
+        smem + kOneBoxOff, tmem, kOneBN, kOneBN / 2, warp, lane, my_tiles, acc_full, abort_flag, &omap, a,
+        [&](int i) { return (tile_of(i) / a.n_ctiles) * kBM; },
+        [&](int i) { return (tile_of(i) % a.n_ctiles) * kOneBN; }, [&](int acc) { mbar_arrive(&acc_empty[acc]); });
+    if (!ok) watchdog_fire(kWdQ8Epilogue);
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc(tmem, kOneTmemCols);
+}
+
+// ---------------------------------------------------------------- CTA pairs (cta_group::2)
+// Each CTA loads its own 128 rows of q and half of the 256 rows of wq; the even CTA issues M256 N256 K32 MMAs that
+// read both CTAs' shared memory and accumulate into both CTAs' TMEM.
+constexpr int kPairBN = 256;
+constexpr int kPairStages = 6;
+constexpr uint32_t kPairStageBytes = 2 * kATile;                     // 32 KB
+constexpr uint32_t kPairBoxOff = kPairStages * kPairStageBytes;
+constexpr uint32_t kPairBarOff = kPairBoxOff + kEpiWarps * kBoxBytes;
+constexpr uint32_t kPairMiscOff = kPairBarOff + (2 * kPairStages + 2 + 2 + 1) * 8;
+constexpr uint32_t kPairSmem = kPairMiscOff + 16 + 1024;
+constexpr uint32_t kPairTmemCols = 2 * kPairBN;
+static_assert(kPairSmem <= 232448, "shared memory budget");
+
+template <int DT, bool TMA>
+__global__ void __launch_bounds__(kThreads, 1)
+linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap,
+                      const __grid_constant__ CUtensorMap omap, const Q8Args a) {
+  pdl_enter();   // before any global access and before claiming TMEM
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairBarOff);   // used in the even CTA
+  uint64_t* empty = full + kPairStages;
+  uint64_t* acc_full = empty + kPairStages;
+  uint64_t* acc_empty = acc_full + 2;                                 // used in the even CTA
+  uint64_t* drain = acc_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kPairMiscOff);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kPairMiscOff + 4);
+
+  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const uint32_t rank = cluster_ctarank();
+  const bool even = rank == 0;
+  const int pair = (int)blockIdx.x / 2, n_pairs = (int)gridDim.x / 2;
+  const int my_tiles = pair < a.n_tiles ? (a.n_tiles - 1 - pair) / n_pairs + 1 : 0;
+  auto tile_of = [&](int i) { return pair + i * n_pairs; };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full[s], 1);      // the even CTA's expect_tx arrival + both CTAs' TMA bytes
+      mbar_init(&empty[s], 1);     // the even CTA's tcgen05.commit
+    }
+    for (int b = 0; b < 2; ++b) {
+      mbar_init(&acc_full[b], 1);
+      mbar_init(&acc_empty[b], 2 * kEpiWarps);   // one arrival per epilogue warp of both CTAs
+    }
+    mbar_init(drain, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 0 && lane == 0) {
+    prefetch_tensormap(&qmap);
+    prefetch_tensormap(&wmap);
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(tmem_slot, kPairTmemCols);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  cluster_sync();   // both CTAs' barriers initialised and TMEM allocated before either signals the other
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    // ------------------------------------------------------------ TMA producer (both CTAs)
+    bool ok = true;
+    int it = 0;
+    for (int i = 0; i < my_tiles && ok; ++i) {
+      const int t = tile_of(i);
+      const int m0 = (t / a.n_ctiles) * (2 * kBM) + (int)rank * kBM;
+      const int n0 = (t % a.n_ctiles) * kPairBN + (int)rank * (kPairBN / 2);
+      for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
+        const int s = it % kPairStages;
+        if (it >= kPairStages && !__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((it / kPairStages) - 1) & 1,
+                                                                            abort_flag, a.spin_limit))) {
+          ok = false;
+          break;
+        }
+        if (lane == 0) {
+          uint8_t* st = smem + s * kPairStageBytes;
+          const uint32_t bar = mapa_shared(&full[s], 0);
+          if (even) mbar_arrive_expect_tx(&full[s], 2 * kPairStageBytes);
+          tma_load_2d_pair(st, &qmap, bar, kb * kBK, m0);
+          tma_load_2d_pair(st + kATile, &wmap, bar, kb * kBK, n0);
+        }
+        __syncwarp();
+      }
+    }
+    if (!ok) {
+      watchdog_fire(kWdQ8Load);
+      if (even) drain_loads<kPairStages>(full, it, a.spin_limit);   // covers both CTAs' loads of each stage
+    }
+  } else if (warp == 1 && even) {
+    // ------------------------------------------------------------ MMA issuer (even CTA, elected lane)
+    auto wait = [&](uint64_t* bar, uint32_t parity) {
+      return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit));
+    };
+    constexpr uint32_t idesc = idesc_e4m3(2 * kBM, kPairBN);
+    const uint64_t desc0 = kmajor_sw128(smem_u32(smem));
+    bool ok = true;
+    int it = 0;
+    for (int i = 0; i < my_tiles && ok; ++i) {
+      const int acc = i & 1;
+      if (i >= 2 && !wait(&acc_empty[acc], ((i >> 1) - 1) & 1)) {
+        ok = false;
+        break;
+      }
+      tc_fence_after();
+      for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
+        const int s = it % kPairStages;
+        if (!wait(&full[s], (it / kPairStages) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        const uint64_t ad = desc0 + (uint64_t)s * (kPairStageBytes >> 4), bd = ad + (kATile >> 4);
+#pragma unroll
+        for (int kk = 0; kk < kBK / 32; ++kk)
+          mma_q8_pair_e(tmem + acc * kPairBN, ad + kk * 2, bd + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+        mma_commit_pair_e(mapa_shared(&empty[s], 0));   // stage s free in both CTAs
+        mma_commit_pair_e(mapa_shared(&empty[s], 1));
+      }
+      if (!ok) break;
+      mma_commit_pair_e(mapa_shared(&acc_full[acc], 0));
+      mma_commit_pair_e(mapa_shared(&acc_full[acc], 1));
+    }
+    if (!ok && my_tiles > 0) watchdog_fire(kWdQ8Mma);
+    mma_commit_pair_e(mapa_shared(drain, 0));
+    for (uint32_t i = 0; i < a.spin_limit && !mbar_try_wait(drain, 0); ++i) {
+    }
+  } else if (warp >= kEpiWarp0) {
+    // ------------------------------------------------------------ epilogue (both CTAs, own rows)
+    const bool ok = q8_epilogue<DT, TMA>(
+        smem + kPairBoxOff, tmem, kPairBN, kPairBN / 2, warp, lane, my_tiles, acc_full, abort_flag, &omap, a,
+        [&](int i) { return (tile_of(i) / a.n_ctiles) * (2 * kBM) + (int)rank * kBM; },
+        [&](int i) { return (tile_of(i) % a.n_ctiles) * kPairBN; },
+        [&](int acc) {
+          if (even) mbar_arrive(&acc_empty[acc]);
+          else mbar_arrive_cluster(mapa_shared(&acc_empty[acc], 0));
+        });
+    if (!ok) watchdog_fire(kWdQ8Epilogue);
+  }
+
+  tc_fence_before();
+  cluster_sync();   // the even CTA's MMAs (which read this CTA's shared memory and TMEM) are done
+  tc_fence_after();
+  if (warp == 1) tmem_dealloc_pair(tmem, kPairTmemCols);
+}
+
+// ---------------------------------------------------------------- host side
+// 2-D map (cols, rows) of a row-major matrix, `pitch` bytes between rows.
+bool map_2d(CUtensorMap* map, CUtensorMapDataType type, const void* base, int64_t rows, int64_t cols, int64_t pitch,
+            uint32_t box_cols, uint32_t box_rows, CUtensorMapSwizzle swizzle) {
+  attn::EncodeTiledFn enc = attn::encode_fn();
+  if (!enc) return false;
+  memset(map, 0, sizeof(*map));
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)pitch};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  return enc(map, type, 2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+             CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+cudaLaunchConfig_t pair_config(cudaLaunchAttribute* attr, int clusters, cudaStream_t stream) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(2 * clusters);
+  cfg.blockDim = dim3(kThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.stream = stream;
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 2;
+  return cfg;
+}
+
+// Clusters of two that fit on the device at once (0: none can be launched), per device, queried once.
+template <int DT, bool TMA>
+int pair_clusters() {
+  static std::atomic<int> cached[64];   // clusters + 1 once queried; races only repeat the query
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  int v = cached[dev].load(std::memory_order_relaxed);
+  if (v == 0) {
+    auto kern = linear_q8_pair_kernel<DT, TMA>;
+    int n = 0;
+    if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem) == cudaSuccess) {
+      cudaLaunchAttribute attr[2];
+      cudaLaunchConfig_t cfg = pair_config(attr, device_sm_count() / 2, nullptr);
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&n, kern, &cfg) != cudaSuccess) n = 0;
+    }
+    cudaGetLastError();   // a refused query leaves no sticky error behind
+    v = n + 1;
+    cached[dev].store(v, std::memory_order_relaxed);
+  }
+  return v - 1;
+}
+
+template <int DT, bool TMA>
+int launch(const CUtensorMap& qm, const CUtensorMap& om, const void* wq, int64_t w_pitch, int64_t K, Q8Args a,
+           cudaStream_t stream) {
+  CUtensorMap wm;
+  const int clusters = a.rows > kBM ? pair_clusters<DT, TMA>() : 0;
+  const int bn = clusters > 0 ? kPairBN : kOneBN;
+  // (a box of the weight: each CTA's half of a pair's columns, or the one CTA's)
+  if (!map_2d(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, a.M, K, w_pitch, kBK, clusters > 0 ? kPairBN / 2 : kOneBN,
+              CU_TENSOR_MAP_SWIZZLE_128B))
+    return KRSI_ERR_CUDA;
+  const int64_t bm = clusters > 0 ? 2 * kBM : kBM;
+  const int64_t rt = (a.rows + bm - 1) / bm, ct = ((int64_t)a.M + bn - 1) / bn;
+  if (rt * ct > INT32_MAX / 2) return KRSI_ERR_UNSUPPORTED;
+  a.n_ctiles = (int)ct;
+  a.n_tiles = (int)(rt * ct);
+  if (clusters > 0) {
+    cudaLaunchAttribute attr[2];
+    const cudaLaunchConfig_t cfg = pair_config(attr, a.n_tiles < clusters ? a.n_tiles : clusters, stream);
+    KRSI_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_q8_pair_kernel<DT, TMA>, qm, wm, om, a));
+    return KRSI_OK;
+  }
+  KRSI_CUDA_TRY((allow_smem<linear_q8_kernel<DT, TMA>>((int)kOneSmem)));
+  const int sms = device_sm_count();
+  KRSI_CUDA_TRY(launch_pdl(linear_q8_kernel<DT, TMA>, dim3(a.n_tiles < sms ? a.n_tiles : sms), dim3(kThreads), kOneSmem,
+                           stream, qm, wm, om, a));
+  return KRSI_OK;
+}
+
+}  // namespace
+}  // namespace krsi
+
+using namespace krsi;
+
+extern "C" int krsi_linear_q8(const void* q, int64_t q_stride, const float* scale, const void* wq, int64_t w_stride,
+                              const float* wscale, void* out, int64_t rows, int64_t K, int64_t M, int out_dtype,
+                              cudaStream_t stream) {
+  KRSI_CHECK_ARG(rows >= 0 && K > 0 && M > 0);
+  if (out_dtype != KRSI_F32 && out_dtype != KRSI_BF16 && out_dtype != KRSI_F16) return KRSI_ERR_INVALID_ARGUMENT;
+  if (rows == 0) return KRSI_OK;
+  KRSI_CHECK_ARG(q && scale && wq && wscale && out && q_stride >= K && w_stride >= K);
+  if (!aligned16(q) || !aligned16(wq) || q_stride % 16 != 0 || w_stride % 16 != 0) return KRSI_ERR_MISALIGNED;
+  if (rows > INT32_MAX - 2 * kBM || K > INT32_MAX - kBK || M > INT32_MAX - kPairBN) return KRSI_ERR_UNSUPPORTED;
+  const int es = out_dtype == KRSI_F32 ? 4 : 2;
+  const bool tma = aligned16(out) && M * es % 16 == 0;
+  KRSI_CUDA_TRY(gemm::bind_context());
+  CUtensorMap qm, om;
+  if (!map_2d(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, rows, K, q_stride, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B))
+    return KRSI_ERR_CUDA;
+  if (tma) {
+    const CUtensorMapDataType type = out_dtype == KRSI_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                     : out_dtype == KRSI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+    if (!map_2d(&om, type, out, rows, M, M * es, 64 / es, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return KRSI_ERR_CUDA;
+  } else {
+    memset(&om, 0, sizeof(om));
+  }
+  const Q8Args a{scale, wscale, out, (int)rows, (int)M, 0, 0, (int)((K + kBK - 1) / kBK), kSpinLimit};
+#define KRSI_OUT(DT)                                                            \
+  if (out_dtype == DT)                                                          \
+    return tma ? launch<DT, true>(qm, om, wq, w_stride, K, a, stream) : launch<DT, false>(qm, om, wq, w_stride, K, a, stream)
+  KRSI_OUT(KRSI_F32);
+  KRSI_OUT(KRSI_BF16);
+  KRSI_OUT(KRSI_F16);
+#undef KRSI_OUT
+  return KRSI_ERR_INVALID_ARGUMENT;
+}

@@ -13,6 +13,9 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <algorithm>
+#include <vector>
+
 #include "../../include/krsi_b200.h"
 
 namespace {
@@ -499,6 +502,241 @@ at::Tensor linear_ce_finish(const at::Tensor& grad, const at::Tensor& g_in, cons
   return out;
 }
 
+// ---------------------------------------------------------------- residual addition and RMSNorm
+// The arguments of the three entry points below; a tensor that starts off 16 bytes is taken as it is (the kernels
+// have a path for it).
+struct NormCall {
+  at::Tensor x, res, w;
+};
+NormCall norm_call(const at::Tensor& x_in, const c10::optional<at::Tensor>& res_in, const at::Tensor& w_in,
+                   const char* what) {
+  check_cuda(x_in, "x2d");
+  check_cuda(w_in, "w");
+  check_same_device(x_in, w_in, what);
+  TORCH_CHECK(x_in.dim() == 2, what, ": x2d must be 2-D, got ", x_in.dim(), "-D");
+  TORCH_CHECK(w_in.dim() == 1 && w_in.size(0) == x_in.size(1), what, ": w must be [", x_in.size(1), "]");
+  NormCall c{x_in.contiguous(), {}, w_in.contiguous()};
+  if (res_in.has_value() && res_in->defined()) {
+    check_cuda(*res_in, "res");
+    check_same_device(x_in, *res_in, what);
+    TORCH_CHECK(res_in->sizes() == x_in.sizes() && res_in->scalar_type() == x_in.scalar_type(), what,
+                ": res must have x2d's shape and dtype");
+    c.res = res_in->contiguous();
+  }
+  return c;
+}
+
+// (y, z, rstd): z is empty where there is no res (it is x2d then).
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rmsnorm_fwd(const at::Tensor& x_in,
+                                                               const c10::optional<at::Tensor>& res_in,
+                                                               const at::Tensor& w_in, double eps) {
+  TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const NormCall c = norm_call(x_in, res_in, w_in, "add_rmsnorm");
+  const int64_t rows = c.x.size(0), n = c.x.size(1);
+  auto y = at::empty({rows, n}, c.x.options());
+  auto z = at::empty({c.res.defined() ? rows : 0, n}, c.x.options());
+  auto rstd = at::empty({rows}, c.x.options().dtype(at::kFloat));
+  check_rc(krsi_add_rmsnorm_fwd(c.x.data_ptr(), c.res.defined() ? c.res.data_ptr() : nullptr, c.w.data_ptr(),
+                                c.res.defined() ? z.data_ptr() : nullptr, y.data_ptr(), rstd.data_ptr<float>(), rows, n,
+                                (float)eps, krsi_dtype_of(c.x), krsi_dtype_of(c.w), at::cuda::getCurrentCUDAStream()),
+           "krsi_add_rmsnorm_fwd");
+  return {y, z, rstd};
+}
+
+// (dz, dw) for the gradients of y and z, either of which may be missing (dw is then empty, or z's is not added).
+std::tuple<at::Tensor, at::Tensor> add_rmsnorm_bwd(const c10::optional<at::Tensor>& gy,
+                                                   const c10::optional<at::Tensor>& gz, const at::Tensor& z,
+                                                   const at::Tensor& w, const at::Tensor& rstd) {
+  const bool have_z = gz.has_value() && gz->defined();
+  if (!gy.has_value() || !gy->defined())
+    return {have_z ? gz->to(z.scalar_type()) : at::zeros_like(z), at::zeros_like(w)};
+  if (!have_z) return rmsnorm_bwd(*gy, z, w, rstd);
+  auto g = gz->to(z.scalar_type()).contiguous();
+  if ((reinterpret_cast<uintptr_t>(g.data_ptr()) & 15u) != 0) g = g.clone();
+  return rmsnorm_bwd_add(*gy, z, w, rstd, g);
+}
+
+// Rows of 8-bit values, each row padded to whole 16 bytes (what a TMA copy of them needs).
+at::Tensor empty_q8(int64_t rows, int64_t n, const at::Tensor& like) {
+  auto q = at::empty({rows, (n + 15) / 16 * 16}, like.options().dtype(at::kFloat8_e4m3fn));
+  return q.size(1) == n ? q : q.narrow(1, 0, n);
+}
+
+// (q, scale, z): z is empty where there is no res.
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rmsnorm_q8(const at::Tensor& x_in,
+                                                              const c10::optional<at::Tensor>& res_in,
+                                                              const at::Tensor& w_in, double eps) {
+  TORCH_CHECK(x_in.is_cuda(), "krsi: x2d must be a CUDA tensor");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const NormCall c = norm_call(x_in, res_in, w_in, "add_rmsnorm_q8");
+  const int64_t rows = c.x.size(0), n = c.x.size(1);
+  auto q = empty_q8(rows, n, c.x);
+  auto z = at::empty({c.res.defined() ? rows : 0, n}, c.x.options());
+  auto scale = at::empty({rows}, c.x.options().dtype(at::kFloat));
+  check_rc(krsi_add_rmsnorm_q8_fwd(c.x.data_ptr(), c.res.defined() ? c.res.data_ptr() : nullptr, c.w.data_ptr(),
+                                   c.res.defined() ? z.data_ptr() : nullptr, q.data_ptr(), (n + 15) / 16 * 16,
+                                   scale.data_ptr<float>(), rows, n, (float)eps, krsi_dtype_of(c.x), krsi_dtype_of(c.w),
+                                   at::cuda::getCurrentCUDAStream()),
+           "krsi_add_rmsnorm_q8_fwd");
+  return {q, scale, z};
+}
+
+std::tuple<at::Tensor, at::Tensor> quantise_rows(const at::Tensor& x_in) {
+  check_cuda(x_in, "x2d");
+  TORCH_CHECK(x_in.dim() == 2, "quantise: x2d must be 2-D, got ", x_in.dim(), "-D");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  auto x = x_in.contiguous();
+  const int64_t rows = x.size(0), n = x.size(1);
+  auto q = empty_q8(rows, n, x);
+  auto scale = at::empty({rows}, x.options().dtype(at::kFloat));
+  check_rc(krsi_quantise_rows(x.data_ptr(), q.data_ptr(), (n + 15) / 16 * 16, scale.data_ptr<float>(), rows, n,
+                              krsi_dtype_of(x), at::cuda::getCurrentCUDAStream()),
+           "krsi_quantise_rows");
+  return {q, scale};
+}
+
+// ---------------------------------------------------------------- product in 8 bits
+at::Tensor linear_q8(const at::Tensor& q_in, const at::Tensor& scale_in, const at::Tensor& wq_in,
+                     const at::Tensor& wscale_in, at::ScalarType out_dtype) {
+  check_cuda(q_in, "q");
+  for (const at::Tensor* t : {&scale_in, &wq_in, &wscale_in}) check_same_device(q_in, *t, "linear_q8");
+  TORCH_CHECK(q_in.dim() == 2 && wq_in.dim() == 2 && q_in.size(1) == wq_in.size(1) && q_in.size(1) > 0 &&
+                  wq_in.size(0) > 0,
+              "linear_q8: q must be [rows, K] and wq [M, K], got ", q_in.sizes(), " and ", wq_in.sizes());
+  TORCH_CHECK(q_in.scalar_type() == at::kFloat8_e4m3fn && wq_in.scalar_type() == at::kFloat8_e4m3fn,
+              "linear_q8: q and wq must be float8_e4m3fn");
+  TORCH_CHECK(scale_in.scalar_type() == at::kFloat && scale_in.dim() == 1 && scale_in.size(0) == q_in.size(0),
+              "linear_q8: scale must be float32 [", q_in.size(0), "]");
+  TORCH_CHECK(wscale_in.scalar_type() == at::kFloat && wscale_in.dim() == 1 && wscale_in.size(0) == wq_in.size(0),
+              "linear_q8: wscale must be float32 [", wq_in.size(0), "]");
+  c10::cuda::CUDAGuard guard(q_in.device());
+  const int64_t K = q_in.size(1), pitch = (K + 15) / 16 * 16;
+  // rows on 16 bytes; others are copied
+  auto rows_of = [&](const at::Tensor& t, int64_t* stride) {
+    const bool one = t.size(0) <= 1;
+    if (t.stride(1) == 1 && (one || (t.stride(0) >= K && t.stride(0) % 16 == 0)) &&
+        (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15u) == 0) {
+      *stride = one ? pitch : t.stride(0);
+      return t;
+    }
+    auto c = empty_q8(t.size(0), K, t);
+    c.copy_(t);
+    *stride = pitch;
+    return c;
+  };
+  int64_t qs = 0, ws = 0;
+  auto q = rows_of(q_in, &qs), wq = rows_of(wq_in, &ws);
+  auto scale = scale_in.contiguous(), wscale = wscale_in.contiguous();
+  auto out = at::empty({q.size(0), wq.size(0)}, q.options().dtype(out_dtype));
+  check_rc(krsi_linear_q8(q.data_ptr(), qs, scale.data_ptr<float>(), wq.data_ptr(), ws, wscale.data_ptr<float>(),
+                          out.data_ptr(), q.size(0), K, wq.size(0), krsi_dtype_of(out),
+                          at::cuda::getCurrentCUDAStream()),
+           "krsi_linear_q8");
+  return out;
+}
+
+// ---------------------------------------------------------------- AdamW
+// One step for every tensor, in place; returns the norm of all gradients (empty where max_norm is 0).  masters and
+// exponents: a tensor for each parameter, one without elements where it has none, or an empty list.
+at::Tensor adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
+                      at::TensorList masters, at::TensorList exponents, const at::Tensor& step,
+                      const c10::optional<at::Tensor>& lr_tensor, double lr, double beta1, double beta2, double eps,
+                      double weight_decay, double max_norm) {
+  const size_t count = params.size();
+  TORCH_CHECK(grads.size() == count && exp_avgs.size() == count && exp_avg_sqs.size() == count,
+              "adamw_step: as many grads, exp_avgs and exp_avg_sqs as params are needed");
+  TORCH_CHECK(masters.empty() || masters.size() == count, "adamw_step: as many masters as params are needed, or none");
+  TORCH_CHECK(exponents.empty() || exponents.size() == count,
+              "adamw_step: as many exponents as params are needed, or none");
+  TORCH_CHECK(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1, "adamw_step: betas must be in [0, 1)");
+  TORCH_CHECK(eps >= 0 && max_norm >= 0, "adamw_step: eps and max_norm must not be negative");
+  check_cuda(step, "step");
+  TORCH_CHECK(step.scalar_type() == at::kLong && step.numel() == 1, "adamw_step: step must be one int64");
+  const bool device_lr = lr_tensor.has_value() && lr_tensor->defined();
+  if (device_lr)
+    TORCH_CHECK(lr_tensor->scalar_type() == at::kFloat && lr_tensor->numel() == 1 &&
+                    lr_tensor->device() == step.device(),
+                "adamw_step: a tensor lr must be one float32 on the step's device");
+  c10::cuda::CUDAGuard guard(step.device());
+  std::vector<krsi_adamw_tensor> table(count);
+  std::vector<at::Tensor> copies;   // gradients that were not contiguous, until the launch
+  std::vector<std::pair<uintptr_t, uintptr_t>> spans;   // no tensor may be updated twice
+  spans.reserve(count);
+  auto own = [&](const at::Tensor& t, const at::Tensor& p, at::ScalarType type, const char* what) {
+    TORCH_CHECK(t.device() == step.device() && t.scalar_type() == type && t.numel() == p.numel() && t.is_contiguous(),
+                "adamw_step: ", what, " must be contiguous ", type, " of the parameter's size on the step's device");
+  };
+  for (size_t i = 0; i < count; ++i) {
+    const at::Tensor& p = params[i];
+    TORCH_CHECK(p.device() == step.device(), "adamw_step: parameters and step must be on one CUDA device");
+    TORCH_CHECK(p.is_contiguous(), "adamw_step: parameters must be contiguous");
+    TORCH_CHECK(grads[i].layout() == at::kStrided, "adamw_step: gradients must be dense");
+    TORCH_CHECK(grads[i].device() == p.device() && grads[i].sizes() == p.sizes(),
+                "adamw_step: a gradient must have its parameter's shape and device");
+    krsi_adamw_tensor& t = table[i];
+    t = krsi_adamw_tensor{};
+    t.n = p.numel();
+    t.p_dtype = krsi_dtype_of(p);
+    t.g_dtype = krsi_dtype_of(grads[i]);
+    TORCH_CHECK(t.g_dtype == t.p_dtype || t.g_dtype == KRSI_F32,
+                "adamw_step: a gradient must have its parameter's dtype or float32");
+    const bool q8 = exp_avgs[i].scalar_type() == at::kFloat8_e4m3fn;
+    t.state_bits = q8 ? 8 : 32;
+    own(exp_avgs[i], p, q8 ? at::kFloat8_e4m3fn : at::kFloat, "exp_avgs");
+    own(exp_avg_sqs[i], p, q8 ? at::kFloat8_e4m3fn : at::kFloat, "exp_avg_sqs");
+    t.p = p.data_ptr();
+    t.m = exp_avgs[i].data_ptr();
+    t.v = exp_avg_sqs[i].data_ptr();
+    if (grads[i].is_contiguous()) {
+      t.g = grads[i].data_ptr();
+    } else {
+      copies.push_back(grads[i].contiguous());
+      t.g = copies.back().data_ptr();
+    }
+    if (!masters.empty() && masters[i].numel() > 0) {
+      TORCH_CHECK(p.scalar_type() != at::kFloat, "adamw_step: a float32 parameter has no master");
+      own(masters[i], p, at::kFloat, "masters");
+      t.master = masters[i].data_ptr<float>();
+    } else {
+      TORCH_CHECK(masters.empty() || t.n == 0 || p.scalar_type() == at::kFloat || masters[i].dim() == 1,
+                  "adamw_step: masters must have their parameters' size, or no elements");
+    }
+    if (q8 && t.n > 0) {
+      TORCH_CHECK(!exponents.empty(), "adamw_step: 8-bit states need exponents");
+      const at::Tensor& e = exponents[i];
+      TORCH_CHECK(e.device() == step.device() && e.scalar_type() == at::kByte && e.is_contiguous() &&
+                      e.numel() == 2 * ((t.n + 255) / 256),
+                  "adamw_step: exponents must be contiguous uint8 [ceil(n / 256), 2]");
+      t.exponents = e.data_ptr<uint8_t>();
+    }
+    if (t.n > 0) {
+      const uintptr_t at = reinterpret_cast<uintptr_t>(t.p);
+      spans.emplace_back(at, at + (uintptr_t)p.nbytes());
+    }
+  }
+  std::sort(spans.begin(), spans.end());
+  for (size_t i = 1; i < spans.size(); ++i)
+    TORCH_CHECK(spans[i].first >= spans[i - 1].second, "adamw_step: two parameters share memory");
+  auto norm = at::empty(max_norm > 0 ? at::IntArrayRef{} : at::IntArrayRef{0}, step.options().dtype(at::kFloat));
+  size_t ws = 0;
+  check_rc(krsi_adamw_workspace_size((int64_t)count, &ws), "krsi_adamw_workspace_size");
+  auto wsp = workspace(step, ws);
+  check_rc(krsi_adamw_step(table.data(), (int64_t)count, step.data_ptr<int64_t>(),
+                           device_lr ? lr_tensor->data_ptr<float>() : nullptr, lr, beta1, beta2, eps, weight_decay,
+                           max_norm, max_norm > 0 ? norm.data_ptr<float>() : nullptr, wsp.data_ptr(),
+                           (size_t)wsp.numel(), at::cuda::getCurrentCUDAStream()),
+           "krsi_adamw_step");
+  // what was written counts as changed in place (a graph that still needs the old values is told so)
+  auto bump = [](at::TensorList l) {
+    for (const at::Tensor& t : l)
+      if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+  };
+  for (const at::TensorList& l : {params, exp_avgs, exp_avg_sqs, masters, exponents}) bump(l);
+  if (!step.is_inference()) step.unsafeGetTensorImpl()->bump_version();
+  return norm;
+}
+
 // ---------------------------------------------------------------- eager autograd
 // Autograd nodes of the vocabulary operators and the 8-bit checkpoint, in C++: at small sizes a pass is
 // bound by the host, and a Python autograd.Function costs it some 25 us more a step than these do (5,003 tokens
@@ -628,6 +866,74 @@ at::Tensor linear_ce_autograd(const at::Tensor& x, const at::Tensor& w, const at
   return linear_ce_plain(x, w, targets, scale, ignore_index, z_loss, reduction, keep);
 }
 
+// (y, z): z is x2d itself where there is no res.
+std::tuple<at::Tensor, at::Tensor> add_rmsnorm_plain(const at::Tensor& x, const c10::optional<at::Tensor>& res,
+                                                     const at::Tensor& w, double eps) {
+  auto [y, z, rstd] = KRSI_OP(add_rmsnorm_fwd).call(x, res, w, eps);
+  return {y, res.has_value() && res->defined() ? z : x.alias()};
+}
+struct AddRmsnormNode : public torch::autograd::Function<AddRmsnormNode> {
+  static variable_list forward(AutogradContext* ctx, const at::Tensor& x, const c10::optional<at::Tensor>& res,
+                               const at::Tensor& w, double eps) {
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto [y, z, rstd] = KRSI_OP(add_rmsnorm_fwd).call(x, res, w, eps);
+    const bool add = res.has_value() && res->defined();
+    if (!add) z = x;
+    ctx->save_for_backward({z, w, rstd});
+    ctx->saved_data["add"] = add;
+    ctx->set_materialize_grads(false);
+    return {y, z};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list g) {
+    check_once("add_rmsnorm");
+    const auto saved = ctx->get_saved_variables();
+    if (!g[0].defined() && !g[1].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    at::AutoDispatchBelowADInplaceOrView below;
+    auto opt = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
+    auto [dz, dw] = KRSI_OP(add_rmsnorm_bwd).call(opt(g[0]), opt(g[1]), saved[0], saved[1], saved[2]);
+    return {dz, ctx->saved_data["add"].toBool() ? dz : at::Tensor(), dw, at::Tensor()};
+  }
+};
+std::tuple<at::Tensor, at::Tensor> add_rmsnorm_autograd(const at::Tensor& x, const c10::optional<at::Tensor>& res,
+                                                        const at::Tensor& w, double eps) {
+  const bool add = res.has_value() && res->defined();
+  check_no_tangent({&x, &w}, "add_rmsnorm");
+  if (add) check_no_tangent({&*res}, "add_rmsnorm");
+  if (at::GradMode::is_enabled() && (x.requires_grad() || w.requires_grad() || (add && res->requires_grad()))) {
+    auto out = AddRmsnormNode::apply(x, res, w, eps);
+    return {out[0], out[1]};
+  }
+  at::AutoDispatchBelowADInplaceOrView below;
+  return add_rmsnorm_plain(x, res, w, eps);
+}
+
+// 8 bits carry no gradient: where one would be asked for, it is refused rather than lost.
+void check_no_grad(std::initializer_list<const at::Tensor*> inputs, const char* what) {
+  check_no_tangent(inputs, what);
+  if (!at::GradMode::is_enabled()) return;
+  for (const at::Tensor* t : inputs)
+    TORCH_CHECK(!t->requires_grad(), what, ": has no gradient; call it under torch.no_grad()");
+}
+std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rmsnorm_q8_autograd(const at::Tensor& x,
+                                                                       const c10::optional<at::Tensor>& res,
+                                                                       const at::Tensor& w, double eps) {
+  check_no_grad({&x, &w}, "add_rmsnorm_q8");
+  if (res.has_value() && res->defined()) check_no_grad({&*res}, "add_rmsnorm_q8");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return KRSI_OP(add_rmsnorm_q8).call(x, res, w, eps);
+}
+std::tuple<at::Tensor, at::Tensor> quantise_rows_autograd(const at::Tensor& x) {
+  check_no_grad({&x}, "quantise");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return KRSI_OP(quantise_rows).call(x);
+}
+at::Tensor linear_q8_autograd(const at::Tensor& q, const at::Tensor& scale, const at::Tensor& wq,
+                              const at::Tensor& wscale, at::ScalarType out_dtype) {
+  check_no_grad({&q, &scale, &wq, &wscale}, "linear_q8");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return KRSI_OP(linear_q8).call(q, scale, wq, wscale, out_dtype);
+}
+
 }  // namespace
 
 TORCH_LIBRARY(krsi, m) {
@@ -657,6 +963,15 @@ TORCH_LIBRARY(krsi, m) {
   m.def("linear_ce_finish(Tensor grad, Tensor g, Tensor weight, float scale, Tensor like) -> Tensor");
   m.def("geglu_q8_fwd(Tensor u, bool keep) -> (Tensor, Tensor, Tensor)");
   m.def("geglu_q8_bwd(Tensor g, Tensor q, Tensor exponents, bool want_out) -> (Tensor, Tensor)");
+  m.def("add_rmsnorm(Tensor x2d, Tensor? res, Tensor w, float eps) -> (Tensor, Tensor)");
+  m.def("add_rmsnorm_fwd(Tensor x2d, Tensor? res, Tensor w, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("add_rmsnorm_bwd(Tensor? gy, Tensor? gz, Tensor z, Tensor w, Tensor rstd) -> (Tensor, Tensor)");
+  m.def("add_rmsnorm_q8(Tensor x2d, Tensor? res, Tensor w, float eps) -> (Tensor, Tensor, Tensor)");
+  m.def("quantise_rows(Tensor x2d) -> (Tensor, Tensor)");
+  m.def("linear_q8(Tensor q, Tensor scale, Tensor wq, Tensor wscale, ScalarType out_dtype) -> Tensor");
+  m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
+        "Tensor(d!)[] masters, Tensor(e!)[] exponents, Tensor(f!) step, Tensor? lr_tensor, float lr, float beta1, "
+        "float beta2, float eps, float weight_decay, float max_norm) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
@@ -682,10 +997,21 @@ TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
   m.impl("linear_ce_finish", &linear_ce_finish);
   m.impl("geglu_q8_fwd", &geglu_q8_fwd);
   m.impl("geglu_q8_bwd", &geglu_q8_bwd);
+  m.impl("add_rmsnorm", &add_rmsnorm_plain);
+  m.impl("add_rmsnorm_fwd", &add_rmsnorm_fwd);
+  m.impl("add_rmsnorm_bwd", &add_rmsnorm_bwd);
+  m.impl("add_rmsnorm_q8", &add_rmsnorm_q8);
+  m.impl("quantise_rows", &quantise_rows);
+  m.impl("linear_q8", &linear_q8);
+  m.impl("adamw_step", &adamw_step);
 }
 
 TORCH_LIBRARY_IMPL(krsi, AutogradCUDA, m) {
   m.impl("embedding", &embedding_autograd);
   m.impl("geglu_q8", &geglu_q8_autograd);
   m.impl("linear_ce", &linear_ce_autograd);
+  m.impl("add_rmsnorm", &add_rmsnorm_autograd);
+  m.impl("add_rmsnorm_q8", &add_rmsnorm_q8_autograd);
+  m.impl("quantise_rows", &quantise_rows_autograd);
+  m.impl("linear_q8", &linear_q8_autograd);
 }

@@ -24,6 +24,9 @@ enum WatchdogRole : unsigned {
   kWdCeLoad = 25,     // vocabulary cross entropy GEMMs: the same three roles
   kWdCeMma = 26,
   kWdCeEpilogue = 27,
+  kWdQ8Load = 33,     // 8-bit product: the same three roles
+  kWdQ8Mma = 34,
+  kWdQ8Epilogue = 35,
   kWdTest = 0x7f      // the self-test kernel's deliberately unsatisfied wait
 };
 
@@ -38,9 +41,10 @@ cudaError_t watchdog_read_attn_bwd(unsigned* word, bool clear);
 cudaError_t watchdog_read_diag(unsigned* word, bool clear);
 cudaError_t watchdog_read_gemm(unsigned* word, bool clear);
 cudaError_t watchdog_read_ce(unsigned* word, bool clear);
+cudaError_t watchdog_read_q8(unsigned* word, bool clear);
 
 inline cudaError_t watchdog_read(unsigned* word, bool clear) {
-  unsigned a = 0, b = 0, c = 0, d = 0, f = 0;
+  unsigned a = 0, b = 0, c = 0, d = 0, f = 0, g = 0;
   cudaError_t e = watchdog_read_attn_fwd(&a, clear);
   if (e != cudaSuccess) return e;
   e = watchdog_read_attn_bwd(&b, clear);
@@ -50,7 +54,9 @@ inline cudaError_t watchdog_read(unsigned* word, bool clear) {
   e = watchdog_read_gemm(&d, clear);
   if (e != cudaSuccess) return e;
   e = watchdog_read_ce(&f, clear);
-  *word = a | b | c | d | f;
+  if (e != cudaSuccess) return e;
+  e = watchdog_read_q8(&g, clear);
+  *word = a | b | c | d | f | g;
   return e;
 }
 

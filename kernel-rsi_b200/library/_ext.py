@@ -176,6 +176,42 @@ def _register_compile_support() -> None:
     def _(x2d, w, targets, scale, ignore_index, z_loss, reduction, keep):
         return x2d.new_empty(() if reduction else (x2d.shape[0],), dtype=torch.float32)
 
+    @reg_fake("krsi::add_rmsnorm_fwd")
+    def _(x2d, res, w, eps):
+        return (x2d.new_empty(x2d.shape), x2d.new_empty((0 if res is None else x2d.shape[0], x2d.shape[1])),
+                x2d.new_empty((x2d.shape[0],), dtype=torch.float32))
+
+    @reg_fake("krsi::add_rmsnorm_bwd")
+    def _(gy, gz, z, w, rstd):
+        return z.new_empty(z.shape), w.new_empty(w.shape)
+
+    @reg_fake("krsi::add_rmsnorm")
+    def _(x2d, res, w, eps):
+        return x2d.new_empty(x2d.shape), x2d.new_empty(x2d.shape)
+
+    def padded_q8(rows, n, like):   # each row on whole 16 bytes
+        return like.new_empty_strided((rows, n), ((n + 15) // 16 * 16, 1), dtype=torch.float8_e4m3fn)
+
+    @reg_fake("krsi::add_rmsnorm_q8")
+    def _(x2d, res, w, eps):
+        rows, n = x2d.shape
+        return (padded_q8(rows, n, x2d), x2d.new_empty((rows,), dtype=torch.float32),
+                x2d.new_empty((0 if res is None else rows, n)))
+
+    @reg_fake("krsi::quantise_rows")
+    def _(x2d):
+        rows, n = x2d.shape
+        return padded_q8(rows, n, x2d), x2d.new_empty((rows,), dtype=torch.float32)
+
+    @reg_fake("krsi::linear_q8")
+    def _(q, scale, wq, wscale, out_dtype):
+        return q.new_empty((q.shape[0], wq.shape[0]), dtype=out_dtype)
+
+    @reg_fake("krsi::adamw_step")
+    def _(params, grads, exp_avgs, exp_avg_sqs, masters, exponents, step, lr_tensor, lr, beta1, beta2, eps,
+          weight_decay, max_norm):
+        return step.new_empty(() if max_norm > 0 else (0,), dtype=torch.float32)
+
     # Autograd of the forward ops, used when a compiled graph contains them (the eager path
     # uses the autograd.Function classes of each module instead).
     def rms_setup(ctx, inputs, output):
@@ -277,6 +313,21 @@ def _register_compile_support() -> None:
         return ops.geglu_q8_bwd(g, *ctx.saved_tensors, False)[0], None
 
     torch.library.register_autograd("krsi::geglu_q8_fwd", q8_backward, setup_context=q8_setup)
+
+    def add_norm_setup(ctx, inputs, output):
+        x2d, res, w, _ = inputs
+        _, z, rstd = output
+        ctx.save_for_backward(x2d if res is None else z, w, rstd)
+        ctx.add = res is not None
+        ctx.set_materialize_grads(False)
+
+    def add_norm_backward(ctx, gy, gz, _grstd):
+        if gy is None and (gz is None or not ctx.add):
+            return None, None, None, None
+        dz, dw = ops.add_rmsnorm_bwd(gy, gz if ctx.add else None, *ctx.saved_tensors)
+        return dz, (dz if ctx.add else None), dw, None
+
+    torch.library.register_autograd("krsi::add_rmsnorm_fwd", add_norm_backward, setup_context=add_norm_setup)
 
 
 _register_compile_support()
