@@ -22,6 +22,7 @@
 #include <cuda_fp8.h>
 
 #include "common.cuh"
+#include "sm100.cuh"
 
 namespace krsi {
 namespace {
@@ -31,6 +32,8 @@ constexpr int kThreads = 256;
 constexpr int kGroupsPerWarp = 4;
 constexpr int kChunk = kThreads / 32 * kGroupsPerWarp * kGroup;   // values of one block: 8192
 constexpr int kLane = 8;                           // values of one lane
+constexpr int kSpan = 8;                           // 8-bit states: groups that a warp takes at a time, at most
+constexpr int kBlocks8 = 592;                      // and its persistent blocks, four an SM
 constexpr int kNormBlocks = 592;                   // a fixed cap, so that the sum's order does not depend on the GPU
 constexpr int kSmallCap = 24, kLargeCap = 440;     // tensors of one launch: 1.6 and 28 KB of kernel arguments
 
@@ -42,14 +45,14 @@ struct Tensor {
   float* master;
   uint8_t* exponents;
   int64_t n;
-  int first_chunk;   // chunks of the tensors before it in the launch
+  int first_chunk;   // chunks (8-bit states: spans) of the tensors before it in the launch
   int aligned;       // whether every pointer allows a lane's vector accesses
 };
 
 template <int CAP>
 struct Table {
   Tensor t[CAP];
-  int count, n_chunks;
+  int count, n_chunks, chunk;   // chunk: values of one
 };
 
 // What the update takes from the device.
@@ -123,50 +126,14 @@ __device__ __forceinline__ void store8(void* base, int64_t at, bool vec, int liv
   }
 }
 
-// ---------------------------------------------------------------- eight codes
-__device__ __forceinline__ void decode8(const void* base, int64_t at, bool vec, int live, float scale, float* o) {
-  const uint8_t* p = static_cast<const uint8_t*>(base) + at;
-  uint32_t u[2] = {0, 0};
-  if (vec) {
-    const uint2 w = *reinterpret_cast<const uint2*>(p);
-    u[0] = w.x;
-    u[1] = w.y;
-  } else {
-#pragma unroll
-    for (int e = 0; e < kLane; ++e)
-      if (e < live) u[e / 4] |= (uint32_t)p[e] << (8 * (e % 4));
-  }
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    const __half2_raw h =
-        __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)((u[k / 2] >> (16 * (k % 2))) & 0xffff), __NV_E4M3);
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
-    o[2 * k] = __fmul_rn(f.x, scale);
-    o[2 * k + 1] = __fmul_rn(f.y, scale);
-  }
-}
-__device__ __forceinline__ void encode8(void* base, int64_t at, bool vec, int live, const float* o) {
-  uint8_t* p = static_cast<uint8_t*>(base) + at;
-  uint32_t u[2] = {0, 0};
-#pragma unroll
-  for (int k = 0; k < 4; ++k)
-    u[k / 2] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(o[2 * k], o[2 * k + 1]), __NV_SATFINITE, __NV_E4M3)
-                << (16 * (k % 2));
-  if (vec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
-  } else {
-#pragma unroll
-    for (int e = 0; e < kLane; ++e)
-      if (e < live) p[e] = (uint8_t)(u[e / 4] >> (8 * (e % 4)));
-  }
-}
+// ---------------------------------------------------------------- codes
 // 2^(byte - 127), NaN for the mark of a group that is not finite.
 __device__ __forceinline__ float scale_of(uint32_t byte) {
   return __uint_as_float(byte == 255 ? 0x7fffffffu : byte << 23);
 }
-// 2^(127 - byte)
+// 2^(127 - byte), byte at most 253
 __device__ __forceinline__ float inverse_scale_of(uint32_t byte) {
-  return __uint_as_float(byte == 255 ? 0x7fffffffu : (254 - byte) << 23);
+  return __uint_as_float((254 - byte) << 23);
 }
 // 16 random bits for each of a pair of places (low half: the even one).
 __device__ __forceinline__ uint32_t dither(uint32_t pair, uint32_t step) {
@@ -257,85 +224,294 @@ adamw_factors_kernel(const FactorArgs a, Factors* __restrict__ out) {
 struct Rates {
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
 };
+struct RatePairs {   // each twice, for f32x2 operations on kernel arguments
+  float2 beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
+  explicit RatePairs(const Rates& r)
+      : beta1{r.beta1, r.beta1}, one_minus_beta1{r.one_minus_beta1, r.one_minus_beta1}, beta2{r.beta2, r.beta2},
+        one_minus_beta2{r.one_minus_beta2, r.one_minus_beta2}, eps{r.eps, r.eps} {}
+};
 
-template <int PT, int GT, bool MASTER, bool Q8, int CAP>
+template <int PT, int GT, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kThreads)
 adamw_kernel(const __grid_constant__ Table<CAP> tab, const Rates c, const Factors* __restrict__ factors) {
   pdl_enter();
   const Factors f = *factors;
   if (f.skip) return;
-  const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const int lane = threadIdx.x % 32;
   const Tensor& t = tab.t[tensor_of(tab, blockIdx.x)];
-  const int64_t base = (int64_t)(blockIdx.x - t.first_chunk) * kChunk + warp * (kGroupsPerWarp * kGroup);
+  const int64_t base = (int64_t)(blockIdx.x - t.first_chunk) * kChunk + threadIdx.x / 32 * (kGroupsPerWarp * kGroup);
   const int64_t n = t.n;
 #pragma unroll 1
   for (int j = 0; j < kGroupsPerWarp; ++j) {
-    const int64_t at0 = base + j * kGroup;   // the group's first value
-    if (at0 >= n) return;
-    const int64_t at = at0 + lane * kLane, left = n - at;
+    const int64_t at = base + j * kGroup + lane * kLane, left = n - at;
+    if (left <= 0) return;
     const bool vec = t.aligned && left >= kLane;
-    const int live = left > kLane ? kLane : (int)(left < 0 ? 0 : left);
+    const int live = left > kLane ? kLane : (int)left;
     float p[kLane], g[kLane], m[kLane], v[kLane];
     if constexpr (MASTER) load8<KRSI_F32>(t.master, at, vec, live, p);
     else load8<PT>(t.p, at, vec, live, p);
     load8<GT>(t.g, at, vec, live, g);
-    if constexpr (Q8) {
-      const uint8_t* ex = t.exponents + at0 / kGroup * 2;
-      const float sm = scale_of(ex[0]), sr = scale_of(ex[1]);
-      decode8(t.m, at, vec, live, sm, m);
-      decode8(t.v, at, vec, live, sr, v);
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) v[e] = __fmul_rn(v[e], v[e]);
-    } else {
-      load8<KRSI_F32>(t.m, at, vec, live, m);
-      load8<KRSI_F32>(t.v, at, vec, live, v);
-    }
-    float r[kLane];
+    load8<KRSI_F32>(t.m, at, vec, live, m);
+    load8<KRSI_F32>(t.v, at, vec, live, v);
 #pragma unroll
     for (int e = 0; e < kLane; ++e) {
       const float ge = __fmul_rn(g[e], f.clip);
       m[e] = __fadd_rn(__fmul_rn(m[e], c.beta1), __fmul_rn(ge, c.one_minus_beta1));
       v[e] = __fadd_rn(__fmul_rn(v[e], c.beta2), __fmul_rn(__fmul_rn(ge, ge), c.one_minus_beta2));
-      r[e] = __fsqrt_rn(v[e]);
-      p[e] = p[e] * f.decay - f.rate * __fdividef(m[e], fmaf(r[e], f.inv_root, c.eps));
+      p[e] = p[e] * f.decay - f.rate * __fdividef(m[e], fmaf(sqrtf(v[e]), f.inv_root, c.eps));
     }
     if constexpr (MASTER) store8<KRSI_F32>(t.master, at, vec, live, p);
     store8<PT>(t.p, at, vec, live, p);
-    if constexpr (Q8) {
-      uint32_t top_m = 0, top_v = 0;
-#pragma unroll
-      for (int e = 0; e < kLane; ++e) {
-        top_m = max(top_m, __float_as_uint(m[e]) & 0x7fffffffu);
-        top_v = max(top_v, __float_as_uint(v[e]) & 0x7fffffffu);
-      }
-      const int field_m = (int)(__reduce_max_sync(0xffffffffu, top_m) >> 23);
-      const int field_v = (int)(__reduce_max_sync(0xffffffffu, top_v) >> 23);
-      // the group's largest magnitude 2^k f, 1 <= f < 2, becomes 2^7 f
-      const uint32_t em = field_m == 255 ? 255u : (uint32_t)max(field_m - 7, 1);
-      const uint32_t er = field_v == 255 ? 255u : (uint32_t)(((field_v - 127) >> 1) + 120);
-      const float im = inverse_scale_of(em), ir = inverse_scale_of(er);
-#pragma unroll
-      for (int e = 0; e < kLane; e += 2) {
-        const uint32_t h = dither((uint32_t)(at >> 1) + e / 2, f.step);
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          m[e + k] = __fmul_rn(m[e + k], im);
-          // up with the probability of the bits below the code's last one: they and the random bits carry into it.
-          // (Below 2^-6 codes are 2^-9 apart: 2^-6 more puts the sum where fp32's 20th bit is worth that.)
-          const float x = __fmul_rn(r[e + k], ir);
-          const float lift = x < 0.015625f ? 0.015625f : 0.f;
-          const uint32_t random = k == 0 ? (h & 0xffffu) << 4 : (h >> 16) << 4;
-          const uint32_t up = (__float_as_uint(__fadd_rn(x, lift)) + random) & 0xfff00000u;
-          r[e + k] = x > 0.f ? fmaxf(__fadd_rn(__uint_as_float(up), -lift), 0.001953125f) : 0.f;
-        }
-      }
-      encode8(t.m, at, vec, live, m);
-      encode8(t.v, at, vec, live, r);
-      if (lane == 0) *reinterpret_cast<uint16_t*>(t.exponents + at0 / kGroup * 2) = (uint16_t)(em | (er << 8));
-    } else {
-      store8<KRSI_F32>(t.m, at, vec, live, m);
-      store8<KRSI_F32>(t.v, at, vec, live, v);
+    store8<KRSI_F32>(t.m, at, vec, live, m);
+    store8<KRSI_F32>(t.v, at, vec, live, v);
+  }
+}
+
+// ---------------------------------------------------------------- 8-bit states
+// At 10 bytes a bf16 weight the memory leaves some 50 issued instructions to each, so the arithmetic is what has to be
+// short: pairs of fp32 (f32x2) where IEEE operations are wanted, one SFU instruction each for the root and the
+// quotient, and the next group's loads in flight meanwhile. The codes nevertheless follow the correctly rounded root:
+// where the SFU's could round the other way (once in 2^17 values) the lane takes __fsqrt_rn.
+
+// A lane's eight values as they are in memory.
+template <int DT>
+struct Raw8 {
+  static constexpr int W = DT == KRSI_F32 ? 8 : 4;
+  uint32_t w[W];
+  __device__ __forceinline__ uint64_t pair(int k) const {   // values 2k and 2k + 1 in fp32
+    if constexpr (DT == KRSI_F32) return sm100::f2_pack(__uint_as_float(w[2 * k]), __uint_as_float(w[2 * k + 1]));
+    else if constexpr (DT == KRSI_BF16)
+      return sm100::f2_pack(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xffff0000u));
+    else {
+      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[k]));
+      return sm100::f2_pack(f.x, f.y);
     }
+  }
+};
+template <int DT>
+__device__ __forceinline__ void load_raw(Raw8<DT>& r, const void* base, int64_t at, bool vec, int live) {
+  using T = typename Elem<DT>::T;
+  const T* p = static_cast<const T*>(base) + at;
+  if (vec) {
+    if constexpr (DT == KRSI_F32) {
+      float o[8];
+      load8(reinterpret_cast<const float*>(p), o);
+#pragma unroll
+      for (int k = 0; k < 8; ++k) r.w[k] = __float_as_uint(o[k]);
+    } else {
+      const uint4 u = *reinterpret_cast<const uint4*>(p);
+      r.w[0] = u.x; r.w[1] = u.y; r.w[2] = u.z; r.w[3] = u.w;
+    }
+  } else {
+#pragma unroll
+    for (int k = 0; k < Raw8<DT>::W; ++k) r.w[k] = 0;
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) {
+      if (e >= live) continue;
+      if constexpr (DT == KRSI_F32) r.w[e] = __float_as_uint(p[e]);
+      else r.w[e / 2] |= (uint32_t)reinterpret_cast<const uint16_t*>(p)[e] << (16 * (e % 2));
+    }
+  }
+}
+__device__ __forceinline__ uint2 load_codes(const void* base, int64_t at, bool vec, int live) {
+  const uint8_t* p = static_cast<const uint8_t*>(base) + at;
+  if (vec) return *reinterpret_cast<const uint2*>(p);
+  uint32_t u[2] = {0, 0};
+#pragma unroll
+  for (int e = 0; e < kLane; ++e)
+    if (e < live) u[e / 4] |= (uint32_t)p[e] << (8 * (e % 4));
+  return make_uint2(u[0], u[1]);
+}
+__device__ __forceinline__ void store_codes(void* base, int64_t at, bool vec, int live, const float* o) {
+  uint8_t* p = static_cast<uint8_t*>(base) + at;
+  uint32_t u[2];
+#pragma unroll
+  for (int k = 0; k < 2; ++k) {
+    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(o[4 * k], o[4 * k + 1]), __NV_SATFINITE, __NV_E4M3);
+    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(o[4 * k + 2], o[4 * k + 3]), __NV_SATFINITE, __NV_E4M3);
+    u[k] = __byte_perm(lo, hi, 0x5410);
+  }
+  if (vec) {
+    *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < kLane; ++e)
+      if (e < live) p[e] = (uint8_t)(u[e / 4] >> (8 * (e % 4)));
+  }
+}
+// Codes 2k and 2k + 1 as fp32.
+__device__ __forceinline__ uint64_t decode_pair(uint2 u, int k) {
+  const uint32_t w = k < 2 ? u.x : u.y;
+  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2((__nv_fp8x2_storage_t)(k % 2 ? w >> 16 : w & 0xffff), __NV_E4M3);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&h));
+  return sm100::f2_pack(f.x, f.y);
+}
+__device__ __forceinline__ float sqrt_sfu(float x) {
+  float y;
+  asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+// The largest of three magnitudes; NaN if one is.
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+  float d;
+  asm("max.NaN.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+__device__ __forceinline__ float max8_abs(const float* x) {
+  return max3_abs(max3_abs(x[0], x[1], x[2]), max3_abs(x[3], x[4], x[5]), max3_abs(x[6], x[7], x[7]));
+}
+__device__ __forceinline__ float min3(float a, float b, float c) {
+  float d;
+  asm("min.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
+constexpr float kLift = 0.015625f;       // 2^-6: codes below are subnormal, 2^-9 apart
+constexpr float kLeast = 0.001953125f;   // 2^-9, the least positive code
+
+// Scaled roots x >= 2^-6 to codes: up with the probability of the bits below the code's last one.  They and the random
+// bits (below fp32's 20th) carry into it; half a code less, the conversion's rounding to nearest then cuts them off.
+// False if one of them came within 8 units of x's last place of rounding differently.
+__device__ __forceinline__ bool round_roots(const float* x, const uint32_t* h, float* code) {
+  int nearest = 0x7fffffff;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    const uint32_t lo = __float_as_uint(x[2 * k]) + ((h[k] << 4) & 0xffff0u) + (8u - 0x80000u);
+    const uint32_t hi = __float_as_uint(x[2 * k + 1]) + ((h[k] >> 16) << 4) + (8u - 0x80000u);
+    nearest = min(nearest, min((int)(lo << 12), (int)(hi << 12)));   // (half a code less: the sign bit)
+    code[2 * k] = __uint_as_float(lo);
+    code[2 * k + 1] = __uint_as_float(hi);
+  }
+  return nearest >= (int)0x80010000;
+}
+// The same for any v, from its correctly rounded root: 2^-6 more puts roots below 2^-6 where fp32's 20th bit is worth
+// 2^-9; a positive one gives at least the least code.
+__device__ __forceinline__ float round_root(float v, float inverse_scale, uint32_t random16) {
+  const float x = __fmul_rn(__fsqrt_rn(v), inverse_scale);
+  const float lift = x < kLift ? kLift : 0.f;
+  const uint32_t up = (__float_as_uint(__fadd_rn(x, lift)) + (random16 << 4)) & 0xfff00000u;
+  return x > 0.f ? fmaxf(__fadd_rn(__uint_as_float(up), -lift), kLeast) : 0.f;
+}
+
+template <int PT, int GT, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kThreads, 4)
+adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ RatePairs c, const Factors* __restrict__ factors) {
+  pdl_enter();
+  using namespace sm100;
+  constexpr int WT = MASTER ? KRSI_F32 : PT;   // what the weight is read from
+  const Factors f = *factors;
+  if (f.skip) return;
+  const int lane = threadIdx.x % 32;
+  const uint64_t clip = f2_pack(f.clip, f.clip), decay = f2_pack(f.decay, f.decay), rate = f2_pack(-f.rate, -f.rate);
+  const auto pair_of = [](const float2& f) { return *reinterpret_cast<const uint64_t*>(&f); };
+
+  // Warps stay and take span after span: the next group's loads, of the next span too, are in flight while one is
+  // worked on (blocks of four groups each, which began with nothing in flight, took 2 ms where this takes 1.2).
+  const int warps = gridDim.x * (kThreads / 32);
+  int span = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
+  if (span >= tab.n_chunks) return;
+  int next = tensor_of(tab, span);   // the tensor, group and end of span of what is fetched next
+  int64_t next_at = (int64_t)(span - tab.t[next].first_chunk) * tab.chunk;
+  int64_t next_end = min(next_at + tab.chunk, tab.t[next].n);
+  Raw8<WT> pw;
+  Raw8<GT> gw;
+  uint2 mc, rc;
+  uint32_t ex;
+  auto fetch = [&]() {
+    const Tensor& t = tab.t[next];
+    const int64_t at = next_at + lane * kLane, left = t.n - at;
+    const bool vec = t.aligned && left >= kLane;
+    const int live = left > kLane ? kLane : (int)(left < 0 ? 0 : left);
+    load_raw<WT>(pw, MASTER ? (const void*)t.master : t.p, at, vec, live);
+    load_raw<GT>(gw, t.g, at, vec, live);
+    mc = load_codes(t.m, at, vec, live);
+    rc = load_codes(t.v, at, vec, live);
+    ex = *reinterpret_cast<const uint16_t*>(t.exponents + next_at / kGroup * 2);
+  };
+  fetch();
+#pragma unroll 1
+  while (true) {
+    const Tensor& t = tab.t[next];
+    const int64_t at0 = next_at;
+    const int64_t at = at0 + lane * kLane, left = t.n - at;
+    const bool vec = t.aligned && left >= kLane;
+    const int live = left > kLane ? kLane : (int)(left < 0 ? 0 : left);
+    uint64_t p[4], m[4], v[4];
+    {
+      const float sm = scale_of(ex & 0xff), sr = scale_of(ex >> 8);
+      const uint64_t sm2 = f2_pack(sm, sm), sr2 = f2_pack(sr, sr);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        p[k] = pw.pair(k);
+        const uint64_t g = f2_mul(gw.pair(k), clip);
+        m[k] = f2_add(f2_mul(f2_mul(decode_pair(mc, k), sm2), pair_of(c.beta1)), f2_mul(g, pair_of(c.one_minus_beta1)));
+        const uint64_t r = f2_mul(decode_pair(rc, k), sr2);
+        v[k] = f2_add(f2_mul(f2_mul(r, r), pair_of(c.beta2)), f2_mul(f2_mul(g, g), pair_of(c.one_minus_beta2)));
+      }
+    }
+    next_at += kGroup;
+    if (next_at >= next_end) {
+      span += warps;
+      if (span < tab.n_chunks) {
+        while (next + 1 < tab.count && tab.t[next + 1].first_chunk <= span) ++next;
+        next_at = (int64_t)(span - tab.t[next].first_chunk) * tab.chunk;
+        next_end = min(next_at + tab.chunk, tab.t[next].n);
+      }
+    }
+    const bool more = span < tab.n_chunks;
+    if (more) fetch();
+    float mf[kLane], vf[kLane];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f2_unpack(m[k], mf[2 * k], mf[2 * k + 1]);
+      f2_unpack(v[k], vf[2 * k], vf[2 * k + 1]);
+    }
+    const int field_m = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(max8_abs(mf))) >> 23);
+    const int field_v = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(max8_abs(vf))) >> 23);
+    // the group's largest magnitude 2^k f, 1 <= f < 2, becomes 2^7 f (one that is not finite marks the group; its own
+    // weights are still updated one by one)
+    const uint32_t em = field_m >= 255 ? 127u : (uint32_t)max(field_m - 7, 1);
+    const uint32_t er = field_v >= 255 ? 127u : (uint32_t)(((field_v - 127) >> 1) + 120);
+    const float im = inverse_scale_of(em), ir = inverse_scale_of(er);
+    const float back = scale_of(er) * f.inv_root;
+    float x[kLane];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      // (2^-100 keeps the quotient of two zeros finite; roots of 2^-9 and more do not see it)
+      float lo, hi;
+      f2_unpack(f2_fma(f2_mul(v[k], f2_pack(ir, ir)), f2_pack(ir, ir), f2_pack(0x1p-100f, 0x1p-100f)), lo, hi);
+      lo = sqrt_sfu(lo);
+      hi = sqrt_sfu(hi);
+      x[2 * k] = lo;
+      x[2 * k + 1] = hi;
+      f2_unpack(f2_fma(f2_pack(lo, hi), f2_pack(back, back), pair_of(c.eps)), lo, hi);
+      const uint64_t quotient = f2_mul(m[k], f2_pack(rcp_approx(lo), rcp_approx(hi)));
+      p[k] = f2_fma(quotient, rate, f2_mul(p[k], decay));
+      f2_unpack(f2_mul(m[k], f2_pack(im, im)), mf[2 * k], mf[2 * k + 1]);
+    }
+    {
+      float o[kLane];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) f2_unpack(p[k], o[2 * k], o[2 * k + 1]);
+      if constexpr (MASTER) store8<KRSI_F32>(t.master, at, vec, live, o);
+      store8<PT>(t.p, at, vec, live, o);
+    }
+    store_codes(t.m, at, vec, live, mf);
+    uint32_t h[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) h[k] = dither((uint32_t)(at >> 1) + k, f.step);
+    float code[kLane];
+    const float least = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), fminf(x[6], x[7]));
+    if (!round_roots(x, h, code) || !(least >= kLift)) {
+#pragma unroll
+      for (int e = 0; e < kLane; ++e)
+        code[e] = round_root(vf[e], ir, e % 2 ? h[e / 2] >> 16 : h[e / 2] & 0xffffu);
+    }
+    store_codes(t.v, at, vec, live, code);
+    if (lane == 0)
+      *reinterpret_cast<uint16_t*>(t.exponents + at0 / kGroup * 2) =
+          (uint16_t)((field_m >= 255 ? 255u : em) | ((field_v >= 255 ? 255u : er) << 8));
+    if (!more) return;
   }
 }
 
@@ -345,9 +521,10 @@ bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p
 
 int64_t launches_at_most(int64_t count) { return count / kLargeCap + 4; }   // one more for each gradient type
 
-// Calls `launch(table, first, n)` for tables of the tensors that `take` accepts, as few as their number allows.
+// Calls `launch(table)` for tables of the tensors that `take` accepts, as few as their number allows, in chunks of
+// `chunk` values.
 template <typename Take, typename Launch>
-int for_tables(const krsi_adamw_tensor* tensors, int64_t count, Take take, Launch launch) {
+int for_tables(const krsi_adamw_tensor* tensors, int64_t count, int chunk, Take take, Launch launch) {
   int64_t i = 0;
   while (i < count) {
     int n = 0;
@@ -357,10 +534,11 @@ int for_tables(const krsi_adamw_tensor* tensors, int64_t count, Take take, Launc
       constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
       int64_t chunks = 0;
       tab.count = 0;
+      tab.chunk = chunk;
       for (; i < count && tab.count < cap; ++i) {
         const krsi_adamw_tensor& s = tensors[i];
         if (!take(s) || s.n == 0) continue;
-        const int64_t own = (s.n + kChunk - 1) / kChunk;
+        const int64_t own = (s.n + chunk - 1) / chunk;
         if (own > INT32_MAX) return KRSI_ERR_UNSUPPORTED;
         if (chunks + own > INT32_MAX) break;   // the next launch takes it
         Tensor& t = tab.t[tab.count++];
@@ -388,22 +566,34 @@ int for_tables(const krsi_adamw_tensor* tensors, int64_t count, Take take, Launc
 
 template <int PT, int GT, bool MASTER, bool Q8>
 int update(const krsi_adamw_tensor* tensors, int64_t count, const Rates& c, const Factors* f, cudaStream_t s) {
-  return for_tables(
-      tensors, count,
-      [](const krsi_adamw_tensor& t) {
-        return t.p_dtype == PT && t.g_dtype == GT && (t.master != nullptr) == MASTER && (t.state_bits == 8) == Q8;
-      },
-      [&](const auto& tab) -> int {
-        constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
-        KRSI_CUDA_TRY(launch_pdl(adamw_kernel<PT, GT, MASTER, Q8, cap>, dim3(tab.n_chunks), dim3(kThreads), 0, s, tab, c, f));
-        return KRSI_OK;
-      });
+  auto take = [](const krsi_adamw_tensor& t) {
+    return t.p_dtype == PT && t.g_dtype == GT && (t.master != nullptr) == MASTER && (t.state_bits == 8) == Q8;
+  };
+  int chunk = kChunk;
+  if (Q8) {   // as many groups a span as leave one for every warp, so that few values still use many of them
+    int64_t groups = 0;
+    for (int64_t i = 0; i < count; ++i)
+      if (take(tensors[i])) groups += (tensors[i].n + kGroup - 1) / kGroup;
+    const int64_t each = groups / (kBlocks8 * (kThreads / 32));
+    chunk = kGroup * (int)(each < 1 ? 1 : each > kSpan ? kSpan : each);
+  }
+  return for_tables(tensors, count, chunk, take, [&](const auto& tab) -> int {
+    constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
+    if constexpr (Q8) {
+      const int64_t blocks = ((int64_t)tab.n_chunks + kThreads / 32 - 1) / (kThreads / 32);
+      KRSI_CUDA_TRY(launch_pdl(adamw8_kernel<PT, GT, MASTER, cap>, dim3((unsigned)(blocks < kBlocks8 ? blocks : kBlocks8)),
+                               dim3(kThreads), 0, s, tab, RatePairs(c), f));
+    } else {
+      KRSI_CUDA_TRY(launch_pdl(adamw_kernel<PT, GT, MASTER, cap>, dim3(tab.n_chunks), dim3(kThreads), 0, s, tab, c, f));
+    }
+    return KRSI_OK;
+  });
 }
 
 template <int GT>
 int norm(const krsi_adamw_tensor* tensors, int64_t count, double* partial, int64_t room, int* used, cudaStream_t s) {
   return for_tables(
-      tensors, count, [](const krsi_adamw_tensor& t) { return t.g_dtype == GT; },
+      tensors, count, kChunk, [](const krsi_adamw_tensor& t) { return t.g_dtype == GT; },
       [&](const auto& tab) -> int {
         constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
         const int blocks = tab.n_chunks < kNormBlocks ? tab.n_chunks : kNormBlocks;
