@@ -32,8 +32,7 @@ constexpr int kThreads = 256;
 constexpr int kGroupsPerWarp = 4;
 constexpr int kChunk = kThreads / 32 * kGroupsPerWarp * kGroup;   // values of one block: 8192
 constexpr int kLane = 8;                           // values of one lane
-constexpr int kSpan = 8;                           // 8-bit states: groups that a warp takes at a time, at most
-constexpr int kBlocks8 = 592;                      // and its persistent blocks, four an SM
+constexpr int kBlocks8 = 444;                      // 8-bit states: blocks, three an SM
 constexpr int kNormBlocks = 592;                   // a fixed cap, so that the sum's order does not depend on the GPU
 constexpr int kSmallCap = 24, kLargeCap = 440;     // tensors of one launch: 1.6 and 28 KB of kernel arguments
 
@@ -45,14 +44,14 @@ struct Tensor {
   float* master;
   uint8_t* exponents;
   int64_t n;
-  int first_chunk;   // chunks (8-bit states: spans) of the tensors before it in the launch
+  int first_chunk;   // chunks (8-bit states: groups) of the tensors before it in the launch
   int aligned;       // whether every pointer allows a lane's vector accesses
 };
 
 template <int CAP>
 struct Table {
   Tensor t[CAP];
-  int count, n_chunks, chunk;   // chunk: values of one
+  int count, n_chunks;
 };
 
 // What the update takes from the device.
@@ -322,8 +321,7 @@ __device__ __forceinline__ uint2 load_codes(const void* base, int64_t at, bool v
     if (e < live) u[e / 4] |= (uint32_t)p[e] << (8 * (e % 4));
   return make_uint2(u[0], u[1]);
 }
-__device__ __forceinline__ void store_codes(void* base, int64_t at, bool vec, int live, const float* o) {
-  uint8_t* p = static_cast<uint8_t*>(base) + at;
+__device__ __forceinline__ uint2 pack_codes(const float* o) {
   uint32_t u[2];
 #pragma unroll
   for (int k = 0; k < 2; ++k) {
@@ -331,12 +329,16 @@ __device__ __forceinline__ void store_codes(void* base, int64_t at, bool vec, in
     const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(o[4 * k + 2], o[4 * k + 3]), __NV_SATFINITE, __NV_E4M3);
     u[k] = __byte_perm(lo, hi, 0x5410);
   }
+  return make_uint2(u[0], u[1]);
+}
+__device__ __forceinline__ void store_codes(void* base, int64_t at, bool vec, int live, uint2 u) {
+  uint8_t* p = static_cast<uint8_t*>(base) + at;
   if (vec) {
-    *reinterpret_cast<uint2*>(p) = make_uint2(u[0], u[1]);
+    *reinterpret_cast<uint2*>(p) = u;
   } else {
 #pragma unroll
     for (int e = 0; e < kLane; ++e)
-      if (e < live) p[e] = (uint8_t)(u[e / 4] >> (8 * (e % 4)));
+      if (e < live) p[e] = (uint8_t)((e < 4 ? u.x : u.y) >> (8 * (e % 4)));
   }
 }
 // Codes 2k and 2k + 1 as fp32.
@@ -393,125 +395,153 @@ __device__ __forceinline__ float round_root(float v, float inverse_scale, uint32
   return x > 0.f ? fmaxf(__fadd_rn(__uint_as_float(up), -lift), kLeast) : 0.f;
 }
 
-template <int PT, int GT, bool MASTER, int CAP>
-__global__ void __launch_bounds__(kThreads, 4)
-adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ RatePairs c, const Factors* __restrict__ factors) {
-  pdl_enter();
+// A lane's part of a group: as read, and the results.
+template <int WT, int GT>
+struct Lane8 {
+  Raw8<WT> p;
+  Raw8<GT> g;
+  uint2 m, r;
+  uint32_t ex;   // both exponents
+};
+struct Done8 {
+  float p[kLane];
+  uint2 m, r;
+  uint32_t ex;
+};
+// Called by whole warps.  pair: the place of the lane's first value, halved.
+template <int WT, int GT>
+__device__ __forceinline__ void update8(const Lane8<WT, GT>& in, const RatePairs& c, const Factors& f, uint32_t pair,
+                                        Done8& out) {
   using namespace sm100;
+  const auto pair_of = [](const float2& x) { return *reinterpret_cast<const uint64_t*>(&x); };
+  const auto twice = [](float x) { return f2_pack(x, x); };
+  uint64_t m[4], v[4];
+  {
+    const uint64_t sm = twice(scale_of(in.ex & 0xff)), sr = twice(scale_of(in.ex >> 8)), clip = twice(f.clip);
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const uint64_t g = f2_mul(in.g.pair(k), clip);
+      m[k] = f2_add(f2_mul(f2_mul(decode_pair(in.m, k), sm), pair_of(c.beta1)), f2_mul(g, pair_of(c.one_minus_beta1)));
+      const uint64_t r = f2_mul(decode_pair(in.r, k), sr);
+      v[k] = f2_add(f2_mul(f2_mul(r, r), pair_of(c.beta2)), f2_mul(f2_mul(g, g), pair_of(c.one_minus_beta2)));
+    }
+  }
+  float mf[kLane], vf[kLane];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    f2_unpack(m[k], mf[2 * k], mf[2 * k + 1]);
+    f2_unpack(v[k], vf[2 * k], vf[2 * k + 1]);
+  }
+  const int field_m = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(max8_abs(mf))) >> 23);
+  const int field_v = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(max8_abs(vf))) >> 23);
+  // the group's largest magnitude 2^k f, 1 <= f < 2, becomes 2^7 f (one that is not finite marks the group; its own
+  // weights are still updated one by one)
+  const uint32_t em = field_m >= 255 ? 127u : (uint32_t)max(field_m - 7, 1);
+  const uint32_t er = field_v >= 255 ? 127u : (uint32_t)(((field_v - 127) >> 1) + 120);
+  out.ex = (field_m >= 255 ? 255u : em) | ((field_v >= 255 ? 255u : er) << 8);
+  const float ir = inverse_scale_of(er);
+  const uint64_t im = twice(inverse_scale_of(em)), back = twice(scale_of(er) * f.inv_root);
+  const uint64_t decay = twice(f.decay), rate = twice(-f.rate);
+  float x[kLane];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    // (2^-100 keeps the quotient of two zeros finite; roots of 2^-9 and more do not see it)
+    float lo, hi;
+    f2_unpack(f2_fma(f2_mul(v[k], twice(ir)), twice(ir), twice(0x1p-100f)), lo, hi);
+    x[2 * k] = sqrt_sfu(lo);
+    x[2 * k + 1] = sqrt_sfu(hi);
+    f2_unpack(f2_fma(f2_pack(x[2 * k], x[2 * k + 1]), back, pair_of(c.eps)), lo, hi);
+    const uint64_t quotient = f2_mul(m[k], f2_pack(rcp_approx(lo), rcp_approx(hi)));
+    f2_unpack(f2_fma(quotient, rate, f2_mul(in.p.pair(k), decay)), out.p[2 * k], out.p[2 * k + 1]);
+    f2_unpack(f2_mul(m[k], im), mf[2 * k], mf[2 * k + 1]);
+  }
+  out.m = pack_codes(mf);
+  uint32_t h[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) h[k] = dither(pair + k, f.step);
+  float code[kLane];
+  const float least = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), fminf(x[6], x[7]));
+  if (!round_roots(x, h, code) || !(least >= kLift)) {
+#pragma unroll
+    for (int e = 0; e < kLane; ++e) code[e] = round_root(vf[e], ir, e % 2 ? h[e / 2] >> 16 : h[e / 2] & 0xffffu);
+  }
+  out.r = pack_codes(code);
+}
+
+template <int PT, int GT, bool MASTER, int CAP>
+__global__ void __launch_bounds__(kThreads, 3)
+adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ RatePairs c, const int span,
+              const Factors* __restrict__ factors) {
+  pdl_enter();
   constexpr int WT = MASTER ? KRSI_F32 : PT;   // what the weight is read from
   const Factors f = *factors;
   if (f.skip) return;
   const int lane = threadIdx.x % 32;
-  const uint64_t clip = f2_pack(f.clip, f.clip), decay = f2_pack(f.decay, f.decay), rate = f2_pack(-f.rate, -f.rate);
-  const auto pair_of = [](const float2& f) { return *reinterpret_cast<const uint64_t*>(&f); };
-
-  // Warps stay and take span after span: the next group's loads, of the next span too, are in flight while one is
-  // worked on (blocks of four groups each, which began with nothing in flight, took 2 ms where this takes 1.2).
-  const int warps = gridDim.x * (kThreads / 32);
-  int span = blockIdx.x * (kThreads / 32) + threadIdx.x / 32;
-  if (span >= tab.n_chunks) return;
-  int next = tensor_of(tab, span);   // the tensor, group and end of span of what is fetched next
-  int64_t next_at = (int64_t)(span - tab.t[next].first_chunk) * tab.chunk;
-  int64_t next_end = min(next_at + tab.chunk, tab.t[next].n);
-  Raw8<WT> pw;
-  Raw8<GT> gw;
-  uint2 mc, rc;
-  uint32_t ex;
-  auto fetch = [&]() {
-    const Tensor& t = tab.t[next];
-    const int64_t at = next_at + lane * kLane, left = t.n - at;
-    const bool vec = t.aligned && left >= kLane;
-    const int live = left > kLane ? kLane : (int)(left < 0 ? 0 : left);
-    load_raw<WT>(pw, MASTER ? (const void*)t.master : t.p, at, vec, live);
-    load_raw<GT>(gw, t.g, at, vec, live);
-    mc = load_codes(t.m, at, vec, live);
-    rc = load_codes(t.v, at, vec, live);
-    ex = *reinterpret_cast<const uint16_t*>(t.exponents + next_at / kGroup * 2);
-  };
-  fetch();
+  // Each warp takes `span` consecutive groups, and of them each tensor's part by itself.
+  const int64_t first = (int64_t)(blockIdx.x * (kThreads / 32) + threadIdx.x / 32) * span;
+  if (first >= tab.n_chunks) return;
+  int group = (int)first;
+  int i = tensor_of(tab, group);
+  const int end = tab.n_chunks - group < span ? tab.n_chunks : group + span;
+  while (group < end) {
+    while (i + 1 < tab.count && tab.t[i + 1].first_chunk <= group) ++i;
+    const Tensor& t = tab.t[i];
+    const int64_t at0 = (int64_t)(group - t.first_chunk) * kGroup;
+    int part = min(end - group, (int)((t.n - at0 + kGroup - 1) / kGroup));
+    group += part;
+    const bool ragged = at0 + (int64_t)part * kGroup > t.n;   // its last group is not a whole one
+    const int whole = t.aligned ? part - ragged : 0;
+    using W = typename Elem<WT>::T;
+    using G = typename Elem<GT>::T;
+    int64_t at = at0 + lane * kLane;
+    if (whole > 0) {   // with the next group's loads in flight while one is worked on
+      const W* w = static_cast<const W*>(MASTER ? (const void*)t.master : t.p) + at;
+      const G* g = static_cast<const G*>(t.g) + at;
+      const uint8_t* m = static_cast<const uint8_t*>(t.m) + at;
+      const uint8_t* r = static_cast<const uint8_t*>(t.v) + at;
+      const uint8_t* ex = t.exponents + at0 / kGroup * 2;
+      Lane8<WT, GT> in;
+      auto fetch = [&](int j) {
+        load_raw<WT>(in.p, w, (int64_t)j * kGroup, true, kLane);
+        load_raw<GT>(in.g, g, (int64_t)j * kGroup, true, kLane);
+        in.m = load_codes(m, (int64_t)j * kGroup, true, kLane);
+        in.r = load_codes(r, (int64_t)j * kGroup, true, kLane);
+        in.ex = *reinterpret_cast<const uint16_t*>(ex + 2 * j);
+      };
+      fetch(0);
 #pragma unroll 1
-  while (true) {
-    const Tensor& t = tab.t[next];
-    const int64_t at0 = next_at;
-    const int64_t at = at0 + lane * kLane, left = t.n - at;
-    const bool vec = t.aligned && left >= kLane;
-    const int live = left > kLane ? kLane : (int)(left < 0 ? 0 : left);
-    uint64_t p[4], m[4], v[4];
-    {
-      const float sm = scale_of(ex & 0xff), sr = scale_of(ex >> 8);
-      const uint64_t sm2 = f2_pack(sm, sm), sr2 = f2_pack(sr, sr);
-#pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        p[k] = pw.pair(k);
-        const uint64_t g = f2_mul(gw.pair(k), clip);
-        m[k] = f2_add(f2_mul(f2_mul(decode_pair(mc, k), sm2), pair_of(c.beta1)), f2_mul(g, pair_of(c.one_minus_beta1)));
-        const uint64_t r = f2_mul(decode_pair(rc, k), sr2);
-        v[k] = f2_add(f2_mul(f2_mul(r, r), pair_of(c.beta2)), f2_mul(f2_mul(g, g), pair_of(c.one_minus_beta2)));
+      for (int j = 0; j < whole; ++j) {
+        const Lane8<WT, GT> now = in;
+        if (j + 1 < whole) fetch(j + 1);
+        Done8 out;
+        update8(now, c, f, (uint32_t)((at + (int64_t)j * kGroup) >> 1), out);
+        if constexpr (MASTER) store8<KRSI_F32>(const_cast<W*>(w), (int64_t)j * kGroup, true, kLane, out.p);
+        store8<PT>(t.p, at + (int64_t)j * kGroup, true, kLane, out.p);
+        store_codes(const_cast<uint8_t*>(m), (int64_t)j * kGroup, true, kLane, out.m);
+        store_codes(const_cast<uint8_t*>(r), (int64_t)j * kGroup, true, kLane, out.r);
+        if (lane == 0) *reinterpret_cast<uint16_t*>(const_cast<uint8_t*>(ex) + 2 * j) = (uint16_t)out.ex;
       }
     }
-    next_at += kGroup;
-    if (next_at >= next_end) {
-      span += warps;
-      if (span < tab.n_chunks) {
-        while (next + 1 < tab.count && tab.t[next + 1].first_chunk <= span) ++next;
-        next_at = (int64_t)(span - tab.t[next].first_chunk) * tab.chunk;
-        next_end = min(next_at + tab.chunk, tab.t[next].n);
-      }
+#pragma unroll 1
+    for (int j = whole; j < part; ++j) {
+      const int64_t a = at + (int64_t)j * kGroup, left = t.n - a;
+      const bool vec = t.aligned && left >= kLane;
+      const int live = left > kLane ? kLane : (int)(left < 0 ? 0 : left);
+      uint8_t* ex = t.exponents + (at0 / kGroup + j) * 2;
+      Lane8<WT, GT> in;
+      load_raw<WT>(in.p, MASTER ? (const void*)t.master : t.p, a, vec, live);
+      load_raw<GT>(in.g, t.g, a, vec, live);
+      in.m = load_codes(t.m, a, vec, live);
+      in.r = load_codes(t.v, a, vec, live);
+      in.ex = *reinterpret_cast<const uint16_t*>(ex);
+      Done8 out;
+      update8(in, c, f, (uint32_t)(a >> 1), out);
+      if constexpr (MASTER) store8<KRSI_F32>(t.master, a, vec, live, out.p);
+      store8<PT>(t.p, a, vec, live, out.p);
+      store_codes(t.m, a, vec, live, out.m);
+      store_codes(t.v, a, vec, live, out.r);
+      if (lane == 0) *reinterpret_cast<uint16_t*>(ex) = (uint16_t)out.ex;
     }
-    const bool more = span < tab.n_chunks;
-    if (more) fetch();
-    float mf[kLane], vf[kLane];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      f2_unpack(m[k], mf[2 * k], mf[2 * k + 1]);
-      f2_unpack(v[k], vf[2 * k], vf[2 * k + 1]);
-    }
-    const int field_m = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(max8_abs(mf))) >> 23);
-    const int field_v = (int)(__reduce_max_sync(0xffffffffu, __float_as_uint(max8_abs(vf))) >> 23);
-    // the group's largest magnitude 2^k f, 1 <= f < 2, becomes 2^7 f (one that is not finite marks the group; its own
-    // weights are still updated one by one)
-    const uint32_t em = field_m >= 255 ? 127u : (uint32_t)max(field_m - 7, 1);
-    const uint32_t er = field_v >= 255 ? 127u : (uint32_t)(((field_v - 127) >> 1) + 120);
-    const float im = inverse_scale_of(em), ir = inverse_scale_of(er);
-    const float back = scale_of(er) * f.inv_root;
-    float x[kLane];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      // (2^-100 keeps the quotient of two zeros finite; roots of 2^-9 and more do not see it)
-      float lo, hi;
-      f2_unpack(f2_fma(f2_mul(v[k], f2_pack(ir, ir)), f2_pack(ir, ir), f2_pack(0x1p-100f, 0x1p-100f)), lo, hi);
-      lo = sqrt_sfu(lo);
-      hi = sqrt_sfu(hi);
-      x[2 * k] = lo;
-      x[2 * k + 1] = hi;
-      f2_unpack(f2_fma(f2_pack(lo, hi), f2_pack(back, back), pair_of(c.eps)), lo, hi);
-      const uint64_t quotient = f2_mul(m[k], f2_pack(rcp_approx(lo), rcp_approx(hi)));
-      p[k] = f2_fma(quotient, rate, f2_mul(p[k], decay));
-      f2_unpack(f2_mul(m[k], f2_pack(im, im)), mf[2 * k], mf[2 * k + 1]);
-    }
-    {
-      float o[kLane];
-#pragma unroll
-      for (int k = 0; k < 4; ++k) f2_unpack(p[k], o[2 * k], o[2 * k + 1]);
-      if constexpr (MASTER) store8<KRSI_F32>(t.master, at, vec, live, o);
-      store8<PT>(t.p, at, vec, live, o);
-    }
-    store_codes(t.m, at, vec, live, mf);
-    uint32_t h[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) h[k] = dither((uint32_t)(at >> 1) + k, f.step);
-    float code[kLane];
-    const float least = min3(min3(x[0], x[1], x[2]), min3(x[3], x[4], x[5]), fminf(x[6], x[7]));
-    if (!round_roots(x, h, code) || !(least >= kLift)) {
-#pragma unroll
-      for (int e = 0; e < kLane; ++e)
-        code[e] = round_root(vf[e], ir, e % 2 ? h[e / 2] >> 16 : h[e / 2] & 0xffffu);
-    }
-    store_codes(t.v, at, vec, live, code);
-    if (lane == 0)
-      *reinterpret_cast<uint16_t*>(t.exponents + at0 / kGroup * 2) =
-          (uint16_t)((field_m >= 255 ? 255u : em) | ((field_v >= 255 ? 255u : er) << 8));
-    if (!more) return;
   }
 }
 
@@ -534,7 +564,6 @@ int for_tables(const krsi_adamw_tensor* tensors, int64_t count, int chunk, Take 
       constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
       int64_t chunks = 0;
       tab.count = 0;
-      tab.chunk = chunk;
       for (; i < count && tab.count < cap; ++i) {
         const krsi_adamw_tensor& s = tensors[i];
         if (!take(s) || s.n == 0) continue;
@@ -569,20 +598,14 @@ int update(const krsi_adamw_tensor* tensors, int64_t count, const Rates& c, cons
   auto take = [](const krsi_adamw_tensor& t) {
     return t.p_dtype == PT && t.g_dtype == GT && (t.master != nullptr) == MASTER && (t.state_bits == 8) == Q8;
   };
-  int chunk = kChunk;
-  if (Q8) {   // as many groups a span as leave one for every warp, so that few values still use many of them
-    int64_t groups = 0;
-    for (int64_t i = 0; i < count; ++i)
-      if (take(tensors[i])) groups += (tensors[i].n + kGroup - 1) / kGroup;
-    const int64_t each = groups / (kBlocks8 * (kThreads / 32));
-    chunk = kGroup * (int)(each < 1 ? 1 : each > kSpan ? kSpan : each);
-  }
-  return for_tables(tensors, count, chunk, take, [&](const auto& tab) -> int {
+  return for_tables(tensors, count, Q8 ? kGroup : kChunk, take, [&](const auto& tab) -> int {
     constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
     if constexpr (Q8) {
-      const int64_t blocks = ((int64_t)tab.n_chunks + kThreads / 32 - 1) / (kThreads / 32);
-      KRSI_CUDA_TRY(launch_pdl(adamw8_kernel<PT, GT, MASTER, cap>, dim3((unsigned)(blocks < kBlocks8 ? blocks : kBlocks8)),
-                               dim3(kThreads), 0, s, tab, RatePairs(c), f));
+      // consecutive groups in equal shares (16 at a time, in turns, take 10% more)
+      constexpr int warps = kBlocks8 * (kThreads / 32);
+      const int64_t span = ((int64_t)tab.n_chunks + warps - 1) / warps;
+      const int64_t blocks = (tab.n_chunks + span * (kThreads / 32) - 1) / (span * (kThreads / 32));
+      KRSI_CUDA_TRY(launch_pdl(adamw8_kernel<PT, GT, MASTER, cap>, dim3((unsigned)blocks), dim3(kThreads), 0, s, tab, RatePairs(c), (int)span, f));
     } else {
       KRSI_CUDA_TRY(launch_pdl(adamw_kernel<PT, GT, MASTER, cap>, dim3(tab.n_chunks), dim3(kThreads), 0, s, tab, c, f));
     }
