@@ -271,11 +271,21 @@ int krsi_linear_ce_finish(const float* grad, const float* g, const float* weight
 
 /* ---------------------------------------------------------------- residual addition and RMSNorm
  * z = (x + res) rounded to x_dtype, then krsi_rmsnorm_fwd's norm of z: y and rstd as there.  The reference has no
- * such op (its models add, then call library/rmsnorm.py:22-31).  The backward is krsi_rmsnorm_bwd_add on z.
- * x, res, z, y: [rows, n] of x_dtype; w: [n] of w_dtype; contiguous; dtypes and widths as krsi_rmsnorm_fwd's.
+ * such op (its models add, then call library/rmsnorm.py:22-31).
+ * x, res, z, y: [rows, n] of x_dtype; w: [n] of w_dtype; contiguous; dtypes as krsi_rmsnorm_fwd's; n up to 16384
+ * (32768 for 16-bit x with rows of whole 16 bytes at 16-byte aligned pointers).
  * res null: z is x, and is not written. */
 int krsi_add_rmsnorm_fwd(const void* x, const void* res, const void* w, void* z, void* y, float* rstd,
                          int64_t rows, int64_t n, float eps, int x_dtype, int w_dtype, cudaStream_t stream);
+
+int krsi_add_rmsnorm_bwd_workspace_size(int64_t rows, int64_t n, size_t* bytes);
+
+/* dz = gy * w * rstd - z * rstd^3 * mean(gy * w * z) + gz, the gradient of x and of res, and dw = sum of gy * z * rstd
+ * over the rows, both in fp32 with one rounding (krsi_rmsnorm_bwd_add rounds gy * w and z * rstd on the way); dw's
+ * sum has a fixed order.  gz null: none. */
+int krsi_add_rmsnorm_bwd(const void* gy, const void* gz, const void* z, const void* w, const float* rstd, void* dz,
+                         void* dw, void* workspace, size_t workspace_bytes, int64_t rows, int64_t n, int x_dtype,
+                         int w_dtype, cudaStream_t stream);
 
 /* The same with y in 8 bits: q [rows, n] e4m3, row i at q + i * q_stride bytes, and scale [rows] fp32;
  * y = q * scale, q = e4m3(z * w * (448 / m)) and scale = m * rstd / 448 for the row's largest |z * w| m.

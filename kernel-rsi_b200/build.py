@@ -29,7 +29,7 @@ NVCC = str(CUDA_HOME / "bin" / "nvcc")
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
 CU_SOURCES = ["capi.cu", "diag.cu", "rmsnorm.cu", "geglu.cu", "relpos_attn_fwd.cu", "relpos_attn_bwd.cu", "t5_bias.cu",
               "linear_geglu.cu", "token_rows.cu", "embedding.cu", "geglu_q8.cu", "linear_ce.cu",
-              "add_rmsnorm.cu", "linear_q8.cu", "adamw.cu"]
+              "add_rmsnorm.cu", "add_rmsnorm_bwd.cu", "linear_q8.cu", "adamw.cu"]
 C_ABI_LIB = LIB / "libkrsi_b200.so"
 TORCH_LIB = LIB / "_krsi_torch.so"
 

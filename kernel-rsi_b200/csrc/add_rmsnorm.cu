@@ -6,21 +6,23 @@
 //   (448 / max is 448 times the rounded reciprocal, as torch divides a number by a tensor.)
 // The codes do not depend on r (it cancels), so neither on the order of the sum of squares: the same row gives
 // the same bits in any plan.  Without res, z is x and is not written.
-// The backward is rmsnorm.cu's with the gradient of z added (krsi_rmsnorm_bwd_add).
+// (The backward is in add_rmsnorm_bwd.cu.)
 // Layout as in rmsnorm.cu: TPR threads hold a row in registers, thread t the packets at columns (c*TPR + t)*VEC.
 
 #include <cuda_fp8.h>
 
-#include "common.cuh"
+#include "add_rmsnorm.cuh"
 
 namespace krsi {
 namespace {
+
+using namespace norm;
 
 constexpr float kE4m3Max = 448.0f;
 // Rows whose largest |t| is below this are scaled as if it were that: 448 / max stays finite.
 constexpr float kTinyTop = 7.888609052210118e-31f;   // 2^-100
 
-enum Out : int { kOutRow = 0, kOutQ8 = 1, kOutQuantise = 2 };
+enum Out : int { kOutRow = 0, kOutQ8 = 1 };   // (8 bits without w: the rows themselves)
 
 __device__ __forceinline__ float warp_max(float v) {
 #pragma unroll
@@ -53,33 +55,6 @@ template <int TPR> struct NormCfg {
   static constexpr int kRowsPerBlock = kThreads / TPR;
 };
 
-template <int DT, int VEC>
-__device__ __forceinline__ void load_row(const typename Elem<DT>::T* p, float* out, bool stream) {
-  using E = Elem<DT>;
-  if constexpr (VEC == 1) {
-    out[0] = E::load(*p);
-  } else {
-    constexpr int PK = Vec16<typename E::T>::N;
-#pragma unroll
-    for (int e = 0; e < VEC; e += PK) {
-      const auto v = stream ? ldg16_stream(p + e) : ldg16(p + e);
-#pragma unroll
-      for (int k = 0; k < PK; ++k) out[e + k] = E::load(v.v[k]);
-    }
-  }
-}
-template <int DT, int VEC>
-__device__ __forceinline__ void store_row(typename Elem<DT>::T* p, const float* in) {
-  using E = Elem<DT>;
-  if constexpr (VEC == 1) {
-    *p = E::store(in[0]);
-  } else {
-    Vec16<typename E::T> o;
-#pragma unroll
-    for (int k = 0; k < VEC; ++k) o.v[k] = E::store(in[k]);
-    stg16(p, o);
-  }
-}
 __device__ __forceinline__ uint16_t e4m3x2(float lo, float hi) {
   return (uint16_t)__nv_cvt_float2_to_fp8x2(make_float2(lo, hi), __NV_SATFINITE, __NV_E4M3);
 }
@@ -105,13 +80,12 @@ struct NormArgs {
   float eps;
 };
 
-template <int XT, int WT, int TPR, int VEC, int NCH, int OUT>
+template <int XT, bool WF32, int TPR, int VEC, int NCH, int OUT>
 __global__ void __launch_bounds__(NormCfg<TPR>::kThreads)
 add_rmsnorm_kernel(const NormArgs a) {
   pdl_enter();
   using T = typename Elem<XT>::T;
   using XE = Elem<XT>;
-  using WE = Elem<WT>;
   __shared__ float2 red[32];
   const int t = threadIdx.x % TPR;
   const int64_t row = (int64_t)blockIdx.x * NormCfg<TPR>::kRowsPerBlock + threadIdx.x / TPR;
@@ -119,8 +93,7 @@ add_rmsnorm_kernel(const NormArgs a) {
   const int n = a.n;
   const T* xr = static_cast<const T*>(a.x) + row * n;
   const T* rr = static_cast<const T*>(a.res) + row * n;
-  const auto* w = static_cast<const typename WE::T*>(a.w);
-  const bool add = OUT != kOutQuantise && a.res != nullptr;
+  const bool add = a.res != nullptr;
   float v[NCH][VEC];
   float ss = 0.f, top = 0.f;
 #pragma unroll
@@ -155,17 +128,15 @@ add_rmsnorm_kernel(const NormArgs a) {
   for (int c = 0; c < NCH; ++c)
 #pragma unroll
     for (int e = 0; e < VEC; ++e) ss = fmaf(v[c][e], v[c][e], ss);
-  if constexpr (OUT != kOutRow) {   // v becomes t = z * w
+  if constexpr (OUT == kOutQ8) {   // v becomes t = z * w
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
       const int col = (c * TPR + t) * VEC;
-      if constexpr (OUT == kOutQ8) {
-        if (col < n) {
-          float wv[VEC];
-          load_row<WT, VEC>(w + col, wv, false);
+      if (a.w != nullptr && col < n) {
+        float wv[VEC];
+        load_weight<XT, VEC>(a.w, WF32, col, wv);
 #pragma unroll
-          for (int e = 0; e < VEC; ++e) v[c][e] *= wv[e];
-        }
+        for (int e = 0; e < VEC; ++e) v[c][e] *= wv[e];
       }
 #pragma unroll
       for (int e = 0; e < VEC; ++e) top = fmaxf(top, fabsf(v[c][e]));
@@ -182,9 +153,13 @@ add_rmsnorm_kernel(const NormArgs a) {
       const int col = (c * TPR + t) * VEC;
       if (col < n) {
         float wv[VEC], o[VEC];
-        load_row<WT, VEC>(w + col, wv, false);
+        load_weight<XT, VEC>(a.w, WF32, col, wv);
+        // z * r is rounded to w's type (the store rounds the product to x's)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = WE::round(wv[e] * WE::round(v[c][e] * r));
+        for (int e = 0; e < VEC; ++e) {
+          const float nz = v[c][e] * r;
+          o[e] = wv[e] * (WF32 ? nz : XE::round(nz));
+        }
         store_row<XT, VEC>(yr + col, o);
       }
     }
@@ -193,8 +168,8 @@ add_rmsnorm_kernel(const NormArgs a) {
     const float inv = __fmul_rn(kE4m3Max, __frcp_rn(top));
     if (t == 0) {
       // fmaxf drops NaN: the sum of squares brings it into the scale (0 * ss is 0 or NaN)
-      const float r = OUT == kOutQ8 ? 1.0f / sqrtf(ss / (float)n + a.eps) : 1.0f;
-      a.stat[row] = OUT == kOutQ8 ? top * r / kE4m3Max : isnan(ss) ? ss : top / kE4m3Max;
+      const float r = 1.0f / sqrtf(ss / (float)n + a.eps);
+      a.stat[row] = a.w != nullptr ? top * r / kE4m3Max : isnan(ss) ? ss : top / kE4m3Max;
     }
     uint8_t* qr = static_cast<uint8_t*>(a.y) + row * a.q_stride;
 #pragma unroll
@@ -210,63 +185,58 @@ add_rmsnorm_kernel(const NormArgs a) {
 }
 
 // ---------------------------------------------------------------- host-side planning
-struct NormPlan { int tpr, vec, nch; };
+// (threads a row, packets a thread) for packets of 8, 4 and 1 values: the first that holds the row.  A warp a row up to
+// 40 values a thread (16 one by one), then blocks, as small as can be: several small blocks an SM keep more rows in
+// flight between their barriers.
+#define KRSI_PLANS8(X) \
+  X(32, 1) X(32, 2) X(32, 3) X(32, 4) X(32, 5) X(64, 3) X(64, 5) X(128, 3) X(128, 5) X(256, 3) X(256, 5) X(512, 3) \
+  X(512, 5) X(1024, 4)
+#define KRSI_PLANS4(X) \
+  X(32, 1) X(32, 2) X(32, 4) X(32, 6) X(32, 8) X(32, 10) X(64, 6) X(64, 10) X(128, 6) X(128, 10) X(256, 6) X(256, 10) \
+  X(512, 6) X(512, 10)
+#define KRSI_PLANS1(X) \
+  X(32, 2) X(32, 4) X(32, 8) X(32, 12) X(32, 16) X(64, 9) X(64, 12) X(64, 16) X(128, 9) X(128, 12) X(128, 16) \
+  X(256, 9) X(256, 12) X(256, 16) X(512, 9) X(512, 12) X(512, 16) X(1024, 9) X(1024, 12) X(1024, 16)
 
-constexpr int kWarpChunks[] = {1, 2, 3, 4, 5, 6, 8};
-constexpr int kBlock128Chunks[] = {3, 4, 6, 8};
-constexpr int kBlock512Chunks[] = {4, 8};
-
-bool plan(int64_t n, int vec, NormPlan* p) {
-  p->vec = vec;
-  const int64_t packets = (n + vec - 1) / vec;
-  for (int c : kWarpChunks)
-    if (packets <= 32 * c) { p->tpr = 32; p->nch = c; return true; }
-  for (int c : kBlock128Chunks)
-    if (packets <= 128 * c) { p->tpr = 128; p->nch = c; return true; }
-  for (int c : kBlock512Chunks)
-    if (packets <= 512 * c) { p->tpr = 512; p->nch = c; return true; }
-  if (vec == 1 && packets <= 1024 * 16) { p->tpr = 1024; p->nch = 16; return true; }
-  return false;
-}
-
-template <int XT, int WT, int TPR, int VEC, int NCH, int OUT>
+template <int XT, bool WF32, int TPR, int VEC, int NCH, int OUT>
 int run(const NormArgs& a, cudaStream_t s) {
   using Cfg = NormCfg<TPR>;
   const int64_t grid = (a.rows + Cfg::kRowsPerBlock - 1) / Cfg::kRowsPerBlock;
   if (grid > 0x7fffffff) return KRSI_ERR_UNSUPPORTED;
-  KRSI_CUDA_TRY(launch_pdl(add_rmsnorm_kernel<XT, WT, TPR, VEC, NCH, OUT>, dim3((unsigned)grid), dim3(Cfg::kThreads),
-                           0, s, a));
+  KRSI_CUDA_TRY(launch_pdl(add_rmsnorm_kernel<XT, WF32, TPR, VEC, NCH, OUT>, dim3((unsigned)grid), dim3(Cfg::kThreads), 0, s, a));
   return KRSI_OK;
 }
 
-template <int XT, int WT, int VEC, int OUT>
-int run_plan(const NormPlan& p, const NormArgs& a, cudaStream_t s) {
-#define KRSI_RUN(TPR, NCH) if (p.tpr == TPR && p.nch == NCH) return run<XT, WT, TPR, VEC, NCH, OUT>(a, s)
-  KRSI_RUN(32, 1); KRSI_RUN(32, 2); KRSI_RUN(32, 3); KRSI_RUN(32, 4); KRSI_RUN(32, 5); KRSI_RUN(32, 6);
-  KRSI_RUN(32, 8); KRSI_RUN(128, 3); KRSI_RUN(128, 4); KRSI_RUN(128, 6); KRSI_RUN(128, 8); KRSI_RUN(512, 4);
-  KRSI_RUN(512, 8);
-  if constexpr (VEC == 1) { KRSI_RUN(1024, 16); }
-#undef KRSI_RUN
+template <int XT, bool WF32, int OUT>
+int run_packets(int vec, const NormArgs& a, cudaStream_t s) {
+  const int64_t packets = ((int64_t)a.n + vec - 1) / vec;
+#define KRSI_RUN8(TPR, NCH) if (packets <= TPR * NCH) return run<XT, WF32, TPR, 8, NCH, OUT>(a, s);
+#define KRSI_RUN4(TPR, NCH) if (packets <= TPR * NCH) return run<XT, WF32, TPR, 4, NCH, OUT>(a, s);
+#define KRSI_RUN1(TPR, NCH) if (packets <= TPR * NCH) return run<XT, WF32, TPR, 1, NCH, OUT>(a, s);
+  if (vec == 8) {
+    if constexpr (XT != KRSI_F32) { KRSI_PLANS8(KRSI_RUN8) }
+  } else if (a.n > 16384) {
+    return KRSI_ERR_UNSUPPORTED;
+  } else if (vec == 4) {
+    KRSI_PLANS4(KRSI_RUN4)
+  } else {
+    KRSI_PLANS1(KRSI_RUN1)
+  }
+#undef KRSI_RUN8
+#undef KRSI_RUN4
+#undef KRSI_RUN1
   return KRSI_ERR_UNSUPPORTED;
 }
 
 template <int OUT>
-int dispatch(int x_dtype, int w_dtype, const NormPlan& p, const NormArgs& a, cudaStream_t s) {
-#define KRSI_DT(XT, WT, VW)            \
-  if (x_dtype == XT && w_dtype == WT)  \
-    return p.vec == 1 ? run_plan<XT, WT, 1, OUT>(p, a, s) : run_plan<XT, WT, VW, OUT>(p, a, s)
-  KRSI_DT(KRSI_F32, KRSI_F32, 4);
-  KRSI_DT(KRSI_BF16, KRSI_BF16, 8);
-  KRSI_DT(KRSI_F16, KRSI_F16, 8);
-  if constexpr (OUT != kOutQuantise) {
-    KRSI_DT(KRSI_BF16, KRSI_F32, 8);
-    KRSI_DT(KRSI_F16, KRSI_F32, 8);
+int dispatch(int x_dtype, int w_dtype, int vec, const NormArgs& a, cudaStream_t s) {
+  const bool f32 = w_dtype == KRSI_F32;
+  switch (x_dtype) {
+    case KRSI_F32: return run_packets<KRSI_F32, true, OUT>(vec, a, s);
+    case KRSI_BF16: return f32 ? run_packets<KRSI_BF16, true, OUT>(vec, a, s) : run_packets<KRSI_BF16, false, OUT>(vec, a, s);
+    default: return f32 ? run_packets<KRSI_F16, true, OUT>(vec, a, s) : run_packets<KRSI_F16, false, OUT>(vec, a, s);
   }
-#undef KRSI_DT
-  return KRSI_ERR_UNSUPPORTED;
 }
-
-bool dtype_ok(int d) { return d == KRSI_F32 || d == KRSI_BF16 || d == KRSI_F16; }
 
 }  // namespace
 }  // namespace krsi
@@ -280,12 +250,9 @@ extern "C" int krsi_add_rmsnorm_fwd(const void* x, const void* res, const void* 
   if (rows == 0) return KRSI_OK;
   KRSI_CHECK_ARG(n > 0 && x && w && y && rstd && (!res || z));
   if (n > 0x7fffffff) return KRSI_ERR_UNSUPPORTED;
-  const int vw = x_dtype == KRSI_F32 ? 4 : 8;
-  const bool vec_ok = n % vw == 0 && aligned16(x) && aligned16(y) && aligned16(w) &&
-                      (!res || (aligned16(res) && aligned16(z)));
-  NormPlan p;
-  if (!plan(n, vec_ok ? vw : 1, &p)) return KRSI_ERR_UNSUPPORTED;
-  return dispatch<kOutRow>(x_dtype, w_dtype, p, NormArgs{x, res, w, z, y, rstd, rows, 0, (int)n, eps}, stream);
+  if (!types_ok(x_dtype, w_dtype)) return KRSI_ERR_UNSUPPORTED;
+  return dispatch<kOutRow>(x_dtype, w_dtype, packet_of(x_dtype, n, {x, y, w, res, res ? z : nullptr}),
+                           NormArgs{x, res, w, z, y, rstd, rows, 0, (int)n, eps}, stream);
 }
 
 extern "C" int krsi_add_rmsnorm_q8_fwd(const void* x, const void* res, const void* w, void* z, void* q,
@@ -295,12 +262,10 @@ extern "C" int krsi_add_rmsnorm_q8_fwd(const void* x, const void* res, const voi
   if (rows == 0) return KRSI_OK;
   KRSI_CHECK_ARG(n > 0 && x && w && q && scale && (!res || z) && q_stride >= n);
   if (n > 0x7fffffff) return KRSI_ERR_UNSUPPORTED;
-  const int vw = x_dtype == KRSI_F32 ? 4 : 8;
-  const bool vec_ok = n % vw == 0 && aligned16(x) && aligned16(w) && aligned16(q) && q_stride % 16 == 0 &&
-                      (!res || (aligned16(res) && aligned16(z)));
-  NormPlan p;
-  if (!plan(n, vec_ok ? vw : 1, &p)) return KRSI_ERR_UNSUPPORTED;
-  return dispatch<kOutQ8>(x_dtype, w_dtype, p, NormArgs{x, res, w, z, q, scale, rows, q_stride, (int)n, eps}, stream);
+  const bool q_ok = aligned16(q) && q_stride % 16 == 0;
+  if (!types_ok(x_dtype, w_dtype)) return KRSI_ERR_UNSUPPORTED;
+  return dispatch<kOutQ8>(x_dtype, w_dtype, q_ok ? packet_of(x_dtype, n, {x, w, res, res ? z : nullptr}) : 1,
+                          NormArgs{x, res, w, z, q, scale, rows, q_stride, (int)n, eps}, stream);
 }
 
 extern "C" int krsi_quantise_rows(const void* x, void* q, int64_t q_stride, float* scale, int64_t rows, int64_t n,
@@ -309,10 +274,7 @@ extern "C" int krsi_quantise_rows(const void* x, void* q, int64_t q_stride, floa
   if (rows == 0) return KRSI_OK;
   KRSI_CHECK_ARG(n > 0 && x && q && scale && q_stride >= n);
   if (n > 0x7fffffff) return KRSI_ERR_UNSUPPORTED;
-  const int vw = x_dtype == KRSI_F32 ? 4 : 8;
-  const bool vec_ok = n % vw == 0 && aligned16(x) && aligned16(q) && q_stride % 16 == 0;
-  NormPlan p;
-  if (!plan(n, vec_ok ? vw : 1, &p)) return KRSI_ERR_UNSUPPORTED;
-  return dispatch<kOutQuantise>(x_dtype, x_dtype, p,
-                                NormArgs{x, nullptr, nullptr, nullptr, q, scale, rows, q_stride, (int)n, 0.f}, stream);
+  const bool q_ok = aligned16(q) && q_stride % 16 == 0;
+  return dispatch<kOutQ8>(x_dtype, x_dtype, q_ok ? packet_of(x_dtype, n, {x}) : 1,
+                          NormArgs{x, nullptr, nullptr, nullptr, q, scale, rows, q_stride, (int)n, 0.f}, stream);
 }

@@ -503,8 +503,14 @@ at::Tensor linear_ce_finish(const at::Tensor& grad, const at::Tensor& g_in, cons
 }
 
 // ---------------------------------------------------------------- residual addition and RMSNorm
-// The arguments of the three entry points below; a tensor that starts off 16 bytes is taken as it is (the kernels
-// have a path for it).
+// Contiguous, and rows of whole 16 bytes on 16 bytes: a view that starts elsewhere is copied, so that the bits of a
+// result do not depend on where an operand lies.
+at::Tensor packed(const at::Tensor& t) {
+  auto c = t.contiguous();
+  const bool whole = c.dim() > 0 && c.size(-1) * c.element_size() % 16 == 0;
+  return whole && (reinterpret_cast<uintptr_t>(c.data_ptr()) & 15u) != 0 ? c.clone() : c;
+}
+// The arguments of the entry points below.
 struct NormCall {
   at::Tensor x, res, w;
 };
@@ -515,13 +521,13 @@ NormCall norm_call(const at::Tensor& x_in, const c10::optional<at::Tensor>& res_
   check_same_device(x_in, w_in, what);
   TORCH_CHECK(x_in.dim() == 2, what, ": x2d must be 2-D, got ", x_in.dim(), "-D");
   TORCH_CHECK(w_in.dim() == 1 && w_in.size(0) == x_in.size(1), what, ": w must be [", x_in.size(1), "]");
-  NormCall c{x_in.contiguous(), {}, w_in.contiguous()};
+  NormCall c{packed(x_in), {}, packed(w_in)};
   if (res_in.has_value() && res_in->defined()) {
     check_cuda(*res_in, "res");
     check_same_device(x_in, *res_in, what);
     TORCH_CHECK(res_in->sizes() == x_in.sizes() && res_in->scalar_type() == x_in.scalar_type(), what,
                 ": res must have x2d's shape and dtype");
-    c.res = res_in->contiguous();
+    c.res = packed(*res_in);
   }
   return c;
 }
@@ -548,13 +554,32 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> add_rmsnorm_fwd(const at::Tensor&
 std::tuple<at::Tensor, at::Tensor> add_rmsnorm_bwd(const c10::optional<at::Tensor>& gy,
                                                    const c10::optional<at::Tensor>& gz, const at::Tensor& z,
                                                    const at::Tensor& w, const at::Tensor& rstd) {
+  check_cuda(z, "z");
   const bool have_z = gz.has_value() && gz->defined();
+  TORCH_CHECK(z.dim() == 2 && w.dim() == 1 && w.size(0) == z.size(1), "add_rmsnorm_bwd: z must be [rows, n] and w [n]");
+  TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.numel() == z.size(0), "add_rmsnorm_bwd: bad rstd");
+  TORCH_CHECK(!have_z || gz->sizes() == z.sizes(), "add_rmsnorm_bwd: gz must match z");
   if (!gy.has_value() || !gy->defined())
     return {have_z ? gz->to(z.scalar_type()) : at::zeros_like(z), at::zeros_like(w)};
-  if (!have_z) return rmsnorm_bwd(*gy, z, w, rstd);
-  auto g = gz->to(z.scalar_type()).contiguous();
-  if ((reinterpret_cast<uintptr_t>(g.data_ptr()) & 15u) != 0) g = g.clone();
-  return rmsnorm_bwd_add(*gy, z, w, rstd, g);
+  TORCH_CHECK(gy->sizes() == z.sizes(), "add_rmsnorm_bwd: gy must match z");
+  c10::cuda::CUDAGuard guard(z.device());
+  auto zc = packed(z), wc = packed(w), rc = rstd.contiguous();
+  auto g = packed(gy->to(z.scalar_type()));
+  at::Tensor g2 = have_z ? packed(gz->to(z.scalar_type())) : at::Tensor();
+  for (const at::Tensor* t : {&g, &wc, &rc}) check_same_device(z, *t, "add_rmsnorm_bwd");
+  if (have_z) check_same_device(z, g2, "add_rmsnorm_bwd");
+  const int64_t rows = zc.size(0), n = zc.size(1);
+  auto dz = at::empty({rows, n}, zc.options());
+  auto dw = at::empty({n}, wc.options());
+  size_t ws = 0;
+  check_rc(krsi_add_rmsnorm_bwd_workspace_size(rows, n, &ws), "krsi_add_rmsnorm_bwd_workspace_size");
+  auto wsp = workspace(zc, ws);
+  check_rc(krsi_add_rmsnorm_bwd(g.data_ptr(), have_z ? g2.data_ptr() : nullptr, zc.data_ptr(), wc.data_ptr(),
+                                rc.data_ptr<float>(), dz.data_ptr(), dw.data_ptr(), wsp.data_ptr(),
+                                (size_t)wsp.numel(), rows, n, krsi_dtype_of(zc), krsi_dtype_of(wc),
+                                at::cuda::getCurrentCUDAStream()),
+           "krsi_add_rmsnorm_bwd");
+  return {dz, dw};
 }
 
 // Rows of 8-bit values, each row padded to whole 16 bytes (what a TMA copy of them needs).
@@ -586,7 +611,7 @@ std::tuple<at::Tensor, at::Tensor> quantise_rows(const at::Tensor& x_in) {
   check_cuda(x_in, "x2d");
   TORCH_CHECK(x_in.dim() == 2, "quantise: x2d must be 2-D, got ", x_in.dim(), "-D");
   c10::cuda::CUDAGuard guard(x_in.device());
-  auto x = x_in.contiguous();
+  auto x = packed(x_in);
   const int64_t rows = x.size(0), n = x.size(1);
   auto q = empty_q8(rows, n, x);
   auto scale = at::empty({rows}, x.options().dtype(at::kFloat));
@@ -1014,4 +1039,5 @@ TORCH_LIBRARY_IMPL(krsi, AutogradCUDA, m) {
   m.impl("add_rmsnorm_q8", &add_rmsnorm_q8_autograd);
   m.impl("quantise_rows", &quantise_rows_autograd);
   m.impl("linear_q8", &linear_q8_autograd);
+  m.impl("adamw_step", torch::CppFunction::makeFallthrough());   // an update is no part of a graph
 }

@@ -14,7 +14,7 @@ gradient, and refuses to be called where one could be asked for.
 
 A row with a value that is not finite has a norm, or a scale, that is not finite either.
 add_rmsnorm's autograd node is in csrc/torch_ext.cpp (krsi::add_rmsnorm).
-Kernels: kernel-rsi_b200/csrc/add_rmsnorm.cu, and csrc/rmsnorm.cu for the backward; C ABI: include/krsi_b200.h.
+Kernels: kernel-rsi_b200/csrc/add_rmsnorm.cu; C ABI: include/krsi_b200.h.
 """
 import sys
 from pathlib import Path
