@@ -8,9 +8,17 @@
 // K-major tiles of 128 values), warp 1 the TMEM owner and issuer of tcgen05.mma kind::f8f6f4 (32 values of K an
 // instruction), warps 4-11 the epilogue.  Two accumulators alternate, so a tile's epilogue runs beside the next
 // tile's MMAs.
-//   more than 128 rows   linear_q8_pair_kernel: CTA pairs (cta_group::2) on tiles of 256 rows x 256 columns
-//   up to 128 rows       linear_q8_kernel: one CTA on tiles of 128 rows x 64 columns (the weight's read bounds it:
-//                        narrow tiles spread it over the SMs)
+//   up to 128 rows    linear_q8_kernel: one CTA on tiles of 128 rows x 64 columns (the weight's read bounds it:
+//                     narrow tiles spread it over the SMs)
+//   more              linear_q8_pair_kernel: CTA pairs (cta_group::2) on tiles of 256 rows x up to 256 columns, all
+//                     columns of the same rows at the same time, so that out is written in whole rows
+//
+// What bounds it (32768 x 1152 x 9216 to bf16, 696 GFLOP and 604 MB of output: 299 us, 2.33 PFLOP/s): the output's
+// way out and the power cap.  Without stores the same kernel takes 234 us; writing 604 MB alone takes 156 (3.9 TB/s),
+// and the two do not hide each other wholly.  Measured on the way: boxes of 64 bytes a row, one a warp, in place of
+// two of 128: 312; ordinary stores of the same boxes: 317; the weight's K blocks kept in shared memory while a pair
+// walks down the rows (a third of the L2's reads): 301, and 130 against 116 for 3456 columns, for the shorter ring that
+// leaves; pairs walking along the columns of rows of their own: 355.
 // Every wait is bounded (watchdog.cuh); a stalled pipeline ends the CTA with an error word.
 #include <atomic>
 
@@ -32,17 +40,34 @@ constexpr int kBK = 128;                    // values of K per stage: one 128-by
 constexpr int kThreads = 384;
 constexpr int kEpiWarp0 = 4, kEpiWarps = 8;
 constexpr uint32_t kATile = kBM * kBK;      // 16 KB
-constexpr uint32_t kBoxBytes = 32 * 64;     // one warp's staged [32 rows x 64 bytes] of the output
 
 struct Q8Args {
+  CUtensorMap omap;   // out, in an epilogue warp's boxes, where its rows start on 16 bytes
   const float* scale;
   const float* wscale;
   void* out;
   int rows, M;
+  int bn;             // columns of a tile
   int n_ctiles;       // column tiles
   int n_tiles;        // row tiles x column tiles
   int n_kb;           // K blocks
+  bool vec_scale;     // wscale starts on 16 bytes
   uint32_t spin_limit;
+};
+
+// The tiles of one CTA or pair: every `stride`th, columns first.
+struct Tiles {
+  const Q8Args& a;
+  const int stride;
+  int tile, row = 0, col = 0;
+  __device__ __forceinline__ Tiles(const Q8Args& args, int first, int step) : a(args), stride(step), tile(first - step) {}
+  __device__ __forceinline__ bool next() {   // to the next tile (at first: to the first one)
+    tile += stride;
+    if (tile >= a.n_tiles) return false;
+    row = tile / a.n_ctiles;
+    col = tile % a.n_ctiles;
+    return true;
+  }
 };
 
 // kind::f8f6f4, both operands e4m3 (format 0), K-major, fp32 sums: the bit layout is idesc_f16's.
@@ -65,29 +90,34 @@ __device__ __forceinline__ void mma_q8_pair_e(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
-// The epilogue of one warp: 32 rows (TMEM lanes) x `cols` columns of each of the CTA's tiles, one output box of
-// 64 bytes a row at a time.  `row_of(i)`, `col_of(i)`: the tile's first row and column for this CTA.
-// TMA: boxes leave by TMA stores; else (rows of out that do not start on 16 bytes) by coalesced stores.
-template <int DT, bool TMA, typename RowOf, typename ColOf, typename Release>
+// The epilogue of one warp: 32 rows (TMEM lanes) x `cols` columns of each of the CTA's tiles, ROWB bytes of each row at
+// a time.  A lane has a row of the accumulator, and writes its packets to one of the warp's two boxes in shared memory
+// (rows of ROWB bytes, swizzled).  VEC, rows of out that start on 16 bytes: boxes leave by TMA stores; else by stores
+// value by value.  `row_of(t)`: the first row of a tile for this CTA.
+template <int DT, bool VEC, int ROWB, typename RowOf, typename Release>
 __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int acc_cols, int cols, int warp, int lane,
-                                            int my_tiles, uint64_t* acc_full, volatile int* abort_flag,
-                                            const CUtensorMap* omap, const Q8Args& a, RowOf row_of, ColOf col_of,
-                                            Release release) {
-  using E = Elem<DT>;
-  using T = typename E::T;
-  constexpr int kCols = 64 / (int)sizeof(T);   // columns of a box: 32, or 16 in fp32
+                                            Tiles tiles, uint64_t* acc_full, volatile int* abort_flag, const Q8Args& a,
+                                            RowOf row_of, Release release) {
+  using T = typename Elem<DT>::T;
+  constexpr int kPer = 16 / (int)sizeof(T);          // values of a packet
+  constexpr int kStep = ROWB / (int)sizeof(T);       // columns of a box
+  constexpr int kLoad = kStep < 32 ? kStep : 32;     // columns read from TMEM at a time
   const int ew = warp - kEpiWarp0;
-  const int quarter = ew % 4, part = ew / 4;   // TMEM lane quarter; which `cols` of the tile's columns
+  const int quarter = ew % 4, part = ew / 4;  // TMEM lane quarter; which `cols` of the tile's columns
   const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
-  uint8_t* box = boxes + ew * kBoxBytes;
-  // 16-byte packet p of row r in the 64-byte swizzle
-  auto packet = [&](int r, int p) { return box + r * 64 + ((p ^ ((r >> 1) & 3)) << 4); };
+  uint8_t* box = boxes + ew * 2 * (32 * ROWB);
+  // packet p of row r: the 128- or 64-byte swizzle
+  auto packet = [&](uint8_t* b, int r, int p) {
+    return b + r * ROWB + ((ROWB == 128 ? p ^ (r & 7) : p ^ ((r >> 1) & 3)) << 4);
+  };
+  int turn = 0;
   bool ok = true;
-  for (int i = 0; i < my_tiles; ++i) {
+  for (int i = 0; tiles.next(); ++i) {
     const int acc = i & 1;
-    const int row0 = row_of(i) + quarter * 32;
-    const int c_base = col_of(i) + part * cols;
+    const int row0 = row_of(tiles) + quarter * 32;
+    const int c_base = tiles.col * a.bn + part * cols;
     const float s = row0 + lane < a.rows ? __ldg(a.scale + row0 + lane) : 0.f;
+    const uint64_t s2 = f2_pack(s, s);
     if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], (i >> 1) & 1, abort_flag, a.spin_limit))) {
       ok = false;
       break;
@@ -95,86 +125,103 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
     tc_fence_after();
     const uint32_t acc_addr = tmem + lane_addr + acc * acc_cols + part * cols;
 #pragma unroll 1
-    for (int c0 = 0; c0 < cols; c0 += kCols) {
-      uint32_t v[kCols];
-      if constexpr (kCols == 32) tmem_ld32(acc_addr + c0, v);
-      else tmem_ld16(acc_addr + c0, v);
-      const int col = c_base + c0;
-      float ws[kCols];
-      if (col + kCols <= a.M) {
+    for (int c0 = 0; c0 < cols; c0 += kStep, turn ^= 1) {
+      uint8_t* out_box = box + turn * (32 * ROWB);
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) ws[e] = __ldg(a.wscale + col + e);
-      } else {
+      for (int h = 0; h < kStep; h += kLoad) {
+        const int col = c_base + c0 + h;
+        uint32_t v[kLoad];
+        if constexpr (kLoad == 32) tmem_ld32(acc_addr + c0 + h, v);
+        else tmem_ld16(acc_addr + c0 + h, v);
+        float ws[kLoad];
+        if (a.vec_scale && col + kLoad <= a.M) {
 #pragma unroll
-        for (int e = 0; e < kCols; ++e) ws[e] = col + e < a.M ? __ldg(a.wscale + col + e) : 0.f;
-      }
-      tmem_wait_ld();
-      if (c0 + kCols >= cols) {                  // the accumulator has been read: the MMA may reuse it
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) release(acc);
-      }
-      if (TMA) {
-        if (lane == 0) bulk_wait_read_all();     // the previous box has been read
-        __syncwarp();
-      }
-#pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        uint32_t u[4];
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          if constexpr (DT == KRSI_F32) {
-            const int e = 4 * p + k;
-            u[k] = __float_as_uint(__uint_as_float(v[e]) * s * ws[e]);
-          } else {
-            const int e = 8 * p + 2 * k;
-            const float lo = __uint_as_float(v[e]) * s * ws[e], hi = __uint_as_float(v[e + 1]) * s * ws[e + 1];
-            u[k] = DT == KRSI_F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+          for (int e = 0; e < kLoad; e += 4) {
+            const float4 w4 = __ldg(reinterpret_cast<const float4*>(a.wscale + col + e));
+            ws[e] = w4.x; ws[e + 1] = w4.y; ws[e + 2] = w4.z; ws[e + 3] = w4.w;
           }
+        } else {
+#pragma unroll
+          for (int e = 0; e < kLoad; ++e) ws[e] = col + e < a.M ? __ldg(a.wscale + col + e) : 0.f;
         }
-        *reinterpret_cast<uint4*>(packet(lane, p)) = make_uint4(u[0], u[1], u[2], u[3]);
+        tmem_wait_ld();
+        if (c0 + h + kLoad >= cols) {              // the accumulator has been read: the MMA may reuse it
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) release(acc);
+        }
+        if (VEC && h == 0) {
+          if (lane == 0) bulk_wait_read_but_one();   // the box before the last one has been read
+          __syncwarp();
+        }
+#pragma unroll
+        for (int p = 0; p < kLoad / kPer; ++p) {
+          uint32_t u[4];
+#pragma unroll
+          for (int k = 0; k < kPer / 2; ++k) {
+            const int e = p * kPer + 2 * k;
+            float lo, hi;
+            f2_unpack(f2_mul(f2_mul(f2_pack(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), s2),
+                             f2_pack(ws[e], ws[e + 1])), lo, hi);
+            if constexpr (DT == KRSI_F32) {
+              u[2 * k] = __float_as_uint(lo);
+              u[2 * k + 1] = __float_as_uint(hi);
+            } else {
+              u[k] = DT == KRSI_F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
+            }
+          }
+          *reinterpret_cast<uint4*>(packet(out_box, lane, h / kPer + p)) = make_uint4(u[0], u[1], u[2], u[3]);
+        }
       }
-      if constexpr (TMA) {
+      const int col = c_base + c0;
+      if constexpr (VEC) {
         fence_async_shared();
         __syncwarp();
         if (lane == 0 && col < a.M && row0 < a.rows) {   // the map clips rows >= rows and columns >= M
-          tma_store_2d(omap, box, col, row0);
+          tma_store_2d(&a.omap, out_box, col, row0);
           bulk_commit_group();
         }
-      } else {
+      } else {               // value by value, consecutive lanes on consecutive columns
         __syncwarp();
-        constexpr int kRowsAtOnce = 32 / kCols;
-        const int r_lane = lane / kCols, e = lane % kCols;
-        for (int r = r_lane; r < 32; r += kRowsAtOnce) {
-          if (row0 + r < a.rows && col + e < a.M) {
-            constexpr int kPer = 16 / (int)sizeof(T);
-            const T val = reinterpret_cast<const T*>(packet(r, e / kPer))[e % kPer];
-            static_cast<T*>(a.out)[(int64_t)(row0 + r) * a.M + col + e] = val;
-          }
+        constexpr int kWide = kStep < 32 ? kStep : 32, kRowsAtOnce = 32 / kWide, kTurns = 32 / kRowsAtOnce;
+        const int r0 = lane / kWide;
+#pragma unroll
+        for (int h = 0; h < kStep; h += kWide) {
+          const int e = h + lane % kWide;
+          T* out = static_cast<T*>(a.out) + (int64_t)(row0 + r0) * a.M + col + e;
+          const int left = col + e < a.M ? a.rows - row0 - r0 : 0;
+          T val[kTurns];
+#pragma unroll
+          for (int k = 0; k < kTurns; ++k)
+            val[k] = reinterpret_cast<const T*>(packet(out_box, r0 + k * kRowsAtOnce, e / kPer))[e % kPer];
+#pragma unroll
+          for (int k = 0; k < kTurns; ++k)
+            if (k * kRowsAtOnce < left) out[(int64_t)k * kRowsAtOnce * a.M] = val[k];
         }
         __syncwarp();
       }
     }
   }
-  if (TMA && lane == 0) bulk_wait_all();   // every store has completed before the CTA exits
+  if (VEC && lane == 0) bulk_wait_all();   // every store has completed before the CTA exits
   return ok;
 }
 
 // ---------------------------------------------------------------- up to 128 rows: one CTA, narrow tiles
 constexpr int kOneBN = 64;
 constexpr int kOneStages = 8;
+constexpr int kOneRowB = 64;                                         // bytes of a row in an output box
 constexpr uint32_t kOneStageBytes = kATile + kOneBN * kBK;           // 24 KB
 constexpr uint32_t kOneBoxOff = kOneStages * kOneStageBytes;
-constexpr uint32_t kOneBarOff = kOneBoxOff + kEpiWarps * kBoxBytes;
+constexpr uint32_t kOneBarOff = kOneBoxOff + kEpiWarps * 2 * 32 * kOneRowB;
 constexpr uint32_t kOneMiscOff = kOneBarOff + (2 * kOneStages + 2 + 2 + 1) * 8;
 constexpr uint32_t kOneSmem = kOneMiscOff + 16 + 1024;               // + slack for the 1024-byte alignment
 constexpr uint32_t kOneTmemCols = 2 * kOneBN;
 static_assert(kOneSmem <= 232448, "shared memory budget");
 
-template <int DT, bool TMA>
+template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap,
-                 const __grid_constant__ CUtensorMap omap, const Q8Args a) {
+                 const __grid_constant__ Q8Args a) {
   pdl_enter();   // before any global access and before claiming TMEM
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -187,8 +234,7 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kOneMiscOff + 4);
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const int my_tiles = (int)blockIdx.x < a.n_tiles ? (a.n_tiles - 1 - (int)blockIdx.x) / (int)gridDim.x + 1 : 0;
-  auto tile_of = [&](int i) { return (int)blockIdx.x + i * (int)gridDim.x; };
+  Tiles tiles(a, blockIdx.x, gridDim.x);
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kOneStages; ++s) {
@@ -220,9 +266,8 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     // ------------------------------------------------------------ TMA producer
     bool ok = true;
     int it = 0;
-    for (int i = 0; i < my_tiles && ok; ++i) {
-      const int t = tile_of(i);
-      const int m0 = (t / a.n_ctiles) * kBM, n0 = (t % a.n_ctiles) * kOneBN;
+    while (ok && tiles.next()) {
+      const int m0 = tiles.row * kBM, n0 = tiles.col * kOneBN;
       for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
         const int s = it % kOneStages;
         if (it >= kOneStages && !__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((it / kOneStages) - 1) & 1,
@@ -252,7 +297,7 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     const uint64_t desc0 = kmajor_sw128(smem_u32(smem));
     bool ok = true;
     int it = 0;
-    for (int i = 0; i < my_tiles && ok; ++i) {
+    for (int i = 0; ok && tiles.next(); ++i) {
       const int acc = i & 1;
       if (i >= 2 && !wait(&acc_empty[acc], ((i >> 1) - 1) & 1)) {
         ok = false;
@@ -275,16 +320,15 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
       if (!ok) break;
       mma_commit_e(&acc_full[acc]);
     }
-    if (!ok && my_tiles > 0) watchdog_fire(kWdQ8Mma);
+    if (!ok) watchdog_fire(kWdQ8Mma);
     mma_commit_e(drain);   // every MMA issued above has completed before TMEM is released
     for (uint32_t i = 0; i < a.spin_limit && !mbar_try_wait(drain, 0); ++i) {
     }
   } else if (warp >= kEpiWarp0) {
     // ------------------------------------------------------------ epilogue
-    const bool ok = q8_epilogue<DT, TMA>(
-        smem + kOneBoxOff, tmem, kOneBN, kOneBN / 2, warp, lane, my_tiles, acc_full, abort_flag, &omap, a,
-        [&](int i) { return (tile_of(i) / a.n_ctiles) * kBM; },
-        [&](int i) { return (tile_of(i) % a.n_ctiles) * kOneBN; }, [&](int acc) { mbar_arrive(&acc_empty[acc]); });
+    const bool ok = q8_epilogue<DT, VEC, kOneRowB>(
+        smem + kOneBoxOff, tmem, kOneBN, kOneBN / 2, warp, lane, tiles, acc_full, abort_flag, a,
+        [&](const Tiles& t) { return t.row * kBM; }, [&](int acc) { mbar_arrive(&acc_empty[acc]); });
     if (!ok) watchdog_fire(kWdQ8Epilogue);
   }
 
@@ -295,39 +339,38 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
 }
 
 // ---------------------------------------------------------------- CTA pairs (cta_group::2)
-// Each CTA loads its own 128 rows of q and half of the 256 rows of wq; the even CTA issues M256 N256 K32 MMAs that
-// read both CTAs' shared memory and accumulate into both CTAs' TMEM.
+// Each CTA loads its own 128 rows of q and half of the tile's rows of wq; the even CTA issues M256 K32 MMAs that read
+// both CTAs' shared memory and accumulate into both CTAs' TMEM.
 constexpr int kPairBN = 256;
-constexpr int kPairStages = 6;
+constexpr int kPairStages = 5;
 constexpr uint32_t kPairStageBytes = 2 * kATile;                     // 32 KB
+constexpr int kPairRowB = 128;                                       // bytes of a row in an output box
 constexpr uint32_t kPairBoxOff = kPairStages * kPairStageBytes;
-constexpr uint32_t kPairBarOff = kPairBoxOff + kEpiWarps * kBoxBytes;
+constexpr uint32_t kPairBarOff = kPairBoxOff + kEpiWarps * 2 * 32 * kPairRowB;
 constexpr uint32_t kPairMiscOff = kPairBarOff + (2 * kPairStages + 2 + 2 + 1) * 8;
 constexpr uint32_t kPairSmem = kPairMiscOff + 16 + 1024;
 constexpr uint32_t kPairTmemCols = 2 * kPairBN;
 static_assert(kPairSmem <= 232448, "shared memory budget");
 
-template <int DT, bool TMA>
+template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 1)
 linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant__ CUtensorMap wmap,
-                      const __grid_constant__ CUtensorMap omap, const Q8Args a) {
+                      const __grid_constant__ Q8Args a) {
   pdl_enter();   // before any global access and before claiming TMEM
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairBarOff);   // used in the even CTA
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + kPairBarOff);   // (used in the even CTA)
   uint64_t* empty = full + kPairStages;
   uint64_t* acc_full = empty + kPairStages;
-  uint64_t* acc_empty = acc_full + 2;                                 // used in the even CTA
+  uint64_t* acc_empty = acc_full + 2;                                 // (used in the even CTA)
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kPairMiscOff);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + kPairMiscOff + 4);
-
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   const uint32_t rank = cluster_ctarank();
   const bool even = rank == 0;
-  const int pair = (int)blockIdx.x / 2, n_pairs = (int)gridDim.x / 2;
-  const int my_tiles = pair < a.n_tiles ? (a.n_tiles - 1 - pair) / n_pairs + 1 : 0;
-  auto tile_of = [&](int i) { return pair + i * n_pairs; };
+  Tiles tiles(a, blockIdx.x / 2, gridDim.x / 2);
+  const uint32_t w_bytes = (uint32_t)(a.bn / 2) * kBK;   // one CTA's half of the weight's K block
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < kPairStages; ++s) {
@@ -354,26 +397,27 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
   cluster_sync();   // both CTAs' barriers initialised and TMEM allocated before either signals the other
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  auto wait = [&](uint64_t* bar, uint32_t parity) {   // whole warps
+    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit));
+  };
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
     bool ok = true;
     int it = 0;
-    for (int i = 0; i < my_tiles && ok; ++i) {
-      const int t = tile_of(i);
-      const int m0 = (t / a.n_ctiles) * (2 * kBM) + (int)rank * kBM;
-      const int n0 = (t % a.n_ctiles) * kPairBN + (int)rank * (kPairBN / 2);
+    while (ok && tiles.next()) {
+      const int m0 = tiles.row * (2 * kBM) + (int)rank * kBM;
+      const int n0 = tiles.col * a.bn + (int)rank * (a.bn / 2);
       for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
         const int s = it % kPairStages;
-        if (it >= kPairStages && !__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((it / kPairStages) - 1) & 1,
-                                                                            abort_flag, a.spin_limit))) {
+        if (it >= kPairStages && !wait(&empty[s], ((it / kPairStages) - 1) & 1)) {
           ok = false;
           break;
         }
         if (lane == 0) {
           uint8_t* st = smem + s * kPairStageBytes;
           const uint32_t bar = mapa_shared(&full[s], 0);
-          if (even) mbar_arrive_expect_tx(&full[s], 2 * kPairStageBytes);
+          if (even) mbar_arrive_expect_tx(&full[s], 2 * (kATile + w_bytes));
           tma_load_2d_pair(st, &qmap, bar, kb * kBK, m0);
           tma_load_2d_pair(st + kATile, &wmap, bar, kb * kBK, n0);
         }
@@ -386,14 +430,11 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     }
   } else if (warp == 1 && even) {
     // ------------------------------------------------------------ MMA issuer (even CTA, elected lane)
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit));
-    };
-    constexpr uint32_t idesc = idesc_e4m3(2 * kBM, kPairBN);
+    const uint32_t idesc = idesc_e4m3(2 * kBM, (uint32_t)a.bn);
     const uint64_t desc0 = kmajor_sw128(smem_u32(smem));
     bool ok = true;
     int it = 0;
-    for (int i = 0; i < my_tiles && ok; ++i) {
+    for (int i = 0; ok && tiles.next(); ++i) {
       const int acc = i & 1;
       if (i >= 2 && !wait(&acc_empty[acc], ((i >> 1) - 1) & 1)) {
         ok = false;
@@ -418,16 +459,15 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
       mma_commit_pair_e(mapa_shared(&acc_full[acc], 0));
       mma_commit_pair_e(mapa_shared(&acc_full[acc], 1));
     }
-    if (!ok && my_tiles > 0) watchdog_fire(kWdQ8Mma);
+    if (!ok) watchdog_fire(kWdQ8Mma);
     mma_commit_pair_e(mapa_shared(drain, 0));
     for (uint32_t i = 0; i < a.spin_limit && !mbar_try_wait(drain, 0); ++i) {
     }
   } else if (warp >= kEpiWarp0) {
     // ------------------------------------------------------------ epilogue (both CTAs, own rows)
-    const bool ok = q8_epilogue<DT, TMA>(
-        smem + kPairBoxOff, tmem, kPairBN, kPairBN / 2, warp, lane, my_tiles, acc_full, abort_flag, &omap, a,
-        [&](int i) { return (tile_of(i) / a.n_ctiles) * (2 * kBM) + (int)rank * kBM; },
-        [&](int i) { return (tile_of(i) % a.n_ctiles) * kPairBN; },
+    const bool ok = q8_epilogue<DT, VEC, kPairRowB>(
+        smem + kPairBoxOff, tmem, kPairBN, a.bn / 2, warp, lane, tiles, acc_full, abort_flag, a,
+        [&](const Tiles& t) { return t.row * (2 * kBM) + (int)rank * kBM; },
         [&](int acc) {
           if (even) mbar_arrive(&acc_empty[acc]);
           else mbar_arrive_cluster(mapa_shared(&acc_empty[acc], 0));
@@ -474,14 +514,14 @@ cudaLaunchConfig_t pair_config(cudaLaunchAttribute* attr, int clusters, cudaStre
 }
 
 // Clusters of two that fit on the device at once (0: none can be launched), per device, queried once.
-template <int DT, bool TMA>
+template <int DT, bool VEC>
 int pair_clusters() {
   static std::atomic<int> cached[64];   // clusters + 1 once queried; races only repeat the query
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
   int v = cached[dev].load(std::memory_order_relaxed);
   if (v == 0) {
-    auto kern = linear_q8_pair_kernel<DT, TMA>;
+    auto kern = linear_q8_pair_kernel<DT, VEC>;
     int n = 0;
     if (cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kPairSmem) == cudaSuccess) {
       cudaLaunchAttribute attr[2];
@@ -496,31 +536,60 @@ int pair_clusters() {
   return v - 1;
 }
 
-template <int DT, bool TMA>
-int launch(const CUtensorMap& qm, const CUtensorMap& om, const void* wq, int64_t w_pitch, int64_t K, Q8Args a,
-           cudaStream_t stream) {
-  CUtensorMap wm;
-  const int clusters = a.rows > kBM ? pair_clusters<DT, TMA>() : 0;
-  const int bn = clusters > 0 ? kPairBN : kOneBN;
-  // (a box of the weight: each CTA's half of a pair's columns, or the one CTA's)
-  if (!map_2d(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, a.M, K, w_pitch, kBK, clusters > 0 ? kPairBN / 2 : kOneBN,
-              CU_TENSOR_MAP_SWIZZLE_128B))
-    return KRSI_ERR_CUDA;
-  const int64_t bm = clusters > 0 ? 2 * kBM : kBM;
-  const int64_t rt = (a.rows + bm - 1) / bm, ct = ((int64_t)a.M + bn - 1) / bn;
+bool output_map(Q8Args& a, int dt, int row_bytes) {
+  const int es = dt == KRSI_F32 ? 4 : 2;
+  const CUtensorMapDataType type = dt == KRSI_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : dt == KRSI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
+                                                     : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
+  return map_2d(&a.omap, type, a.out, a.rows, a.M, (int64_t)a.M * es, row_bytes / es, 32,
+                row_bytes == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B);
+}
+
+// Columns of a pair's tile: the width that takes least by this count of cycles.  A K block costs its MMAs (2 cycles a
+// column) or its operands' way from the L2 (some 48 bytes a cycle), whichever is longer; a tile 400 cycles more, and the
+// last one's epilogue is not hidden.  (2001 x 1000 x 2743 to fp32: 192 columns, in two rounds of tiles where 256 take two
+// as well.)  A warp's output box holds 64 columns of 16 bits, or 32 of fp32.
+int tile_columns(int64_t row_tiles, int64_t M, int n_kb, int pairs, bool f32) {
+  int best = kPairBN;
+  int64_t least = INT64_MAX;
+  for (int bn : {256, 192, 128, 64}) {
+    if (!f32 && bn % 128 != 0) continue;
+    const int64_t rounds = (row_tiles * ((M + bn - 1) / bn) + pairs - 1) / pairs;
+    const int64_t block = 2 * bn > (16384 + 64 * bn) / 48 ? 2 * bn : (16384 + 64 * bn) / 48;
+    const int64_t cycles = rounds * (n_kb * block + 400) + 12 * bn;
+    if (cycles < least) {
+      least = cycles;
+      best = bn;
+    }
+  }
+  return best;
+}
+
+template <int DT, bool VEC>
+int launch(const CUtensorMap& qm, const void* wq, int64_t w_pitch, int64_t K, Q8Args a, cudaStream_t stream) {
+  const int clusters = a.rows > kBM ? pair_clusters<DT, VEC>() : 0;
+  const int64_t bm = clusters > 0 ? 2 * kBM : kBM, rt = ((int64_t)a.rows + bm - 1) / bm;
+  a.bn = clusters > 0 ? tile_columns(rt, a.M, a.n_kb, clusters, DT == KRSI_F32) : kOneBN;
+  const int64_t ct = ((int64_t)a.M + a.bn - 1) / a.bn;
   if (rt * ct > INT32_MAX / 2) return KRSI_ERR_UNSUPPORTED;
   a.n_ctiles = (int)ct;
   a.n_tiles = (int)(rt * ct);
+  CUtensorMap wm;
+  // (a box of the weight: each CTA's half of a pair's columns, or the one CTA's)
+  if (!map_2d(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, a.M, K, w_pitch, kBK, clusters > 0 ? a.bn / 2 : a.bn,
+              CU_TENSOR_MAP_SWIZZLE_128B) ||
+      (VEC && !output_map(a, DT, clusters > 0 ? kPairRowB : kOneRowB)))
+    return KRSI_ERR_CUDA;
   if (clusters > 0) {
     cudaLaunchAttribute attr[2];
     const cudaLaunchConfig_t cfg = pair_config(attr, a.n_tiles < clusters ? a.n_tiles : clusters, stream);
-    KRSI_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_q8_pair_kernel<DT, TMA>, qm, wm, om, a));
+    KRSI_CUDA_TRY(cudaLaunchKernelEx(&cfg, linear_q8_pair_kernel<DT, VEC>, qm, wm, a));
     return KRSI_OK;
   }
-  KRSI_CUDA_TRY((allow_smem<linear_q8_kernel<DT, TMA>>((int)kOneSmem)));
+  KRSI_CUDA_TRY((allow_smem<linear_q8_kernel<DT, VEC>>((int)kOneSmem)));
   const int sms = device_sm_count();
-  KRSI_CUDA_TRY(launch_pdl(linear_q8_kernel<DT, TMA>, dim3(a.n_tiles < sms ? a.n_tiles : sms), dim3(kThreads), kOneSmem,
-                           stream, qm, wm, om, a));
+  KRSI_CUDA_TRY(launch_pdl(linear_q8_kernel<DT, VEC>, dim3(a.n_tiles < sms ? a.n_tiles : sms), dim3(kThreads), kOneSmem,
+                           stream, qm, wm, a));
   return KRSI_OK;
 }
 
@@ -539,23 +608,23 @@ extern "C" int krsi_linear_q8(const void* q, int64_t q_stride, const float* scal
   if (!aligned16(q) || !aligned16(wq) || q_stride % 16 != 0 || w_stride % 16 != 0) return KRSI_ERR_MISALIGNED;
   if (rows > INT32_MAX - 2 * kBM || K > INT32_MAX - kBK || M > INT32_MAX - kPairBN) return KRSI_ERR_UNSUPPORTED;
   const int es = out_dtype == KRSI_F32 ? 4 : 2;
-  const bool tma = aligned16(out) && M * es % 16 == 0;
+  const bool vec = aligned16(out) && M * es % 16 == 0;
   KRSI_CUDA_TRY(gemm::bind_context());
-  CUtensorMap qm, om;
+  CUtensorMap qm;
   if (!map_2d(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, rows, K, q_stride, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B))
     return KRSI_ERR_CUDA;
-  if (tma) {
-    const CUtensorMapDataType type = out_dtype == KRSI_F32    ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
-                                     : out_dtype == KRSI_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16
-                                                              : CU_TENSOR_MAP_DATA_TYPE_FLOAT16;
-    if (!map_2d(&om, type, out, rows, M, M * es, 64 / es, 32, CU_TENSOR_MAP_SWIZZLE_64B)) return KRSI_ERR_CUDA;
-  } else {
-    memset(&om, 0, sizeof(om));
-  }
-  const Q8Args a{scale, wscale, out, (int)rows, (int)M, 0, 0, (int)((K + kBK - 1) / kBK), kSpinLimit};
+  Q8Args a{};
+  a.scale = scale;
+  a.wscale = wscale;
+  a.out = out;
+  a.rows = (int)rows;
+  a.M = (int)M;
+  a.n_kb = (int)((K + kBK - 1) / kBK);
+  a.vec_scale = aligned16(wscale);
+  a.spin_limit = kSpinLimit;
 #define KRSI_OUT(DT)                                                            \
   if (out_dtype == DT)                                                          \
-    return tma ? launch<DT, true>(qm, om, wq, w_stride, K, a, stream) : launch<DT, false>(qm, om, wq, w_stride, K, a, stream)
+    return vec ? launch<DT, true>(qm, wq, w_stride, K, a, stream) : launch<DT, false>(qm, wq, w_stride, K, a, stream)
   KRSI_OUT(KRSI_F32);
   KRSI_OUT(KRSI_BF16);
   KRSI_OUT(KRSI_F16);
