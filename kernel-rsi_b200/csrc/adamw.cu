@@ -223,8 +223,11 @@ adamw_factors_kernel(const FactorArgs a, Factors* __restrict__ out) {
 struct Rates {
   float beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
 };
-struct RatePairs {   // each twice, for f32x2 operations on kernel arguments
-  float2 beta1, one_minus_beta1, beta2, one_minus_beta2, eps;
+// Each twice, for f32x2 operations on kernel arguments.  `one` is there for sums of products that are to be rounded
+// before they are added: a paired multiplication and addition, .rn or not, come out of the assembler as one fma; the
+// addition as an fma by a 1 that it does not know cannot be joined to either product.
+struct RatePairs {
+  float2 beta1, one_minus_beta1, beta2, one_minus_beta2, eps, one{1.f, 1.f};
   explicit RatePairs(const Rates& r)
       : beta1{r.beta1, r.beta1}, one_minus_beta1{r.one_minus_beta1, r.one_minus_beta1}, beta2{r.beta2, r.beta2},
         one_minus_beta2{r.one_minus_beta2, r.one_minus_beta2}, eps{r.eps, r.eps} {}
@@ -421,9 +424,11 @@ __device__ __forceinline__ void update8(const Lane8<WT, GT>& in, const RatePairs
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const uint64_t g = f2_mul(in.g.pair(k), clip);
-      m[k] = f2_add(f2_mul(f2_mul(decode_pair(in.m, k), sm), pair_of(c.beta1)), f2_mul(g, pair_of(c.one_minus_beta1)));
+      m[k] = f2_fma(f2_mul(f2_mul(decode_pair(in.m, k), sm), pair_of(c.beta1)), pair_of(c.one),
+                    f2_mul(g, pair_of(c.one_minus_beta1)));
       const uint64_t r = f2_mul(decode_pair(in.r, k), sr);
-      v[k] = f2_add(f2_mul(f2_mul(r, r), pair_of(c.beta2)), f2_mul(f2_mul(g, g), pair_of(c.one_minus_beta2)));
+      v[k] = f2_fma(f2_mul(f2_mul(r, r), pair_of(c.beta2)), pair_of(c.one),
+                    f2_mul(f2_mul(g, g), pair_of(c.one_minus_beta2)));
     }
   }
   float mf[kLane], vf[kLane];

@@ -153,6 +153,23 @@ def test_8_bit_states_follow_their_rule(pt, gt, master, max_norm):
             x[256:512] = 0
 
 
+@pytest.mark.parametrize("pt", [F32, BF16, F16])
+def test_8_bit_codes_on_borders(pt):
+    """0.9 m + 0.1 g of short m and g often lies on the border between two codes, where the last bit of the sum decides:
+    the products are rounded before they are added."""
+    n = 1 << 20
+    l = make([n], pt, bits=8)
+    g = torch.Generator().manual_seed(5)
+    m, r = torch.randint(-40, 41, (n,), generator=g) * 4.0, torch.randint(1, 41, (n,), generator=g) * 4.0
+    l["m"][0].copy_(m.to(torch.float8_e4m3fn)), l["v"][0].copy_(r.to(torch.float8_e4m3fn))
+    l["exponents"][0].copy_(torch.randint(100, 104, (n // GROUP, 2), generator=g))
+    l["g"][0].copy_(torch.randint(-160, 161, (n,), generator=g) * 2.0 ** -26)
+    want = rule(l["g"][0], l["m"][0], l["v"][0], l["exponents"][0], 1.0, 1)
+    call(l, count())
+    for a, b in zip((l["m"][0], l["v"][0], l["exponents"][0]), want):
+        assert (bits(a) != bits(b)).sum().item() == 0
+
+
 def test_8_bit_values():
     """What the codes stand for: m within half a code of its value, the root within one code, positive ones not 0."""
     l = make([100000], F32, bits=8)
