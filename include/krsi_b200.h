@@ -270,8 +270,9 @@ int krsi_linear_ce_finish(const float* grad, const float* g, const float* weight
                           float scale, int dtype, cudaStream_t stream);
 
 /* ---------------------------------------------------------------- residual addition and RMSNorm
- * z = (x + res) rounded to x_dtype, then krsi_rmsnorm_fwd's norm of z: y and rstd as there.  The reference has no
- * such op (its models add, then call library/rmsnorm.py:22-31).
+ * z = (x + res) rounded to x_dtype, rstd = 1 / sqrt(mean(z^2) + eps), y = w * z * rstd in fp32, rounded once
+ * (krsi_rmsnorm_fwd rounds z * rstd first).  The reference has no such op (its models add, then call
+ * library/rmsnorm.py:22-31).
  * x, res, z, y: [rows, n] of x_dtype; w: [n] of w_dtype; contiguous; dtypes as krsi_rmsnorm_fwd's; n up to 16384
  * (32768 for 16-bit x with rows of whole 16 bytes at 16-byte aligned pointers).
  * res null: z is x, and is not written. */

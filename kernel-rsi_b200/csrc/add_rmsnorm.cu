@@ -1,7 +1,7 @@
 // add_rmsnorm.cu - the residual's addition and RMSNorm in one pass, its output in the input's type or in 8 bits,
 // for B200:
 //   z = (x + res) rounded to x's type;   r = 1 / sqrt(mean(z^2) + eps)
-//   y = w * (z * r).to(w.dtype), stored in x's type (rmsnorm.cu's rounding points), or
+//   y = w * (z * r) in fp32, rounded once to x's type (rmsnorm.cu rounds z * r to w's type first), or
 //   q = e4m3(t * (448 / max|t|)), scale = max|t| * r / 448, with t = z * w in fp32: y is q * scale.
 //   (448 / max is 448 times the rounded reciprocal, as torch divides a number by a tensor.)
 // The codes do not depend on r (it cancels), so neither on the order of the sum of squares: the same row gives
@@ -154,12 +154,8 @@ add_rmsnorm_kernel(const NormArgs a) {
       if (col < n) {
         float wv[VEC], o[VEC];
         load_weight<XT, VEC>(a.w, WF32, col, wv);
-        // z * r is rounded to w's type (the store rounds the product to x's)
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) {
-          const float nz = v[c][e] * r;
-          o[e] = wv[e] * (WF32 ? nz : XE::round(nz));
-        }
+        for (int e = 0; e < VEC; ++e) o[e] = wv[e] * (v[c][e] * r);
         store_row<XT, VEC>(yr + col, o);
       }
     }

@@ -1,8 +1,9 @@
 """The residual's addition and RMSNorm in one pass on B200 (hand-written sm_100a CUDA), its output in the
 input's type or in 8 bits. Use add_rmsnorm(x2d, res, w, eps), or add_rmsnorm_q8(...) before a product in 8 bits.
 
-add_rmsnorm(x2d, res, w, eps) -> (y, z): z = x2d + res rounded to their type, y = rmsnorm(z, w, eps) with
-rmsnorm()'s rounding.  z is the residual of the next junction; its gradient is added inside the norm's backward, so
+add_rmsnorm(x2d, res, w, eps) -> (y, z): z = x2d + res rounded to their type, y = w * z / sqrt(mean(z^2) + eps) in
+fp32, rounded once (rmsnorm() rounds the normalised row to w's type before the product, as the reference does,
+rmsnorm.py:22-31); so are the gradients.  z is the residual of the next junction; its gradient is added inside the norm's backward, so
 no pass over memory is left for either sum.  With res None, z is x2d: what remains is that addition.  fp32, bf16 and
 f16, w in the same type or fp32; rows up to 16384 elements (32768 for 16-bit types with rows of whole 16 bytes).
 
@@ -44,7 +45,8 @@ class PassNorm(torch.autograd.Function):
 
 
 def add_rmsnorm(x2d, res, w, eps):
-    """(y, z) with z = x2d + res (x2d where res is None) and y = rmsnorm(z, w, eps), over the rows of 2-D tensors."""
+    """(y, z) with z = x2d + res (x2d where res is None) and y = w * z / sqrt(mean(z^2) + eps), over the rows of 2-D
+    tensors."""
     if compiling():
         return PassNorm.apply(x2d, w, eps) if res is None else ops.add_rmsnorm_fwd(x2d, res, w, eps)[:2]
     return ops.add_rmsnorm(x2d, res, w, eps)
@@ -57,11 +59,11 @@ def add_rmsnorm_q8(x2d, res, w, eps):
 
 
 def reference(x2d, res, w, eps):
-    """The torch expression add_rmsnorm reproduces: the sum, then rmsnorm's reference()."""
+    """The torch expression add_rmsnorm reproduces."""
     z = x2d if res is None else x2d + res
     zf = z.float()
     inv = torch.rsqrt(zf.square().mean(dim=-1, keepdim=True) + eps)
-    return (w * (zf * inv).to(w.dtype)).to(x2d.dtype), z
+    return (w * (zf * inv)).to(x2d.dtype), z
 
 
 def selftest():

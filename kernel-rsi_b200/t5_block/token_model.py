@@ -111,8 +111,8 @@ class TokenModel(nn.Module):
             a = attention(layer, linear_q8.linear_q8(q, scale, *wqkv, dtype), B, S)
             q, scale, x2 = add_rmsnorm.add_rmsnorm_q8(a @ layer.o.weight.t(), x2, layer.ln2.weight, layer.ln2.eps)
             out = geglu.geglu(linear_q8.linear_q8(q, scale, *wi, dtype)) @ layer.wo.weight.t()
-        h = add_rmsnorm.add_rmsnorm(x2 if out is None else out, None if out is None else x2, self.ln.weight,
-                                    self.ln.eps)[0]
+        h = (rmsnorm.rmsnorm(x2, self.ln.weight, self.ln.eps) if out is None else
+             add_rmsnorm.add_rmsnorm(out, x2, self.ln.weight, self.ln.eps)[0])
         return linear_cross_entropy.linear_cross_entropy(h, self.table, targets.reshape(-1), ignore_index=IGNORE,
                                                          z_loss=self.z_loss)
 
