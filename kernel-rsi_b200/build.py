@@ -16,6 +16,7 @@ import os
 import shutil
 import subprocess
 import sys
+import sysconfig
 from pathlib import Path
 
 PKG = Path(__file__).resolve().parent
@@ -90,7 +91,7 @@ def build_torch_ext(force: bool = False) -> Path:
     if not (force or _stale(TORCH_LIB, [src, C_ABI_LIB, *_headers()])):
         return TORCH_LIB
     inc = []
-    for p in ce.include_paths(device_type="cuda"):
+    for p in [*ce.include_paths(device_type="cuda"), sysconfig.get_paths()["include"]]:
         inc += ["-I", p]
     libdirs = ce.library_paths(device_type="cuda")
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
@@ -100,7 +101,7 @@ def build_torch_ext(force: bool = False) -> Path:
            "-L", str(LIB), "-lkrsi_b200", "-Wl,-rpath,$ORIGIN"]
     for d in libdirs:
         cmd += ["-L", d, f"-Wl,-rpath,{d}"]
-    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-lcudart"]
+    cmd += ["-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch", "-ltorch_python", "-lcudart"]
     _run(cmd)
     return TORCH_LIB
 

@@ -29,8 +29,8 @@ namespace {
 
 constexpr int kGroup = 256;                        // values that share the exponents of 8-bit states
 constexpr int kThreads = 256;
-constexpr int kGroupsPerWarp = 4;
-constexpr int kChunk = kThreads / 32 * kGroupsPerWarp * kGroup;   // values of one block: 8192
+constexpr int kGroupsPerWarp = 4;                  // at most
+constexpr int kChunk = kThreads / 32 * kGroupsPerWarp * kGroup;   // values of one block, at most: 8192
 constexpr int kLane = 8;                           // values of one lane
 constexpr int kBlocks8 = 444;                      // 8-bit states: blocks, three an SM
 constexpr int kNormBlocks = 592;                   // a fixed cap, so that the sum's order does not depend on the GPU
@@ -198,26 +198,30 @@ adamw_factors_kernel(const FactorArgs a, Factors* __restrict__ out) {
   for (int o = 16; o > 0; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
   if (lane == 0) red[warp] = sum;
   __syncthreads();
-  if (threadIdx.x != 0) return;
+  if (warp != 0) return;
   Factors f{1.f, 0.f, 0.f, 0.f, 0u, 0};
   if (a.max_norm > 0.f) {
     double total = 0.0;
     for (int i = 0; i < 8; ++i) total += red[i];
     const float norm = (float)sqrt(total);
-    if (a.norm) *a.norm = norm;
+    if (lane == 0) *a.norm = norm;
     f.clip = fminf(__fdiv_rn(a.max_norm, __fadd_rn(norm, 1e-6f)), 1.f);
     f.skip = !isfinite(norm);
   }
   if (!f.skip) {
     const int64_t t = *a.step + 1;
-    *a.step = t;
     const double lr = a.lr_dev ? (double)*a.lr_dev : a.lr;
-    f.rate = (float)(lr / -expm1((double)t * a.log_beta1));
-    f.inv_root = (float)(1.0 / sqrt(-expm1((double)t * a.log_beta2)));
+    // 1 - beta^t, of beta1 in the even lanes and of beta2 in the odd ones
+    const double bias = -expm1((double)t * (lane % 2 == 0 ? a.log_beta1 : a.log_beta2));
+    const double bias2 = __shfl_sync(0xffffffffu, bias, 1);
+    __syncwarp();   // every lane has read the step
+    if (lane == 0) *a.step = t;
+    f.rate = (float)(lr / bias);
+    f.inv_root = (float)(1.0 / sqrt(bias2));
     f.decay = (float)(1.0 - lr * a.decay);
     f.step = (uint32_t)t;
   }
-  *out = f;
+  if (lane == 0) *out = f;
 }
 
 struct Rates {
@@ -235,26 +239,36 @@ struct RatePairs {
 
 template <int PT, int GT, bool MASTER, int CAP>
 __global__ void __launch_bounds__(kThreads)
-adamw_kernel(const __grid_constant__ Table<CAP> tab, const Rates c, const Factors* __restrict__ factors) {
-  pdl_enter();
-  const Factors f = *factors;
-  if (f.skip) return;
+adamw_kernel(const __grid_constant__ Table<CAP> tab, const Rates c, const int groups,
+             const Factors* __restrict__ factors) {
   const int lane = threadIdx.x % 32;
   const Tensor& t = tab.t[tensor_of(tab, blockIdx.x)];
-  const int64_t base = (int64_t)(blockIdx.x - t.first_chunk) * kChunk + threadIdx.x / 32 * (kGroupsPerWarp * kGroup);
+  const int64_t base = ((int64_t)(blockIdx.x - t.first_chunk) * (kThreads / 32) + threadIdx.x / 32) * groups * kGroup;
   const int64_t n = t.n;
-#pragma unroll 1
-  for (int j = 0; j < kGroupsPerWarp; ++j) {
+  float p[kLane], g[kLane], m[kLane], v[kLane];
+  auto load = [&](int j) {
     const int64_t at = base + j * kGroup + lane * kLane, left = n - at;
-    if (left <= 0) return;
     const bool vec = t.aligned && left >= kLane;
-    const int live = left > kLane ? kLane : (int)left;
-    float p[kLane], g[kLane], m[kLane], v[kLane];
+    const int live = left > kLane ? kLane : (int)(left < 0 ? 0 : left);
     if constexpr (MASTER) load8<KRSI_F32>(t.master, at, vec, live, p);
     else load8<PT>(t.p, at, vec, live, p);
     load8<GT>(t.g, at, vec, live, g);
     load8<KRSI_F32>(t.m, at, vec, live, m);
     load8<KRSI_F32>(t.v, at, vec, live, v);
+  };
+  // The first group is loaded before the wait for the kernel before: that is adamw_factors_kernel, which writes none of
+  // it and lets this kernel begin only when all before it has completed.
+  load(0);
+  pdl_enter();
+  const Factors f = *factors;
+  if (f.skip) return;
+#pragma unroll 1
+  for (int j = 0; j < groups; ++j) {
+    const int64_t at = base + j * kGroup + lane * kLane, left = n - at;
+    if (left <= 0) return;
+    const bool vec = t.aligned && left >= kLane;
+    const int live = left > kLane ? kLane : (int)left;
+    if (j > 0) load(j);
 #pragma unroll
     for (int e = 0; e < kLane; ++e) {
       const float ge = __fmul_rn(g[e], f.clip);
@@ -556,37 +570,43 @@ bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p
 
 int64_t launches_at_most(int64_t count) { return count / kLargeCap + 4; }   // one more for each gradient type
 
-// Calls `launch(table)` for tables of the tensors that `take` accepts, as few as their number allows, in chunks of
-// `chunk` values.
+// A tensor's kind: what the update's kernel is compiled for.
+constexpr int kKinds = 3 * 2 * 2 * 2;
+constexpr int kind_of(int p_dtype, int g_dtype, bool master, bool q8) {
+  return ((p_dtype * 2 + (g_dtype != p_dtype)) * 2 + master) * 2 + q8;
+}
+int kind_of(const krsi_adamw_tensor& t) {
+  return kind_of(t.p_dtype, t.g_dtype, t.master != nullptr, t.state_bits == 8);
+}
+
+// Calls `launch(table)` for tables of the tensors that `take` accepts, `left` of them, in chunks of `chunk` values.
 template <typename Take, typename Launch>
-int for_tables(const krsi_adamw_tensor* tensors, int64_t count, int chunk, Take take, Launch launch) {
+int for_tables(const krsi_adamw_tensor* tensors, int64_t left, int chunk, Take take, Launch launch) {
   int64_t i = 0;
-  while (i < count) {
-    int n = 0;
-    for (int64_t j = i; j < count && n <= kSmallCap; ++j) n += take(tensors[j]) && tensors[j].n > 0;
-    if (n == 0) return KRSI_OK;
-    auto fill = [&](auto& tab) -> int {
-      constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
-      int64_t chunks = 0;
-      tab.count = 0;
-      for (; i < count && tab.count < cap; ++i) {
-        const krsi_adamw_tensor& s = tensors[i];
-        if (!take(s) || s.n == 0) continue;
-        const int64_t own = (s.n + chunk - 1) / chunk;
-        if (own > INT32_MAX) return KRSI_ERR_UNSUPPORTED;
-        if (chunks + own > INT32_MAX) break;   // the next launch takes it
-        Tensor& t = tab.t[tab.count++];
-        t = Tensor{s.p, s.g, s.m, s.v, s.master, s.exponents, s.n, (int)chunks, 0};
-        const size_t state = s.state_bits == 8 ? 8 : 32;
-        t.aligned = aligned_to(s.p, s.p_dtype == KRSI_F32 ? 32 : 16) && aligned_to(s.g, s.g_dtype == KRSI_F32 ? 32 : 16) &&
-                    aligned_to(s.m, state) && aligned_to(s.v, state) && aligned_to(s.master, 32);
-        chunks += own;
-      }
-      tab.n_chunks = (int)chunks;
-      return launch(tab);
-    };
+  auto fill = [&](auto& tab) -> int {
+    constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
+    int64_t chunks = 0;
+    tab.count = 0;
+    for (; left > 0 && tab.count < cap; ++i) {
+      const krsi_adamw_tensor& s = tensors[i];
+      if (!take(s)) continue;
+      const int64_t own = (s.n + chunk - 1) / chunk;
+      if (own > INT32_MAX) return KRSI_ERR_UNSUPPORTED;
+      if (chunks + own > INT32_MAX) break;   // the next launch takes it
+      const size_t state = s.state_bits == 8 ? 8 : 32;
+      const bool aligned = aligned_to(s.p, s.p_dtype == KRSI_F32 ? 32 : 16) &&
+                           aligned_to(s.g, s.g_dtype == KRSI_F32 ? 32 : 16) && aligned_to(s.m, state) &&
+                           aligned_to(s.v, state) && aligned_to(s.master, 32);
+      tab.t[tab.count++] = Tensor{s.p, s.g, s.m, s.v, s.master, s.exponents, s.n, (int)chunks, aligned};
+      chunks += own;
+      --left;
+    }
+    tab.n_chunks = (int)chunks;
+    return launch(tab);
+  };
+  while (left > 0) {
     int rc;
-    if (n <= kSmallCap) {
+    if (left <= kSmallCap) {
       Table<kSmallCap> tab;
       rc = fill(tab);
     } else {
@@ -598,38 +618,48 @@ int for_tables(const krsi_adamw_tensor* tensors, int64_t count, int chunk, Take 
   return KRSI_OK;
 }
 
+// How many tensors there are of each kind, and with each gradient type, and the values of each kind; tensors without
+// values count for none.
+struct Counts {
+  int64_t kind[kKinds] = {}, grad[3] = {}, values[kKinds] = {};
+};
+
 template <int PT, int GT, bool MASTER, bool Q8>
-int update(const krsi_adamw_tensor* tensors, int64_t count, const Rates& c, const Factors* f, cudaStream_t s) {
-  auto take = [](const krsi_adamw_tensor& t) {
-    return t.p_dtype == PT && t.g_dtype == GT && (t.master != nullptr) == MASTER && (t.state_bits == 8) == Q8;
-  };
-  return for_tables(tensors, count, Q8 ? kGroup : kChunk, take, [&](const auto& tab) -> int {
+int update(const krsi_adamw_tensor* tensors, const Counts& counts, const Rates& c, const Factors* f, cudaStream_t s) {
+  constexpr int kind = kind_of(PT, GT, MASTER, Q8);
+  auto take = [](const krsi_adamw_tensor& t) { return t.n > 0 && kind_of(t) == kind; };
+  // fp32 states: one group a warp where four would leave SMs without a block (150,000 values: 5 us became 3)
+  const int groups = counts.values[kind] < (int64_t)kNumSMsB200 * kChunk ? 1 : kGroupsPerWarp;
+  const int chunk = Q8 ? kGroup : kThreads / 32 * groups * kGroup;
+  return for_tables(tensors, counts.kind[kind], chunk, take, [&](const auto& tab) -> int {
     constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
     if constexpr (Q8) {
       // consecutive groups in equal shares (16 at a time, in turns, take 10% more)
       constexpr int warps = kBlocks8 * (kThreads / 32);
       const int64_t span = ((int64_t)tab.n_chunks + warps - 1) / warps;
       const int64_t blocks = (tab.n_chunks + span * (kThreads / 32) - 1) / (span * (kThreads / 32));
-      KRSI_CUDA_TRY(launch_pdl(adamw8_kernel<PT, GT, MASTER, cap>, dim3((unsigned)blocks), dim3(kThreads), 0, s, tab, RatePairs(c), (int)span, f));
+      KRSI_CUDA_TRY(launch_pdl(adamw8_kernel<PT, GT, MASTER, cap>, dim3((unsigned)blocks), dim3(kThreads), 0, s, tab,
+                               RatePairs(c), (int)span, f));
     } else {
-      KRSI_CUDA_TRY(launch_pdl(adamw_kernel<PT, GT, MASTER, cap>, dim3(tab.n_chunks), dim3(kThreads), 0, s, tab, c, f));
+      KRSI_CUDA_TRY(launch_pdl(adamw_kernel<PT, GT, MASTER, cap>, dim3(tab.n_chunks), dim3(kThreads), 0, s, tab, c, groups,
+                               f));
     }
     return KRSI_OK;
   });
 }
 
 template <int GT>
-int norm(const krsi_adamw_tensor* tensors, int64_t count, double* partial, int64_t room, int* used, cudaStream_t s) {
-  return for_tables(
-      tensors, count, kChunk, [](const krsi_adamw_tensor& t) { return t.g_dtype == GT; },
-      [&](const auto& tab) -> int {
-        constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
-        const int blocks = tab.n_chunks < kNormBlocks ? tab.n_chunks : kNormBlocks;
-        if (*used + blocks > room) return KRSI_ERR_WORKSPACE;
-        KRSI_CUDA_TRY(launch_pdl(adamw_norm_kernel<GT, cap>, dim3(blocks), dim3(kThreads), 0, s, tab, partial + *used));
-        *used += blocks;
-        return KRSI_OK;
-      });
+int norm(const krsi_adamw_tensor* tensors, const Counts& counts, double* partial, int64_t room, int* used,
+         cudaStream_t s) {
+  auto take = [](const krsi_adamw_tensor& t) { return t.n > 0 && t.g_dtype == GT; };
+  return for_tables(tensors, counts.grad[GT], kChunk, take, [&](const auto& tab) -> int {
+    constexpr int cap = sizeof(tab.t) / sizeof(tab.t[0]);
+    const int blocks = tab.n_chunks < kNormBlocks ? tab.n_chunks : kNormBlocks;
+    if (*used + blocks > room) return KRSI_ERR_WORKSPACE;
+    KRSI_CUDA_TRY(launch_pdl(adamw_norm_kernel<GT, cap>, dim3(blocks), dim3(kThreads), 0, s, tab, partial + *used));
+    *used += blocks;
+    return KRSI_OK;
+  });
 }
 
 }  // namespace
@@ -649,6 +679,7 @@ extern "C" int krsi_adamw_step(const krsi_adamw_tensor* tensors, int64_t count, 
   KRSI_CHECK_ARG(count >= 0 && (count == 0 || tensors) && step);
   KRSI_CHECK_ARG(beta1 >= 0 && beta1 < 1 && beta2 >= 0 && beta2 < 1 && eps >= 0 && max_norm >= 0);
   KRSI_CHECK_ARG(max_norm == 0 || norm_out);
+  Counts counts;
   for (int64_t i = 0; i < count; ++i) {
     const krsi_adamw_tensor& t = tensors[i];
     KRSI_CHECK_ARG(t.n >= 0 && dtype_ok(t.p_dtype) && (t.state_bits == 8 || t.state_bits == 32));
@@ -657,6 +688,9 @@ extern "C" int krsi_adamw_step(const krsi_adamw_tensor* tensors, int64_t count, 
     KRSI_CHECK_ARG(t.p && t.g && t.m && t.v && (t.state_bits == 32 || t.exponents));
     KRSI_CHECK_ARG(t.p_dtype != KRSI_F32 || !t.master);
     if (t.state_bits == 8 && !aligned_to(t.exponents, 2)) return KRSI_ERR_MISALIGNED;
+    ++counts.kind[kind_of(t)];
+    ++counts.grad[t.g_dtype];
+    counts.values[kind_of(t)] += t.n;
   }
   size_t need = 0;
   krsi_adamw_workspace_size(count, &need);
@@ -667,9 +701,9 @@ extern "C" int krsi_adamw_step(const krsi_adamw_tensor* tensors, int64_t count, 
   int used = 0;
   if (max_norm > 0) {
     const int64_t room = launches_at_most(count) * kNormBlocks;
-    int rc = norm<KRSI_F32>(tensors, count, partial, room, &used, stream);
-    if (rc == KRSI_OK) rc = norm<KRSI_BF16>(tensors, count, partial, room, &used, stream);
-    if (rc == KRSI_OK) rc = norm<KRSI_F16>(tensors, count, partial, room, &used, stream);
+    int rc = norm<KRSI_F32>(tensors, counts, partial, room, &used, stream);
+    if (rc == KRSI_OK) rc = norm<KRSI_BF16>(tensors, counts, partial, room, &used, stream);
+    if (rc == KRSI_OK) rc = norm<KRSI_F16>(tensors, counts, partial, room, &used, stream);
     if (rc != KRSI_OK) return rc;
   }
   const FactorArgs fa{partial, used, norm_out, step, lr_dev, lr, log(beta1), log(beta2), weight_decay, (float)max_norm};
@@ -677,8 +711,8 @@ extern "C" int krsi_adamw_step(const krsi_adamw_tensor* tensors, int64_t count, 
   const Rates c{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
 #define KRSI_UPDATE(PT, GT, MASTER)                                                        \
   do {                                                                                     \
-    int rc = update<PT, GT, MASTER, false>(tensors, count, c, factors, stream);            \
-    if (rc == KRSI_OK) rc = update<PT, GT, MASTER, true>(tensors, count, c, factors, stream); \
+    int rc = update<PT, GT, MASTER, false>(tensors, counts, c, factors, stream);            \
+    if (rc == KRSI_OK) rc = update<PT, GT, MASTER, true>(tensors, counts, c, factors, stream); \
     if (rc != KRSI_OK) return rc;                                                          \
   } while (0)
   KRSI_UPDATE(KRSI_F32, KRSI_F32, false);

@@ -7,10 +7,17 @@
 // caching allocator on the input's device), passes the current CUDA stream, and turns a
 // nonzero krsi_status into a Python RuntimeError.  No synchronisation, so the ops can be
 // captured in CUDA graphs.
+#include <torch/csrc/python_headers.h>
+
 #include <ATen/ATen.h>
+#include <ATen/PythonTorchFunctionTLS.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
+#include <pybind11/pybind11.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -740,7 +747,7 @@ at::Tensor adamw_step(at::TensorList params, at::TensorList grads, at::TensorLis
       spans.emplace_back(at, at + (uintptr_t)p.nbytes());
     }
   }
-  std::sort(spans.begin(), spans.end());
+  if (!std::is_sorted(spans.begin(), spans.end())) std::sort(spans.begin(), spans.end());
   for (size_t i = 1; i < spans.size(); ++i)
     TORCH_CHECK(spans[i].first >= spans[i - 1].second, "adamw_step: two parameters share memory");
   auto norm = at::empty(max_norm > 0 ? at::IntArrayRef{} : at::IntArrayRef{0}, step.options().dtype(at::kFloat));
@@ -1030,6 +1037,66 @@ TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
   m.impl("linear_q8", &linear_q8);
   m.impl("adamw_step", &adamw_step);
 }
+
+// ---------------------------------------------------------------- Python lists
+// adamw_step from Python lists as they are.  An operator's list arguments are boxed and unboxed tensor by tensor on the
+// way, which for a model's lists is most of a step's time on the host (0.5 us a tensor; this takes a quarter).  What
+// only the dispatcher can see to, a mode that is on or a tensor that is not torch's own, is left to the operator: the
+// answer is then NotImplemented.
+namespace {
+
+bool unpack(PyObject* list, std::vector<at::Tensor>& out) {
+  if (!PyList_CheckExact(list) && !PyTuple_CheckExact(list)) return false;
+  const Py_ssize_t n = PySequence_Fast_GET_SIZE(list);
+  PyObject** items = PySequence_Fast_ITEMS(list);
+  out.reserve(n);
+  for (Py_ssize_t i = 0; i < n; ++i) {
+    if (!THPVariable_CheckExact(items[i])) return false;
+    out.push_back(THPVariable_Unpack(items[i]));
+  }
+  return true;
+}
+
+PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
+  HANDLE_TH_ERRORS
+  if (nargs != 14) return PyErr_Format(PyExc_TypeError, "adamw_step: 14 arguments expected, got %zd", nargs);
+  const bool modes = c10::impl::TorchDispatchModeTLS::any_modes_set() ||
+                     at::impl::PythonTorchFunctionTLS::stack_len() > 0;
+  std::vector<at::Tensor> lists[6];
+  bool ok = !modes && THPVariable_CheckExact(args[6]) && (args[7] == Py_None || THPVariable_CheckExact(args[7]));
+  for (int k = 0; ok && k < 6; ++k) ok = unpack(args[k], lists[k]);
+  // (the operator's own refusals where there is no CUDA tensor)
+  ok = ok && THPVariable_Unpack(args[6]).is_cuda();
+  for (int k = 0; ok && k < 4; ++k)
+    for (const at::Tensor& t : lists[k]) ok = ok && t.is_cuda();
+  if (!ok) Py_RETURN_NOTIMPLEMENTED;
+  double number[6];
+  for (int k = 0; k < 6; ++k) {
+    number[k] = PyFloat_AsDouble(args[8 + k]);
+    if (number[k] == -1.0 && PyErr_Occurred()) return nullptr;
+  }
+  const at::Tensor step = THPVariable_Unpack(args[6]);
+  const c10::optional<at::Tensor> lr =
+      args[7] == Py_None ? c10::nullopt : c10::optional<at::Tensor>(THPVariable_Unpack(args[7]));
+  at::Tensor norm;
+  {
+    pybind11::gil_scoped_release release;
+    at::AutoDispatchBelowADInplaceOrView below;
+    norm = adamw_step(lists[0], lists[1], lists[2], lists[3], lists[4], lists[5], step, lr, number[0], number[1],
+                      number[2], number[3], number[4], number[5]);
+  }
+  return THPVariable_Wrap(std::move(norm));
+  END_HANDLE_TH_ERRORS
+}
+
+PyMethodDef methods[] = {{"adamw_step", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(&py_adamw_step)),
+                          METH_FASTCALL, "torch.ops.krsi.adamw_step on Python lists, or NotImplemented"},
+                         {nullptr, nullptr, 0, nullptr}};
+PyModuleDef module = {PyModuleDef_HEAD_INIT, "_krsi_torch", nullptr, -1, methods};
+
+}  // namespace
+
+extern "C" __attribute__((visibility("default"))) PyObject* PyInit__krsi_torch() { return PyModule_Create(&module); }
 
 TORCH_LIBRARY_IMPL(krsi, AutogradCUDA, m) {
   m.impl("embedding", &embedding_autograd);

@@ -15,6 +15,7 @@ relative to this file.
 from __future__ import annotations
 
 import ctypes
+import importlib.util
 import os
 from pathlib import Path
 
@@ -46,6 +47,8 @@ capi.krsi_device_status.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.c_int]
 if not hasattr(torch.ops, "krsi") or not hasattr(torch.ops.krsi, "rmsnorm_fwd"):
     torch.ops.load_library(str(TORCH_EXT_PATH))
 ops = torch.ops.krsi
+_spec = importlib.util.spec_from_file_location("_krsi_torch", TORCH_EXT_PATH)
+direct = importlib.util.module_from_spec(_spec)   # functions of Python lists (the same library: loaded once)
 
 
 def device_status(clear: bool = False) -> int:

@@ -26,10 +26,10 @@ from pathlib import Path
 import torch
 
 sys.path.insert(0, str(Path(__file__).resolve().parent))
-from _ext import ops  # noqa: E402
+from _compat import compiling  # noqa: E402
+from _ext import direct, ops  # noqa: E402
 
 GROUP = 256
-_step = ops.adamw_step.default   # (found once: the lookup takes a tenth of a small step)
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
@@ -39,8 +39,11 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     copies of the 16-bit parameters (None, or an entry without elements, where there is none).  Returns the norm of
     all gradients where max_norm > 0, else None.  No two tensors may overlap."""
     device_lr = isinstance(lr, torch.Tensor)
-    norm = _step(params, grads, exp_avgs, exp_avg_sqs, masters or [], exponents or [], step,
-                 lr if device_lr else None, 0.0 if device_lr else lr, betas[0], betas[1], eps, weight_decay, max_norm)
+    args = (params, grads, exp_avgs, exp_avg_sqs, masters or [], exponents or [], step, lr if device_lr else None,
+            0.0 if device_lr else lr, betas[0], betas[1], eps, weight_decay, max_norm)
+    norm = NotImplemented if compiling() else direct.adamw_step(*args)
+    if norm is NotImplemented:
+        norm = ops.adamw_step(*args)
     return norm if max_norm > 0 else None
 
 

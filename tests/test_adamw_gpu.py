@@ -354,6 +354,35 @@ def test_refusals():
     assert all(torch.equal(a, b) for a, b in zip(p, before)) and _ext.device_status() == 0
 
 
+def test_modes_and_subclasses_reach_the_operator():
+    """Lists go past the dispatcher only where nothing there would see to them; either way the bits are the same."""
+    from torch.utils._python_dispatch import TorchDispatchMode
+
+    class Seen(TorchDispatchMode):
+        ops = []
+
+        def __torch_dispatch__(self, func, types, args=(), kwargs=None):
+            self.ops.append(func._opname)
+            return func(*args, **(kwargs or {}))
+
+    class Named(torch.Tensor):
+        pass
+
+    want, moded, named, tupled = (make([300, 20], BF16, master=True, bits=8) for _ in range(4))
+    call(want, count())
+    with Seen():
+        call(moded, count())
+    assert "adamw_step" in Seen.ops
+    named["p"] = [x.as_subclass(Named) for x in named["p"]]
+    call(named, count())
+    call({k: tuple(v) for k, v in tupled.items()}, count())
+    for l in (moded, named, tupled):
+        assert all(torch.equal(bits_of(a), bits_of(b)) for k in want for a, b in zip(l[k], want[k]))
+    compiled = make([300, 20], BF16, master=True, bits=8)
+    torch.compile(lambda: call(compiled, count()))()
+    assert all(torch.equal(bits_of(a), bits_of(b)) for k in want for a, b in zip(compiled[k], want[k]))
+
+
 # ---------------------------------------------------------------- the optimizer
 def small_model(dtype=F32):
     torch.manual_seed(0)
