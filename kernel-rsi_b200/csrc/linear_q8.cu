@@ -51,6 +51,7 @@ struct Q8Args {
   int n_ctiles;       // column tiles
   int n_tiles;        // row tiles x column tiles
   int n_kb;           // K blocks
+  int q_rows, stages; // one CTA: rows of q in a stage, stages
   bool vec_scale;     // wscale starts on 16 bytes
   uint32_t spin_limit;
 };
@@ -207,16 +208,41 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
 }
 
 // ---------------------------------------------------------------- up to 128 rows: one CTA, narrow tiles
+// The weight comes from memory, so its K blocks in flight are what counts: a stage's tile of q has only as many rows as
+// there are, up to eight more (a.q_rows), which leaves room for up to 20 stages of the weight's 8 KB instead of 8.  An
+// MMA nevertheless reads 128 rows: what follows in shared memory, whatever it is, makes rows of the accumulator that
+// nothing reads.  (4 rows of 2792 over 7843: 17.3 us with 8 stages
+// became 9.8.)
 constexpr int kOneBN = 64;
-constexpr int kOneStages = 8;
+constexpr int kOneMaxStages = 20;
+constexpr uint32_t kOneWTile = kOneBN * kBK;                         // 8 KB
 constexpr int kOneRowB = 64;                                         // bytes of a row in an output box
-constexpr uint32_t kOneStageBytes = kATile + kOneBN * kBK;           // 24 KB
-constexpr uint32_t kOneBoxOff = kOneStages * kOneStageBytes;
+constexpr uint32_t kOneRing = 8 * (kATile + kOneWTile);              // 192 KB
+constexpr uint32_t kOneBoxOff = kOneRing;
 constexpr uint32_t kOneBarOff = kOneBoxOff + kEpiWarps * 2 * 32 * kOneRowB;
-constexpr uint32_t kOneMiscOff = kOneBarOff + (2 * kOneStages + 2 + 2 + 1) * 8;
+constexpr uint32_t kOneMiscOff = kOneBarOff + (2 * kOneMaxStages + 2 + 2 + 1) * 8;
 constexpr uint32_t kOneSmem = kOneMiscOff + 16 + 1024;               // + slack for the 1024-byte alignment
 constexpr uint32_t kOneTmemCols = 2 * kOneBN;
 static_assert(kOneSmem <= 232448, "shared memory budget");
+
+// A ring's position: slot, and the parity of its current use.  (A division of the K block's number by a.stages, in its
+// place, took 3 us of 36 K blocks.)
+struct Ring {
+  int slot = 0;
+  uint32_t parity = 0;
+  __device__ __forceinline__ void next(int stages) {
+    if (++slot == stages) {
+      slot = 0;
+      parity ^= 1;
+    }
+  }
+};
+
+// Stages for a.q_rows rows.  The tiles of q come first, so an MMA on the last one reads on into the weight's.
+inline int one_stages(int q_rows) {
+  const int n = (int)(kOneRing / (q_rows * kBK + kOneWTile));
+  return n < kOneMaxStages ? n : kOneMaxStages;
+}
 
 template <int DT, bool VEC>
 __global__ void __launch_bounds__(kThreads, 1)
@@ -226,8 +252,8 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint64_t* full = reinterpret_cast<uint64_t*>(smem + kOneBarOff);
-  uint64_t* empty = full + kOneStages;
-  uint64_t* acc_full = empty + kOneStages;
+  uint64_t* empty = full + kOneMaxStages;
+  uint64_t* acc_full = empty + kOneMaxStages;
   uint64_t* acc_empty = acc_full + 2;
   uint64_t* drain = acc_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + kOneMiscOff);
@@ -235,9 +261,10 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   Tiles tiles(a, blockIdx.x, gridDim.x);
+  const uint32_t q_bytes = (uint32_t)a.q_rows * kBK, w_off = a.stages * q_bytes;
 
   if (threadIdx.x == 0) {
-    for (int s = 0; s < kOneStages; ++s) {
+    for (int s = 0; s < a.stages; ++s) {
       mbar_init(&full[s], 1);
       mbar_init(&empty[s], 1);
     }
@@ -265,28 +292,31 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     bool ok = true;
+    Ring ring;
     int it = 0;
     while (ok && tiles.next()) {
       const int m0 = tiles.row * kBM, n0 = tiles.col * kOneBN;
       for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
-        const int s = it % kOneStages;
-        if (it >= kOneStages && !__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ((it / kOneStages) - 1) & 1,
-                                                                           abort_flag, a.spin_limit))) {
+        const int s = ring.slot;
+        if (it >= a.stages &&
+            !__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ring.parity ^ 1, abort_flag, a.spin_limit))) {
           ok = false;
           break;
         }
+        ring.next(a.stages);
         if (lane == 0) {
-          uint8_t* st = smem + s * kOneStageBytes;
-          mbar_arrive_expect_tx(&full[s], kOneStageBytes);
-          tma_load_2d(st, &qmap, &full[s], kb * kBK, m0);
-          tma_load_2d(st + kATile, &wmap, &full[s], kb * kBK, n0);
+          mbar_arrive_expect_tx(&full[s], q_bytes + kOneWTile);
+          tma_load_2d(smem + w_off + s * kOneWTile, &wmap, &full[s], kb * kBK, n0);
+          tma_load_2d(smem + s * q_bytes, &qmap, &full[s], kb * kBK, m0);
         }
         __syncwarp();
       }
     }
-    if (!ok) {
+    if (!ok) {   // every load issued has landed before this CTA exits
       watchdog_fire(kWdQ8Load);
-      drain_loads<kOneStages>(full, it, a.spin_limit);
+      for (int j = it > a.stages ? it - a.stages : 0; j < it; ++j)
+        for (uint32_t n = 0; n < a.spin_limit && !mbar_try_wait(&full[j % a.stages], (j / a.stages) & 1); ++n) {
+        }
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ MMA issuer (whole warp, elected lane)
@@ -294,9 +324,9 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
       return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit));
     };
     constexpr uint32_t idesc = idesc_e4m3(kBM, kOneBN);
-    const uint64_t desc0 = kmajor_sw128(smem_u32(smem));
+    const uint64_t q0 = kmajor_sw128(smem_u32(smem)), w0 = kmajor_sw128(smem_u32(smem + w_off));
     bool ok = true;
-    int it = 0;
+    Ring ring;
     for (int i = 0; ok && tiles.next(); ++i) {
       const int acc = i & 1;
       if (i >= 2 && !wait(&acc_empty[acc], ((i >> 1) - 1) & 1)) {
@@ -304,14 +334,15 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         break;
       }
       tc_fence_after();
-      for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
-        const int s = it % kOneStages;
-        if (!wait(&full[s], (it / kOneStages) & 1)) {
+      for (int kb = 0; kb < a.n_kb; ++kb) {
+        const int s = ring.slot;
+        if (!wait(&full[s], ring.parity)) {
           ok = false;
           break;
         }
+        ring.next(a.stages);
         tc_fence_after();
-        const uint64_t ad = desc0 + (uint64_t)s * (kOneStageBytes >> 4), bd = ad + (kATile >> 4);
+        const uint64_t ad = q0 + (uint64_t)s * (q_bytes >> 4), bd = w0 + (uint64_t)s * (kOneWTile >> 4);
 #pragma unroll
         for (int kk = 0; kk < kBK / 32; ++kk)
           mma_q8_e(tmem + acc * kOneBN, ad + kk * 2, bd + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
@@ -566,7 +597,7 @@ int tile_columns(int64_t row_tiles, int64_t M, int n_kb, int pairs, bool f32) {
 }
 
 template <int DT, bool VEC>
-int launch(const CUtensorMap& qm, const void* wq, int64_t w_pitch, int64_t K, Q8Args a, cudaStream_t stream) {
+int launch(const void* q, int64_t q_pitch, const void* wq, int64_t w_pitch, int64_t K, Q8Args a, cudaStream_t stream) {
   const int clusters = a.rows > kBM ? pair_clusters<DT, VEC>() : 0;
   const int64_t bm = clusters > 0 ? 2 * kBM : kBM, rt = ((int64_t)a.rows + bm - 1) / bm;
   a.bn = clusters > 0 ? tile_columns(rt, a.M, a.n_kb, clusters, DT == KRSI_F32) : kOneBN;
@@ -574,9 +605,12 @@ int launch(const CUtensorMap& qm, const void* wq, int64_t w_pitch, int64_t K, Q8
   if (rt * ct > INT32_MAX / 2) return KRSI_ERR_UNSUPPORTED;
   a.n_ctiles = (int)ct;
   a.n_tiles = (int)(rt * ct);
-  CUtensorMap wm;
+  a.q_rows = a.rows < kBM ? (a.rows + 7) / 8 * 8 : kBM;
+  a.stages = one_stages(a.q_rows);
+  CUtensorMap qm, wm;
   // (a box of the weight: each CTA's half of a pair's columns, or the one CTA's)
-  if (!map_2d(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, a.M, K, w_pitch, kBK, clusters > 0 ? a.bn / 2 : a.bn,
+  if (!map_2d(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, a.rows, K, q_pitch, kBK, a.q_rows, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !map_2d(&wm, CU_TENSOR_MAP_DATA_TYPE_UINT8, wq, a.M, K, w_pitch, kBK, clusters > 0 ? a.bn / 2 : a.bn,
               CU_TENSOR_MAP_SWIZZLE_128B) ||
       (VEC && !output_map(a, DT, clusters > 0 ? kPairRowB : kOneRowB)))
     return KRSI_ERR_CUDA;
@@ -610,9 +644,6 @@ extern "C" int krsi_linear_q8(const void* q, int64_t q_stride, const float* scal
   const int es = out_dtype == KRSI_F32 ? 4 : 2;
   const bool vec = aligned16(out) && M * es % 16 == 0;
   KRSI_CUDA_TRY(gemm::bind_context());
-  CUtensorMap qm;
-  if (!map_2d(&qm, CU_TENSOR_MAP_DATA_TYPE_UINT8, q, rows, K, q_stride, kBK, kBM, CU_TENSOR_MAP_SWIZZLE_128B))
-    return KRSI_ERR_CUDA;
   Q8Args a{};
   a.scale = scale;
   a.wscale = wscale;
@@ -624,7 +655,7 @@ extern "C" int krsi_linear_q8(const void* q, int64_t q_stride, const float* scal
   a.spin_limit = kSpinLimit;
 #define KRSI_OUT(DT)                                                            \
   if (out_dtype == DT)                                                          \
-    return vec ? launch<DT, true>(qm, wq, w_stride, K, a, stream) : launch<DT, false>(qm, wq, w_stride, K, a, stream)
+    return vec ? launch<DT, true>(q, q_stride, wq, w_stride, K, a, stream) : launch<DT, false>(q, q_stride, wq, w_stride, K, a, stream)
   KRSI_OUT(KRSI_F32);
   KRSI_OUT(KRSI_BF16);
   KRSI_OUT(KRSI_F16);
