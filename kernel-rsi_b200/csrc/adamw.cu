@@ -256,8 +256,9 @@ adamw_kernel(const __grid_constant__ Table<CAP> tab, const Rates c, const int gr
     load8<KRSI_F32>(t.m, at, vec, live, m);
     load8<KRSI_F32>(t.v, at, vec, live, v);
   };
-  // The first group is loaded before the wait for the kernel before: that is adamw_factors_kernel, which writes none of
-  // it and lets this kernel begin only when all before it has completed.
+  // The first group is loaded before the wait for the kernel before, which is adamw_factors_kernel or the update of
+  // another kind of tensors: neither writes any of it, and both let this kernel begin only after their own wait, when all
+  // that came before the factors has completed.
   load(0);
   pdl_enter();
   const Factors f = *factors;
