@@ -247,7 +247,7 @@ extern "C" int krsi_add_rmsnorm_fwd(const void* x, const void* res, const void* 
   KRSI_CHECK_ARG(n > 0 && x && w && y && rstd && (!res || z));
   if (n > 0x7fffffff) return KRSI_ERR_UNSUPPORTED;
   if (!types_ok(x_dtype, w_dtype)) return KRSI_ERR_UNSUPPORTED;
-  return dispatch<kOutRow>(x_dtype, w_dtype, packet_of(x_dtype, n, {x, y, w, res, res ? z : nullptr}),
+  return dispatch<kOutRow>(x_dtype, w_dtype, packet_of(x_dtype, w_dtype, n, w, {x, y, res, res ? z : nullptr}),
                            NormArgs{x, res, w, z, y, rstd, rows, 0, (int)n, eps}, stream);
 }
 
@@ -260,7 +260,7 @@ extern "C" int krsi_add_rmsnorm_q8_fwd(const void* x, const void* res, const voi
   if (n > 0x7fffffff) return KRSI_ERR_UNSUPPORTED;
   const bool q_ok = aligned16(q) && q_stride % 16 == 0;
   if (!types_ok(x_dtype, w_dtype)) return KRSI_ERR_UNSUPPORTED;
-  return dispatch<kOutQ8>(x_dtype, w_dtype, q_ok ? packet_of(x_dtype, n, {x, w, res, res ? z : nullptr}) : 1,
+  return dispatch<kOutQ8>(x_dtype, w_dtype, q_ok ? packet_of(x_dtype, w_dtype, n, w, {x, res, res ? z : nullptr}) : 1,
                           NormArgs{x, res, w, z, q, scale, rows, q_stride, (int)n, eps}, stream);
 }
 
@@ -271,6 +271,6 @@ extern "C" int krsi_quantise_rows(const void* x, void* q, int64_t q_stride, floa
   KRSI_CHECK_ARG(n > 0 && x && q && scale && q_stride >= n);
   if (n > 0x7fffffff) return KRSI_ERR_UNSUPPORTED;
   const bool q_ok = aligned16(q) && q_stride % 16 == 0;
-  return dispatch<kOutQ8>(x_dtype, x_dtype, q_ok ? packet_of(x_dtype, n, {x}) : 1,
+  return dispatch<kOutQ8>(x_dtype, x_dtype, q_ok ? packet_of(x_dtype, x_dtype, n, nullptr, {x}) : 1,
                           NormArgs{x, nullptr, nullptr, nullptr, q, scale, rows, q_stride, (int)n, 0.f}, stream);
 }

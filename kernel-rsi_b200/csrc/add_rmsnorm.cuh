@@ -69,13 +69,15 @@ __device__ __forceinline__ void load_weight(const void* w, bool f32, int col, fl
   }
 }
 
-// The widest packets that rows of n values at these addresses allow (an fp32 weight beside 16-bit rows: 16 bytes).
-inline int packet_of(int x_dtype, int64_t n, std::initializer_list<const void*> pointers) {
+// The widest packets, in values, that rows of n values at these addresses allow: 16 or 8 bytes, or 1 value.  A packet's
+// values of w are as many bytes as the row's, or in fp32 beside 16 bits 16 at a time.
+inline int packet_of(int x_dtype, int w_dtype, int64_t n, const void* w, std::initializer_list<const void*> rows) {
   const int es = x_dtype == KRSI_F32 ? 4 : 2;
   for (int bytes : {16, 8}) {
     if (es == 4 && bytes == 8) break;
-    bool ok = n * es % bytes == 0;
-    for (const void* p : pointers) ok = ok && (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0;
+    auto on = [](const void* p, int bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; };
+    bool ok = n * es % bytes == 0 && on(w, w_dtype == KRSI_F32 ? 16 : bytes);
+    for (const void* p : rows) ok = ok && on(p, bytes);
     if (ok) return bytes / es;
   }
   return 1;

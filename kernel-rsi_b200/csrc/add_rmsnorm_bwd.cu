@@ -385,7 +385,7 @@ extern "C" int krsi_add_rmsnorm_bwd(const void* gy, const void* gz, const void* 
   krsi_add_rmsnorm_bwd_workspace_size(rows, n, &need);
   if (!workspace || workspace_bytes < need) return KRSI_ERR_WORKSPACE;
   const BwdArgs a{gy, gz, z, w, rstd, dz, static_cast<float*>(workspace), rows, (int)n, w_dtype == KRSI_F32};
-  const int vec = packet_of(x_dtype, n, {gy, gz, z, w, dz});
+  const int vec = packet_of(x_dtype, w_dtype, n, w, {gy, gz, z, dz});
   int64_t blocks = 0;
   const int rc = x_dtype == KRSI_F32    ? run_packets<KRSI_F32>(vec, a, &blocks, stream)
                  : x_dtype == KRSI_BF16 ? run_packets<KRSI_BF16>(vec, a, &blocks, stream)

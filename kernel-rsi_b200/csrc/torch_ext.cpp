@@ -567,7 +567,7 @@ std::tuple<at::Tensor, at::Tensor> add_rmsnorm_bwd(const c10::optional<at::Tenso
   TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.numel() == z.size(0), "add_rmsnorm_bwd: bad rstd");
   TORCH_CHECK(!have_z || gz->sizes() == z.sizes(), "add_rmsnorm_bwd: gz must match z");
   if (!gy.has_value() || !gy->defined())
-    return {have_z ? gz->to(z.scalar_type()) : at::zeros_like(z), at::zeros_like(w)};
+    return {have_z ? gz->to(z.scalar_type(), /*non_blocking=*/false, /*copy=*/true) : at::zeros_like(z), at::zeros_like(w)};
   TORCH_CHECK(gy->sizes() == z.sizes(), "add_rmsnorm_bwd: gy must match z");
   c10::cuda::CUDAGuard guard(z.device());
   auto zc = packed(z), wc = packed(w), rc = rstd.contiguous();
@@ -919,11 +919,12 @@ struct AddRmsnormNode : public torch::autograd::Function<AddRmsnormNode> {
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     check_once("add_rmsnorm");
     const auto saved = ctx->get_saved_variables();
-    if (!g[0].defined() && !g[1].defined()) return {at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const bool add = ctx->saved_data["add"].toBool();
+    if (!g[0].defined()) return {g[1], add ? g[1] : at::Tensor(), at::Tensor(), at::Tensor()};   // (z's alone, or none)
     at::AutoDispatchBelowADInplaceOrView below;
     auto opt = [](const at::Tensor& t) { return t.defined() ? c10::optional<at::Tensor>(t) : c10::nullopt; };
-    auto [dz, dw] = KRSI_OP(add_rmsnorm_bwd).call(opt(g[0]), opt(g[1]), saved[0], saved[1], saved[2]);
-    return {dz, ctx->saved_data["add"].toBool() ? dz : at::Tensor(), dw, at::Tensor()};
+    auto [dz, dw] = KRSI_OP(add_rmsnorm_bwd).call(g[0], opt(g[1]), saved[0], saved[1], saved[2]);
+    return {dz, add ? dz : at::Tensor(), dw, at::Tensor()};
   }
 };
 std::tuple<at::Tensor, at::Tensor> add_rmsnorm_autograd(const at::Tensor& x, const c10::optional<at::Tensor>& res,

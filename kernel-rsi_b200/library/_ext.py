@@ -47,8 +47,10 @@ capi.krsi_device_status.argtypes = [ctypes.POINTER(ctypes.c_int), ctypes.c_int]
 if not hasattr(torch.ops, "krsi") or not hasattr(torch.ops.krsi, "rmsnorm_fwd"):
     torch.ops.load_library(str(TORCH_EXT_PATH))
 ops = torch.ops.krsi
-_spec = importlib.util.spec_from_file_location("_krsi_torch", TORCH_EXT_PATH)
-direct = importlib.util.module_from_spec(_spec)   # functions of Python lists (the same library: loaded once)
+# Functions of Python lists, of the same library (loaded once); None where the operators came from another file.
+direct = None
+if os.path.realpath(TORCH_EXT_PATH) in map(os.path.realpath, torch.ops.loaded_libraries):
+    direct = importlib.util.module_from_spec(importlib.util.spec_from_file_location("_krsi_torch", TORCH_EXT_PATH))
 
 
 def device_status(clear: bool = False) -> int:

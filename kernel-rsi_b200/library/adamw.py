@@ -41,7 +41,7 @@ def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.
     device_lr = isinstance(lr, torch.Tensor)
     args = (params, grads, exp_avgs, exp_avg_sqs, masters or [], exponents or [], step, lr if device_lr else None,
             0.0 if device_lr else lr, betas[0], betas[1], eps, weight_decay, max_norm)
-    norm = NotImplemented if compiling() else direct.adamw_step(*args)
+    norm = NotImplemented if direct is None or compiling() else direct.adamw_step(*args)
     if norm is NotImplemented:
         norm = ops.adamw_step(*args)
     return norm if max_norm > 0 else None

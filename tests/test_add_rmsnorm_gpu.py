@@ -4,11 +4,14 @@ can go wrong.
 Tolerances: u is half a step of a type relative to the value (torch.finfo(t).eps / 2).  z is exact (one rounding,
 done alike).  y, dz and dw are rounded once; fp32 sums of k terms in chains of at most k / 32 + 32 are off by that many
 2^-24 of the sum of magnitudes."""
+import ctypes
+
 import pytest
 import torch
 
 import _ext
 from add_rmsnorm import add_rmsnorm, add_rmsnorm_q8
+from gpu_util import DT, capi, ptr, stream
 from linear_q8 import dequantise
 
 pytestmark = pytest.mark.gpu
@@ -146,6 +149,49 @@ def test_layouts_and_streams():
     gy_t = gy.t().contiguous().t()
     got = torch.autograd.grad(out, args, (gy_t, odd[1:].view(40, 264)))
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_the_same_operand_twice():
+    """x as its own residual: both gradients reach it."""
+    x, _, w, gy, gz = inputs(40, 264, BF16, BF16)
+    leaf, lw = x.clone().requires_grad_(True), w.clone().requires_grad_(True)
+    y, z = add_rmsnorm(leaf, leaf, lw, EPS)
+    (dx,) = torch.autograd.grad((y, z), leaf, (gy, gz))
+    _, dz, _, size, _ = formula(z, w, gy, gz)
+    ux = u(BF16)   # dz is rounded once, twice it once more
+    assert ((dx.double() - 2 * dz).abs() <= 2.1 * 2 * ux * dz.abs() + 4 * (264 / 32 + 64) * 2 ** -24 * size + 1e-30).all()
+
+
+@pytest.mark.parametrize("dt,wt", TYPES)
+@pytest.mark.parametrize("off", [4, 8])
+def test_c_abi_at_addresses_off_16_bytes(dt, wt, off):
+    """Every operand, the weight among them, `off` bytes past a 16-byte boundary; rows of whole 8 bytes, and odd ones."""
+    lib = capi()
+    for n, d in ((5, 260), (5, 264), (3, 77)):
+        x, res, w, gy, gz = inputs(n, d, dt, wt)
+
+        def shifted(t):
+            k = off // t.element_size()
+            room = torch.zeros(t.numel() + k, dtype=t.dtype, device=dev)
+            room[k:] = t.reshape(-1)
+            return room[k:].view(t.shape)
+
+        a = [shifted(t) for t in (x, res, w, gy, gz)]
+        y, z, dz, dw = (shifted(torch.zeros_like(t)) for t in (x, x, x, w))
+        rstd, scale = torch.zeros(n, device=dev), torch.zeros(n, device=dev)
+        q = shifted(torch.zeros(n, d, dtype=torch.uint8, device=dev))
+        ws = torch.zeros(n * d, device=dev)
+        i64, kinds = ctypes.c_int64, (ctypes.c_int64(n), ctypes.c_int64(d))
+        eps = ctypes.c_float(EPS)
+        assert lib.krsi_add_rmsnorm_fwd(*map(ptr, (a[0], a[1], a[2], z, y, rstd)), *kinds, eps, DT[dt], DT[wt], stream()) == 0
+        assert lib.krsi_add_rmsnorm_bwd(*map(ptr, (a[3], a[4], z, a[2], rstd, dz, dw, ws)), ctypes.c_size_t(n * d * 4),
+                                        *kinds, DT[dt], DT[wt], stream()) == 0
+        assert torch.equal(z, x + res)
+        check(z, w, gy, gz, y, dz, dw)
+        assert lib.krsi_add_rmsnorm_q8_fwd(*map(ptr, (a[0], a[1], a[2], z, q)), i64(d), ptr(scale), *kinds, eps, DT[dt],
+                                           DT[wt], stream()) == 0
+        assert torch.equal(q, codes(z, w)[0].view(torch.uint8))
+    torch.cuda.synchronize()
 
 
 def test_empty():

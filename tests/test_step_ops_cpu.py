@@ -51,6 +51,17 @@ def test_fake_impls_give_the_shapes():
     assert out.shape == (6, 24) and out.dtype == torch.float16
 
 
+def test_lists_have_their_way_past_the_dispatcher():
+    import adamw
+
+    assert adamw.direct is not None and callable(adamw.direct.adamw_step)
+    x, step = torch.zeros(4), torch.zeros((), dtype=torch.int64)
+    args = ([x], [x], [x], [x], [], [], step, None, 1e-3, 0.9, 0.999, 1e-8, 0.0, 0.0)
+    assert adamw.direct.adamw_step(*args) is NotImplemented       # no CUDA tensors: the operator's to refuse
+    with pytest.raises(TypeError):
+        adamw.direct.adamw_step(x)
+
+
 def test_cpu_tensors_are_rejected():
     import adamw
     import add_rmsnorm
@@ -121,6 +132,6 @@ def test_adamw_argument_checks(lib):
     assert f(p_dtype=5) == f(state_bits=16) == f(p_dtype=BF16, g_dtype=F16) == f(p_dtype=F32, g_dtype=BF16) == 1
     assert f(state_bits=8) == 1                                   # no exponents
     assert f(master=16) == 1                                      # of an fp32 parameter
-    assert f(beta1=1.0) == f(beta2=-0.1) == f(eps=-1.0) == f(max_norm=-1.0) == f(max_norm=1.0) == 1
+    assert f(beta1=1.0) == f(beta2=-0.1) == f(eps=-1.0) == f(max_norm=-1.0) == f(max_norm=1.0) == f(max_norm=1e-60, norm=16) == 1
     assert f(state_bits=8, exponents=17) == 3 and f(ws=8) == 3
     assert f(ws=0) == f(room=64) == 4
