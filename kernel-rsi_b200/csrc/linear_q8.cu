@@ -52,6 +52,7 @@ struct Q8Args {
   int n_tiles;        // row tiles x column tiles
   int n_kb;           // K blocks
   int q_rows, stages; // one CTA: rows of q in a stage, stages
+  int unit;           // bytes that every row of out starts on: 8, 4 or less (16: TMA stores)
   bool vec_scale;     // wscale starts on 16 bytes
   uint32_t spin_limit;
 };
@@ -91,10 +92,33 @@ __device__ __forceinline__ void mma_q8_pair_e(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
+// A box of rows that start on a U but not on 16 bytes: consecutive lanes on consecutive U.  `at(r, byte)`: the box in
+// shared memory; out: its first value, rows M values apart; `cols`, `rows`: what is left of the matrix from there.
+// (17261 x 965 to M bf16, indexed value by value it took 96 to 99 us: 76 for M 3436 by 8 bytes, 80 for 3438
+// by 4, 87 for 3439 by 2; 71 for 3440 by TMA.  Words put together from an odd row's neighbouring values: 102.)
+template <typename T, typename U, int ROWB, typename At>
+__device__ __forceinline__ void store_box(At at, T* out, int M, int cols, int rows, int lane) {
+  constexpr int kUnits = ROWB / (int)sizeof(U), kLanes = kUnits < 32 ? kUnits : 32;
+  constexpr int kRowsAtOnce = 32 / kLanes, kTurns = 32 / kRowsAtOnce, kPer = sizeof(U) / sizeof(T);
+  const int r0 = lane / kLanes;
+#pragma unroll
+  for (int h = 0; h < kUnits; h += kLanes) {
+    const int u = h + lane % kLanes;
+    const int left = u * kPer < cols ? rows - r0 : 0;
+    U val[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) val[k] = *reinterpret_cast<const U*>(at(r0 + k * kRowsAtOnce, u * (int)sizeof(U)));
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k)
+      if (k * kRowsAtOnce < left)
+        *reinterpret_cast<U*>(out + (int64_t)(r0 + k * kRowsAtOnce) * M + u * kPer) = val[k];
+  }
+}
+
 // The epilogue of one warp: 32 rows (TMEM lanes) x `cols` columns of each of the CTA's tiles, ROWB bytes of each row at
 // a time.  A lane has a row of the accumulator, and writes its packets to one of the warp's two boxes in shared memory
-// (rows of ROWB bytes, swizzled).  VEC, rows of out that start on 16 bytes: boxes leave by TMA stores; else by stores
-// value by value.  `row_of(t)`: the first row of a tile for this CTA.
+// (rows of ROWB bytes, swizzled).  VEC, rows of out that start on 16 bytes: boxes leave by TMA stores; else by store_box.
+// `row_of(t)`: the first row of a tile for this CTA.
 template <int DT, bool VEC, int ROWB, typename RowOf, typename Release>
 __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int acc_cols, int cols, int warp, int lane,
                                             Tiles tiles, uint64_t* acc_full, volatile int* abort_flag, const Q8Args& a,
@@ -182,23 +206,14 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
           tma_store_2d(&a.omap, out_box, col, row0);
           bulk_commit_group();
         }
-      } else {               // value by value, consecutive lanes on consecutive columns
+      } else {
         __syncwarp();
-        constexpr int kWide = kStep < 32 ? kStep : 32, kRowsAtOnce = 32 / kWide, kTurns = 32 / kRowsAtOnce;
-        const int r0 = lane / kWide;
-#pragma unroll
-        for (int h = 0; h < kStep; h += kWide) {
-          const int e = h + lane % kWide;
-          T* out = static_cast<T*>(a.out) + (int64_t)(row0 + r0) * a.M + col + e;
-          const int left = col + e < a.M ? a.rows - row0 - r0 : 0;
-          T val[kTurns];
-#pragma unroll
-          for (int k = 0; k < kTurns; ++k)
-            val[k] = reinterpret_cast<const T*>(packet(out_box, r0 + k * kRowsAtOnce, e / kPer))[e % kPer];
-#pragma unroll
-          for (int k = 0; k < kTurns; ++k)
-            if (k * kRowsAtOnce < left) out[(int64_t)k * kRowsAtOnce * a.M] = val[k];
-        }
+        const int left = a.rows - row0;
+        T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.M + col;
+        auto at = [&](int r, int byte) { return packet(out_box, r, byte >> 4) + (byte & 15); };
+        if (a.unit == 8) store_box<T, uint64_t, ROWB>(at, out, a.M, a.M - col, left, lane);
+        else if (sizeof(T) == 4 || a.unit == 4) store_box<T, uint32_t, ROWB>(at, out, a.M, a.M - col, left, lane);
+        else if constexpr (sizeof(T) == 2) store_box<T, uint16_t, ROWB>(at, out, a.M, a.M - col, left, lane);
         __syncwarp();
       }
     }
@@ -651,6 +666,8 @@ extern "C" int krsi_linear_q8(const void* q, int64_t q_stride, const float* scal
   a.rows = (int)rows;
   a.M = (int)M;
   a.n_kb = (int)((K + kBK - 1) / kBK);
+  for (a.unit = 8; (reinterpret_cast<uintptr_t>(out) | (uintptr_t)(M * es)) & (a.unit - 1); a.unit /= 2) {
+  }
   a.vec_scale = aligned16(wscale);
   a.spin_limit = kSpinLimit;
 #define KRSI_OUT(DT)                                                            \
