@@ -52,7 +52,7 @@ struct Q8Args {
   int n_tiles;        // row tiles x column tiles
   int n_kb;           // K blocks
   int q_rows, stages; // one CTA: rows of q in a stage, stages
-  int unit;           // bytes that every row of out starts on: 8, 4 or less (16: TMA stores)
+  int unit;           // bytes that every row of out starts on: 8, 4 or less (16: TMA stores); of 16-bit types
   bool vec_scale;     // wscale starts on 16 bytes
   uint32_t spin_limit;
 };
@@ -92,10 +92,10 @@ __device__ __forceinline__ void mma_q8_pair_e(uint32_t d_tmem, uint64_t a_desc, 
       : "memory");
 }
 
-// A box of rows that start on a U but not on 16 bytes: consecutive lanes on consecutive U.  `at(r, byte)`: the box in
-// shared memory; out: its first value, rows M values apart; `cols`, `rows`: what is left of the matrix from there.
-// (17261 x 965 to M bf16, indexed value by value it took 96 to 99 us: 76 for M 3436 by 8 bytes, 80 for 3438
-// by 4, 87 for 3439 by 2; 71 for 3440 by TMA.  Words put together from an odd row's neighbouring values: 102.)
+// A box of rows of 16-bit values that start on a U but not on 16 bytes: consecutive lanes on consecutive U.  `at(r, byte)`:
+// the box in shared memory; out: its first value, rows M values apart; `cols`, `rows`: what is left of the matrix from
+// there.  (17261 x 965 to M bf16, indexed value by value it took 96 to 99 us: 76 for M 3436 by 8 bytes, 80 for 3438 by 4, 87
+// for 3439 by 2; 71 for 3440 by TMA.  As LooseRows: 86, 93 and 98, for the shifts by half a word and longer ends.)
 template <typename T, typename U, int ROWB, typename At>
 __device__ __forceinline__ void store_box(At at, T* out, int M, int cols, int rows, int lane) {
   constexpr int kUnits = ROWB / (int)sizeof(U), kLanes = kUnits < 32 ? kUnits : 32;
@@ -115,15 +115,83 @@ __device__ __forceinline__ void store_box(At at, T* out, int M, int cols, int ro
   }
 }
 
+// 32 rows of fp32 that do not start on 16 bytes: each lane writes its own row to shared memory where the values lie in
+// the 32-byte sectors of memory, and the row's packets are read and stored whole.  What passes the end of a box comes
+// first in the next one; only the packets at both ends of a row leave value by value.  (17261 x 965 to 3439 fp32: 99 us;
+// as words of a box, lane by lane, 115; 3440 by TMA: 85.  An even M, whose lanes share banks: 108 either way for 3438.)
+template <int ROWB>
+struct LooseRows {
+  static constexpr int kBox = ROWB / 4;   // values of a row in a box
+  // Where row r starts in a box: between two rows is room for what passes the end (which nothing reads there); 8 values
+  // more every 8 rows put lanes of different shift or row / 8 on different banks.
+  static __device__ __forceinline__ int at(int r) { return 8 + r * (kBox + 8) + (r >> 3) * 8; }
+
+  float* box;
+  float* out;            // the first value of the rows
+  int M, n, rows, lane;  // values between two rows; of each row; rows that are left
+  int own;               // the values of a sector before this lane's row
+  float carry[8];        // the last values of the box before
+
+  __device__ __forceinline__ LooseRows(uint8_t* box_, float* out_, int M_, int n_, int rows_, int lane_)
+      : box(reinterpret_cast<float*>(box_)), out(out_), M(M_), n(n_), rows(rows_), lane(lane_), own(shift(lane_)) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) carry[i] = 0.f;
+  }
+  __device__ __forceinline__ int shift(int r) const {
+    return (int)(((uint32_t)(reinterpret_cast<uintptr_t>(out) / 4) + (uint32_t)r * (uint32_t)M) % 8);
+  }
+  __device__ __forceinline__ void begin() {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) box[at(lane) + own + i - 8] = carry[i];
+  }
+  __device__ __forceinline__ void put(int k, float v) {   // value k of this lane's row in the box
+    box[at(lane) + own + k] = v;
+    if (k >= kBox - 8) carry[k - (kBox - 8)] = v;
+  }
+  // PACKETS of each row of box b, and the ends of this lane's row.
+  template <int PACKETS>
+  __device__ __forceinline__ void leave(int b) {
+    constexpr int kRows = 32 / PACKETS, kTurns = 32 / kRows;
+    const int e0 = b * kBox + lane % PACKETS * 4;
+    __syncwarp();
+    float4 val[kTurns];
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k)
+      val[k] = *reinterpret_cast<const float4*>(box + at(k * kRows + lane / PACKETS) + lane % PACKETS * 4);
+#pragma unroll
+    for (int k = 0; k < kTurns; ++k) {
+      const int r = k * kRows + lane / PACKETS, e = e0 - shift(r);   // from the row's first value
+      if (r < rows && e >= 0 && e + 4 <= n) *reinterpret_cast<float4*>(out + (int64_t)r * M + e) = val[k];
+    }
+    if (lane < rows && n > 0) {
+      const float* row = box + at(lane);
+      float* to = out + (int64_t)lane * M - own;
+      const int end = own + n, last = end / 4 * 4;   // (`last`: the packet that the row ends in)
+#pragma unroll
+      for (int k = 0; k < 3; ++k) {
+        if (b == 0 && own + k < end && own + k < (own + 3) / 4 * 4) to[own + k] = row[own + k];
+        if (last >= b * kBox && last < b * kBox + PACKETS * 4 && last + k < end && last + k >= own)
+          to[last + k] = row[last + k - b * kBox];
+      }
+    }
+    __syncwarp();
+  }
+  __device__ __forceinline__ void finish(int b) {   // what passed the end of the last box, b - 1
+    begin();
+    leave<2>(b);
+  }
+};
+
 // The epilogue of one warp: 32 rows (TMEM lanes) x `cols` columns of each of the CTA's tiles, ROWB bytes of each row at
 // a time.  A lane has a row of the accumulator, and writes its packets to one of the warp's two boxes in shared memory
-// (rows of ROWB bytes, swizzled).  VEC, rows of out that start on 16 bytes: boxes leave by TMA stores; else by store_box.
-// `row_of(t)`: the first row of a tile for this CTA.
+// (rows of ROWB bytes, swizzled).  VEC, rows of out that start on 16 bytes: boxes leave by TMA stores; else by
+// LooseRows (fp32) or store_box.  `row_of(t)`: the first row of a tile for this CTA.
 template <int DT, bool VEC, int ROWB, typename RowOf, typename Release>
 __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int acc_cols, int cols, int warp, int lane,
                                             Tiles tiles, uint64_t* acc_full, volatile int* abort_flag, const Q8Args& a,
                                             RowOf row_of, Release release) {
   using T = typename Elem<DT>::T;
+  constexpr bool kLoose = !VEC && DT == KRSI_F32;
   constexpr int kPer = 16 / (int)sizeof(T);          // values of a packet
   constexpr int kStep = ROWB / (int)sizeof(T);       // columns of a box
   constexpr int kLoad = kStep < 32 ? kStep : 32;     // columns read from TMEM at a time
@@ -149,6 +217,8 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
     }
     tc_fence_after();
     const uint32_t acc_addr = tmem + lane_addr + acc * acc_cols + part * cols;
+    LooseRows<ROWB> loose(box, static_cast<float*>(a.out) + (int64_t)row0 * a.M + c_base, a.M,
+                          a.M - c_base < cols ? a.M - c_base : cols, a.rows - row0, lane);   // (kLoose alone)
 #pragma unroll 1
     for (int c0 = 0; c0 < cols; c0 += kStep, turn ^= 1) {
       uint8_t* out_box = box + turn * (32 * ROWB);
@@ -175,6 +245,7 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
           __syncwarp();
           if (lane == 0) release(acc);
         }
+        if (kLoose && h == 0) loose.begin();
         if (VEC && h == 0) {
           if (lane == 0) bulk_wait_read_but_one();   // the box before the last one has been read
           __syncwarp();
@@ -195,7 +266,12 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
               u[k] = DT == KRSI_F16 ? pack_f16x2(lo, hi) : pack_bf16x2(lo, hi);
             }
           }
-          *reinterpret_cast<uint4*>(packet(out_box, lane, h / kPer + p)) = make_uint4(u[0], u[1], u[2], u[3]);
+          if constexpr (kLoose) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) loose.put(h + p * 4 + k, __uint_as_float(u[k]));
+          } else {
+            *reinterpret_cast<uint4*>(packet(out_box, lane, h / kPer + p)) = make_uint4(u[0], u[1], u[2], u[3]);
+          }
         }
       }
       const int col = c_base + c0;
@@ -206,17 +282,20 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
           tma_store_2d(&a.omap, out_box, col, row0);
           bulk_commit_group();
         }
+      } else if constexpr (kLoose) {
+        loose.template leave<ROWB / 16>(c0 / kStep);
       } else {
         __syncwarp();
         const int left = a.rows - row0;
         T* out = static_cast<T*>(a.out) + (int64_t)row0 * a.M + col;
         auto at = [&](int r, int byte) { return packet(out_box, r, byte >> 4) + (byte & 15); };
         if (a.unit == 8) store_box<T, uint64_t, ROWB>(at, out, a.M, a.M - col, left, lane);
-        else if (sizeof(T) == 4 || a.unit == 4) store_box<T, uint32_t, ROWB>(at, out, a.M, a.M - col, left, lane);
-        else if constexpr (sizeof(T) == 2) store_box<T, uint16_t, ROWB>(at, out, a.M, a.M - col, left, lane);
+        else if (a.unit == 4) store_box<T, uint32_t, ROWB>(at, out, a.M, a.M - col, left, lane);
+        else store_box<T, uint16_t, ROWB>(at, out, a.M, a.M - col, left, lane);
         __syncwarp();
       }
     }
+    if constexpr (kLoose) loose.finish(cols / kStep);
   }
   if (VEC && lane == 0) bulk_wait_all();   // every store has completed before the CTA exits
   return ok;
