@@ -182,12 +182,13 @@ struct LooseRows {
   }
 };
 
-// The epilogue of one warp: 32 rows (TMEM lanes) x `cols` columns of each of the CTA's tiles, ROWB bytes of each row at
-// a time.  A lane has a row of the accumulator, and writes its packets to one of the warp's two boxes in shared memory
-// (rows of ROWB bytes, swizzled).  VEC, rows of out that start on 16 bytes: boxes leave by TMA stores; else by
-// LooseRows (fp32) or store_box.  `row_of(t)`: the first row of a tile for this CTA.
+// The epilogue of one warp: 32 rows (TMEM lanes) x the first `first` columns of each of the CTA's tiles, or the others,
+// ROWB bytes of each row at a time (both parts are whole boxes, one at least).  A lane has a row of the accumulator, and
+// writes its packets to one of the warp's two boxes in shared memory (rows of ROWB bytes, swizzled).  VEC, rows of out that
+// start on 16 bytes: boxes leave by TMA stores; else by LooseRows (fp32) or store_box.  `row_of(t)`: the first row of a tile
+// for this CTA.
 template <int DT, bool VEC, int ROWB, typename RowOf, typename Release>
-__device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int acc_cols, int cols, int warp, int lane,
+__device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int acc_cols, int first, int warp, int lane,
                                             Tiles tiles, uint64_t* acc_full, volatile int* abort_flag, const Q8Args& a,
                                             RowOf row_of, Release release) {
   using T = typename Elem<DT>::T;
@@ -196,7 +197,8 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
   constexpr int kStep = ROWB / (int)sizeof(T);       // columns of a box
   constexpr int kLoad = kStep < 32 ? kStep : 32;     // columns read from TMEM at a time
   const int ew = warp - kEpiWarp0;
-  const int quarter = ew % 4, part = ew / 4;  // TMEM lane quarter; which `cols` of the tile's columns
+  const int quarter = ew % 4, part = ew / 4;  // TMEM lane quarter; which of the tile's columns
+  const int base = part * first, cols = part ? a.bn - first : first;
   const uint32_t lane_addr = (uint32_t)(quarter * 32) << 16;
   uint8_t* box = boxes + ew * 2 * (32 * ROWB);
   // packet p of row r: the 128- or 64-byte swizzle
@@ -208,7 +210,7 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
   for (int i = 0; tiles.next(); ++i) {
     const int acc = i & 1;
     const int row0 = row_of(tiles) + quarter * 32;
-    const int c_base = tiles.col * a.bn + part * cols;
+    const int c_base = tiles.col * a.bn + base;
     const float s = row0 + lane < a.rows ? __ldg(a.scale + row0 + lane) : 0.f;
     const uint64_t s2 = f2_pack(s, s);
     if (!__all_sync(0xffffffffu, mbar_wait_bounded(&acc_full[acc], (i >> 1) & 1, abort_flag, a.spin_limit))) {
@@ -216,7 +218,7 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
       break;
     }
     tc_fence_after();
-    const uint32_t acc_addr = tmem + lane_addr + acc * acc_cols + part * cols;
+    const uint32_t acc_addr = tmem + lane_addr + acc * acc_cols + base;
     LooseRows<ROWB> loose(box, static_cast<float*>(a.out) + (int64_t)row0 * a.M + c_base, a.M,
                           a.M - c_base < cols ? a.M - c_base : cols, a.rows - row0, lane);   // (kLoose alone)
 #pragma unroll 1
@@ -590,8 +592,9 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     }
   } else if (warp >= kEpiWarp0) {
     // ------------------------------------------------------------ epilogue (both CTAs, own rows)
+    constexpr int kStep = kPairRowB / (int)sizeof(typename Elem<DT>::T);   // columns of a box
     const bool ok = q8_epilogue<DT, VEC, kPairRowB>(
-        smem + kPairBoxOff, tmem, kPairBN, a.bn / 2, warp, lane, tiles, acc_full, abort_flag, a,
+        smem + kPairBoxOff, tmem, kPairBN, (a.bn / kStep + 1) / 2 * kStep, warp, lane, tiles, acc_full, abort_flag, a,
         [&](const Tiles& t) { return t.row * (2 * kBM) + (int)rank * kBM; },
         [&](int acc) {
           if (even) mbar_arrive(&acc_empty[acc]);
@@ -672,16 +675,16 @@ bool output_map(Q8Args& a, int dt, int row_bytes) {
 
 // Columns of a pair's tile: the width that takes least by this count of cycles.  A K block costs its MMAs (2 cycles a
 // column) or its operands' way from the L2 (some 48 bytes a cycle), whichever is longer; a tile 400 cycles more, and the
-// last one's epilogue is not hidden.  (2001 x 1000 x 2743 to fp32: 192 columns, in two rounds of tiles where 256 take two
-// as well.)  A warp's output box holds 64 columns of 16 bits, or 32 of fp32.
-int tile_columns(int64_t row_tiles, int64_t M, int n_kb, int pairs, bool f32) {
+// last one's epilogue (its longer part) is not hidden.  Widths are whole output boxes (`step` columns: 64 of 16 bits, 32 of
+// fp32).  (2001 x 1000 x 2743 to fp32: 160 columns 16.1 us, 192 17.6, 256 19.4, all in two rounds of tiles, 128 in three
+// 19.1; 700 x 1152 x 4608 to bf16: 192 columns 8.8 us, 256 9.7, 128 11.0.)
+int tile_columns(int64_t row_tiles, int64_t M, int n_kb, int pairs, int step) {
   int best = kPairBN;
   int64_t least = INT64_MAX;
-  for (int bn : {256, 192, 128, 64}) {
-    if (!f32 && bn % 128 != 0) continue;
+  for (int bn = kPairBN; bn >= 2 * step; bn -= step) {
     const int64_t rounds = (row_tiles * ((M + bn - 1) / bn) + pairs - 1) / pairs;
     const int64_t block = 2 * bn > (16384 + 64 * bn) / 48 ? 2 * bn : (16384 + 64 * bn) / 48;
-    const int64_t cycles = rounds * (n_kb * block + 400) + 12 * bn;
+    const int64_t cycles = rounds * (n_kb * block + 400) + 20 * ((bn / step + 1) / 2 * step);
     if (cycles < least) {
       least = cycles;
       best = bn;
@@ -694,7 +697,7 @@ template <int DT, bool VEC>
 int launch(const void* q, int64_t q_pitch, const void* wq, int64_t w_pitch, int64_t K, Q8Args a, cudaStream_t stream) {
   const int clusters = a.rows > kBM ? pair_clusters<DT, VEC>() : 0;
   const int64_t bm = clusters > 0 ? 2 * kBM : kBM, rt = ((int64_t)a.rows + bm - 1) / bm;
-  a.bn = clusters > 0 ? tile_columns(rt, a.M, a.n_kb, clusters, DT == KRSI_F32) : kOneBN;
+  a.bn = clusters > 0 ? tile_columns(rt, a.M, a.n_kb, clusters, kPairRowB / (int)sizeof(typename Elem<DT>::T)) : kOneBN;
   const int64_t ct = ((int64_t)a.M + a.bn - 1) / a.bn;
   if (rt * ct > INT32_MAX / 2) return KRSI_ERR_UNSUPPORTED;
   a.n_ctiles = (int)ct;

@@ -44,6 +44,18 @@ def test_against_float64(rows, K, M, dtype):
     assert _ext.device_status() == 0
 
 
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("M", [-1, 0, 2])
+@pytest.mark.parametrize("rows,K,M0", [(260, 642, 2400), (257, 145, 3624), (257, 1061, 4768), (523, 86, 3888),
+                                       (521, 902, 4640), (781, 1033, 4056)])
+def test_widths_of_tiles(rows, K, M0, M, dtype):
+    """On 148 SMs: fp32 tiles of 96 to 256 columns, 16-bit ones of 128 to 256, uneven parts among them; rows of out on
+    16, 8 or 4 bytes and less."""
+    ops = operands(rows, K, M0 + M)
+    check(linear_q8(*ops, dtype), *ops)
+    assert _ext.device_status() == 0
+
+
 @pytest.mark.parametrize("rows", [64, 400])
 def test_whole_numbers_are_exact(rows):
     """Small whole numbers have exact products and sums: every element, whatever the order."""
