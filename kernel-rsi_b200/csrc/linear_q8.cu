@@ -75,21 +75,44 @@ struct Tiles {
 // kind::f8f6f4, both operands e4m3 (format 0), K-major, fp32 sums: the bit layout is idesc_f16's.
 __host__ __device__ constexpr uint32_t idesc_e4m3(uint32_t M, uint32_t N) { return idesc_f16(M, N, 0, false, false); }
 
-__device__ __forceinline__ void mma_q8_e(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                         uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
-      : "memory");
+// One lane of a converged warp.  It alone runs the producer's or the issuer's loop: where all 32 lanes waited, voted and
+// elected for each instruction a K block took 430 cycles to issue (2048 x 4608 x 1152 to bf16: 16.7 us, 12.7 by one lane).
+__device__ __forceinline__ bool elect_one() {
+  uint32_t e;
+  asm volatile("{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\tselp.u32 %0, 1, 0, e;\n\t}" : "=r"(e));
+  return e != 0;
 }
-__device__ __forceinline__ void mma_q8_pair_e(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
-                                              uint32_t accumulate) {
+// Whether `bar` has reached the phase, without waiting.  With up to 128 rows the issuer asks for the next stage before it
+// issues this one's MMAs, which hide the 220 cycles of an answer (16 x 4608 x 1152: 10.9 us became 9.95).  The pair kernel,
+// which waits for its operands, does not: 700 x 1152 x 4608 to fp32 took 11.6 us instead of 9.3.
+__device__ __forceinline__ uint32_t mbar_test(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
   asm volatile(
-      "{\n\t.reg .pred e, p;\n\telect.sync _|e, 0xffffffff;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "@e tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
-      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+      "{\n\t.reg .pred p;\n\tmbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
       : "memory");
+  return ok;
+}
+template <int CTAS>
+__device__ __forceinline__ void mma_q8(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                       uint32_t accumulate) {
+  if constexpr (CTAS == 1)
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+  else
+    asm volatile(
+        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}" ::"r"(d_tmem),
+        "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate)
+        : "memory");
+}
+// Arrive on `bar` (an address in the cluster) when every MMA that this thread issued so far has completed.
+__device__ __forceinline__ void mma_commit_pair(uint32_t bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
 }
 
 // A box of rows of 16-bit values that start on a U but not on 16 bytes: consecutive lanes on consecutive U.  `at(r, byte)`:
@@ -305,12 +328,12 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
 
 // ---------------------------------------------------------------- up to 128 rows: one CTA, narrow tiles
 // The weight comes from memory, so its K blocks in flight are what counts: a stage's tile of q has only as many rows as
-// there are, up to eight more (a.q_rows), which leaves room for up to 20 stages of the weight's 8 KB instead of 8.  An
+// there are, up to eight more (a.q_rows), which leaves room for up to 20 K blocks of the weight's 8 KB instead of 8.  An
 // MMA nevertheless reads 128 rows: what follows in shared memory, whatever it is, makes rows of the accumulator that
-// nothing reads.  (4 rows of 2792 over 7843: 17.3 us with 8 stages
-// became 9.8.)
+// nothing reads.  (4 rows of 2792 over 7843: 17.3 us with 8 blocks became 9.8.)  A stage has two K blocks, for half the
+// waits and commits: 16 x 4608 x 1152 9.95 us became 9.3.
 constexpr int kOneBN = 64;
-constexpr int kOneMaxStages = 20;
+constexpr int kOneMaxStages = 10;   // of two K blocks
 constexpr uint32_t kOneWTile = kOneBN * kBK;                         // 8 KB
 constexpr int kOneRowB = 64;                                         // bytes of a row in an output box
 constexpr uint32_t kOneRing = 8 * (kATile + kOneWTile);              // 192 KB
@@ -336,7 +359,7 @@ struct Ring {
 
 // Stages for a.q_rows rows.  The tiles of q come first, so an MMA on the last one reads on into the weight's.
 inline int one_stages(int q_rows) {
-  const int n = (int)(kOneRing / (q_rows * kBK + kOneWTile));
+  const int n = (int)(kOneRing / (2 * (q_rows * kBK + kOneWTile)));
   return n < kOneMaxStages ? n : kOneMaxStages;
 }
 
@@ -357,7 +380,7 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
 
   const int warp = threadIdx.x / 32, lane = threadIdx.x % 32;
   Tiles tiles(a, blockIdx.x, gridDim.x);
-  const uint32_t q_bytes = (uint32_t)a.q_rows * kBK, w_off = a.stages * q_bytes;
+  const uint32_t q_bytes = (uint32_t)a.q_rows * kBK, w_off = 2 * a.stages * q_bytes;
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < a.stages; ++s) {
@@ -385,27 +408,29 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
 
-  if (warp == 0) {
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit); };
+
+  if (warp == 0 && elect_one()) {
     // ------------------------------------------------------------ TMA producer
     bool ok = true;
     Ring ring;
     int it = 0;
     while (ok && tiles.next()) {
       const int m0 = tiles.row * kBM, n0 = tiles.col * kOneBN;
-      for (int kb = 0; kb < a.n_kb; ++kb, ++it) {
-        const int s = ring.slot;
-        if (it >= a.stages &&
-            !__all_sync(0xffffffffu, mbar_wait_bounded(&empty[s], ring.parity ^ 1, abort_flag, a.spin_limit))) {
+      for (int kb = 0; kb < a.n_kb; kb += 2, ++it) {
+        const int s = ring.slot, blocks = kb + 1 < a.n_kb ? 2 : 1;
+        if (it >= a.stages && !wait(&empty[s], ring.parity ^ 1)) {
           ok = false;
           break;
         }
         ring.next(a.stages);
-        if (lane == 0) {
-          mbar_arrive_expect_tx(&full[s], q_bytes + kOneWTile);
-          tma_load_2d(smem + w_off + s * kOneWTile, &wmap, &full[s], kb * kBK, n0);
-          tma_load_2d(smem + s * q_bytes, &qmap, &full[s], kb * kBK, m0);
+        mbar_arrive_expect_tx(&full[s], blocks * (q_bytes + kOneWTile));
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          if (b >= blocks) break;
+          tma_load_2d(smem + w_off + (2 * s + b) * kOneWTile, &wmap, &full[s], (kb + b) * kBK, n0);
+          tma_load_2d(smem + (2 * s + b) * q_bytes, &qmap, &full[s], (kb + b) * kBK, m0);
         }
-        __syncwarp();
       }
     }
     if (!ok) {   // every load issued has landed before this CTA exits
@@ -414,15 +439,13 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         for (uint32_t n = 0; n < a.spin_limit && !mbar_try_wait(&full[j % a.stages], (j / a.stages) & 1); ++n) {
         }
     }
-  } else if (warp == 1) {
-    // ------------------------------------------------------------ MMA issuer (whole warp, elected lane)
-    auto wait = [&](uint64_t* bar, uint32_t parity) {
-      return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit));
-    };
+  } else if (warp == 1 && elect_one()) {
+    // ------------------------------------------------------------ MMA issuer
     constexpr uint32_t idesc = idesc_e4m3(kBM, kOneBN);
     const uint64_t q0 = kmajor_sw128(smem_u32(smem)), w0 = kmajor_sw128(smem_u32(smem + w_off));
     bool ok = true;
     Ring ring;
+    uint32_t ready = 0;
     for (int i = 0; ok && tiles.next(); ++i) {
       const int acc = i & 1;
       if (i >= 2 && !wait(&acc_empty[acc], ((i >> 1) - 1) & 1)) {
@@ -430,25 +453,30 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
         break;
       }
       tc_fence_after();
-      for (int kb = 0; kb < a.n_kb; ++kb) {
+      for (int kb = 0; kb < a.n_kb; kb += 2) {
         const int s = ring.slot;
-        if (!wait(&full[s], ring.parity)) {
+        if (!ready && !wait(&full[s], ring.parity)) {
           ok = false;
           break;
         }
         ring.next(a.stages);
+        ready = mbar_test(&full[ring.slot], ring.parity);
         tc_fence_after();
-        const uint64_t ad = q0 + (uint64_t)s * (q_bytes >> 4), bd = w0 + (uint64_t)s * (kOneWTile >> 4);
 #pragma unroll
-        for (int kk = 0; kk < kBK / 32; ++kk)
-          mma_q8_e(tmem + acc * kOneBN, ad + kk * 2, bd + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-        mma_commit_e(&empty[s]);
+        for (int b = 0; b < 2; ++b) {
+          if (kb + b >= a.n_kb) break;
+          const uint64_t ad = q0 + (uint64_t)(2 * s + b) * (q_bytes >> 4), bd = w0 + (uint64_t)(2 * s + b) * (kOneWTile >> 4);
+#pragma unroll
+          for (int kk = 0; kk < kBK / 32; ++kk)
+            mma_q8<1>(tmem + acc * kOneBN, ad + kk * 2, bd + kk * 2, idesc, (kb + b > 0 || kk > 0) ? 1u : 0u);
+        }
+        mma_commit(&empty[s]);
       }
       if (!ok) break;
-      mma_commit_e(&acc_full[acc]);
+      mma_commit(&acc_full[acc]);
     }
     if (!ok) watchdog_fire(kWdQ8Mma);
-    mma_commit_e(drain);   // every MMA issued above has completed before TMEM is released
+    mma_commit(drain);   // every MMA issued above has completed before TMEM is released
     for (uint32_t i = 0; i < a.spin_limit && !mbar_try_wait(drain, 0); ++i) {
     }
   } else if (warp >= kEpiWarp0) {
@@ -459,6 +487,7 @@ linear_q8_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_constant
     if (!ok) watchdog_fire(kWdQ8Epilogue);
   }
 
+  __syncwarp();   // (the lanes that were not elected)
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
@@ -524,11 +553,9 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
   cluster_sync();   // both CTAs' barriers initialised and TMEM allocated before either signals the other
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  auto wait = [&](uint64_t* bar, uint32_t parity) {   // whole warps
-    return __all_sync(0xffffffffu, mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit));
-  };
+  auto wait = [&](uint64_t* bar, uint32_t parity) { return mbar_wait_bounded(bar, parity, abort_flag, a.spin_limit); };
 
-  if (warp == 0) {
+  if (warp == 0 && elect_one()) {
     // ------------------------------------------------------------ TMA producer (both CTAs)
     bool ok = true;
     int it = 0;
@@ -541,22 +568,19 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
           ok = false;
           break;
         }
-        if (lane == 0) {
-          uint8_t* st = smem + s * kPairStageBytes;
-          const uint32_t bar = mapa_shared(&full[s], 0);
-          if (even) mbar_arrive_expect_tx(&full[s], 2 * (kATile + w_bytes));
-          tma_load_2d_pair(st, &qmap, bar, kb * kBK, m0);
-          tma_load_2d_pair(st + kATile, &wmap, bar, kb * kBK, n0);
-        }
-        __syncwarp();
+        uint8_t* st = smem + s * kPairStageBytes;
+        const uint32_t bar = mapa_shared(&full[s], 0);
+        if (even) mbar_arrive_expect_tx(&full[s], 2 * (kATile + w_bytes));
+        tma_load_2d_pair(st, &qmap, bar, kb * kBK, m0);
+        tma_load_2d_pair(st + kATile, &wmap, bar, kb * kBK, n0);
       }
     }
     if (!ok) {
       watchdog_fire(kWdQ8Load);
       if (even) drain_loads<kPairStages>(full, it, a.spin_limit);   // covers both CTAs' loads of each stage
     }
-  } else if (warp == 1 && even) {
-    // ------------------------------------------------------------ MMA issuer (even CTA, elected lane)
+  } else if (warp == 1 && even && elect_one()) {
+    // ------------------------------------------------------------ MMA issuer (even CTA)
     const uint32_t idesc = idesc_e4m3(2 * kBM, (uint32_t)a.bn);
     const uint64_t desc0 = kmajor_sw128(smem_u32(smem));
     bool ok = true;
@@ -578,16 +602,16 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
         const uint64_t ad = desc0 + (uint64_t)s * (kPairStageBytes >> 4), bd = ad + (kATile >> 4);
 #pragma unroll
         for (int kk = 0; kk < kBK / 32; ++kk)
-          mma_q8_pair_e(tmem + acc * kPairBN, ad + kk * 2, bd + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
-        mma_commit_pair_e(mapa_shared(&empty[s], 0));   // stage s free in both CTAs
-        mma_commit_pair_e(mapa_shared(&empty[s], 1));
+          mma_q8<2>(tmem + acc * kPairBN, ad + kk * 2, bd + kk * 2, idesc, (kb > 0 || kk > 0) ? 1u : 0u);
+        mma_commit_pair(mapa_shared(&empty[s], 0));   // stage s free in both CTAs
+        mma_commit_pair(mapa_shared(&empty[s], 1));
       }
       if (!ok) break;
-      mma_commit_pair_e(mapa_shared(&acc_full[acc], 0));
-      mma_commit_pair_e(mapa_shared(&acc_full[acc], 1));
+      mma_commit_pair(mapa_shared(&acc_full[acc], 0));
+      mma_commit_pair(mapa_shared(&acc_full[acc], 1));
     }
     if (!ok) watchdog_fire(kWdQ8Mma);
-    mma_commit_pair_e(mapa_shared(drain, 0));
+    mma_commit_pair(mapa_shared(drain, 0));
     for (uint32_t i = 0; i < a.spin_limit && !mbar_try_wait(drain, 0); ++i) {
     }
   } else if (warp >= kEpiWarp0) {
@@ -603,6 +627,7 @@ linear_q8_pair_kernel(const __grid_constant__ CUtensorMap qmap, const __grid_con
     if (!ok) watchdog_fire(kWdQ8Epilogue);
   }
 
+  __syncwarp();   // (the lanes that were not elected)
   tc_fence_before();
   cluster_sync();   // the even CTA's MMAs (which read this CTA's shared memory and TMEM) are done
   tc_fence_after();
