@@ -6,8 +6,8 @@
 //
 // Structure (as linear_geglu.cu): a persistent grid, 12 warps a CTA: warp 0 the TMA producer (128-byte swizzled
 // K-major tiles of 128 values), warp 1 the TMEM owner and issuer of tcgen05.mma kind::f8f6f4 (32 values of K an
-// instruction), warps 4-11 the epilogue.  Two accumulators alternate, so a tile's epilogue runs beside the next
-// tile's MMAs.
+// instruction), one lane of each, warps 4-11 the epilogue.  Two accumulators alternate, so a tile's epilogue runs beside
+// the next tile's MMAs.
 //   up to 128 rows    linear_q8_kernel: one CTA on tiles of 128 rows x 64 columns (the weight's read bounds it:
 //                     narrow tiles spread it over the SMs)
 //   more              linear_q8_pair_kernel: CTA pairs (cta_group::2) on tiles of 256 rows x up to 256 columns, all
