@@ -303,9 +303,9 @@ __device__ __forceinline__ bool q8_epilogue(uint8_t* boxes, uint32_t tmem, int a
       if constexpr (VEC) {
         fence_async_shared();
         __syncwarp();
-        if (lane == 0 && col < a.M && row0 < a.rows) {   // the map clips rows >= rows and columns >= M
-          tma_store_2d(&a.omap, out_box, col, row0);
-          bulk_commit_group();
+        if (lane == 0) {
+          if (col < a.M && row0 < a.rows) tma_store_2d(&a.omap, out_box, col, row0);   // (the map clips the box)
+          bulk_commit_group();   // of a box that stays too: the wait above counts groups
         }
       } else if constexpr (kLoose) {
         loose.template leave<ROWB / 16>(c0 / kStep);

@@ -56,6 +56,19 @@ def test_widths_of_tiles(rows, K, M0, M, dtype):
     assert _ext.device_status() == 0
 
 
+@pytest.mark.parametrize("rows,K,M,dtype", [(3748, 2608, 4768, F32), (3748, 300, 4768, F32), (3000, 256, 4704, F32),
+                                            (3748, 512, 4800, BF16), (3748, 130, 4736, F16), (100, 2000, 20488, F32)])
+def test_columns_end_inside_a_tile(rows, K, M, dtype):
+    """A tile's last boxes may lie past M: what is written to shared memory for them must not reach the boxes before,
+    which are still on their way to memory."""
+    g = torch.Generator(device=dev).manual_seed(5)
+    q, wq = (torch.randint(-3, 4, (n, K), generator=g, device=dev).to(torch.float8_e4m3fn) for n in (rows, M))
+    one = lambda n: torch.ones(n, device=dev)  # noqa: E731
+    want = (q.double() @ wq.double().t()).to(dtype)
+    for _ in range(3):
+        assert torch.equal(linear_q8(q, one(rows), wq, one(M), dtype), want)
+
+
 @pytest.mark.parametrize("rows", [64, 400])
 def test_whole_numbers_are_exact(rows):
     """Small whole numbers have exact products and sums: every element, whatever the order."""
