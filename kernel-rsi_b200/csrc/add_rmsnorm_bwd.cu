@@ -1,7 +1,8 @@
 // add_rmsnorm_bwd.cu - the backward of the residual norm (add_rmsnorm.cu), for B200.  From z, r and the gradients gy
 // of y and gz of z, in fp32 with one rounding at the end:
-//   dz = r * gy * w - z * r^3 * mean(gy * w * z) + gz,   dw = sum over the rows of gy * z * r
-// (x and res both have the gradient dz).  dw: each block adds up its rows, a second kernel the blocks, in a fixed
+//   dz = r * (gy * w - n * mean(gy * w * n)) + gz with n = z * r,   dw = sum over the rows of gy * n
+// (x and res both have the gradient dz).  In this order nothing leaves fp32's range where dz does not: r^3, which the
+// product taken apart has, is subnormal for rows of 5e12 and infinite for those of 1e-13.  dw: each block adds up its rows, a second kernel the blocks, in a fixed
 // order.
 #include "add_rmsnorm.cuh"
 #include "sm100.cuh"
@@ -128,14 +129,14 @@ add_rmsnorm_bwd_staged_kernel(const BwdArgs a) {
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const uint64_t gk = widen2<XT>(gu[k]), zk = widen2<XT>(zu[k]);
-        acc[c][k] = f2_fma(gk, f2_mul(zk, r2), acc[c][k]);
-        dot2 = f2_fma(f2_mul(gk, w[k]), zk, dot2);
+        const uint64_t nk = f2_mul(zk, r2);
+        acc[c][k] = f2_fma(gk, nk, acc[c][k]);
+        dot2 = f2_fma(f2_mul(gk, w[k]), nk, dot2);
       }
     }
     float lo, hi;
     f2_unpack(dot2, lo, hi);
-    const float dot = warp_sum(lo + hi);
-    const float m = -r * r * r * (dot / (float)n);
+    const float m = -(warp_sum(lo + hi) / (float)n);
     const uint64_t m2 = f2_pack(m, m);
     uint4* out = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.dz) + row * n);
 #pragma unroll
@@ -149,8 +150,8 @@ add_rmsnorm_bwd_staged_kernel(const BwdArgs a) {
       weight(c, w);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
-        const uint64_t gw = f2_mul(widen2<XT>(gu[k]), w[k]);
-        o[k] = narrow2<XT>(f2_fma(gw, r2, f2_fma(widen2<XT>(zu[k]), m2, widen2<XT>(au[k]))));
+        const uint64_t gw = f2_mul(widen2<XT>(gu[k]), w[k]), nk = f2_mul(widen2<XT>(zu[k]), r2);
+        o[k] = narrow2<XT>(f2_fma(f2_fma(nk, m2, gw), r2, widen2<XT>(au[k])));
       }
       if ((c * 32 + lane) * 8 < n) out[c * 32 + lane] = make_uint4(o[0], o[1], o[2], o[3]);
     }
@@ -222,7 +223,8 @@ add_rmsnorm_bwd_kernel(const BwdArgs a) {
     for (int c = 0; c < NCH; ++c)
 #pragma unroll
       for (int e = 0; e < VEC; ++e) {
-        acc[c][e] = fmaf(g[c][e], zv[c][e] * r, acc[c][e]);
+        zv[c][e] *= r;
+        acc[c][e] = fmaf(g[c][e], zv[c][e], acc[c][e]);
         g[c][e] *= wv[c][e];
         dot = fmaf(g[c][e], zv[c][e], dot);
       }
@@ -234,7 +236,7 @@ add_rmsnorm_bwd_kernel(const BwdArgs a) {
 #pragma unroll
       for (int i = 0; i < TPR / 32; ++i) dot += red[turn][i];
     }
-    const float m = -r * r * r * (dot / (float)n);
+    const float m = -(dot / (float)n);
     T* dz = static_cast<T*>(a.dz) + row * n;
 #pragma unroll
     for (int c = 0; c < NCH; ++c) {
@@ -242,7 +244,7 @@ add_rmsnorm_bwd_kernel(const BwdArgs a) {
       if (col < n) {
         float o[VEC];
 #pragma unroll
-        for (int e = 0; e < VEC; ++e) o[e] = fmaf(g[c][e], r, fmaf(zv[c][e], m, add[c][e]));
+        for (int e = 0; e < VEC; ++e) o[e] = fmaf(fmaf(zv[c][e], m, g[c][e]), r, add[c][e]);
         store_row<XT, VEC>(dz + col, o);
       }
     }
