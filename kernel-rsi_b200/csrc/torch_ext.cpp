@@ -566,10 +566,14 @@ std::tuple<at::Tensor, at::Tensor> add_rmsnorm_bwd(const c10::optional<at::Tenso
   TORCH_CHECK(z.dim() == 2 && w.dim() == 1 && w.size(0) == z.size(1), "add_rmsnorm_bwd: z must be [rows, n] and w [n]");
   TORCH_CHECK(rstd.scalar_type() == at::kFloat && rstd.numel() == z.size(0), "add_rmsnorm_bwd: bad rstd");
   TORCH_CHECK(!have_z || gz->sizes() == z.sizes(), "add_rmsnorm_bwd: gz must match z");
-  if (!gy.has_value() || !gy->defined())
-    return {have_z ? gz->to(z.scalar_type(), /*non_blocking=*/false, /*copy=*/true) : at::zeros_like(z), at::zeros_like(w)};
-  TORCH_CHECK(gy->sizes() == z.sizes(), "add_rmsnorm_bwd: gy must match z");
   c10::cuda::CUDAGuard guard(z.device());
+  if (!gy.has_value() || !gy->defined()) {   // contiguous like the kernel's, whatever gz's and z's strides
+    auto dz = at::empty(z.sizes(), z.options());
+    if (have_z) dz.copy_(*gz);
+    else dz.zero_();
+    return {dz, at::zeros(w.sizes(), w.options())};
+  }
+  TORCH_CHECK(gy->sizes() == z.sizes(), "add_rmsnorm_bwd: gy must match z");
   auto zc = packed(z), wc = packed(w), rc = rstd.contiguous();
   auto g = packed(gy->to(z.scalar_type()));
   at::Tensor g2 = have_z ? packed(gz->to(z.scalar_type())) : at::Tensor();
