@@ -139,8 +139,13 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict):
-        """The base class casts states to their parameter's type; they keep their own here."""
+        """The base class casts states to their parameter's type; they keep their own here.  It leaves a group's tensors
+        where the dictionary has them; the step count and a tensor lr go to the group's parameters' device."""
         super().load_state_dict(state_dict)
+        for group in self.param_groups:
+            for key in ("step", "lr"):
+                if isinstance(group.get(key), torch.Tensor) and group["params"]:
+                    group[key] = group[key].to(group["params"][0].device)
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(ids, params):
