@@ -313,13 +313,19 @@ int krsi_linear_q8(const void* q, int64_t q_stride, const float* scale, const vo
  *   t = t + 1,  m = b1 m + (1 - b1) g',  v = b2 v + (1 - b2) g'^2,
  *   p = p (1 - lr wd) - lr / (1 - b1^t) * m / (sqrt(v) / sqrt(1 - b2^t) + eps)
  * A norm that is not finite leaves everything as it is, the step included. */
+
+/* Added to state_bits 8: m's codes are rounded up or down at random, right on average, as those of sqrt(v) always are.
+ * Without it m's codes are the nearest ones, which is right for one step and not for a run of them: m stops wherever
+ * (1 - b1) |g' - m| is below half a code. */
+#define KRSI_ADAMW_RANDOM_M 256
+
 typedef struct {
   void* p;            /* [n] of p_dtype */
   const void* g;      /* [n] of g_dtype: p_dtype or F32 */
-  void* m;            /* state_bits 32: fp32 m and v; 8: e4m3 codes of m and of sqrt(v) */
+  void* m;            /* state_bits 32: fp32 m and v; 8, alone or + KRSI_ADAMW_RANDOM_M: e4m3 codes of m and of sqrt(v) */
   void* v;
   float* master;      /* fp32 copy of a 16-bit p that is updated in its place (p: its rounding), or null */
-  uint8_t* exponents; /* state_bits 8: [ceil(n / 256), 2]: a group of 256 codes stands for code * 2^(e - 127),
+  uint8_t* exponents; /* 8-bit states: [ceil(n / 256), 2]: a group of 256 codes stands for code * 2^(e - 127),
                          e of m and of sqrt(v); 255 marks a group that is not finite (it reads back as NaN).
                          2-byte aligned */
   int64_t n;

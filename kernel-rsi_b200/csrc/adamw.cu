@@ -11,10 +11,13 @@
 //
 // 8-bit states: m and r = sqrt(v) as e4m3 at a power of two for each group of 256 values, which puts the group's
 // largest magnitude into [128, 256): 13 binades below it keep 3 bits of mantissa, three more lose one each.  r and not
-// v, because a square takes twice the binades.  m is rounded to nearest: it moves by a tenth a step, more than half
-// a code.  v moves by a thousandth, far less than half a code: rounded to nearest it would stay where it is, so r
-// is rounded up or down at random, right on average.  The randomness is a hash of the element's place and t, so a
-// step has the same bits every time.  A positive v never becomes 0, which eps alone would divide by.
+// v, because a square takes twice the binades.  r is rounded up or down at random, right on average: it moves by far
+// less than half a code a step, and rounded to nearest it would stay where it is.  So does m wherever (1 - b1) |g' - m|
+// is below half a code: rounded to nearest it stops at 0.71 of a constant gradient (b1 0.9; 0.54 at 0.95), and the last
+// codes of an element without gradients never go.  With KRSI_ADAMW_RANDOM_M it is rounded at random too, by other
+// bits, which holds over a run of steps; without, one step's codes are the nearest ones.  The randomness is a hash of
+// the element's place and t, so a step has the same bits every time.  A positive v never becomes 0, which eps alone
+// would divide by.
 // A group with a value that is not finite reads back as NaN.
 // The moments and their codes are formed by IEEE operations in a fixed order without contraction.
 #include <math.h>
@@ -140,6 +143,12 @@ __device__ __forceinline__ uint32_t dither(uint32_t pair, uint32_t step) {
   h = (h ^ (h >> 16)) * 0x21F0AAADu;
   h = (h ^ (h >> 15)) * 0x735A2D97u;
   return h ^ (h >> 15);
+}
+// As many for m, independent of those that round r: counted over all h, each combination of the first six bits of a half
+// of either is equally frequent, to 0.2%.
+__device__ __forceinline__ uint32_t dither_m(uint32_t h) {
+  h *= 0x2C1B3C6Du;
+  return h ^ (h >> 16);
 }
 
 // ---------------------------------------------------------------- kernels
@@ -383,6 +392,13 @@ __device__ __forceinline__ float min3(float a, float b, float c) {
   return d;
 }
 
+// The least of three magnitudes.
+__device__ __forceinline__ float min3_abs(float a, float b, float c) {
+  float d;
+  asm("min.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 constexpr float kLift = 0.015625f;       // 2^-6: codes below are subnormal, 2^-9 apart
 constexpr float kLeast = 0.001953125f;   // 2^-9, the least positive code
 
@@ -410,6 +426,22 @@ __device__ __forceinline__ float round_root(float v, float inverse_scale, uint32
   return x > 0.f ? fmaxf(__fadd_rn(__uint_as_float(up), -lift), kLeast) : 0.f;
 }
 
+// Scaled m, |x| >= 2^-6, to codes, up in magnitude with the probability of the bits below the code's last one: as
+// round_roots, but x is exact, so its last bit is set instead of 8 units added: the sum is never on the conversion's border.
+__device__ __forceinline__ void round_moments(const float* x, const uint32_t* h, float* code) {
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    code[2 * k] = __uint_as_float((__float_as_uint(x[2 * k]) | 1u) + ((h[k] << 4) & 0xffff0u) - 0x80000u);
+    code[2 * k + 1] = __uint_as_float((__float_as_uint(x[2 * k + 1]) | 1u) + ((h[k] >> 16) << 4) - 0x80000u);
+  }
+}
+// The same for any x; the least codes go to 0 as well.
+__device__ __forceinline__ float round_moment(float x, uint32_t random16) {
+  const float a = fabsf(x), lift = a < kLift ? kLift : 0.f;
+  const uint32_t up = (__float_as_uint(__fadd_rn(a, lift)) + (random16 << 4)) & 0xfff00000u;
+  return copysignf(__fadd_rn(__uint_as_float(up), -lift), x);
+}
+
 // A lane's part of a group: as read, and the results.
 template <int WT, int GT>
 struct Lane8 {
@@ -424,7 +456,7 @@ struct Done8 {
   uint32_t ex;
 };
 // Called by whole warps.  pair: the place of the lane's first value, halved.
-template <int WT, int GT>
+template <int WT, int GT, bool RANDOM_M>
 __device__ __forceinline__ void update8(const Lane8<WT, GT>& in, const RatePairs& c, const Factors& f, uint32_t pair,
                                         Done8& out) {
   using namespace sm100;
@@ -459,6 +491,24 @@ __device__ __forceinline__ void update8(const Lane8<WT, GT>& in, const RatePairs
   const float ir = inverse_scale_of(er);
   const uint64_t im = twice(inverse_scale_of(em)), back = twice(scale_of(er) * f.inv_root);
   const uint64_t decay = twice(f.decay), rate = twice(-f.rate);
+  if constexpr (RANDOM_M) {   // (before the roots, for fewer live registers)
+    uint32_t h[4];
+    float code[kLane];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      f2_unpack(f2_mul(m[k], im), mf[2 * k], mf[2 * k + 1]);
+      h[k] = dither_m(dither(pair + k, f.step));
+    }
+    const float least =
+        min3_abs(min3_abs(mf[0], mf[1], mf[2]), min3_abs(mf[3], mf[4], mf[5]), min3_abs(mf[6], mf[7], mf[7]));
+    if (least >= kLift) {
+      round_moments(mf, h, code);
+    } else {
+#pragma unroll
+      for (int e = 0; e < kLane; ++e) code[e] = round_moment(mf[e], e % 2 ? h[e / 2] >> 16 : h[e / 2] & 0xffffu);
+    }
+    out.m = pack_codes(code);
+  }
   float x[kLane];
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
@@ -470,9 +520,9 @@ __device__ __forceinline__ void update8(const Lane8<WT, GT>& in, const RatePairs
     f2_unpack(f2_fma(f2_pack(x[2 * k], x[2 * k + 1]), back, pair_of(c.eps)), lo, hi);
     const uint64_t quotient = f2_mul(m[k], f2_pack(rcp_approx(lo), rcp_approx(hi)));
     f2_unpack(f2_fma(quotient, rate, f2_mul(in.p.pair(k), decay)), out.p[2 * k], out.p[2 * k + 1]);
-    f2_unpack(f2_mul(m[k], im), mf[2 * k], mf[2 * k + 1]);
+    if constexpr (!RANDOM_M) f2_unpack(f2_mul(m[k], im), mf[2 * k], mf[2 * k + 1]);
   }
-  out.m = pack_codes(mf);
+  if constexpr (!RANDOM_M) out.m = pack_codes(mf);
   uint32_t h[4];
 #pragma unroll
   for (int k = 0; k < 4; ++k) h[k] = dither(pair + k, f.step);
@@ -485,7 +535,7 @@ __device__ __forceinline__ void update8(const Lane8<WT, GT>& in, const RatePairs
   out.r = pack_codes(code);
 }
 
-template <int PT, int GT, bool MASTER, int CAP>
+template <int PT, int GT, bool MASTER, bool RANDOM_M, int CAP>
 __global__ void __launch_bounds__(kThreads, 3)
 adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ RatePairs c, const int span,
               const Factors* __restrict__ factors) {
@@ -531,7 +581,7 @@ adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Ra
         const Lane8<WT, GT> now = in;
         if (j + 1 < whole) fetch(j + 1);
         Done8 out;
-        update8(now, c, f, (uint32_t)((at + (int64_t)j * kGroup) >> 1), out);
+        update8<WT, GT, RANDOM_M>(now, c, f, (uint32_t)((at + (int64_t)j * kGroup) >> 1), out);
         if constexpr (MASTER) store8<KRSI_F32>(const_cast<W*>(w), (int64_t)j * kGroup, true, kLane, out.p);
         store8<PT>(t.p, at + (int64_t)j * kGroup, true, kLane, out.p);
         store_codes(const_cast<uint8_t*>(m), (int64_t)j * kGroup, true, kLane, out.m);
@@ -552,7 +602,7 @@ adamw8_kernel(const __grid_constant__ Table<CAP> tab, const __grid_constant__ Ra
       in.r = load_codes(t.v, a, vec, live);
       in.ex = *reinterpret_cast<const uint16_t*>(ex);
       Done8 out;
-      update8(in, c, f, (uint32_t)(a >> 1), out);
+      update8<WT, GT, RANDOM_M>(in, c, f, (uint32_t)(a >> 1), out);
       if constexpr (MASTER) store8<KRSI_F32>(t.master, a, vec, live, out.p);
       store8<PT>(t.p, a, vec, live, out.p);
       store_codes(t.m, a, vec, live, out.m);
@@ -569,12 +619,16 @@ bool aligned_to(const void* p, size_t a) { return (reinterpret_cast<uintptr_t>(p
 int64_t launches_at_most(int64_t count) { return count / kLargeCap + 4; }   // one more for each gradient type
 
 // A tensor's kind: what the update's kernel is compiled for.
-constexpr int kKinds = 3 * 2 * 2 * 2;
-constexpr int kind_of(int p_dtype, int g_dtype, bool master, bool q8) {
-  return ((p_dtype * 2 + (g_dtype != p_dtype)) * 2 + master) * 2 + q8;
+enum States : int { kStates32 = 0, kStates8 = 1, kStates8Random = 2 };
+constexpr int kKinds = 3 * 2 * 2 * 3;
+constexpr int kind_of(int p_dtype, int g_dtype, bool master, int states) {
+  return ((p_dtype * 2 + (g_dtype != p_dtype)) * 2 + master) * 3 + states;
 }
+constexpr int kBits8Random = 8 + KRSI_ADAMW_RANDOM_M;
+bool in_8_bits(const krsi_adamw_tensor& t) { return t.state_bits == 8 || t.state_bits == kBits8Random; }
 int kind_of(const krsi_adamw_tensor& t) {
-  return kind_of(t.p_dtype, t.g_dtype, t.master != nullptr, t.state_bits == 8);
+  const int states = t.state_bits == 8 ? kStates8 : t.state_bits == kBits8Random ? kStates8Random : kStates32;
+  return kind_of(t.p_dtype, t.g_dtype, t.master != nullptr, states);
 }
 
 // Calls `launch(table)` for tables of the tensors that `take` accepts, `left` of them, in chunks of `chunk` values.
@@ -591,7 +645,7 @@ int for_tables(const krsi_adamw_tensor* tensors, int64_t left, int chunk, Take t
       const int64_t own = (s.n + chunk - 1) / chunk;
       if (own > INT32_MAX) return KRSI_ERR_UNSUPPORTED;
       if (chunks + own > INT32_MAX) break;   // the next launch takes it
-      const size_t state = s.state_bits == 8 ? 8 : 32;
+      const size_t state = in_8_bits(s) ? 8 : 32;
       const bool aligned = aligned_to(s.p, s.p_dtype == KRSI_F32 ? 32 : 16) &&
                            aligned_to(s.g, s.g_dtype == KRSI_F32 ? 32 : 16) && aligned_to(s.m, state) &&
                            aligned_to(s.v, state) && aligned_to(s.master, 32);
@@ -622,9 +676,10 @@ struct Counts {
   int64_t kind[kKinds] = {}, grad[3] = {}, values[kKinds] = {};
 };
 
-template <int PT, int GT, bool MASTER, bool Q8>
+template <int PT, int GT, bool MASTER, int STATES>
 int update(const krsi_adamw_tensor* tensors, const Counts& counts, const Rates& c, const Factors* f, cudaStream_t s) {
-  constexpr int kind = kind_of(PT, GT, MASTER, Q8);
+  constexpr int kind = kind_of(PT, GT, MASTER, STATES);
+  constexpr bool Q8 = STATES != kStates32;
   auto take = [](const krsi_adamw_tensor& t) { return t.n > 0 && kind_of(t) == kind; };
   // fp32 states: one group a warp where four would leave SMs without a block (150,000 values: 5 us became 3)
   const int groups = counts.values[kind] < (int64_t)kNumSMsB200 * kChunk ? 1 : kGroupsPerWarp;
@@ -636,8 +691,8 @@ int update(const krsi_adamw_tensor* tensors, const Counts& counts, const Rates& 
       constexpr int warps = kBlocks8 * (kThreads / 32);
       const int64_t span = ((int64_t)tab.n_chunks + warps - 1) / warps;
       const int64_t blocks = (tab.n_chunks + span * (kThreads / 32) - 1) / (span * (kThreads / 32));
-      KRSI_CUDA_TRY(launch_pdl(adamw8_kernel<PT, GT, MASTER, cap>, dim3((unsigned)blocks), dim3(kThreads), 0, s, tab,
-                               RatePairs(c), (int)span, f));
+      KRSI_CUDA_TRY(launch_pdl(adamw8_kernel<PT, GT, MASTER, STATES == kStates8Random, cap>, dim3((unsigned)blocks),
+                               dim3(kThreads), 0, s, tab, RatePairs(c), (int)span, f));
     } else {
       KRSI_CUDA_TRY(launch_pdl(adamw_kernel<PT, GT, MASTER, cap>, dim3(tab.n_chunks), dim3(kThreads), 0, s, tab, c, groups,
                                f));
@@ -680,12 +735,12 @@ extern "C" int krsi_adamw_step(const krsi_adamw_tensor* tensors, int64_t count, 
   Counts counts;
   for (int64_t i = 0; i < count; ++i) {
     const krsi_adamw_tensor& t = tensors[i];
-    KRSI_CHECK_ARG(t.n >= 0 && dtype_ok(t.p_dtype) && (t.state_bits == 8 || t.state_bits == 32));
+    KRSI_CHECK_ARG(t.n >= 0 && dtype_ok(t.p_dtype) && (t.state_bits == 32 || in_8_bits(t)));
     KRSI_CHECK_ARG(t.g_dtype == t.p_dtype || t.g_dtype == KRSI_F32);
     if (t.n == 0) continue;
     KRSI_CHECK_ARG(t.p && t.g && t.m && t.v && (t.state_bits == 32 || t.exponents));
     KRSI_CHECK_ARG(t.p_dtype != KRSI_F32 || !t.master);
-    if (t.state_bits == 8 && !aligned_to(t.exponents, 2)) return KRSI_ERR_MISALIGNED;
+    if (in_8_bits(t) && !aligned_to(t.exponents, 2)) return KRSI_ERR_MISALIGNED;
     ++counts.kind[kind_of(t)];
     ++counts.grad[t.g_dtype];
     counts.values[kind_of(t)] += t.n;
@@ -709,8 +764,9 @@ extern "C" int krsi_adamw_step(const krsi_adamw_tensor* tensors, int64_t count, 
   const Rates c{(float)beta1, (float)(1.0 - beta1), (float)beta2, (float)(1.0 - beta2), (float)eps};
 #define KRSI_UPDATE(PT, GT, MASTER)                                                        \
   do {                                                                                     \
-    int rc = update<PT, GT, MASTER, false>(tensors, counts, c, factors, stream);            \
-    if (rc == KRSI_OK) rc = update<PT, GT, MASTER, true>(tensors, counts, c, factors, stream); \
+    int rc = update<PT, GT, MASTER, kStates32>(tensors, counts, c, factors, stream);       \
+    if (rc == KRSI_OK) rc = update<PT, GT, MASTER, kStates8>(tensors, counts, c, factors, stream); \
+    if (rc == KRSI_OK) rc = update<PT, GT, MASTER, kStates8Random>(tensors, counts, c, factors, stream); \
     if (rc != KRSI_OK) return rc;                                                          \
   } while (0)
   KRSI_UPDATE(KRSI_F32, KRSI_F32, false);

@@ -674,11 +674,12 @@ at::Tensor linear_q8(const at::Tensor& q_in, const at::Tensor& scale_in, const a
 
 // ---------------------------------------------------------------- AdamW
 // One step for every tensor, in place; returns the norm of all gradients (empty where max_norm is 0).  masters and
-// exponents: a tensor for each parameter, one without elements where it has none, or an empty list.
+// exponents: a tensor for each parameter, one without elements where it has none, or an empty list.  random_m: of the 8-bit
+// states, m's codes at random too.
 at::Tensor adamw_step(at::TensorList params, at::TensorList grads, at::TensorList exp_avgs, at::TensorList exp_avg_sqs,
                       at::TensorList masters, at::TensorList exponents, const at::Tensor& step,
                       const c10::optional<at::Tensor>& lr_tensor, double lr, double beta1, double beta2, double eps,
-                      double weight_decay, double max_norm) {
+                      double weight_decay, double max_norm, bool random_m) {
   const size_t count = params.size();
   TORCH_CHECK(grads.size() == count && exp_avgs.size() == count && exp_avg_sqs.size() == count,
               "adamw_step: as many grads, exp_avgs and exp_avg_sqs as params are needed");
@@ -718,7 +719,7 @@ at::Tensor adamw_step(at::TensorList params, at::TensorList grads, at::TensorLis
     TORCH_CHECK(t.g_dtype == t.p_dtype || t.g_dtype == KRSI_F32,
                 "adamw_step: a gradient must have its parameter's dtype or float32");
     const bool q8 = exp_avgs[i].scalar_type() == at::kFloat8_e4m3fn;
-    t.state_bits = q8 ? 8 : 32;
+    t.state_bits = !q8 ? 32 : random_m ? 8 + KRSI_ADAMW_RANDOM_M : 8;
     own(exp_avgs[i], p, q8 ? at::kFloat8_e4m3fn : at::kFloat, "exp_avgs");
     own(exp_avg_sqs[i], p, q8 ? at::kFloat8_e4m3fn : at::kFloat, "exp_avg_sqs");
     t.p = p.data_ptr();
@@ -1008,7 +1009,7 @@ TORCH_LIBRARY(krsi, m) {
   m.def("linear_q8(Tensor q, Tensor scale, Tensor wq, Tensor wscale, ScalarType out_dtype) -> Tensor");
   m.def("adamw_step(Tensor(a!)[] params, Tensor[] grads, Tensor(b!)[] exp_avgs, Tensor(c!)[] exp_avg_sqs, "
         "Tensor(d!)[] masters, Tensor(e!)[] exponents, Tensor(f!) step, Tensor? lr_tensor, float lr, float beta1, "
-        "float beta2, float eps, float weight_decay, float max_norm) -> Tensor");
+        "float beta2, float eps, float weight_decay, float max_norm, bool random_m=False) -> Tensor");
 }
 
 TORCH_LIBRARY_IMPL(krsi, CUDA, m) {
@@ -1064,7 +1065,8 @@ bool unpack(PyObject* list, std::vector<at::Tensor>& out) {
 
 PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
   HANDLE_TH_ERRORS
-  if (nargs != 14) return PyErr_Format(PyExc_TypeError, "adamw_step: 14 arguments expected, got %zd", nargs);
+  if (nargs != 14 && nargs != 15)
+    return PyErr_Format(PyExc_TypeError, "adamw_step: 14 or 15 arguments expected, got %zd", nargs);
   const bool modes = c10::impl::TorchDispatchModeTLS::any_modes_set() ||
                      at::impl::PythonTorchFunctionTLS::stack_len() > 0;
   std::vector<at::Tensor> lists[6];
@@ -1080,6 +1082,8 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     number[k] = PyFloat_AsDouble(args[8 + k]);
     if (number[k] == -1.0 && PyErr_Occurred()) return nullptr;
   }
+  const int random_m = nargs == 15 ? PyObject_IsTrue(args[14]) : 0;
+  if (random_m < 0) return nullptr;
   const at::Tensor step = THPVariable_Unpack(args[6]);
   const c10::optional<at::Tensor> lr =
       args[7] == Py_None ? c10::nullopt : c10::optional<at::Tensor>(THPVariable_Unpack(args[7]));
@@ -1088,7 +1092,7 @@ PyObject* py_adamw_step(PyObject*, PyObject* const* args, Py_ssize_t nargs) {
     pybind11::gil_scoped_release release;
     at::AutoDispatchBelowADInplaceOrView below;
     norm = adamw_step(lists[0], lists[1], lists[2], lists[3], lists[4], lists[5], step, lr, number[0], number[1],
-                      number[2], number[3], number[4], number[5]);
+                      number[2], number[3], number[4], number[5], random_m != 0);
   }
   return THPVariable_Wrap(std::move(norm));
   END_HANDLE_TH_ERRORS

@@ -214,7 +214,7 @@ def _register_compile_support() -> None:
 
     @reg_fake("krsi::adamw_step")
     def _(params, grads, exp_avgs, exp_avg_sqs, masters, exponents, step, lr_tensor, lr, beta1, beta2, eps,
-          weight_decay, max_norm):
+          weight_decay, max_norm, random_m=False):
         return step.new_empty(() if max_norm > 0 else (0,), dtype=torch.float32)
 
     # Autograd of the forward ops, used when a compiled graph contains them (the eager path

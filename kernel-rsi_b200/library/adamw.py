@@ -14,13 +14,17 @@ parameter's last place are lost).
 
 States in 8 bits: m and sqrt(v) as float8_e4m3fn and, for each group of 256 elements, an exponent byte for either;
 a value is code * 2^(exponent - 127).  The group's largest magnitude lies in [128, 256), so 13 binades below it keep
-3 bits of mantissa.  m is rounded to nearest; sqrt(v), which a step moves by far less than half a code, is rounded up
-or down by a hash of the element's place and t, right on average (the same bits every run).  10 bytes a bf16
-parameter are read and written where fp32 states take 22.  A group with a value that is not finite reads back as NaN.
+3 bits of mantissa.  A step moves sqrt(v) and often m by far less than half a code, so both are rounded up or down by a
+hash of the element's place and t, right on average (the same bits every run): rounding="random", which AdamW takes.
+With "nearest" m's codes are the nearest ones, as one step alone would have them; over a run of steps m then stops
+wherever (1 - b1) |g' - m| is below half a code (0.71 of a constant gradient for b1 0.9), and an element whose gradients
+have ended keeps moving.  10 bytes a bf16 parameter are read and written where fp32 states take 22.  A group with a
+value that is not finite reads back as NaN.
 
 Kernels: kernel-rsi_b200/csrc/adamw.cu; C ABI: include/krsi_b200.h.
 """
 import sys
+import warnings
 from pathlib import Path
 
 import torch
@@ -30,21 +34,38 @@ from _compat import compiling  # noqa: E402
 from _ext import direct, ops  # noqa: E402
 
 GROUP = 256
+_warned = False
 
 
 def adamw_step(params, grads, exp_avgs, exp_avg_sqs, step, *, lr, betas=(0.9, 0.999), eps=1e-8, weight_decay=0.01,
-               max_norm=0.0, masters=None, exponents=None):
+               max_norm=0.0, masters=None, exponents=None, rounding=None):
     """One AdamW step on lists of tensors, in place; step: an int64 CUDA tensor, counted on.  exp_avgs and exp_avg_sqs
     are fp32, or float8_e4m3fn codes of m and sqrt(v) with exponents (new_state() makes either).  masters: fp32
     copies of the 16-bit parameters (None, or an entry without elements, where there is none).  Returns the norm of
-    all gradients where max_norm > 0, else None.  No two tensors may overlap."""
+    all gradients where max_norm > 0, else None.  No two tensors may overlap.
+
+    rounding: of m's 8-bit codes, "random" (right on average: what a run of steps needs) or "nearest" (right for a single
+    step; over a run m stops short of its mean).  Where it is not given it is "nearest", with a warning."""
+    if rounding is None:
+        if exponents and not _warned and not compiling():
+            _warn_nearest(exp_avgs)
+    elif rounding not in ("random", "nearest"):
+        raise ValueError(f'adamw_step: rounding must be "random" or "nearest", got {rounding!r}')
     device_lr = isinstance(lr, torch.Tensor)
     args = (params, grads, exp_avgs, exp_avg_sqs, masters or [], exponents or [], step, lr if device_lr else None,
-            0.0 if device_lr else lr, betas[0], betas[1], eps, weight_decay, max_norm)
+            0.0 if device_lr else lr, betas[0], betas[1], eps, weight_decay, max_norm, rounding == "random")
     norm = NotImplemented if direct is None or compiling() else direct.adamw_step(*args)
     if norm is NotImplemented:
         norm = ops.adamw_step(*args)
     return norm if max_norm > 0 else None
+
+
+def _warn_nearest(exp_avgs):
+    global _warned
+    if any(m.dtype == torch.float8_e4m3fn for m in exp_avgs):
+        _warned = True
+        warnings.warn('adamw_step: 8-bit states are rounded to nearest, which is right for a single step only; a run of '
+                      'steps needs rounding="random" ("nearest" is this, without the warning)', stacklevel=3)
 
 
 def new_state(p, bits=32):
@@ -67,7 +88,8 @@ def dequantise(exp_avg, exp_avg_sq, exponents):
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's role on adamw_step(): each parameter group is one call.
 
-    bits: of the states; parameters with fewer than min_8bit_size elements keep fp32 ones.  master: keep an fp32
+    bits: of the states (8: m and sqrt(v) rounded at random, right on average over a run, for any betas); parameters with
+    fewer than min_8bit_size elements keep fp32 ones.  master: keep an fp32
     master of each 16-bit parameter.  max_norm: clip by the norm of the group's gradients (0: not); grad_norm holds
     the last step's, one a group.  lr may be a 0-dim fp32 CUDA tensor.  Parameters without a gradient are left
     alone; the step counts the group's calls, not each parameter's.  States are made by the first step, or by
@@ -135,7 +157,8 @@ class AdamW(torch.optim.Optimizer):
             self.grad_norm.append(adamw_step(
                 params, [p.grad for p in params], columns["exp_avg"], columns["exp_avg_sq"], group["step"],
                 lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"],
-                max_norm=group["max_norm"], masters=columns["master"], exponents=columns["exponents"]))
+                max_norm=group["max_norm"], masters=columns["master"], exponents=columns["exponents"],
+                rounding="random"))
         return loss
 
     def load_state_dict(self, state_dict):
