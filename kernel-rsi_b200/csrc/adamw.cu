@@ -281,6 +281,7 @@ adamw_kernel(const __grid_constant__ Table<CAP> tab, const Rates c, const int gr
       const float ge = __fmul_rn(g[e], f.clip);
       m[e] = __fadd_rn(__fmul_rn(m[e], c.beta1), __fmul_rn(ge, c.one_minus_beta1));
       v[e] = __fadd_rn(__fmul_rn(v[e], c.beta2), __fmul_rn(__fmul_rn(ge, ge), c.one_minus_beta2));
+      // (the quotient to 2 units of its last place, of a move that is some thousandth of p)
       p[e] = p[e] * f.decay - f.rate * __fdividef(m[e], fmaf(sqrtf(v[e]), f.inv_root, c.eps));
     }
     if constexpr (MASTER) store8<KRSI_F32>(t.master, at, vec, live, p);

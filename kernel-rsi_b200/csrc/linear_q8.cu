@@ -13,9 +13,10 @@
 //   more              linear_q8_pair_kernel: CTA pairs (cta_group::2) on tiles of 256 rows x up to 256 columns, all
 //                     columns of the same rows at the same time, so that out is written in whole rows
 //
-// What bounds it (32768 x 1152 x 9216 to bf16, 696 GFLOP and 604 MB of output: 299 us, 2.33 PFLOP/s): the output's
-// way out and the power cap.  Without stores the same kernel takes 234 us; writing 604 MB alone takes 156 (3.9 TB/s),
-// and the two do not hide each other wholly.  Measured on the way: boxes of 64 bytes a row, one a warp, in place of
+// What bounds it (32768 x 1152 x 9216 to bf16, 696 GFLOP and 604 MB of output: 332 to 339 us in a long loop, 2.1 PFLOP/s at
+// 1.46 GHz under the power cap; 299 in short runs, 2.33, as are all figures from here): the output's way out and the power
+// cap.  Without stores the same kernel takes 234 us; writing 604 MB alone takes 156 (3.9 TB/s), and the two do not hide
+// each other wholly.  Measured on the way: boxes of 64 bytes a row, one a warp, in place of
 // two of 128: 312; ordinary stores of the same boxes: 317; the weight's K blocks kept in shared memory while a pair
 // walks down the rows (a third of the L2's reads): 301, and 130 against 116 for 3456 columns, for the shorter ring that
 // leaves; pairs walking along the columns of rows of their own: 355.

@@ -88,10 +88,10 @@ def dequantise(exp_avg, exp_avg_sq, exponents):
 class AdamW(torch.optim.Optimizer):
     """torch.optim.AdamW's role on adamw_step(): each parameter group is one call.
 
-    bits: of the states (8: m and sqrt(v) rounded at random, right on average over a run, for any betas); parameters with
-    fewer than min_8bit_size elements keep fp32 ones.  master: keep an fp32
-    master of each 16-bit parameter.  max_norm: clip by the norm of the group's gradients (0: not); grad_norm holds
-    the last step's, one a group.  lr may be a 0-dim fp32 CUDA tensor.  Parameters without a gradient are left
+    bits: of the states (8: m and sqrt(v) rounded at random, right on average over a run for b1 up to 0.999); parameters
+    with fewer than min_8bit_size elements keep fp32 ones.  master: keep an fp32 master of each 16-bit parameter.  max_norm: clip by the norm of the group's gradients (0: not), which is the model's
+    where there is one group alone (else torch.nn.utils.clip_grad_norm_ before the step); grad_norm holds the last
+    step's, one a group.  lr may be a 0-dim fp32 CUDA tensor.  Parameters without a gradient are left
     alone; the step counts the group's calls, not each parameter's.  States are made by the first step, or by
     init_states(), which has to come before a step is captured into a CUDA graph."""
 
